@@ -600,6 +600,63 @@ mml_status mml_wrmf_auc(mml_wrmf* h, const int32_t* candidates, int32_t n_candid
                         const int32_t* users, int32_t n_users, const int64_t* test_off,
                         const int32_t* test_items, double* out_auc);
 
+/* ------------------------------------------------------------------ softmax over the catalogue
+ * For row r (user u = users[r], or r) and item j: s_rj = <U_u, V_j> + b_j and p_rj the softmax of
+ * row r over the items that are not excluded.  No reference counterpart (the reference ranks by
+ * score; these give the scores a probability).  These calls take device pointers and are
+ * stream-ordered: they return once the kernels are enqueued on `stream` (a hipStream_t, NULL = the
+ * default stream) of `device`, allocate nothing, read nothing back and may be captured into a
+ * graph.  `workspace` (256-byte aligned, mml_item_log_probs_workspace bytes) belongs to the call
+ * until its work is done: two calls that can overlap need one each.
+ *
+ * Excluded from row r: the items of user u's list in the CSR exclude_offsets / exclude_items
+ * (n_exclude entries; e.g. the training items; unsorted and repeated ids allowed, ids outside the
+ * catalogue skipped), and for every row the items whose bias is -1e30 or lower (-inf included);
+ * what their factors hold does not matter.  A row with no item left has log_norm -inf, entropy 0,
+ * log_probs -inf, top_items -1 and no gradient.  A user id outside [0, n_users) gives NaN (top
+ * items -1) and no gradient; a factor or bias that is not finite (or above 3e38) and not excluded
+ * makes its rows NaN. */
+enum { MML_DTYPE_F32 = 0, MML_DTYPE_BF16 = 1, MML_DTYPE_F16 = 2 };
+typedef struct {
+    int32_t dtype;                  /* MML_DTYPE_* of both factor matrices */
+    int32_t num_factors;            /* 1 .. 256 */
+    int64_t n_rows;
+    int32_t n_users, n_items;       /* rows of the factor matrices */
+    const void* user_factors;       /* element (u, f) at u * ld_users + f */
+    const void* item_factors;
+    int64_t ld_users, ld_items;     /* >= num_factors, in elements */
+    const float* item_bias;         /* [n_items], NULL: 0 */
+    const int32_t* users;           /* [n_rows], NULL: row r is user r */
+    const int32_t* items;           /* [n_rows] the given items, NULL: none; an id outside the
+                                       catalogue (-1) means none for that row */
+    const int64_t* exclude_offsets; /* [n_users + 1], NULL: nothing excluded */
+    const int32_t* exclude_items;   /* [n_exclude] */
+    int64_t n_exclude;
+    int32_t n_top;                  /* 0 .. 128 */
+} mml_item_softmax_args;
+/* Workspace of the two calls below (grad 0 / 1) for these sizes. */
+mml_status mml_item_log_probs_workspace(const mml_item_softmax_args* args, int32_t grad,
+                                        int64_t* bytes);
+/* log_probs[r] = log p_r(items[r]) (0 without one, -inf for an excluded one), log_norm[r] =
+ * log sum_j exp(s_rj), entropy[r] = -sum_j p_rj log p_rj, top_items / top_log_probs [n_rows x n_top]:
+ * the n_top likeliest items and their log p, ordered by the exact score (64-bit sums), the lower
+ * id first among equals, -1 / -inf behind the last item. */
+mml_status mml_item_log_probs_device(const mml_item_softmax_args* args, float* log_probs,
+                                     float* log_norm, float* entropy, int32_t* top_items,
+                                     float* top_log_probs, void* workspace,
+                                     int64_t workspace_bytes, int32_t device, void* stream);
+/* The gradient of a loss L with grad_log_probs[r] = dL / d log_probs[r] and grad_entropy[r] =
+ * dL / d entropy[r] (either NULL: 0), log_norm and entropy as mml_item_log_probs_device gave them
+ * (entropy only read with grad_entropy): grad_users [n_rows x num_factors] per row (a user listed
+ * twice has two), grad_items [n_items x num_factors] in the factors' type with the row strides
+ * ld_*, grad_bias [n_items].  Every element is written, in the same order of sums every time. */
+mml_status mml_item_log_probs_grad_device(const mml_item_softmax_args* args, const float* log_norm,
+                                          const float* entropy, const float* grad_log_probs,
+                                          const float* grad_entropy, void* grad_users,
+                                          int64_t ld_grad_users, void* grad_items,
+                                          int64_t ld_grad_items, float* grad_bias, void* workspace,
+                                          int64_t workspace_bytes, int32_t device, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -16,6 +16,15 @@ from .rating_prediction import (BiasedMatrixFactorization, MatrixFactorization,
                                 SigmoidCombinedAsymmetricFactorModel, SigmoidSVDPlusPlus,
                                 SVDPlusPlus)
 
+
+def __getattr__(name):
+    """The operators on torch tensors, loaded on first use: the recommenders need no torch."""
+    if name in ("item_log_probs", "item_log_probs_grad", "ItemLogProbs"):
+        from . import item_softmax
+        return getattr(item_softmax, name)
+    raise AttributeError(f"module {__name__!r} has no attribute {name!r}")
+
+
 __all__ = ["BiasedMatrixFactorization", "MatrixFactorization", "SocialMF",
            "SigmoidItemAsymmetricFactorModel", "SigmoidUserAsymmetricFactorModel",
            "SigmoidCombinedAsymmetricFactorModel", "SVDPlusPlus", "SigmoidSVDPlusPlus", "BPRMF", "WRMF",
@@ -23,4 +32,5 @@ __all__ = ["BiasedMatrixFactorization", "MatrixFactorization", "SocialMF",
            "PosOnlyFeedback", "Mapping", "IdentityMapping", "read_ratings", "read_items", "Random",
            "DeviceRatingFile",
            "SystemRandom", "create_rating_predictor", "create_item_recommender",
-           "create_recommender", "list_recommenders"]
+           "create_recommender", "list_recommenders", "item_log_probs", "item_log_probs_grad",
+           "ItemLogProbs"]

@@ -67,6 +67,21 @@ class WrmfParams(ctypes.Structure):
     _fields_ = [("num_factors", ctypes.c_int32), ("refine_passes", ctypes.c_int32),
                 ("alpha", ctypes.c_double), ("regularization", ctypes.c_double)]
 
+
+
+DTYPE_F32, DTYPE_BF16, DTYPE_F16 = 0, 1, 2
+
+
+class ItemSoftmaxArgs(ctypes.Structure):
+    """mml_item_softmax_args (include/mml.h)."""
+    _fields_ = [("dtype", ctypes.c_int32), ("num_factors", ctypes.c_int32),
+                ("n_rows", ctypes.c_int64), ("n_users", ctypes.c_int32),
+                ("n_items", ctypes.c_int32), ("user_factors", _vp), ("item_factors", _vp),
+                ("ld_users", ctypes.c_int64), ("ld_items", ctypes.c_int64), ("item_bias", _vp),
+                ("users", _vp), ("items", _vp), ("exclude_offsets", _vp), ("exclude_items", _vp),
+                ("n_exclude", ctypes.c_int64), ("n_top", ctypes.c_int32)]
+
+
 # every exported symbol of include/mml.h: name -> (restype, argtypes)
 SIGNATURES = {
     "mml_abi_version": (ctypes.c_int, []),
@@ -184,6 +199,12 @@ SIGNATURES = {
     "mml_wrmf_last_refine_passes": (_st, [_vp, _i32p, _f32p]),
     "mml_wrmf_auc": (_st, [_vp, _i32p, ctypes.c_int32, _i32p, ctypes.c_int32, _i64p, _i32p,
                            _f64p]),
+    "mml_item_log_probs_workspace": (_st, [ctypes.POINTER(ItemSoftmaxArgs), ctypes.c_int32, _i64p]),
+    "mml_item_log_probs_device": (_st, [ctypes.POINTER(ItemSoftmaxArgs), _vp, _vp, _vp, _vp, _vp,
+                                        _vp, ctypes.c_int64, ctypes.c_int32, _vp]),
+    "mml_item_log_probs_grad_device": (_st, [ctypes.POINTER(ItemSoftmaxArgs), _vp, _vp, _vp, _vp,
+                                             _vp, ctypes.c_int64, _vp, ctypes.c_int64, _vp, _vp,
+                                             ctypes.c_int64, ctypes.c_int32, _vp]),
 }
 
 _lib = None

@@ -1,0 +1,968 @@
+// item_softmax.hip -- the softmax over the catalogue of a matrix-factorization model: log
+// probabilities of given items, the entropy, the top items (mml_item_log_probs_device) and the
+// gradient of a loss on them (mml_item_log_probs_grad_device).
+//
+// For a row r (a user) and item j:  s_rj = <U_r, V_j> + b_j,  lse_r = log sum_j exp(s_rj),
+// log p_rj = s_rj - lse_r,  H_r = -sum_j p_rj log p_rj.  With w_r = dL / d log p_r(given item t_r)
+// and h_r = dL / dH_r:
+//   G_rj = dL / ds_rj = w_r ([j = t_r] - p_rj) - h_r p_rj (log p_rj + H_r),
+//   dL/dU = G V,  dL/dV = G^T U,  dL/db_j = sum_r G_rj.
+// The R x N matrices s, p and G are never stored: 32 x 32 tiles of s are made on the matrix cores,
+// used in registers and dropped (flash style: a running maximum m, sum l and sum of e y).
+//
+// f32 factors run on the bf16 matrix cores at f32 accuracy: every value is split into three bf16
+// planes (8 significant bits each) and a product takes the six plane products a b with
+// plane(a) + plane(b) <= 2, accumulated in f32; the dropped ones are below 2^-23 of |a b|.
+// v_mfma_f32_32x32x16_bf16 does 1,024 flops per cycle and SIMD against 64 of the f32 form, so six
+// products are 2.7 times as fast.  bf16 factors are one plane; f16 factors one f16 plane for the
+// scores and two bf16 planes (exact: 11 bits) for the gradient products.  G is split into three
+// (f32) or two (bf16, f16: 16 bits, against outputs of 8 and 11 bits) planes.
+//
+// Tile layout.  v_mfma_f32_32x32x16: A (32 x 16), lane l holds row l % 32, k = 8 (l / 32) .. + 7;
+// B (16 x 32) the same with the column; C: lane l holds column l % 32, register i row
+// 8 (i / 4) + 4 (l / 32) + i % 4.  The streamed side is A, the side a wave keeps is B, so a lane
+// owns one row of the kept side: in the forward pass and the users' gradient one user per lane
+// pair (l, l + 32) and its softmax state needs no lane exchange; in the items' gradient one item.
+// The next product contracts over the streamed side.  Its B operand (16 x 32) for step s takes, in
+// lane l, the C registers 8 s .. 8 s + 7 as they are when the A operand's k order is
+// 16 s + 8 (e / 4) + 4 (l / 32) + e % 4, which the "transposed" fragments are laid out for.
+//
+// A preparation kernel writes both sides as fragments in that order (16 bytes per lane, 1 KB per
+// fragment), so every operand load is a linear 1 KB.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <cmath>
+
+#include "mml_device.h"
+#include "mml_internal.h"
+
+namespace {
+
+using f32x16 = __attribute__((ext_vector_type(16))) float;
+using f32x4 = __attribute__((ext_vector_type(4))) float;
+using u32x4 = __attribute__((ext_vector_type(4))) uint32_t;
+using bf16x8 = __attribute__((ext_vector_type(8))) __bf16;
+using f16x8 = __attribute__((ext_vector_type(8))) _Float16;
+
+constexpr float kLog2e = 1.44269504088896340736f;
+constexpr float kLn2 = 0.69314718055994530942f;
+// The score of an excluded item.  Finite, so that e * y below is 0 * finite = 0 and not 0 * inf.
+constexpr float kGone = -1e30f;
+// Where the running maximum starts: above kGone, so that an excluded item's e is 0 before the first
+// score too (a row whose scores are all below it counts as empty).
+constexpr float kFloor = -1e28f;
+constexpr int kMaxTop = 128;
+
+// Planes of a factor type: PS of the score product, PG of the gradient product's factors, GP of G.
+template <int T>
+struct Planes;
+template <>
+struct Planes<MML_DTYPE_F32> {
+    static constexpr int PS = 3, PG = 3, GP = 3;
+};
+template <>
+struct Planes<MML_DTYPE_BF16> {
+    static constexpr int PS = 1, PG = 1, GP = 2;
+};
+template <>
+struct Planes<MML_DTYPE_F16> {
+    static constexpr int PS = 1, PG = 2, GP = 2;
+};
+
+template <int T>
+__device__ __forceinline__ float load_factor(const void* p, int64_t i) {
+    if constexpr (T == MML_DTYPE_F32) return ((const float*)p)[i];
+    if constexpr (T == MML_DTYPE_BF16) return __uint_as_float((uint32_t)((const uint16_t*)p)[i] << 16);
+    if constexpr (T == MML_DTYPE_F16) return (float)((const _Float16*)p)[i];
+}
+__device__ __forceinline__ uint32_t bf16_rn(float x) {
+    const uint32_t b = __float_as_uint(x);
+    return (b + 0x7FFFu + ((b >> 16) & 1u)) >> 16;
+}
+template <int T>
+__device__ __forceinline__ void store_factor(void* p, int64_t i, float x) {
+    if constexpr (T == MML_DTYPE_F32) ((float*)p)[i] = x;
+    if constexpr (T == MML_DTYPE_BF16)  // one rounding, to nearest; a NaN stays one
+        ((uint16_t*)p)[i] = x != x ? 0x7FC0u : (uint16_t)bf16_rn(x);
+    if constexpr (T == MML_DTYPE_F16) ((_Float16*)p)[i] = (_Float16)x;
+}
+
+// ------------------------------------------------------------------ arguments of the kernels
+struct Side {  // one factor matrix as fragments
+    const void* src;
+    int64_t ld;
+    const int32_t* index;  // row x of the side is src row index[x] (nullptr: x)
+    int32_t n_src;         // rows of src
+    int64_t n;             // rows of the side
+    int32_t tiles;         // tiles of 32 rows written (>= ceil(n / 32))
+    uint4* frag;           // [tiles][PS][KT][64]
+    uint4* trans;          // [tiles][PG][MT][2][64] (nullptr: not needed)
+};
+
+struct RowMeta {  // per row of the users' side, gradient only
+    float lse2;   // lse * log2 e; 1e30 for a row without a gradient (p = 0)
+    float c0, c1; // G = -p (c0 + c1 x) + [j = t] w,  x = log2 p
+    int32_t t;    // the given item, -1: none
+};
+
+struct Job {
+    Side u, v;
+    const float* bias;   // items (nullptr: 0)
+    float* vbias;        // [v.tiles * 32]: bias, kGone for an excluded or padding item, NaN where
+                         // the factors are not finite
+    uint8_t* ubad;       // [u.tiles * 32]: 1 = factors not finite, 2 = unknown user
+    uint32_t* mask;      // [v.tiles][rows_pad]: bit i of word (tile, r): item 32 tile + i excluded
+    int64_t rows_pad;    // u.tiles * 32
+    const int64_t* ex_off;
+    const int32_t* ex_items;
+    int64_t n_ex;
+    const int32_t* target;
+    int32_t k, n_items;
+    int64_t n_rows;
+    int32_t splits;
+    // forward
+    float* part;    // [splits][3][rows_pad]: m, l, w
+    float* cmax;    // [rows_pad][cpad]: every tile's largest score (n_top > 0)
+    int64_t cpad;
+    int32_t n_top;
+    float *log_probs, *log_norm, *entropy, *top_lp;
+    int32_t* top_items;
+    // gradient
+    const float *in_norm, *in_entropy, *g_lp, *g_ent;
+    RowMeta* meta;  // [rows_pad]
+    float* w;       // [rows_pad]
+    float *du_part, *dv_part, *db_part;
+    int32_t vsplits;
+    void *gu, *gv;
+    int64_t ld_gu, ld_gv;
+    float* gb;
+};
+
+__device__ __forceinline__ int64_t clamp64(int64_t x, int64_t lo, int64_t hi) {
+    return x < lo ? lo : (x > hi ? hi : x);
+}
+__device__ __forceinline__ int64_t source_row(const Side& s, int64_t x) {  // -1: none
+    if (x >= s.n) return -1;
+    const int64_t r = s.index ? (int64_t)s.index[x] : x;
+    return r >= 0 && r < s.n_src ? r : -1;
+}
+
+// ------------------------------------------------------------------ preparation
+__global__ __launch_bounds__(256) void softmax_clear_kernel(uint32_t* p, int64_t n) {
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256)
+        p[i] = 0;
+}
+
+// One wave per row sets the bits of its user's exclusion list.  The lists may be unsorted and may
+// repeat an item (an OR of bits does not depend on the order); ids outside the catalogue and
+// offsets outside the array are skipped.
+__global__ __launch_bounds__(256) void softmax_mask_kernel(Job j) {
+    const int64_t r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (r >= j.n_rows) return;
+    const int64_t u = source_row(j.u, r);
+    if (u < 0) return;
+    const int64_t b = clamp64(j.ex_off[u], 0, j.n_ex), e = clamp64(j.ex_off[u + 1], 0, j.n_ex);
+    for (int64_t x = b + (threadIdx.x & 63); x < e; x += 64) {
+        const int32_t i = j.ex_items[x];
+        if (i >= 0 && i < j.n_items)
+            atomicOr(&j.mask[(int64_t)(i >> 5) * j.rows_pad + r], 1u << (i & 31));
+    }
+}
+
+// Fragments of both sides, one block per tile of 32 rows (the users' tiles first).  A row with a
+// value that is not finite is written as zeros and marked, so that 0 * NaN cannot reach the other
+// rows' sums: an item that is not excluded gets the bias NaN, a user the mark in ubad.
+template <int T, int KT>
+__global__ __launch_bounds__(256) void softmax_prep_kernel(Job j) {
+    using P = Planes<T>;
+    constexpr int KP = KT * 16, MT = KT > 1 ? KT / 2 : 1, LD = KP + 1;
+    __shared__ float tile[32 * LD];
+    __shared__ int bad[32];
+    const bool users = blockIdx.x < (uint32_t)j.u.tiles;
+    const Side& s = users ? j.u : j.v;
+    const int64_t tl = users ? blockIdx.x : blockIdx.x - j.u.tiles;
+    const int t = threadIdx.x;
+    if (t < 32) {
+        int b = 0;
+        if (users && tl * 32 + t < s.n && source_row(s, tl * 32 + t) < 0) b = 2;
+        bad[t] = b;
+    }
+    __syncthreads();
+    for (int x = t; x < 32 * KP; x += 256) {
+        const int row = x / KP, f = x % KP;
+        const int64_t src = source_row(s, tl * 32 + row);
+        float v = 0.0f;
+        if (src >= 0 && f < j.k) v = load_factor<T>(s.src, src * s.ld + f);
+        if (!(fabsf(v) < 3e38f)) atomicOr(&bad[row], 1);
+        tile[row * LD + f] = v;
+    }
+    __syncthreads();
+    if (t < 32) {
+        const int64_t row = tl * 32 + t;
+        if (users) {
+            j.ubad[row] = (uint8_t)bad[t];
+        } else {
+            float b = row < s.n ? (j.bias ? j.bias[row] : 0.0f) : kGone;
+            if (b <= kGone) b = kGone;
+            else if (bad[t] || !(fabsf(b) < 3e38f)) b = __builtin_nanf("");
+            j.vbias[row] = b;
+        }
+    }
+    for (int x = t; x < KT * 64; x += 256) {
+        const int ks = x >> 6, lane = x & 63, row = lane & 31;
+        const float* src = &tile[row * LD + ks * 16 + 8 * (lane >> 5)];
+        uint32_t q[P::PS][8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            float v = bad[row] ? 0.0f : src[e];
+            if constexpr (T == MML_DTYPE_F16) {
+                q[0][e] = (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)v);
+            } else {
+#pragma unroll
+                for (int p = 0; p < P::PS; ++p) {
+                    q[p][e] = bf16_rn(v);
+                    v -= __uint_as_float(q[p][e] << 16);
+                }
+            }
+        }
+#pragma unroll
+        for (int p = 0; p < P::PS; ++p)
+            s.frag[((tl * P::PS + p) * KT + ks) * 64 + lane] =
+                make_uint4(q[p][0] | q[p][1] << 16, q[p][2] | q[p][3] << 16,
+                           q[p][4] | q[p][5] << 16, q[p][6] | q[p][7] << 16);
+    }
+    if (!s.trans) return;
+    for (int x = t; x < MT * 128; x += 256) {
+        const int mt = x >> 7, step = (x >> 6) & 1, lane = x & 63, f = 32 * mt + (lane & 31);
+        uint32_t q[P::PG][8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const int row = 16 * step + 8 * (e >> 2) + 4 * (lane >> 5) + (e & 3);
+            float v = f < KP && !bad[row] ? tile[row * LD + f] : 0.0f;
+#pragma unroll
+            for (int p = 0; p < P::PG; ++p) {
+                q[p][e] = bf16_rn(v);
+                v -= __uint_as_float(q[p][e] << 16);
+            }
+        }
+#pragma unroll
+        for (int p = 0; p < P::PG; ++p)
+            s.trans[((tl * P::PG + p) * MT * 2 + mt * 2 + step) * 64 + lane] =
+                make_uint4(q[p][0] | q[p][1] << 16, q[p][2] | q[p][3] << 16,
+                           q[p][4] | q[p][5] << 16, q[p][6] | q[p][7] << 16);
+    }
+}
+
+// The rows' constants of the gradient.  A row without one -- both coefficients 0, no items left, an
+// unknown user -- gets lse2 = 1e30, so that its p are 0.
+__global__ __launch_bounds__(256) void softmax_meta_kernel(Job j) {
+    const int64_t r = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (r >= j.rows_pad) return;
+    RowMeta m{1e30f, 0.0f, 0.0f, -1};
+    float w = 0.0f;
+    if (r < j.n_rows && j.ubad[r] < 2) {
+        const float lse = j.in_norm[r], h = j.g_ent ? j.g_ent[r] : 0.0f;
+        int32_t t = j.target ? j.target[r] : -1;
+        if (t < 0 || t >= j.n_items || j.vbias[t] <= kGone ||
+            (j.mask && (j.mask[(int64_t)(t >> 5) * j.rows_pad + r] >> (t & 31) & 1u)))
+            t = -1;
+        w = t >= 0 && j.g_lp ? j.g_lp[r] : 0.0f;
+        if ((w != 0.0f || h != 0.0f) && lse != -INFINITY) {
+            const float H = h != 0.0f ? j.in_entropy[r] : 0.0f;
+            m = RowMeta{j.ubad[r] ? __builtin_nanf("") : lse * kLog2e, w + h * H, h * kLn2, t};
+        } else {
+            w = 0.0f;
+        }
+    }
+    j.meta[r] = m;
+    j.w[r] = w;
+}
+
+// ------------------------------------------------------------------ tiles
+// c + A B over the PS planes of KT steps (smallest products first).  A: fragments in memory.
+template <int T, int KT>
+__device__ __forceinline__ f32x16 score_tile(const uint4* __restrict__ a,
+                                             const uint4 (&b)[Planes<T>::PS][KT], f32x16 c,
+                                             int lane) {
+    constexpr int PS = Planes<T>::PS;
+#pragma unroll
+    for (int ks = 0; ks < KT; ++ks) {
+        uint4 x[PS];
+#pragma unroll
+        for (int p = 0; p < PS; ++p) x[p] = a[(p * KT + ks) * 64 + lane];
+        if constexpr (T == MML_DTYPE_F16) {
+            c = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, x[0]),
+                                                       __builtin_bit_cast(f16x8, b[0][ks]), c, 0, 0,
+                                                       0);
+        } else {
+#pragma unroll
+            for (int sum = PS - 1; sum >= 0; --sum)
+#pragma unroll
+                for (int p = sum; p >= 0; --p)
+                    c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
+                        __builtin_bit_cast(bf16x8, x[p]), __builtin_bit_cast(bf16x8, b[sum - p][ks]),
+                        c, 0, 0, 0);
+        }
+    }
+    return c;
+}
+
+// The planes of G's registers 8 s .. 8 s + 7 as B operands: the leading planes are cut off (the
+// next plane holds the rest exactly), the last is rounded to nearest.
+template <int GP>
+__device__ __forceinline__ void split_g(const float (&g)[16], int step, uint4 (&q)[GP]) {
+    uint32_t w[GP][4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        float x = g[8 * step + 2 * e], y = g[8 * step + 2 * e + 1];
+#pragma unroll
+        for (int p = 0; p < GP; ++p) {
+            const uint32_t a = __float_as_uint(x), b = __float_as_uint(y);
+            if (p + 1 < GP) {
+                w[p][e] = __builtin_amdgcn_perm(b, a, 0x07060302u);
+                x -= __uint_as_float(a & 0xFFFF0000u);
+                y -= __uint_as_float(b & 0xFFFF0000u);
+            } else {
+                w[p][e] = bf16_rn(x) | bf16_rn(y) << 16;
+            }
+        }
+    }
+#pragma unroll
+    for (int p = 0; p < GP; ++p) q[p] = make_uint4(w[p][0], w[p][1], w[p][2], w[p][3]);
+}
+
+// acc[mt] += A B for the MT tiles of 32 factors: A the transposed fragments, B the planes of G
+template <int T, int KT>
+__device__ __forceinline__ void grad_tile(const uint4* __restrict__ a, const float (&g)[16],
+                                          f32x16 (&acc)[(KT > 1 ? KT / 2 : 1)], int lane) {
+    using P = Planes<T>;
+    constexpr int MT = KT > 1 ? KT / 2 : 1, MAXSUM = P::PG > P::GP ? P::PG - 1 : P::GP - 1;
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+        uint4 q[P::GP];
+        split_g<P::GP>(g, s, q);
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) {
+            uint4 x[P::PG];
+#pragma unroll
+            for (int p = 0; p < P::PG; ++p) x[p] = a[(p * MT * 2 + mt * 2 + s) * 64 + lane];
+#pragma unroll
+            for (int sum = MAXSUM; sum >= 0; --sum)
+#pragma unroll
+                for (int p = P::PG - 1; p >= 0; --p)
+                    if (sum - p >= 0 && sum - p < P::GP)
+                        acc[mt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
+                            __builtin_bit_cast(bf16x8, x[p]), __builtin_bit_cast(bf16x8, q[sum - p]),
+                            acc[mt], 0, 0, 0);
+        }
+    }
+}
+
+__device__ __forceinline__ int reg_row(int i, int h) { return 8 * (i >> 2) + 4 * h + (i & 3); }
+
+// ------------------------------------------------------------------ forward
+// A wave keeps 32 users and streams the item tiles of its split.  Lane l: user l % 32, 16 of a
+// tile's 32 items.  m, l, w: the running maximum, sum of e = exp(s - m) and of e y, y = log2 e.
+template <int T, int KT, bool TOP>
+__global__ __launch_bounds__(256) void softmax_forward_kernel(Job j) {
+    constexpr int PS = Planes<T>::PS;
+    const int lane = threadIdx.x & 63, h = lane >> 5;
+    const int split = blockIdx.x % j.splits;
+    const int64_t ut = (int64_t)(blockIdx.x / j.splits) * 4 + (threadIdx.x >> 6);
+    if (ut >= j.u.tiles) return;
+    const int64_t row = ut * 32 + (lane & 31);
+    uint4 b[PS][KT];
+#pragma unroll
+    for (int p = 0; p < PS; ++p)
+#pragma unroll
+        for (int ks = 0; ks < KT; ++ks) b[p][ks] = j.u.frag[((ut * PS + p) * KT + ks) * 64 + lane];
+    const int t0 = (int)((int64_t)j.v.tiles * split / j.splits);
+    const int t1 = (int)((int64_t)j.v.tiles * (split + 1) / j.splits);
+    float m = kFloor, l = 0.0f, w = 0.0f;
+    for (int tl = t0; tl < t1; ++tl) {
+        f32x16 c;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const f32x4 bias = *(const f32x4*)&j.vbias[tl * 32 + 8 * q + 4 * h];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) c[4 * q + e] = bias[e];
+        }
+        c = score_tile<T, KT>(j.v.frag + (int64_t)tl * PS * KT * 64, b, c, lane);
+        if (j.mask) {
+            const uint32_t bits = j.mask[(int64_t)tl * j.rows_pad + row] >> (4 * h);
+            if (__any(bits & 0x0F0F0F0Fu)) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    if (bits >> reg_row(i, 0) & 1u) c[i] = kGone;
+            }
+        }
+        float mt = c[0];
+#pragma unroll
+        for (int i = 1; i < 16; ++i) mt = fmaxf(mt, c[i]);
+        if constexpr (TOP) {
+            const float both = fmaxf(mt, __shfl_xor(mt, 32));
+            if (h == 0) j.cmax[row * j.cpad + tl] = both;
+        }
+        if (__any(mt > m)) {
+            const float mn = fmaxf(m, mt), d = (m - mn) * kLog2e, f = __builtin_amdgcn_exp2f(d);
+            w = f * fmaf(l, d, w);
+            l *= f;
+            m = mn;
+        }
+        const float m2 = m * kLog2e;
+        float sl = 0.0f, sw = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const float y = fmaf(c[i], kLog2e, -m2), e = __builtin_amdgcn_exp2f(y);
+            sl += e;
+            sw = fmaf(e, y, sw);
+        }
+        l += sl;
+        w += sw;
+    }
+    // the halves' states joined: lanes l and l + 32 hold the same user
+    const float mo = __shfl_xor(m, 32), mn = fmaxf(m, mo), d = (m - mn) * kLog2e;
+    const float f = __builtin_amdgcn_exp2f(d);
+    w = f * fmaf(l, d, w);
+    l *= f;
+    w += __shfl_xor(w, 32);
+    l += __shfl_xor(l, 32);
+    if (h == 0) {
+        float* p = j.part + (int64_t)split * 3 * j.rows_pad + row;
+        p[0] = mn;
+        p[j.rows_pad] = l;
+        p[2 * j.rows_pad] = w;
+    }
+}
+
+// s_rj in 64 bits for the given and the top items (exact f32 products)
+template <int T>
+__device__ __forceinline__ double exact_score(const Job& j, int64_t u, int64_t i) {
+    double a = 0.0;
+    for (int f = 0; f < j.k; ++f)
+        a = fma((double)load_factor<T>(j.u.src, u * j.u.ld + f),
+                (double)load_factor<T>(j.v.src, i * j.v.ld + f), a);
+    return a + (j.bias ? (double)j.bias[i] : 0.0);
+}
+__device__ __forceinline__ bool is_excluded(const Job& j, int64_t r, int64_t i) {
+    return j.vbias[i] <= kGone ||
+           (j.mask && (j.mask[(i >> 5) * j.rows_pad + r] >> (i & 31) & 1u));
+}
+
+// One block per row: the splits' states joined, the outputs, and the top items.  The tiles' largest
+// scores select n + 2 tiles: the n best items lie in the n tiles with the largest maxima (lower
+// tile first among equals), two more cover the rounding of the maxima.  Their items are scored
+// again in 64 bits, so the order is that of the exact scores, the lowest id first among equals.
+struct Best {  // (value, index): larger value first, then lower index
+    double v;
+    int32_t i;
+};
+__device__ __forceinline__ bool before(double va, int32_t ia, double vb, int32_t ib) {
+    return va > vb || (va == vb && ia < ib);
+}
+__device__ __forceinline__ Best block_best(Best b, Best* red) {
+#pragma unroll
+    for (int s = 32; s > 0; s >>= 1) {
+        const double v = __shfl_xor(b.v, s);
+        const int32_t i = __shfl_xor(b.i, s);
+        if (before(v, i, b.v, b.i)) b = Best{v, i};
+    }
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = b;
+    __syncthreads();
+    b = red[0];
+    for (int w = 1; w < 4; ++w)
+        if (before(red[w].v, red[w].i, b.v, b.i)) b = red[w];
+    return b;
+}
+
+template <int T>
+__global__ __launch_bounds__(256) void softmax_finish_kernel(Job j) {
+    __shared__ Best red[4];
+    __shared__ int32_t chosen[kMaxTop + 2];
+    __shared__ double score[(kMaxTop + 2) * 32];
+    const int64_t r = blockIdx.x;
+    const int t = threadIdx.x;
+    // every thread joins the splits' states (they are few)
+    float m = kFloor;
+    for (int s = 0; s < j.splits; ++s) m = fmaxf(m, j.part[(int64_t)s * 3 * j.rows_pad + r]);
+    double l = 0.0, w = 0.0;
+    for (int s = 0; s < j.splits; ++s) {
+        const float* p = j.part + (int64_t)s * 3 * j.rows_pad + r;
+        const double d = ((double)p[0] - m) * 1.4426950408889634;
+        const double f = exp2(d);
+        w += f * ((double)p[2 * j.rows_pad] + (double)p[j.rows_pad] * d);
+        l += f * p[j.rows_pad];
+    }
+    const bool empty = m <= kFloor && l == l;
+    const int bad = j.ubad[r];
+    double lse = (double)m + log(l), H = log(l) - 0.69314718055994531 * w / l;
+    if (empty) lse = -INFINITY, H = 0.0;
+    if (bad) lse = H = __builtin_nan("");
+    const int64_t u = source_row(j.u, r);
+    if (t == 0) {
+        const int32_t g = j.target ? j.target[r] : -1;
+        double lp = 0.0;
+        if (lse != lse) lp = lse;
+        else if (g >= 0 && g < j.n_items)
+            lp = is_excluded(j, r, g) ? -INFINITY : exact_score<T>(j, u, g) - lse;
+        j.log_probs[r] = (float)lp;
+        j.log_norm[r] = (float)lse;
+        j.entropy[r] = (float)(H < 0.0 ? 0.0 : H);
+    }
+    if (j.n_top == 0) return;
+    const int n = j.n_top;
+    if (lse != lse || empty) {
+        for (int x = t; x < n; x += 256) {
+            j.top_items[r * n + x] = -1;
+            j.top_lp[r * n + x] = (float)(empty ? -INFINITY : lse);
+        }
+        return;
+    }
+    const int want = min(n + 2, j.v.tiles);
+    const float* cm = j.cmax + r * j.cpad;
+    Best last{INFINITY, -1};
+    for (int c = 0; c < want; ++c) {
+        Best b{-INFINITY, 0x7FFFFFFF};
+        for (int x = t; x < j.v.tiles; x += 256) {
+            const double v = cm[x];
+            if (before(last.v, last.i, v, x) && before(v, x, b.v, b.i)) b = Best{v, x};
+        }
+        last = block_best(b, red);
+        if (t == 0) chosen[c] = last.i;
+    }
+    __syncthreads();
+    for (int x = t; x < want * 32; x += 256) {
+        const int64_t i = (int64_t)chosen[x >> 5] * 32 + (x & 31);
+        score[x] = i < j.n_items && !is_excluded(j, r, i) ? exact_score<T>(j, u, i) : -INFINITY;
+    }
+    __syncthreads();
+    last = Best{INFINITY, -1};
+    for (int c = 0; c < n; ++c) {
+        Best b{-INFINITY, 0x7FFFFFFF};
+        for (int x = t; x < want * 32; x += 256) {
+            const double v = score[x];
+            const int32_t i = chosen[x >> 5] * 32 + (x & 31);
+            if (v != -INFINITY && before(last.v, last.i, v, i) && before(v, i, b.v, b.i))
+                b = Best{v, i};
+        }
+        last = block_best(b, red);
+        if (t == 0) {
+            const bool none = last.v == -INFINITY;
+            j.top_items[r * n + c] = none ? -1 : last.i;
+            j.top_lp[r * n + c] = none ? -INFINITY : (float)(last.v - lse);
+        }
+        if (last.v == -INFINITY) last.i = -1;
+    }
+}
+
+// ------------------------------------------------------------------ gradient
+// Users' side: as the forward pass, G in place of the softmax state, dU += G V.
+template <int T, int KT>
+__global__ __launch_bounds__(256) void softmax_grad_users_kernel(Job j) {
+    using P = Planes<T>;
+    constexpr int PS = P::PS, MT = KT > 1 ? KT / 2 : 1, KP = MT * 32;
+    const int lane = threadIdx.x & 63, h = lane >> 5;
+    const int split = blockIdx.x % j.splits;
+    const int64_t ut = (int64_t)(blockIdx.x / j.splits) * 4 + (threadIdx.x >> 6);
+    if (ut >= j.u.tiles) return;
+    const int64_t row = ut * 32 + (lane & 31);
+    uint4 b[PS][KT];
+#pragma unroll
+    for (int p = 0; p < PS; ++p)
+#pragma unroll
+        for (int ks = 0; ks < KT; ++ks) b[p][ks] = j.u.frag[((ut * PS + p) * KT + ks) * 64 + lane];
+    const RowMeta mr = j.meta[row];
+    f32x16 acc[MT] = {};
+    const int t0 = (int)((int64_t)j.v.tiles * split / j.splits);
+    const int t1 = (int)((int64_t)j.v.tiles * (split + 1) / j.splits);
+    for (int tl = t0; tl < t1; ++tl) {
+        f32x16 c;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const f32x4 bias = *(const f32x4*)&j.vbias[tl * 32 + 8 * q + 4 * h];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) c[4 * q + e] = bias[e];
+        }
+        c = score_tile<T, KT>(j.v.frag + (int64_t)tl * PS * KT * 64, b, c, lane);
+        if (j.mask) {
+            const uint32_t bits = j.mask[(int64_t)tl * j.rows_pad + row] >> (4 * h);
+            if (__any(bits & 0x0F0F0F0Fu)) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    if (bits >> reg_row(i, 0) & 1u) c[i] = kGone;
+            }
+        }
+        float g[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const float x = fmaf(c[i], kLog2e, -mr.lse2);
+            g[i] = -__builtin_amdgcn_exp2f(x) * fmaf(mr.c1, x, mr.c0);
+        }
+        grad_tile<T, KT>(j.v.trans + (int64_t)tl * P::PG * MT * 128, g, acc, lane);
+    }
+    float* out = j.du_part + ((int64_t)split * j.rows_pad + row) * KP;
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+            *(f32x4*)&out[32 * mt + 8 * q + 4 * h] =
+                f32x4{acc[mt][4 * q], acc[mt][4 * q + 1], acc[mt][4 * q + 2], acc[mt][4 * q + 3]};
+}
+
+// Items' side: a wave keeps 32 items and streams the user tiles of its split; dV += G^T U,
+// db = the sum of G.  The given items add w to G's element here.
+template <int T, int KT>
+__global__ __launch_bounds__(256) void softmax_grad_items_kernel(Job j) {
+    using P = Planes<T>;
+    constexpr int PS = P::PS, MT = KT > 1 ? KT / 2 : 1, KP = MT * 32;
+    const int lane = threadIdx.x & 63, h = lane >> 5;
+    const int split = blockIdx.x % j.vsplits;
+    const int64_t vt = (int64_t)(blockIdx.x / j.vsplits) * 4 + (threadIdx.x >> 6);
+    if (vt >= j.v.tiles) return;
+    const int64_t item = vt * 32 + (lane & 31);
+    uint4 b[PS][KT];
+#pragma unroll
+    for (int p = 0; p < PS; ++p)
+#pragma unroll
+        for (int ks = 0; ks < KT; ++ks) b[p][ks] = j.v.frag[((vt * PS + p) * KT + ks) * 64 + lane];
+    const float bias = j.vbias[item];
+    f32x16 acc[MT] = {};
+    float db = 0.0f;
+    const int t0 = (int)((int64_t)j.u.tiles * split / j.vsplits);
+    const int t1 = (int)((int64_t)j.u.tiles * (split + 1) / j.vsplits);
+    for (int tl = t0; tl < t1; ++tl) {
+        f32x16 c;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) c[i] = bias;
+        c = score_tile<T, KT>(j.u.frag + (int64_t)tl * PS * KT * 64, b, c, lane);
+        const RowMeta* meta = j.meta + tl * 32;
+        if (j.mask) {
+            const uint32_t* words = j.mask + vt * j.rows_pad + tl * 32;
+            if (__any(words[lane & 31])) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    if (words[reg_row(i, h)] >> (lane & 31) & 1u) c[i] = kGone;
+            }
+        }
+        float g[16], sum = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const RowMeta mr = meta[reg_row(i, h)];
+            const float x = fmaf(c[i], kLog2e, -mr.lse2);
+            g[i] = -__builtin_amdgcn_exp2f(x) * fmaf(mr.c1, x, mr.c0);
+        }
+        if (__any(meta[lane & 31].t >> 5 == (int32_t)vt)) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+                if (meta[reg_row(i, h)].t == (int32_t)item) g[i] += j.w[tl * 32 + reg_row(i, h)];
+        }
+#pragma unroll
+        for (int i = 0; i < 16; ++i) sum += g[i];
+        db += sum;
+        grad_tile<T, KT>(j.u.trans + (int64_t)tl * P::PG * MT * 128, g, acc, lane);
+    }
+    const int64_t items_pad = (int64_t)j.v.tiles * 32;
+    float* out = j.dv_part + ((int64_t)split * items_pad + item) * KP;
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+            *(f32x4*)&out[32 * mt + 8 * q + 4 * h] =
+                f32x4{acc[mt][4 * q], acc[mt][4 * q + 1], acc[mt][4 * q + 2], acc[mt][4 * q + 3]};
+    db += __shfl_xor(db, 32);
+    if (h == 0) j.db_part[split * items_pad + item] = db;
+}
+
+// The splits' sums in split order (the same result every time), the users' rows with w V_t added.
+template <int T>
+__global__ __launch_bounds__(256) void softmax_join_users_kernel(Job j, int32_t kp) {
+    const int64_t x = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (x >= j.n_rows * j.k) return;
+    const int64_t r = x / j.k;
+    const int f = (int)(x % j.k);
+    float a = 0.0f;
+    for (int s = 0; s < j.splits; ++s) a += j.du_part[((int64_t)s * j.rows_pad + r) * kp + f];
+    const int32_t t = j.meta[r].t;
+    if (t >= 0) a = fmaf(j.w[r], load_factor<T>(j.v.src, (int64_t)t * j.v.ld + f), a);
+    store_factor<T>(j.gu, r * j.ld_gu + f, a);
+}
+template <int T>
+__global__ __launch_bounds__(256) void softmax_join_items_kernel(Job j, int32_t kp) {
+    const int64_t x = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    const int64_t items_pad = (int64_t)j.v.tiles * 32;
+    if (x < (int64_t)j.n_items * j.k) {
+        const int64_t i = x / j.k;
+        const int f = (int)(x % j.k);
+        float a = 0.0f;
+        for (int s = 0; s < j.vsplits; ++s) a += j.dv_part[((int64_t)s * items_pad + i) * kp + f];
+        store_factor<T>(j.gv, i * j.ld_gv + f, a);
+    }
+    if (x < j.n_items) {
+        float a = 0.0f;
+        for (int s = 0; s < j.vsplits; ++s) a += j.db_part[s * items_pad + x];
+        j.gb[x] = a;
+    }
+}
+
+// ------------------------------------------------------------------ host side
+int steps_of(int32_t k) {  // KT: the factors padded to 16, 32, 64, 128 or 256
+    int kt = 1;
+    while (kt * 16 < k) kt *= 2;
+    return kt;
+}
+
+struct Carve {  // a workspace cut into arrays of 256-byte alignment (base null: sizes only)
+    char* base;
+    int64_t used = 0;
+    template <class X>
+    X* take(int64_t n) {
+        X* p = base ? reinterpret_cast<X*>(base + used) : nullptr;
+        used += (n * (int64_t)sizeof(X) + 255) & ~(int64_t)255;
+        return p;
+    }
+};
+
+void check_args(const mml_item_softmax_args* a) {
+    MML_REQUIRE(a, "args is null");
+    MML_REQUIRE(a->dtype >= MML_DTYPE_F32 && a->dtype <= MML_DTYPE_F16, "unknown dtype");
+    MML_REQUIRE(a->num_factors >= 1 && a->num_factors <= 256, "num_factors must be in [1, 256]");
+    MML_REQUIRE(a->n_rows >= 0 && a->n_rows <= (int64_t)1 << 30, "bad n_rows");
+    MML_REQUIRE(a->n_users >= 0 && a->n_items >= 1, "bad n_users or n_items");
+    MML_REQUIRE(a->n_items <= 0x7FFFFF00, "n_items too large");
+    MML_REQUIRE(a->users || a->n_rows <= a->n_users, "more rows than users");
+    MML_REQUIRE(a->ld_users >= a->num_factors && a->ld_items >= a->num_factors,
+                "a row stride is shorter than a row");
+    MML_REQUIRE(a->n_top >= 0 && a->n_top <= kMaxTop, "n_top must be in [0, 128]");
+    MML_REQUIRE(a->n_exclude >= 0, "bad n_exclude");
+}
+
+// The launch's numbers and its arrays in the workspace at `base` (nullptr: sizes only).
+int64_t plan(const mml_item_softmax_args* a, bool grad, void* base, Job& j) {
+    const int T = a->dtype, kt = steps_of(a->num_factors), mt = kt > 1 ? kt / 2 : 1;
+    const int ps = T == MML_DTYPE_F32 ? 3 : 1;
+    const int pg = T == MML_DTYPE_F32 ? 3 : T == MML_DTYPE_F16 ? 2 : 1;
+    j = Job{};
+    j.k = a->num_factors;
+    j.n_items = a->n_items;
+    j.n_rows = a->n_rows;
+    j.n_top = grad ? 0 : a->n_top;
+    j.u = Side{a->user_factors, a->ld_users, a->users, a->n_users, a->n_rows,
+               (int32_t)((a->n_rows + 31) / 32), nullptr, nullptr};
+    j.v = Side{a->item_factors, a->ld_items, nullptr, a->n_items, a->n_items,
+               (int32_t)(((int64_t)a->n_items + 31) / 32), nullptr, nullptr};
+    j.rows_pad = (int64_t)j.u.tiles * 32;
+    const int64_t items_pad = (int64_t)j.v.tiles * 32;
+    j.bias = a->item_bias;
+    j.target = a->items;
+    j.ex_off = a->exclude_offsets;
+    j.ex_items = a->exclude_items;
+    j.n_ex = a->n_exclude;
+    // about 2,048 waves, a split not under 4 tiles
+    const auto splits = [](int64_t kept, int64_t streamed) {
+        const int64_t s = std::min<int64_t>((2048 + kept - 1) / std::max<int64_t>(kept, 1),
+                                            (streamed + 3) / 4);
+        return (int32_t)std::max<int64_t>(1, s);
+    };
+    j.splits = splits(j.u.tiles, j.v.tiles);
+    j.vsplits = splits(j.v.tiles, j.u.tiles);
+    Carve c{(char*)base};
+    j.u.frag = c.take<uint4>((int64_t)j.u.tiles * ps * kt * 64);
+    j.v.frag = c.take<uint4>((int64_t)j.v.tiles * ps * kt * 64);
+    j.vbias = c.take<float>(items_pad);
+    j.ubad = c.take<uint8_t>(j.rows_pad);
+    if (a->exclude_offsets) j.mask = c.take<uint32_t>((int64_t)j.v.tiles * j.rows_pad);
+    if (!grad) {
+        j.part = c.take<float>((int64_t)j.splits * 3 * j.rows_pad);
+        j.cpad = (j.v.tiles + 31) / 32 * 32;
+        if (j.n_top) j.cmax = c.take<float>(j.rows_pad * j.cpad);
+    } else {
+        j.u.trans = c.take<uint4>((int64_t)j.u.tiles * pg * mt * 128);
+        j.v.trans = c.take<uint4>((int64_t)j.v.tiles * pg * mt * 128);
+        j.meta = c.take<RowMeta>(j.rows_pad);
+        j.w = c.take<float>(j.rows_pad);
+        j.du_part = c.take<float>((int64_t)j.splits * j.rows_pad * mt * 32);
+        j.dv_part = c.take<float>((int64_t)j.vsplits * items_pad * mt * 32);
+        j.db_part = c.take<float>((int64_t)j.vsplits * items_pad);
+    }
+    return c.used;
+}
+
+template <class F>
+void dispatch(int T, int kt, F&& f) {
+#define MML_KT(TT)                                                       \
+    switch (kt) {                                                        \
+        case 1: return f(std::integral_constant<int, TT>{}, std::integral_constant<int, 1>{});   \
+        case 2: return f(std::integral_constant<int, TT>{}, std::integral_constant<int, 2>{});   \
+        case 4: return f(std::integral_constant<int, TT>{}, std::integral_constant<int, 4>{});   \
+        case 8: return f(std::integral_constant<int, TT>{}, std::integral_constant<int, 8>{});   \
+        default: return f(std::integral_constant<int, TT>{}, std::integral_constant<int, 16>{}); \
+    }
+    switch (T) {
+        case MML_DTYPE_F32: MML_KT(MML_DTYPE_F32)
+        case MML_DTYPE_BF16: MML_KT(MML_DTYPE_BF16)
+        default: MML_KT(MML_DTYPE_F16)
+    }
+#undef MML_KT
+}
+
+uint32_t grid_of(int64_t n) {
+    if (n > 0x7FFFFFFF) mml::fail(MML_ERR_ARG, "too many rows or items for one launch");
+    return (uint32_t)n;
+}
+
+void mask_and_prep(const Job& j, int T, hipStream_t st) {
+    if (j.mask) {
+        const int64_t words = (int64_t)j.v.tiles * j.rows_pad;
+        softmax_clear_kernel<<<(uint32_t)std::min<int64_t>((words + 255) / 256, 8192), 256, 0, st>>>(
+            j.mask, words);
+        softmax_mask_kernel<<<grid_of((j.n_rows + 3) / 4), 256, 0, st>>>(j);
+    }
+    dispatch(T, steps_of(j.k), [&](auto tt, auto kt) {
+        softmax_prep_kernel<decltype(tt)::value, decltype(kt)::value>
+            <<<grid_of((int64_t)j.u.tiles + j.v.tiles), 256, 0, st>>>(j);
+    });
+}
+
+void check_pointers(const mml_item_softmax_args* a, const void* ws, int64_t ws_bytes,
+                    int64_t need) {
+    MML_REQUIRE(a->user_factors && a->item_factors, "null factors");
+    MML_REQUIRE(!a->exclude_offsets || a->n_exclude == 0 || a->exclude_items,
+                "exclude_offsets without exclude_items");
+    MML_REQUIRE(ws && ws_bytes >= need, "workspace too small");
+    MML_REQUIRE((uintptr_t)ws % 256 == 0, "workspace must be aligned to 256 bytes");
+}
+
+}  // namespace
+
+namespace mml {
+
+void item_log_probs(const mml_item_softmax_args* a, float* log_probs, float* log_norm,
+                    float* entropy, int32_t* top_items, float* top_log_probs, void* ws,
+                    int64_t ws_bytes, hipStream_t st) {
+    check_args(a);
+    if (a->n_rows == 0) return;
+    Job j;
+    const int64_t need = plan(a, false, ws, j);
+    check_pointers(a, ws, ws_bytes, need);
+    MML_REQUIRE(log_probs && log_norm && entropy, "null output");
+    MML_REQUIRE(a->n_top == 0 || (top_items && top_log_probs), "n_top without its outputs");
+    j.log_probs = log_probs;
+    j.log_norm = log_norm;
+    j.entropy = entropy;
+    j.top_items = top_items;
+    j.top_lp = top_log_probs;
+    mask_and_prep(j, a->dtype, st);
+    const uint32_t blocks = grid_of((int64_t)((j.u.tiles + 3) / 4) * j.splits);
+    dispatch(a->dtype, steps_of(j.k), [&](auto tt, auto kt) {
+        if (j.n_top)
+            softmax_forward_kernel<decltype(tt)::value, decltype(kt)::value, true>
+                <<<blocks, 256, 0, st>>>(j);
+        else
+            softmax_forward_kernel<decltype(tt)::value, decltype(kt)::value, false>
+                <<<blocks, 256, 0, st>>>(j);
+    });
+    switch (a->dtype) {
+        case MML_DTYPE_F32:
+            softmax_finish_kernel<MML_DTYPE_F32><<<grid_of(j.n_rows), 256, 0, st>>>(j);
+            break;
+        case MML_DTYPE_BF16:
+            softmax_finish_kernel<MML_DTYPE_BF16><<<grid_of(j.n_rows), 256, 0, st>>>(j);
+            break;
+        default:
+            softmax_finish_kernel<MML_DTYPE_F16><<<grid_of(j.n_rows), 256, 0, st>>>(j);
+    }
+    MML_HIP(hipGetLastError());
+}
+
+int64_t item_log_probs_workspace(const mml_item_softmax_args* a, bool grad) {
+    check_args(a);
+    Job j;
+    return plan(a, grad, nullptr, j);
+}
+
+void item_log_probs_grad(const mml_item_softmax_args* a, const float* log_norm,
+                         const float* entropy, const float* g_lp, const float* g_ent, void* gu,
+                         int64_t ld_gu, void* gv, int64_t ld_gv, float* gb, void* ws,
+                         int64_t ws_bytes, hipStream_t st) {
+    check_args(a);
+    Job j;
+    const int64_t need = plan(a, true, ws, j);
+    MML_REQUIRE(gv && gb && (gu || a->n_rows == 0), "null output");
+    MML_REQUIRE(ld_gu >= a->num_factors && ld_gv >= a->num_factors,
+                "a gradient's row stride is shorter than a row");
+    if (a->n_rows > 0) {
+        check_pointers(a, ws, ws_bytes, need);
+        MML_REQUIRE(log_norm, "null log_norm");
+        MML_REQUIRE(!g_ent || entropy, "grad_entropy without entropy");
+        MML_REQUIRE(!g_lp || a->items, "grad_log_probs without items");
+    } else {
+        MML_REQUIRE(ws && ws_bytes >= need, "workspace too small");
+    }
+    j.in_norm = log_norm;
+    j.in_entropy = entropy;
+    j.g_lp = g_lp;
+    j.g_ent = g_ent;
+    j.gu = gu;
+    j.gv = gv;
+    j.ld_gu = ld_gu;
+    j.ld_gv = ld_gv;
+    j.gb = gb;
+    const int kt0 = steps_of(j.k), kp = std::max(32, kt0 * 16);
+    if (a->n_rows > 0) {
+        mask_and_prep(j, a->dtype, st);
+        softmax_meta_kernel<<<grid_of((j.rows_pad + 255) / 256), 256, 0, st>>>(j);
+    }
+    const uint32_t ub = grid_of((int64_t)((j.u.tiles + 3) / 4) * j.splits);
+    const uint32_t vb = grid_of((int64_t)((j.v.tiles + 3) / 4) * j.vsplits);
+    const uint32_t ju = grid_of((j.n_rows * j.k + 255) / 256);
+    const uint32_t ji = grid_of(((int64_t)j.n_items * j.k + 255) / 256);
+    dispatch(a->dtype, kt0, [&](auto tt, auto kt) {
+        constexpr int T = decltype(tt)::value, KT = decltype(kt)::value;
+        if (j.n_rows > 0) {
+            softmax_grad_users_kernel<T, KT><<<ub, 256, 0, st>>>(j);
+            softmax_join_users_kernel<T><<<ju, 256, 0, st>>>(j, kp);
+        }
+        softmax_grad_items_kernel<T, KT><<<vb, 256, 0, st>>>(j);
+        softmax_join_items_kernel<T><<<ji, 256, 0, st>>>(j, kp);
+    });
+    MML_HIP(hipGetLastError());
+}
+
+}  // namespace mml
+
+using mml::guard;
+
+extern "C" mml_status mml_item_log_probs_workspace(const mml_item_softmax_args* args, int32_t grad,
+                                                   int64_t* bytes) {
+    return guard([&] {
+        MML_REQUIRE(bytes, "bytes is null");
+        *bytes = mml::item_log_probs_workspace(args, grad != 0);
+    });
+}
+
+extern "C" mml_status mml_item_log_probs_device(const mml_item_softmax_args* args, float* log_probs,
+                                                float* log_norm, float* entropy, int32_t* top_items,
+                                                float* top_log_probs, void* workspace,
+                                                int64_t workspace_bytes, int32_t device,
+                                                void* stream) {
+    return guard([&] {
+        mml::DeviceScope on(device);
+        mml::item_log_probs(args, log_probs, log_norm, entropy, top_items, top_log_probs, workspace,
+                            workspace_bytes, (hipStream_t)stream);
+    });
+}
+
+extern "C" mml_status mml_item_log_probs_grad_device(
+    const mml_item_softmax_args* args, const float* log_norm, const float* entropy,
+    const float* grad_log_probs, const float* grad_entropy, void* grad_users, int64_t ld_grad_users,
+    void* grad_items, int64_t ld_grad_items, float* grad_bias, void* workspace,
+    int64_t workspace_bytes, int32_t device, void* stream) {
+    return guard([&] {
+        mml::DeviceScope on(device);
+        mml::item_log_probs_grad(args, log_norm, entropy, grad_log_probs, grad_entropy, grad_users,
+                                 ld_grad_users, grad_items, ld_grad_items, grad_bias, workspace,
+                                 workspace_bytes, (hipStream_t)stream);
+    });
+}

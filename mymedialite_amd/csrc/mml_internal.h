@@ -81,6 +81,27 @@ inline void rccl_check(ncclResult_t r, const char* what) {
         if (!(cond)) ::mml::fail(MML_ERR_ARG, (msg)); \
     } while (0)
 
+// The current device for the calls that name one: `device` inside the scope, the caller's after it.
+struct DeviceScope {
+    int before = -1;
+    explicit DeviceScope(int32_t device) {
+        int n = 0;
+        if (hipGetDeviceCount(&n) != hipSuccess || n == 0)
+            fail(MML_ERR_NODEV, "no HIP device visible");
+        MML_REQUIRE(device >= 0 && device < n, "device out of range");
+        int now = -1;
+        MML_HIP(hipGetDevice(&now));
+        if (now == device) return;
+        MML_HIP(hipSetDevice(device));
+        before = now;
+    }
+    ~DeviceScope() {
+        if (before >= 0) (void)hipSetDevice(before);
+    }
+    DeviceScope(const DeviceScope&) = delete;
+    DeviceScope& operator=(const DeviceScope&) = delete;
+};
+
 // Owning device allocation (HBM of the context's device).
 template <class T>
 struct DeviceArray {
@@ -131,6 +152,18 @@ void item_auc(hipStream_t st, const float* U, int32_t ldu, int32_t n_users_model
               const int64_t* tr_off, const int32_t* tr_cols, int32_t n_tr_rows,
               const int32_t* candidates, int32_t n_cand, const int32_t* users, int32_t n_eval,
               const int64_t* test_off, const int32_t* test_items, double* out_auc);
+
+// The softmax over the catalogue (item_softmax.hip), stream-ordered: mml_item_log_probs_* without
+// the device scope and the status.
+void item_log_probs(const mml_item_softmax_args* a, float* log_probs, float* log_norm,
+                    float* entropy, int32_t* top_items, float* top_log_probs, void* ws,
+                    int64_t ws_bytes, hipStream_t st);
+void item_log_probs_grad(const mml_item_softmax_args* a, const float* log_norm,
+                         const float* entropy, const float* grad_log_probs,
+                         const float* grad_entropy, void* grad_users, int64_t ld_grad_users,
+                         void* grad_items, int64_t ld_grad_items, float* grad_bias, void* ws,
+                         int64_t ws_bytes, hipStream_t st);
+int64_t item_log_probs_workspace(const mml_item_softmax_args* a, bool grad);
 
 // contiguous row shards with balanced work (weight deg + k/2), bounds[parts + 1] (mml_core.cpp)
 std::vector<int64_t> balanced_rows(const std::vector<int64_t>& deg, int32_t k, int32_t parts);
