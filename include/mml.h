@@ -657,6 +657,42 @@ mml_status mml_item_log_probs_grad_device(const mml_item_softmax_args* args, con
                                           int64_t ld_grad_items, float* grad_bias, void* workspace,
                                           int64_t workspace_bytes, int32_t device, void* stream);
 
+/* ------------------------------------------------------------------ AdamW
+ * One step over n_tensors parameter tensors in place, t = step_state[0] + 1 (the models' own
+ * trainers step by SGD; this is the step for dense gradients such as mml_item_log_probs_grad_device's):
+ *   m <- beta1 m + (1 - beta1) g,  v <- beta2 v + (1 - beta2) g^2,
+ *   p <- p - learn_rate weight_decay p
+ *          - learn_rate m / (1 - beta1^t) / (sqrt(v / (1 - beta2^t)) + epsilon),
+ * in f32, a half-precision parameter rounded once to nearest.  state_bits 32: m and v are float[n].
+ * 8: m and v are e4m3 codes (uint8_t[n], the OCP format without infinities), value = code x scale
+ * of its MML_ADAMW_BLOCK consecutive values, scale = largest magnitude / 448 (float[ceil(n / 256)]);
+ * v's codes hold sqrt(v), and one that is not zero never gets code 0.  A gradient that is not
+ * finite (8 bits: or whose square is not) makes that value's parameter and moments NaN or infinite
+ * and no other's.  All zero is the start of
+ * both forms.  Stream-ordered like mml_item_log_probs_device, nothing allocated or read back; a
+ * captured step counts on at every replay (learn_rate is replayed as captured).  step_state:
+ * int32_t[2] on the device, {steps done, 0}; one step at a time may use it.  Tensors must not
+ * overlap. */
+enum { MML_ADAMW_BLOCK = 256 };
+typedef struct {
+    void* param;
+    const void* grad;
+    void* m;                 /* float[n] or uint8_t[n] */
+    void* v;
+    float* m_scale;          /* 8 bits: [ceil(n / MML_ADAMW_BLOCK)] */
+    float* v_scale;
+    int64_t n;
+    int32_t param_dtype;     /* MML_DTYPE_* */
+    int32_t grad_dtype;
+} mml_adamw_tensor;
+typedef struct {
+    double learn_rate, beta1, beta2, epsilon, weight_decay;
+    int32_t state_bits;      /* 32 or 8 */
+} mml_adamw_params;
+mml_status mml_adamw_step_device(const mml_adamw_tensor* tensors, int32_t n_tensors,
+                                 const mml_adamw_params* params, int32_t* step_state,
+                                 int32_t device, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -22,6 +22,9 @@ def __getattr__(name):
     if name in ("item_log_probs", "item_log_probs_grad", "ItemLogProbs"):
         from . import item_softmax
         return getattr(item_softmax, name)
+    if name == "AdamW":
+        from .adamw import AdamW
+        return AdamW
     raise AttributeError(f"module {__name__!r} has no attribute {name!r}")
 
 
@@ -33,4 +36,4 @@ __all__ = ["BiasedMatrixFactorization", "MatrixFactorization", "SocialMF",
            "DeviceRatingFile",
            "SystemRandom", "create_rating_predictor", "create_item_recommender",
            "create_recommender", "list_recommenders", "item_log_probs", "item_log_probs_grad",
-           "ItemLogProbs"]
+           "ItemLogProbs", "AdamW"]

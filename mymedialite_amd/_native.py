@@ -82,6 +82,24 @@ class ItemSoftmaxArgs(ctypes.Structure):
                 ("n_exclude", ctypes.c_int64), ("n_top", ctypes.c_int32)]
 
 
+
+ADAMW_BLOCK = 256
+
+
+class AdamwTensor(ctypes.Structure):
+    """mml_adamw_tensor (include/mml.h)."""
+    _fields_ = [("param", _vp), ("grad", _vp), ("m", _vp), ("v", _vp), ("m_scale", _vp),
+                ("v_scale", _vp), ("n", ctypes.c_int64), ("param_dtype", ctypes.c_int32),
+                ("grad_dtype", ctypes.c_int32)]
+
+
+class AdamwParams(ctypes.Structure):
+    """mml_adamw_params (include/mml.h)."""
+    _fields_ = [("learn_rate", ctypes.c_double), ("beta1", ctypes.c_double),
+                ("beta2", ctypes.c_double), ("epsilon", ctypes.c_double),
+                ("weight_decay", ctypes.c_double), ("state_bits", ctypes.c_int32)]
+
+
 # every exported symbol of include/mml.h: name -> (restype, argtypes)
 SIGNATURES = {
     "mml_abi_version": (ctypes.c_int, []),
@@ -205,6 +223,8 @@ SIGNATURES = {
     "mml_item_log_probs_grad_device": (_st, [ctypes.POINTER(ItemSoftmaxArgs), _vp, _vp, _vp, _vp,
                                              _vp, ctypes.c_int64, _vp, ctypes.c_int64, _vp, _vp,
                                              ctypes.c_int64, ctypes.c_int32, _vp]),
+    "mml_adamw_step_device": (_st, [ctypes.POINTER(AdamwTensor), ctypes.c_int32,
+                                    ctypes.POINTER(AdamwParams), _vp, ctypes.c_int32, _vp]),
 }
 
 _lib = None
