@@ -126,6 +126,7 @@ struct Job {
     float* cmax;    // [rows_pad][cpad]: every tile's largest score (n_top > 0)
     int64_t cpad;
     int32_t n_top;
+    int32_t vec4;   // the items' rows can be loaded 4 factors at a time
     float *log_probs, *log_norm, *entropy, *top_lp;
     int32_t* top_items;
     // gradient
@@ -436,124 +437,255 @@ __global__ __launch_bounds__(256) void softmax_forward_kernel(Job j) {
     }
 }
 
-// s_rj in 64 bits for the given and the top items (exact f32 products)
-template <int T>
-__device__ __forceinline__ double exact_score(const Job& j, int64_t u, int64_t i) {
+// s_rj in 64 bits for the given and the top items: exact products, f64 sums.  LANES neighbouring
+// lanes share an item (every lane gets the sum); u: the user's row in LDS.
+template <int T, int LANES>
+__device__ __forceinline__ double exact_score(const Job& j, const float* u, int64_t i, int lane) {
     double a = 0.0;
-    for (int f = 0; f < j.k; ++f)
-        a = fma((double)load_factor<T>(j.u.src, u * j.u.ld + f),
-                (double)load_factor<T>(j.v.src, i * j.v.ld + f), a);
+    const int64_t at = i * j.v.ld;
+    if (j.vec4) {  // rows of whole groups of 4 factors, aligned: one load per group
+        for (int f = 4 * lane; f < j.k; f += 4 * LANES) {
+            float x[4];
+            if constexpr (T == MML_DTYPE_F32) {
+                const f32x4 v = *(const f32x4*)((const float*)j.v.src + at + f);
+                x[0] = v[0], x[1] = v[1], x[2] = v[2], x[3] = v[3];
+            } else {
+                const uint2 v = *(const uint2*)((const uint16_t*)j.v.src + at + f);
+                const uint32_t w[2] = {v.x, v.y};
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const uint16_t b = (uint16_t)(w[e >> 1] >> (16 * (e & 1)));
+                    x[e] = T == MML_DTYPE_F16 ? (float)__builtin_bit_cast(_Float16, b)
+                                              : __uint_as_float((uint32_t)b << 16);
+                }
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) a = fma((double)u[f + e], (double)x[e], a);
+        }
+    } else {
+        for (int f = lane; f < j.k; f += LANES)
+            a = fma((double)u[f], (double)load_factor<T>(j.v.src, at + f), a);
+    }
+#pragma unroll
+    for (int d = 1; d < LANES; d <<= 1) a += __shfl_xor(a, d);
     return a + (j.bias ? (double)j.bias[i] : 0.0);
 }
 __device__ __forceinline__ bool is_excluded(const Job& j, int64_t r, int64_t i) {
     return j.vbias[i] <= kGone ||
            (j.mask && (j.mask[(i >> 5) * j.rows_pad + r] >> (i & 31) & 1u));
 }
-
-// One block per row: the splits' states joined, the outputs, and the top items.  The tiles' largest
-// scores select n + 2 tiles: the n best items lie in the n tiles with the largest maxima (lower
-// tile first among equals), two more cover the rounding of the maxima.  Their items are scored
-// again in 64 bits, so the order is that of the exact scores, the lowest id first among equals.
-struct Best {  // (value, index): larger value first, then lower index
-    double v;
-    int32_t i;
-};
-__device__ __forceinline__ bool before(double va, int32_t ia, double vb, int32_t ib) {
-    return va > vb || (va == vb && ia < ib);
+// A double as an unsigned key in the same order (-inf is the smallest that occurs)
+__device__ __forceinline__ uint64_t key_of(double x) {
+    const uint64_t b = (uint64_t)__double_as_longlong(x);
+    return b >> 63 ? ~b : b | 1ull << 63;
 }
-__device__ __forceinline__ Best block_best(Best b, Best* red) {
-#pragma unroll
-    for (int s = 32; s > 0; s >>= 1) {
-        const double v = __shfl_xor(b.v, s);
-        const int32_t i = __shfl_xor(b.i, s);
-        if (before(v, i, b.v, b.i)) b = Best{v, i};
+__device__ __forceinline__ double value_of(uint64_t k) {
+    return __longlong_as_double((long long)(k >> 63 ? k & ~(1ull << 63) : ~k));
+}
+__device__ __forceinline__ bool before(uint64_t va, int32_t ia, uint64_t vb, int32_t ib) {
+    return va > vb || (va == vb && ia < ib);  // larger value first, then lower index
+}
+__device__ __forceinline__ uint32_t key_of(float x) {
+    const uint32_t b = __float_as_uint(x);
+    return b >> 31 ? ~b : b | 1u << 31;
+}
+
+constexpr int kListed = 1024;  // tiles that the selection below lists at most
+
+// The `want` tiles with the largest maxima cm[0 .. tiles), ordered, the lower tile first among
+// equals.  The want-th largest of the 256 threads' own maxima is a lower bound of the want-th
+// largest maximum, so few tiles are at or above it; they are listed and ranked by counting.  Where
+// more than kListed are (many equal maxima), they are taken one after another.
+__device__ __forceinline__ void select_tiles(const float* __restrict__ cm, int tiles, int want,
+                                             int32_t* chosen, uint32_t* key, int32_t* index) {
+    __shared__ int32_t count;
+    __shared__ uint32_t bound;
+    const int t = threadIdx.x;
+    uint32_t mine = 0;
+    for (int x = t; x < tiles; x += 256) mine = max(mine, key_of(cm[x]));
+    key[t] = mine;
+    if (t == 0) count = 0;
+    __syncthreads();
+    int rank = 0;
+    for (int x = 0; x < 256; ++x) rank += before(key[x], x, mine, t);
+    if (rank == want - 1) bound = mine;
+    __syncthreads();
+    const uint32_t least = bound;
+    for (int x = t; x < tiles; x += 256) {
+        const uint32_t v = key_of(cm[x]);
+        if (v >= least) {
+            const int at = atomicAdd(&count, 1);
+            if (at < kListed) {
+                key[at] = v;
+                index[at] = x;
+            }
+        }
     }
     __syncthreads();
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = b;
+    const int n = count;
+    if (n <= kListed) {
+        for (int x = t; x < n; x += 256) {
+            const uint32_t v = key[x];
+            const int32_t i = index[x];
+            int r = 0;
+            for (int y = 0; y < n; ++y) r += before(key[y], index[y], v, i);
+            if (r < want) chosen[r] = i;
+        }
+        __syncthreads();
+        return;
+    }
+    uint32_t lv = 0xFFFFFFFFu;
+    int32_t li = -1;
+    for (int c = 0; c < want; ++c) {
+        uint32_t bv = 0;
+        int32_t bi = 0x7FFFFFFF;
+        for (int x = t; x < tiles; x += 256) {
+            const uint32_t v = key_of(cm[x]);
+            if (before(lv, li, v, x) && before(v, x, bv, bi)) bv = v, bi = x;
+        }
+#pragma unroll
+        for (int d = 32; d > 0; d >>= 1) {
+            const uint32_t v = (uint32_t)__shfl_xor((int)bv, d);
+            const int32_t i = __shfl_xor(bi, d);
+            if (before(v, i, bv, bi)) bv = v, bi = i;
+        }
+        __syncthreads();
+        if ((t & 63) == 0) key[t >> 6] = bv, index[t >> 6] = bi;
+        __syncthreads();
+        bv = key[0], bi = index[0];
+        for (int w = 1; w < 4; ++w)
+            if (before(key[w], index[w], bv, bi)) bv = key[w], bi = index[w];
+        lv = bv, li = bi;
+        if (t == 0) chosen[c] = bi;
+    }
     __syncthreads();
-    b = red[0];
-    for (int w = 1; w < 4; ++w)
-        if (before(red[w].v, red[w].i, b.v, b.i)) b = red[w];
-    return b;
 }
 
-template <int T>
-__global__ __launch_bounds__(256) void softmax_finish_kernel(Job j) {
-    __shared__ Best red[4];
-    __shared__ int32_t chosen[kMaxTop + 2];
-    __shared__ double score[(kMaxTop + 2) * 32];
+// One block per row (256 threads with top items, 64 without): the splits' states joined, the
+// outputs, and the top items.  The n best items lie in the n tiles with the largest maxima (lower
+// tile first among equals); two more tiles cover the rounding of the maxima.  Their items are
+// scored again in 64 bits, so the order is that of the exact scores.  The n-th largest of the tiles'
+// exact maxima bounds the n-th best score from below: the items at or above it are ranked by
+// counting.  Dynamic LDS: the candidates' keys, 8 bytes each.
+template <int T, bool TOP>
+__global__ __launch_bounds__(TOP ? 256 : 64) void softmax_finish_kernel(Job j) {
+    constexpr int NT = TOP ? 256 : 64;
+    __shared__ float urow[256];
+    __shared__ double join[3][NT / 64];
     const int64_t r = blockIdx.x;
     const int t = threadIdx.x;
-    // every thread joins the splits' states (they are few)
+    const int64_t u = source_row(j.u, r);
+    for (int f = t; f < j.k; f += NT)
+        urow[f] = u >= 0 ? load_factor<T>(j.u.src, u * j.u.ld + f) : 0.0f;
     float m = kFloor;
-    for (int s = 0; s < j.splits; ++s) m = fmaxf(m, j.part[(int64_t)s * 3 * j.rows_pad + r]);
+    for (int s = t; s < j.splits; s += NT) m = fmaxf(m, j.part[(int64_t)s * 3 * j.rows_pad + r]);
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor(m, d));
+    if (TOP) {
+        if ((t & 63) == 0) join[0][t >> 6] = m;
+        __syncthreads();
+        for (int w = 0; w < NT / 64; ++w) m = fmaxf(m, (float)join[0][w]);
+    }
     double l = 0.0, w = 0.0;
-    for (int s = 0; s < j.splits; ++s) {
+    for (int s = t; s < j.splits; s += NT) {
         const float* p = j.part + (int64_t)s * 3 * j.rows_pad + r;
         const double d = ((double)p[0] - m) * 1.4426950408889634;
         const double f = exp2(d);
         w += f * ((double)p[2 * j.rows_pad] + (double)p[j.rows_pad] * d);
         l += f * p[j.rows_pad];
     }
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) {
+        l += __shfl_xor(l, d);
+        w += __shfl_xor(w, d);
+    }
+    if (TOP) {
+        if ((t & 63) == 0) join[1][t >> 6] = l, join[2][t >> 6] = w;
+        __syncthreads();
+        l = w = 0.0;
+        for (int x = 0; x < NT / 64; ++x) l += join[1][x], w += join[2][x];
+    } else {
+        __syncthreads();
+    }
     const bool empty = m <= kFloor && l == l;
-    const int bad = j.ubad[r];
     double lse = (double)m + log(l), H = log(l) - 0.69314718055994531 * w / l;
     if (empty) lse = -INFINITY, H = 0.0;
-    if (bad) lse = H = __builtin_nan("");
-    const int64_t u = source_row(j.u, r);
-    if (t == 0) {
+    if (j.ubad[r]) lse = H = __builtin_nan("");
+    if (t < 64) {
         const int32_t g = j.target ? j.target[r] : -1;
         double lp = 0.0;
         if (lse != lse) lp = lse;
         else if (g >= 0 && g < j.n_items)
-            lp = is_excluded(j, r, g) ? -INFINITY : exact_score<T>(j, u, g) - lse;
-        j.log_probs[r] = (float)lp;
-        j.log_norm[r] = (float)lse;
-        j.entropy[r] = (float)(H < 0.0 ? 0.0 : H);
-    }
-    if (j.n_top == 0) return;
-    const int n = j.n_top;
-    if (lse != lse || empty) {
-        for (int x = t; x < n; x += 256) {
-            j.top_items[r * n + x] = -1;
-            j.top_lp[r * n + x] = (float)(empty ? -INFINITY : lse);
-        }
-        return;
-    }
-    const int want = min(n + 2, j.v.tiles);
-    const float* cm = j.cmax + r * j.cpad;
-    Best last{INFINITY, -1};
-    for (int c = 0; c < want; ++c) {
-        Best b{-INFINITY, 0x7FFFFFFF};
-        for (int x = t; x < j.v.tiles; x += 256) {
-            const double v = cm[x];
-            if (before(last.v, last.i, v, x) && before(v, x, b.v, b.i)) b = Best{v, x};
-        }
-        last = block_best(b, red);
-        if (t == 0) chosen[c] = last.i;
-    }
-    __syncthreads();
-    for (int x = t; x < want * 32; x += 256) {
-        const int64_t i = (int64_t)chosen[x >> 5] * 32 + (x & 31);
-        score[x] = i < j.n_items && !is_excluded(j, r, i) ? exact_score<T>(j, u, i) : -INFINITY;
-    }
-    __syncthreads();
-    last = Best{INFINITY, -1};
-    for (int c = 0; c < n; ++c) {
-        Best b{-INFINITY, 0x7FFFFFFF};
-        for (int x = t; x < want * 32; x += 256) {
-            const double v = score[x];
-            const int32_t i = chosen[x >> 5] * 32 + (x & 31);
-            if (v != -INFINITY && before(last.v, last.i, v, i) && before(v, i, b.v, b.i))
-                b = Best{v, i};
-        }
-        last = block_best(b, red);
+            lp = is_excluded(j, r, g) ? -INFINITY : exact_score<T, 64>(j, urow, g, t) - lse;
         if (t == 0) {
-            const bool none = last.v == -INFINITY;
-            j.top_items[r * n + c] = none ? -1 : last.i;
-            j.top_lp[r * n + c] = none ? -INFINITY : (float)(last.v - lse);
+            j.log_probs[r] = (float)lp;
+            j.log_norm[r] = (float)lse;
+            j.entropy[r] = (float)(H < 0.0 ? 0.0 : H);
         }
-        if (last.v == -INFINITY) last.i = -1;
+    }
+    if constexpr (TOP) {
+        extern __shared__ uint64_t cand[];
+        __shared__ uint32_t key[kListed];
+        __shared__ int32_t index[kListed], chosen[kMaxTop + 2], count;
+        __shared__ unsigned long long tmax[kMaxTop + 2], bound;
+        const int n = j.n_top;
+        if (lse != lse || empty) {
+            for (int x = t; x < n; x += 256) {
+                j.top_items[r * n + x] = -1;
+                j.top_lp[r * n + x] = (float)(empty ? -INFINITY : lse);
+            }
+            return;
+        }
+        const int want = min(n + 2, j.v.tiles);
+        if (t < want) tmax[t] = 0;
+        if (t == 0) count = 0, bound = 0;
+        select_tiles(j.cmax + r * j.cpad, j.v.tiles, want, chosen, key, index);
+        const uint64_t none = key_of(-INFINITY);
+        for (int x = t >> 2; x < want * 32; x += 64) {
+            const int64_t i = (int64_t)chosen[x >> 5] * 32 + (x & 31);
+            uint64_t k = none;
+            if (i < j.n_items && !is_excluded(j, r, i))
+                k = key_of(exact_score<T, 4>(j, urow, i, t & 3));
+            if ((t & 3) == 0) {
+                cand[x] = k;
+                atomicMax(&tmax[x >> 5], (unsigned long long)k);
+            }
+        }
+        __syncthreads();
+        if (t < want) {  // the n-th largest of the tiles' maxima (none where there are fewer tiles)
+            int rank = 0;
+            for (int x = 0; x < want; ++x) rank += before(tmax[x], x, tmax[t], t);
+            if (rank == n - 1) bound = tmax[t];
+        }
+        __syncthreads();
+        const uint64_t least = max((uint64_t)bound, none + 1);
+        for (int x = t; x < want * 32; x += 256)
+            if (cand[x] >= least) {
+                const int at = atomicAdd(&count, 1);
+                if (at < kListed) index[at] = x;
+            }
+        __syncthreads();
+        const int found = count;
+        const bool listed = found <= kListed;
+        for (int y = t; y < (listed ? found : want * 32); y += 256) {
+            const int x = listed ? index[y] : y;
+            const uint64_t v = cand[x];
+            if (v < least) continue;
+            const int32_t i = chosen[x >> 5] * 32 + (x & 31);
+            int rank = 0;
+            for (int z = 0; z < (listed ? found : want * 32); ++z) {
+                const int o = listed ? index[z] : z;
+                rank += before(cand[o], chosen[o >> 5] * 32 + (o & 31), v, i);
+            }
+            if (rank < n) {
+                j.top_items[r * n + rank] = i;
+                j.top_lp[r * n + rank] = (float)(value_of(v) - lse);
+            }
+        }
+        for (int x = found + t; x < n; x += 256) {
+            j.top_items[r * n + x] = -1;
+            j.top_lp[r * n + x] = -INFINITY;
+        }
     }
 }
 
@@ -756,6 +888,9 @@ int64_t plan(const mml_item_softmax_args* a, bool grad, void* base, Job& j) {
     const int64_t items_pad = (int64_t)j.v.tiles * 32;
     j.bias = a->item_bias;
     j.target = a->items;
+    const int size = T == MML_DTYPE_F32 ? 4 : 2;
+    j.vec4 = a->num_factors % 4 == 0 && a->ld_items % 4 == 0 &&
+             (uintptr_t)a->item_factors % (4 * size) == 0;
     j.ex_off = a->exclude_offsets;
     j.ex_items = a->exclude_items;
     j.n_ex = a->n_exclude;
@@ -863,16 +998,14 @@ void item_log_probs(const mml_item_softmax_args* a, float* log_probs, float* log
             softmax_forward_kernel<decltype(tt)::value, decltype(kt)::value, false>
                 <<<blocks, 256, 0, st>>>(j);
     });
-    switch (a->dtype) {
-        case MML_DTYPE_F32:
-            softmax_finish_kernel<MML_DTYPE_F32><<<grid_of(j.n_rows), 256, 0, st>>>(j);
-            break;
-        case MML_DTYPE_BF16:
-            softmax_finish_kernel<MML_DTYPE_BF16><<<grid_of(j.n_rows), 256, 0, st>>>(j);
-            break;
-        default:
-            softmax_finish_kernel<MML_DTYPE_F16><<<grid_of(j.n_rows), 256, 0, st>>>(j);
-    }
+    const uint32_t lds = std::min(j.n_top + 2, j.v.tiles) * 32 * sizeof(uint64_t);
+    dispatch(a->dtype, 1, [&](auto tt, auto) {
+        constexpr int T = decltype(tt)::value;
+        if (j.n_top)
+            softmax_finish_kernel<T, true><<<grid_of(j.n_rows), 256, lds, st>>>(j);
+        else
+            softmax_finish_kernel<T, false><<<grid_of(j.n_rows), 64, 0, st>>>(j);
+    });
     MML_HIP(hipGetLastError());
 }
 
