@@ -106,6 +106,8 @@ struct RowMeta {  // per row of the users' side, gradient only
     int32_t t;    // the given item, -1: none
 };
 
+static_assert(sizeof(RowMeta) == 16, "staged 16 bytes per lane");
+
 struct Job {
     Side u, v;
     const float* bias;   // items (nullptr: 0)
@@ -280,10 +282,27 @@ __global__ __launch_bounds__(256) void softmax_meta_kernel(Job j) {
     j.w[r] = w;
 }
 
+// ------------------------------------------------------------------ staging
+// n KB of fragments into LDS, asynchronously (global_load_lds: 16 bytes per lane, no registers), the
+// 1 KB pieces dealt over the block's waves.  stage_wait: this wave's pieces have landed; with the
+// barrier behind it, everyone's have.
+template <int WAVES>
+__device__ __forceinline__ void stage(const uint4* __restrict__ src, uint4* dst, int n) {
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    for (int c = wave; c < n; c += WAVES)
+        __builtin_amdgcn_global_load_lds(
+            (const __attribute__((address_space(1))) void*)(src + c * 64 + lane),
+            (__attribute__((address_space(3))) void*)(dst + c * 64), 16, 0, 0);
+}
+__device__ __forceinline__ void stage_wait() {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+}
+
 // ------------------------------------------------------------------ tiles
-// c + A B over the PS planes of KT steps (smallest products first).  A: fragments in memory.
+// c + A B over the PS planes of KT steps (smallest products first).  A: fragments in LDS.
 template <int T, int KT>
-__device__ __forceinline__ f32x16 score_tile(const uint4* __restrict__ a,
+__device__ __forceinline__ f32x16 score_tile(const uint4* a,
                                              const uint4 (&b)[Planes<T>::PS][KT], f32x16 c,
                                              int lane) {
     constexpr int PS = Planes<T>::PS;
@@ -335,7 +354,7 @@ __device__ __forceinline__ void split_g(const float (&g)[16], int step, uint4 (&
 
 // acc[mt] += A B for the MT tiles of 32 factors: A the transposed fragments, B the planes of G
 template <int T, int KT>
-__device__ __forceinline__ void grad_tile(const uint4* __restrict__ a, const float (&g)[16],
+__device__ __forceinline__ void grad_tile(const uint4* a, const float (&g)[16],
                                           f32x16 (&acc)[(KT > 1 ? KT / 2 : 1)], int lane) {
     using P = Planes<T>;
     constexpr int MT = KT > 1 ? KT / 2 : 1, MAXSUM = P::PG > P::GP ? P::PG - 1 : P::GP - 1;
@@ -363,65 +382,107 @@ __device__ __forceinline__ void grad_tile(const uint4* __restrict__ a, const flo
 __device__ __forceinline__ int reg_row(int i, int h) { return 8 * (i >> 2) + 4 * h + (i & 3); }
 
 // ------------------------------------------------------------------ forward
-// A wave keeps 32 users and streams the item tiles of its split.  Lane l: user l % 32, 16 of a
-// tile's 32 items.  m, l, w: the running maximum, sum of e = exp(s - m) and of e y, y = log2 e.
+// Waves of a block: as many as the registers of two blocks' waves per SIMD allow, since the block
+// shares each streamed tile.
+template <int T, int KT>
+constexpr int forward_waves() {
+    return Planes<T>::PS * KT > 24 ? 4 : 8;
+}
+
+// A block's waves keep 32 users each and stream the item tiles of a split through LDS, TPS tiles a
+// turn in two buffers: the next turn's tiles are on the way while this one's are used.  Lane l: user
+// l % 32, 16 of a tile's 32 items.  m, l, w: the running maximum, sum of e = exp(s - m) and of e y,
+// y = log2 e.  The tiles' maxima gather in LDS and leave 32 at a time, a row's 128 bytes together.
 template <int T, int KT, bool TOP>
-__global__ __launch_bounds__(256) void softmax_forward_kernel(Job j) {
-    constexpr int PS = Planes<T>::PS;
-    const int lane = threadIdx.x & 63, h = lane >> 5;
+__global__ __launch_bounds__((forward_waves<T, KT>() * 64)) void softmax_forward_kernel(Job j) {
+    constexpr int PS = Planes<T>::PS, WAVES = forward_waves<T, KT>();
+    constexpr int TPS = PS * KT < 8 ? 8 / (PS * KT) : 1;
+    __shared__ uint4 buf[2][TPS * PS * KT * 64];
+    __shared__ f32x4 bias[2][TPS * 8];
+    __shared__ float tmax[TOP ? WAVES : 1][TOP ? 32 * 33 : 1];
+    const int lane = threadIdx.x & 63, h = lane >> 5, wave = threadIdx.x >> 6;
     const int split = blockIdx.x % j.splits;
-    const int64_t ut = (int64_t)(blockIdx.x / j.splits) * 4 + (threadIdx.x >> 6);
-    if (ut >= j.u.tiles) return;
-    const int64_t row = ut * 32 + (lane & 31);
+    const int64_t ut = (int64_t)(blockIdx.x / j.splits) * WAVES + wave;
+    const bool mine = ut < j.u.tiles;  // the others only help to stage
+    const int64_t row = (mine ? ut : 0) * 32 + (lane & 31);
     uint4 b[PS][KT];
 #pragma unroll
     for (int p = 0; p < PS; ++p)
 #pragma unroll
-        for (int ks = 0; ks < KT; ++ks) b[p][ks] = j.u.frag[((ut * PS + p) * KT + ks) * 64 + lane];
+        for (int ks = 0; ks < KT; ++ks)
+            b[p][ks] = j.u.frag[(((mine ? ut : 0) * PS + p) * KT + ks) * 64 + lane];
     const int t0 = (int)((int64_t)j.v.tiles * split / j.splits);
     const int t1 = (int)((int64_t)j.v.tiles * (split + 1) / j.splits);
+    const auto load = [&](int tl, int at) {
+        const int n = min(TPS, t1 - tl);
+        stage<WAVES>(j.v.frag + (int64_t)tl * PS * KT * 64, buf[at], n * PS * KT);
+        if (wave == WAVES - 1 && lane < n * 8)  // n * 32 floats
+            __builtin_amdgcn_global_load_lds(
+                (const __attribute__((address_space(1))) void*)((const f32x4*)j.vbias + tl * 8 +
+                                                                lane),
+                (__attribute__((address_space(3))) void*)bias[at], 16, 0, 0);
+    };
     float m = kFloor, l = 0.0f, w = 0.0f;
-    for (int tl = t0; tl < t1; ++tl) {
-        f32x16 c;
+    uint32_t next_bits = j.mask && t0 < t1 ? j.mask[(int64_t)t0 * j.rows_pad + row] : 0;
+    if (t0 < t1) load(t0, 0);
+    for (int ts = t0, at = 0; ts < t1; ts += TPS, at ^= 1) {
+        stage_wait();
+        if (ts + TPS < t1) load(ts + TPS, at ^ 1);
+        if (!mine) continue;
+        for (int x = 0; x < TPS && ts + x < t1; ++x) {
+            const int tl = ts + x;
+            const uint32_t bits = next_bits >> (4 * h);
+            if (j.mask && tl + 1 < t1) next_bits = j.mask[(int64_t)(tl + 1) * j.rows_pad + row];
+            f32x16 c;
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-            const f32x4 bias = *(const f32x4*)&j.vbias[tl * 32 + 8 * q + 4 * h];
+            for (int q = 0; q < 4; ++q) {
+                const f32x4 v = bias[at][x * 8 + 2 * q + h];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) c[4 * q + e] = bias[e];
-        }
-        c = score_tile<T, KT>(j.v.frag + (int64_t)tl * PS * KT * 64, b, c, lane);
-        if (j.mask) {
-            const uint32_t bits = j.mask[(int64_t)tl * j.rows_pad + row] >> (4 * h);
+                for (int e = 0; e < 4; ++e) c[4 * q + e] = v[e];
+            }
+            c = score_tile<T, KT>(buf[at] + x * PS * KT * 64, b, c, lane);
             if (__any(bits & 0x0F0F0F0Fu)) {
 #pragma unroll
                 for (int i = 0; i < 16; ++i)
                     if (bits >> reg_row(i, 0) & 1u) c[i] = kGone;
             }
-        }
-        float mt = c[0];
+            float mt = c[0];
 #pragma unroll
-        for (int i = 1; i < 16; ++i) mt = fmaxf(mt, c[i]);
-        if constexpr (TOP) {
-            const float both = fmaxf(mt, __shfl_xor(mt, 32));
-            if (h == 0) j.cmax[row * j.cpad + tl] = both;
-        }
-        if (__any(mt > m)) {
-            const float mn = fmaxf(m, mt), d = (m - mn) * kLog2e, f = __builtin_amdgcn_exp2f(d);
-            w = f * fmaf(l, d, w);
-            l *= f;
-            m = mn;
-        }
-        const float m2 = m * kLog2e;
-        float sl = 0.0f, sw = 0.0f;
+            for (int i = 1; i < 16; ++i) mt = fmaxf(mt, c[i]);
+            if constexpr (TOP) {
+                const float both = fmaxf(mt, __shfl_xor(mt, 32));
+                if (h == 0) tmax[wave][lane * 33 + (tl & 31)] = both;
+                if ((tl & 31) == 31 || tl + 1 == t1) {  // 32 tiles, or the split's ends
+                    const int first = max(t0, tl & ~31);
+                    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+                    const int col = lane & 31;
+                    if (col >= (first & 31) && col <= (tl & 31))
+                        for (int r = h; r < 32; r += 2)
+                            j.cmax[(ut * 32 + r) * j.cpad + (tl & ~31) + col] =
+                                tmax[wave][r * 33 + col];
+                    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+                }
+            }
+            if (__any(mt > m)) {
+                const float mn = fmaxf(m, mt), d = (m - mn) * kLog2e;
+                const float f = __builtin_amdgcn_exp2f(d);
+                w = f * fmaf(l, d, w);
+                l *= f;
+                m = mn;
+            }
+            const float m2 = m * kLog2e;
+            float sl = 0.0f, sw = 0.0f;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            const float y = fmaf(c[i], kLog2e, -m2), e = __builtin_amdgcn_exp2f(y);
-            sl += e;
-            sw = fmaf(e, y, sw);
+            for (int i = 0; i < 16; ++i) {
+                const float y = fmaf(c[i], kLog2e, -m2), e = __builtin_amdgcn_exp2f(y);
+                sl += e;
+                sw = fmaf(e, y, sw);
+            }
+            l += sl;
+            w += sw;
         }
-        l += sl;
-        w += sw;
     }
+    if (!mine) return;
     // the halves' states joined: lanes l and l + 32 hold the same user
     const float mo = __shfl_xor(m, 32), mn = fmaxf(m, mo), d = (m - mn) * kLog2e;
     const float f = __builtin_amdgcn_exp2f(d);
@@ -690,50 +751,77 @@ __global__ __launch_bounds__(TOP ? 256 : 64) void softmax_finish_kernel(Job j) {
 }
 
 // ------------------------------------------------------------------ gradient
+// Both kernels stage a tile's score fragments in one LDS buffer and its transposed ones in another:
+// while one is used, the other is on the way, with a barrier between.  Waves of a block: 4 where
+// the accumulators (8 x 16) and the kept side fill half of the registers.
+template <int KT>
+constexpr int grad_waves() {
+    return KT > 8 ? 4 : 8;
+}
+
 // Users' side: as the forward pass, G in place of the softmax state, dU += G V.
 template <int T, int KT>
-__global__ __launch_bounds__(256) void softmax_grad_users_kernel(Job j) {
+__global__ __launch_bounds__(grad_waves<KT>() * 64) void softmax_grad_users_kernel(Job j) {
     using P = Planes<T>;
-    constexpr int PS = P::PS, MT = KT > 1 ? KT / 2 : 1, KP = MT * 32;
-    const int lane = threadIdx.x & 63, h = lane >> 5;
+    constexpr int PS = P::PS, MT = KT > 1 ? KT / 2 : 1, KP = MT * 32, WAVES = grad_waves<KT>();
+    constexpr int NS = PS * KT, NT = P::PG * MT * 2;  // KB of score and of transposed fragments
+    __shared__ uint4 sbuf[NS * 64], tbuf[NT * 64];
+    __shared__ f32x4 bias[2][8];
+    const int lane = threadIdx.x & 63, h = lane >> 5, wave = threadIdx.x >> 6;
     const int split = blockIdx.x % j.splits;
-    const int64_t ut = (int64_t)(blockIdx.x / j.splits) * 4 + (threadIdx.x >> 6);
-    if (ut >= j.u.tiles) return;
-    const int64_t row = ut * 32 + (lane & 31);
+    const int64_t ut = (int64_t)(blockIdx.x / j.splits) * WAVES + wave;
+    const bool mine = ut < j.u.tiles;
+    const int64_t row = (mine ? ut : 0) * 32 + (lane & 31);
     uint4 b[PS][KT];
 #pragma unroll
     for (int p = 0; p < PS; ++p)
 #pragma unroll
-        for (int ks = 0; ks < KT; ++ks) b[p][ks] = j.u.frag[((ut * PS + p) * KT + ks) * 64 + lane];
+        for (int ks = 0; ks < KT; ++ks)
+            b[p][ks] = j.u.frag[(((mine ? ut : 0) * PS + p) * KT + ks) * 64 + lane];
     const RowMeta mr = j.meta[row];
     f32x16 acc[MT] = {};
     const int t0 = (int)((int64_t)j.v.tiles * split / j.splits);
     const int t1 = (int)((int64_t)j.v.tiles * (split + 1) / j.splits);
+    const auto load = [&](int tl) {
+        stage<WAVES>(j.v.frag + (int64_t)tl * NS * 64, sbuf, NS);
+        if (wave == WAVES - 1 && lane < 8)
+            __builtin_amdgcn_global_load_lds(
+                (const __attribute__((address_space(1))) void*)((const f32x4*)j.vbias + tl * 8 +
+                                                                lane),
+                (__attribute__((address_space(3))) void*)bias[tl & 1], 16, 0, 0);
+    };
+    if (t0 < t1) load(t0);
     for (int tl = t0; tl < t1; ++tl) {
-        f32x16 c;
+        const uint32_t bits =
+            j.mask ? j.mask[(int64_t)tl * j.rows_pad + row] >> (4 * h) : 0;
+        stage_wait();
+        stage<WAVES>(j.v.trans + (int64_t)tl * NT * 64, tbuf, NT);
+        float g[16];
+        if (mine) {
+            f32x16 c;
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-            const f32x4 bias = *(const f32x4*)&j.vbias[tl * 32 + 8 * q + 4 * h];
+            for (int q = 0; q < 4; ++q) {
+                const f32x4 v = bias[tl & 1][2 * q + h];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) c[4 * q + e] = bias[e];
-        }
-        c = score_tile<T, KT>(j.v.frag + (int64_t)tl * PS * KT * 64, b, c, lane);
-        if (j.mask) {
-            const uint32_t bits = j.mask[(int64_t)tl * j.rows_pad + row] >> (4 * h);
+                for (int e = 0; e < 4; ++e) c[4 * q + e] = v[e];
+            }
+            c = score_tile<T, KT>(sbuf, b, c, lane);
             if (__any(bits & 0x0F0F0F0Fu)) {
 #pragma unroll
                 for (int i = 0; i < 16; ++i)
                     if (bits >> reg_row(i, 0) & 1u) c[i] = kGone;
             }
-        }
-        float g[16];
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            const float x = fmaf(c[i], kLog2e, -mr.lse2);
-            g[i] = -__builtin_amdgcn_exp2f(x) * fmaf(mr.c1, x, mr.c0);
+            for (int i = 0; i < 16; ++i) {
+                const float x = fmaf(c[i], kLog2e, -mr.lse2);
+                g[i] = -__builtin_amdgcn_exp2f(x) * fmaf(mr.c1, x, mr.c0);
+            }
         }
-        grad_tile<T, KT>(j.v.trans + (int64_t)tl * P::PG * MT * 128, g, acc, lane);
+        stage_wait();
+        if (tl + 1 < t1) load(tl + 1);
+        if (mine) grad_tile<T, KT>(tbuf, g, acc, lane);
     }
+    if (!mine) return;
     float* out = j.du_part + ((int64_t)split * j.rows_pad + row) * KP;
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt)
@@ -746,55 +834,76 @@ __global__ __launch_bounds__(256) void softmax_grad_users_kernel(Job j) {
 // Items' side: a wave keeps 32 items and streams the user tiles of its split; dV += G^T U,
 // db = the sum of G.  The given items add w to G's element here.
 template <int T, int KT>
-__global__ __launch_bounds__(256) void softmax_grad_items_kernel(Job j) {
+__global__ __launch_bounds__(grad_waves<KT>() * 64) void softmax_grad_items_kernel(Job j) {
     using P = Planes<T>;
-    constexpr int PS = P::PS, MT = KT > 1 ? KT / 2 : 1, KP = MT * 32;
-    const int lane = threadIdx.x & 63, h = lane >> 5;
+    constexpr int PS = P::PS, MT = KT > 1 ? KT / 2 : 1, KP = MT * 32, WAVES = grad_waves<KT>();
+    constexpr int NS = PS * KT, NT = P::PG * MT * 2;
+    __shared__ uint4 sbuf[NS * 64], tbuf[NT * 64];
+    __shared__ uint4 mbuf[2][32];  // the tile's RowMeta
+    const int lane = threadIdx.x & 63, h = lane >> 5, wave = threadIdx.x >> 6;
     const int split = blockIdx.x % j.vsplits;
-    const int64_t vt = (int64_t)(blockIdx.x / j.vsplits) * 4 + (threadIdx.x >> 6);
-    if (vt >= j.v.tiles) return;
-    const int64_t item = vt * 32 + (lane & 31);
+    const int64_t vt = (int64_t)(blockIdx.x / j.vsplits) * WAVES + wave;
+    const bool mine = vt < j.v.tiles;
+    const int64_t item = (mine ? vt : 0) * 32 + (lane & 31);
     uint4 b[PS][KT];
 #pragma unroll
     for (int p = 0; p < PS; ++p)
 #pragma unroll
-        for (int ks = 0; ks < KT; ++ks) b[p][ks] = j.v.frag[((vt * PS + p) * KT + ks) * 64 + lane];
+        for (int ks = 0; ks < KT; ++ks)
+            b[p][ks] = j.v.frag[(((mine ? vt : 0) * PS + p) * KT + ks) * 64 + lane];
     const float bias = j.vbias[item];
     f32x16 acc[MT] = {};
     float db = 0.0f;
     const int t0 = (int)((int64_t)j.u.tiles * split / j.vsplits);
     const int t1 = (int)((int64_t)j.u.tiles * (split + 1) / j.vsplits);
+    const auto load = [&](int tl) {
+        stage<WAVES>(j.u.frag + (int64_t)tl * NS * 64, sbuf, NS);
+        if (wave == WAVES - 1 && lane < 32)
+            __builtin_amdgcn_global_load_lds(
+                (const __attribute__((address_space(1))) void*)((const uint4*)j.meta + tl * 32 +
+                                                                lane),
+                (__attribute__((address_space(3))) void*)mbuf[tl & 1], 16, 0, 0);
+    };
+    if (t0 < t1) load(t0);
     for (int tl = t0; tl < t1; ++tl) {
-        f32x16 c;
+        const uint32_t word =
+            j.mask ? j.mask[(mine ? vt : 0) * j.rows_pad + tl * 32 + (lane & 31)] : 0;
+        stage_wait();
+        stage<WAVES>(j.u.trans + (int64_t)tl * NT * 64, tbuf, NT);
+        float g[16];
+        if (mine) {
+            f32x16 c;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) c[i] = bias;
-        c = score_tile<T, KT>(j.u.frag + (int64_t)tl * PS * KT * 64, b, c, lane);
-        const RowMeta* meta = j.meta + tl * 32;
-        if (j.mask) {
-            const uint32_t* words = j.mask + vt * j.rows_pad + tl * 32;
-            if (__any(words[lane & 31])) {
+            for (int i = 0; i < 16; ++i) c[i] = bias;
+            c = score_tile<T, KT>(sbuf, b, c, lane);
+            const RowMeta* meta = (const RowMeta*)mbuf[tl & 1];
+            if (__any(word)) {
 #pragma unroll
                 for (int i = 0; i < 16; ++i)
-                    if (words[reg_row(i, h)] >> (lane & 31) & 1u) c[i] = kGone;
+                    if (__shfl((int)word, reg_row(i, h)) >> (lane & 31) & 1) c[i] = kGone;
             }
-        }
-        float g[16], sum = 0.0f;
+            float sum = 0.0f;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            const RowMeta mr = meta[reg_row(i, h)];
-            const float x = fmaf(c[i], kLog2e, -mr.lse2);
-            g[i] = -__builtin_amdgcn_exp2f(x) * fmaf(mr.c1, x, mr.c0);
-        }
-        if (__any(meta[lane & 31].t >> 5 == (int32_t)vt)) {
+            for (int i = 0; i < 16; ++i) {
+                const RowMeta mr = meta[reg_row(i, h)];
+                const float x = fmaf(c[i], kLog2e, -mr.lse2);
+                g[i] = -__builtin_amdgcn_exp2f(x) * fmaf(mr.c1, x, mr.c0);
+            }
+            if (__any(meta[lane & 31].t >> 5 == (int32_t)vt)) {
 #pragma unroll
-            for (int i = 0; i < 16; ++i)
-                if (meta[reg_row(i, h)].t == (int32_t)item) g[i] += j.w[tl * 32 + reg_row(i, h)];
-        }
+                for (int i = 0; i < 16; ++i)
+                    if (meta[reg_row(i, h)].t == (int32_t)item)
+                        g[i] += j.w[tl * 32 + reg_row(i, h)];
+            }
 #pragma unroll
-        for (int i = 0; i < 16; ++i) sum += g[i];
-        db += sum;
-        grad_tile<T, KT>(j.u.trans + (int64_t)tl * P::PG * MT * 128, g, acc, lane);
+            for (int i = 0; i < 16; ++i) sum += g[i];
+            db += sum;
+        }
+        stage_wait();
+        if (tl + 1 < t1) load(tl + 1);
+        if (mine) grad_tile<T, KT>(tbuf, g, acc, lane);
     }
+    if (!mine) return;
     const int64_t items_pad = (int64_t)j.v.tiles * 32;
     float* out = j.dv_part + ((int64_t)split * items_pad + item) * KP;
 #pragma unroll
@@ -894,10 +1003,12 @@ int64_t plan(const mml_item_softmax_args* a, bool grad, void* base, Job& j) {
     j.ex_off = a->exclude_offsets;
     j.ex_items = a->exclude_items;
     j.n_ex = a->n_exclude;
-    // about 2,048 waves, a split not under 4 tiles
+    // about 4,096 waves, a split not under 4 tiles; a multiple of the 8 XCDs where there are more,
+    // so that the blocks of one split share an L2 (block b runs on XCD b mod 8)
     const auto splits = [](int64_t kept, int64_t streamed) {
-        const int64_t s = std::min<int64_t>((2048 + kept - 1) / std::max<int64_t>(kept, 1),
-                                            (streamed + 3) / 4);
+        int64_t s = std::min<int64_t>((4096 + kept - 1) / std::max<int64_t>(kept, 1),
+                                      (streamed + 3) / 4);
+        if (s > 8) s &= ~(int64_t)7;
         return (int32_t)std::max<int64_t>(1, s);
     };
     j.splits = splits(j.u.tiles, j.v.tiles);
@@ -989,14 +1100,14 @@ void item_log_probs(const mml_item_softmax_args* a, float* log_probs, float* log
     j.top_items = top_items;
     j.top_lp = top_log_probs;
     mask_and_prep(j, a->dtype, st);
-    const uint32_t blocks = grid_of((int64_t)((j.u.tiles + 3) / 4) * j.splits);
     dispatch(a->dtype, steps_of(j.k), [&](auto tt, auto kt) {
+        constexpr int T = decltype(tt)::value, KT = decltype(kt)::value;
+        constexpr int W = forward_waves<T, KT>();
+        const uint32_t blocks = grid_of((int64_t)((j.u.tiles + W - 1) / W) * j.splits);
         if (j.n_top)
-            softmax_forward_kernel<decltype(tt)::value, decltype(kt)::value, true>
-                <<<blocks, 256, 0, st>>>(j);
+            softmax_forward_kernel<T, KT, true><<<blocks, W * 64, 0, st>>>(j);
         else
-            softmax_forward_kernel<decltype(tt)::value, decltype(kt)::value, false>
-                <<<blocks, 256, 0, st>>>(j);
+            softmax_forward_kernel<T, KT, false><<<blocks, W * 64, 0, st>>>(j);
     });
     const uint32_t lds = std::min(j.n_top + 2, j.v.tiles) * 32 * sizeof(uint64_t);
     dispatch(a->dtype, 1, [&](auto tt, auto) {
@@ -1047,17 +1158,17 @@ void item_log_probs_grad(const mml_item_softmax_args* a, const float* log_norm,
         mask_and_prep(j, a->dtype, st);
         softmax_meta_kernel<<<grid_of((j.rows_pad + 255) / 256), 256, 0, st>>>(j);
     }
-    const uint32_t ub = grid_of((int64_t)((j.u.tiles + 3) / 4) * j.splits);
-    const uint32_t vb = grid_of((int64_t)((j.v.tiles + 3) / 4) * j.vsplits);
     const uint32_t ju = grid_of((j.n_rows * j.k + 255) / 256);
     const uint32_t ji = grid_of(((int64_t)j.n_items * j.k + 255) / 256);
     dispatch(a->dtype, kt0, [&](auto tt, auto kt) {
-        constexpr int T = decltype(tt)::value, KT = decltype(kt)::value;
+        constexpr int T = decltype(tt)::value, KT = decltype(kt)::value, W = grad_waves<KT>();
+        const uint32_t ub = grid_of((int64_t)((j.u.tiles + W - 1) / W) * j.splits);
+        const uint32_t vb = grid_of((int64_t)((j.v.tiles + W - 1) / W) * j.vsplits);
         if (j.n_rows > 0) {
-            softmax_grad_users_kernel<T, KT><<<ub, 256, 0, st>>>(j);
+            softmax_grad_users_kernel<T, KT><<<ub, W * 64, 0, st>>>(j);
             softmax_join_users_kernel<T><<<ju, 256, 0, st>>>(j, kp);
         }
-        softmax_grad_items_kernel<T, KT><<<vb, 256, 0, st>>>(j);
+        softmax_grad_items_kernel<T, KT><<<vb, W * 64, 0, st>>>(j);
         softmax_join_items_kernel<T><<<ji, 256, 0, st>>>(j, kp);
     });
     MML_HIP(hipGetLastError());
