@@ -88,6 +88,27 @@ __device__ __forceinline__ void store_factor(void* p, int64_t i, float x) {
     if constexpr (T == MML_DTYPE_F16) ((_Float16*)p)[i] = (_Float16)x;
 }
 
+// Factors f .. f + 3 of the row at `at`: one store where the rows allow it
+template <int T>
+__device__ __forceinline__ void store_factors(void* p, int64_t at, int f, int k, int vec4, f32x4 x) {
+    if (f >= k) return;
+    if (vec4) {  // k, the stride and the base are multiples of 4 factors
+        if constexpr (T == MML_DTYPE_F32) {
+            *(f32x4*)((float*)p + at + f) = x;
+        } else {
+            uint16_t v[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) store_factor<T>(v, e, x[e]);
+            *(uint2*)((uint16_t*)p + at + f) =
+                make_uint2(v[0] | (uint32_t)v[1] << 16, v[2] | (uint32_t)v[3] << 16);
+        }
+        return;
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+        if (f + e < k) store_factor<T>(p, at + f + e, x[e]);
+}
+
 // ------------------------------------------------------------------ arguments of the kernels
 struct Side {  // one factor matrix as fragments
     const void* src;
@@ -98,6 +119,7 @@ struct Side {  // one factor matrix as fragments
     int32_t tiles;         // tiles of 32 rows written (>= ceil(n / 32))
     uint4* frag;           // [tiles][PS][KT][64]
     uint4* trans;          // [tiles][PG][MT][2][64] (nullptr: not needed)
+    int32_t vec8;          // the rows begin at multiples of 16 bytes
 };
 
 struct RowMeta {  // per row of the users' side, gradient only
@@ -139,6 +161,7 @@ struct Job {
     int32_t vsplits;
     void *gu, *gv;
     int64_t ld_gu, ld_gv;
+    int32_t gv_vec4;
     float* gb;
 };
 
@@ -179,26 +202,50 @@ __global__ __launch_bounds__(256) void softmax_mask_kernel(Job j) {
 template <int T, int KT>
 __global__ __launch_bounds__(256) void softmax_prep_kernel(Job j) {
     using P = Planes<T>;
-    constexpr int KP = KT * 16, MT = KT > 1 ? KT / 2 : 1, LD = KP + 1;
-    __shared__ float tile[32 * LD];
+    constexpr int KP = KT * 16, MT = KT > 1 ? KT / 2 : 1, LD = KP + 4;
+    __shared__ __align__(16) float tile[32 * LD];
     __shared__ int bad[32];
     const bool users = blockIdx.x < (uint32_t)j.u.tiles;
     const Side& s = users ? j.u : j.v;
     const int64_t tl = users ? blockIdx.x : blockIdx.x - j.u.tiles;
     const int t = threadIdx.x;
-    if (t < 32) {
-        int b = 0;
-        if (users && tl * 32 + t < s.n && source_row(s, tl * 32 + t) < 0) b = 2;
-        bad[t] = b;
-    }
+    if (t < 32)
+        bad[t] = users && tl * 32 + t < s.n && source_row(s, tl * 32 + t) < 0 ? 2 : 0;
     __syncthreads();
-    for (int x = t; x < 32 * KP; x += 256) {
-        const int row = x / KP, f = x % KP;
+    for (int x = t; x < 64 * KT; x += 256) {  // 8 factors each
+        const int row = x / (2 * KT), f = 8 * (x % (2 * KT));
         const int64_t src = source_row(s, tl * 32 + row);
-        float v = 0.0f;
-        if (src >= 0 && f < j.k) v = load_factor<T>(s.src, src * s.ld + f);
-        if (!(fabsf(v) < 3e38f)) atomicOr(&bad[row], 1);
-        tile[row * LD + f] = v;
+        float v[8] = {};
+        if (src >= 0) {
+            const int64_t at = src * s.ld + f;
+            if (s.vec8 && f + 8 <= j.k) {
+                if constexpr (T == MML_DTYPE_F32) {
+                    const f32x4 lo = *(const f32x4*)((const float*)s.src + at);
+                    const f32x4 hi = *(const f32x4*)((const float*)s.src + at + 4);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) v[e] = lo[e], v[4 + e] = hi[e];
+                } else {
+                    const uint4 q = *(const uint4*)((const uint16_t*)s.src + at);
+                    const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        const uint16_t b = (uint16_t)(w[e >> 1] >> (16 * (e & 1)));
+                        v[e] = T == MML_DTYPE_F16 ? (float)__builtin_bit_cast(_Float16, b)
+                                                  : __uint_as_float((uint32_t)b << 16);
+                    }
+                }
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    if (f + e < j.k) v[e] = load_factor<T>(s.src, at + e);
+            }
+        }
+        bool ok = true;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) ok = ok && fabsf(v[e]) < 3e38f;
+        if (!ok) atomicOr(&bad[row], 1);
+        *(f32x4*)&tile[row * LD + f] = f32x4{v[0], v[1], v[2], v[3]};
+        *(f32x4*)&tile[row * LD + f + 4] = f32x4{v[4], v[5], v[6], v[7]};
     }
     __syncthreads();
     if (t < 32) {
@@ -214,11 +261,12 @@ __global__ __launch_bounds__(256) void softmax_prep_kernel(Job j) {
     }
     for (int x = t; x < KT * 64; x += 256) {
         const int ks = x >> 6, lane = x & 63, row = lane & 31;
-        const float* src = &tile[row * LD + ks * 16 + 8 * (lane >> 5)];
+        const f32x4* src = (const f32x4*)&tile[row * LD + ks * 16 + 8 * (lane >> 5)];
+        const f32x4 lo = src[0], hi = src[1];
         uint32_t q[P::PS][8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-            float v = bad[row] ? 0.0f : src[e];
+            float v = bad[row] ? 0.0f : e < 4 ? lo[e & 3] : hi[e & 3];
             if constexpr (T == MML_DTYPE_F16) {
                 q[0][e] = (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)v);
             } else {
@@ -456,8 +504,9 @@ __global__ __launch_bounds__((forward_waves<T, KT>() * 64)) void softmax_forward
                     const int first = max(t0, tl & ~31);
                     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
                     const int col = lane & 31;
-                    if (col >= (first & 31) && col <= (tl & 31))
-                        for (int r = h; r < 32; r += 2)
+                    const bool in = col >= (first & 31) && col <= (tl & 31);
+                    for (int r = h; r < 32; r += 2)
+                        if (in)
                             j.cmax[(ut * 32 + r) * j.cpad + (tl & ~31) + col] =
                                 tmax[wave][r * 33 + col];
                     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
@@ -905,6 +954,19 @@ __global__ __launch_bounds__(grad_waves<KT>() * 64) void softmax_grad_items_kern
     }
     if (!mine) return;
     const int64_t items_pad = (int64_t)j.v.tiles * 32;
+    db += __shfl_xor(db, 32);
+    if (j.vsplits == 1) {  // nothing to join: the result itself
+        if (item >= j.n_items) return;
+        if (h == 0) j.gb[item] = db;
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+                store_factors<T>(j.gv, item * j.ld_gv, 32 * mt + 8 * q + 4 * h, j.k, j.gv_vec4,
+                                 f32x4{acc[mt][4 * q], acc[mt][4 * q + 1], acc[mt][4 * q + 2],
+                                       acc[mt][4 * q + 3]});
+        return;
+    }
     float* out = j.dv_part + ((int64_t)split * items_pad + item) * KP;
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt)
@@ -912,7 +974,6 @@ __global__ __launch_bounds__(grad_waves<KT>() * 64) void softmax_grad_items_kern
         for (int q = 0; q < 4; ++q)
             *(f32x4*)&out[32 * mt + 8 * q + 4 * h] =
                 f32x4{acc[mt][4 * q], acc[mt][4 * q + 1], acc[mt][4 * q + 2], acc[mt][4 * q + 3]};
-    db += __shfl_xor(db, 32);
     if (h == 0) j.db_part[split * items_pad + item] = db;
 }
 
@@ -990,14 +1051,16 @@ int64_t plan(const mml_item_softmax_args* a, bool grad, void* base, Job& j) {
     j.n_rows = a->n_rows;
     j.n_top = grad ? 0 : a->n_top;
     j.u = Side{a->user_factors, a->ld_users, a->users, a->n_users, a->n_rows,
-               (int32_t)((a->n_rows + 31) / 32), nullptr, nullptr};
+               (int32_t)((a->n_rows + 31) / 32), nullptr, nullptr, 0};
     j.v = Side{a->item_factors, a->ld_items, nullptr, a->n_items, a->n_items,
-               (int32_t)(((int64_t)a->n_items + 31) / 32), nullptr, nullptr};
+               (int32_t)(((int64_t)a->n_items + 31) / 32), nullptr, nullptr, 0};
+    const int size = T == MML_DTYPE_F32 ? 4 : 2;
+    j.u.vec8 = (uintptr_t)a->user_factors % 16 == 0 && a->ld_users * size % 16 == 0;
+    j.v.vec8 = (uintptr_t)a->item_factors % 16 == 0 && a->ld_items * size % 16 == 0;
     j.rows_pad = (int64_t)j.u.tiles * 32;
     const int64_t items_pad = (int64_t)j.v.tiles * 32;
     j.bias = a->item_bias;
     j.target = a->items;
-    const int size = T == MML_DTYPE_F32 ? 4 : 2;
     j.vec4 = a->num_factors % 4 == 0 && a->ld_items % 4 == 0 &&
              (uintptr_t)a->item_factors % (4 * size) == 0;
     j.ex_off = a->exclude_offsets;
@@ -1029,8 +1092,10 @@ int64_t plan(const mml_item_softmax_args* a, bool grad, void* base, Job& j) {
         j.meta = c.take<RowMeta>(j.rows_pad);
         j.w = c.take<float>(j.rows_pad);
         j.du_part = c.take<float>((int64_t)j.splits * j.rows_pad * mt * 32);
-        j.dv_part = c.take<float>((int64_t)j.vsplits * items_pad * mt * 32);
-        j.db_part = c.take<float>((int64_t)j.vsplits * items_pad);
+        if (j.vsplits > 1) {
+            j.dv_part = c.take<float>((int64_t)j.vsplits * items_pad * mt * 32);
+            j.db_part = c.take<float>((int64_t)j.vsplits * items_pad);
+        }
     }
     return c.used;
 }
@@ -1153,6 +1218,8 @@ void item_log_probs_grad(const mml_item_softmax_args* a, const float* log_norm,
     j.ld_gu = ld_gu;
     j.ld_gv = ld_gv;
     j.gb = gb;
+    const int size = a->dtype == MML_DTYPE_F32 ? 4 : 2;
+    j.gv_vec4 = j.k % 4 == 0 && ld_gv % 4 == 0 && (uintptr_t)gv % (4 * size) == 0;
     const int kt0 = steps_of(j.k), kp = std::max(32, kt0 * 16);
     if (a->n_rows > 0) {
         mask_and_prep(j, a->dtype, st);
@@ -1169,7 +1236,7 @@ void item_log_probs_grad(const mml_item_softmax_args* a, const float* log_norm,
             softmax_join_users_kernel<T><<<ju, 256, 0, st>>>(j, kp);
         }
         softmax_grad_items_kernel<T, KT><<<vb, W * 64, 0, st>>>(j);
-        softmax_join_items_kernel<T><<<ji, 256, 0, st>>>(j, kp);
+        if (j.vsplits > 1) softmax_join_items_kernel<T><<<ji, 256, 0, st>>>(j, kp);
     });
     MML_HIP(hipGetLastError());
 }
