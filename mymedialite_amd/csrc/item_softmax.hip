@@ -376,8 +376,15 @@ __device__ __forceinline__ f32x16 score_tile(const uint4* a,
     return c;
 }
 
-// The planes of G's registers 8 s .. 8 s + 7 as B operands: the leading planes are cut off (the
-// next plane holds the rest exactly), the last is rounded to nearest.
+// Two values as bf16, to nearest even (v_cvt_pk_bf16_f32)
+__device__ __forceinline__ uint32_t pack_bf16(float x, float y) {
+    using f32x2 = __attribute__((ext_vector_type(2))) float;
+    using bf16x2 = __attribute__((ext_vector_type(2))) __bf16;
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{x, y}), bf16x2));
+}
+// The planes of G's registers 8 s .. 8 s + 7 as B operands.  The leading planes are cut off, so the
+// next holds the rest exactly; of three planes the last has its 8 bits left and is cut too, of two
+// it is rounded to nearest.
 template <int GP>
 __device__ __forceinline__ void split_g(const float (&g)[16], int step, uint4 (&q)[GP]) {
     uint32_t w[GP][4];
@@ -387,13 +394,10 @@ __device__ __forceinline__ void split_g(const float (&g)[16], int step, uint4 (&
 #pragma unroll
         for (int p = 0; p < GP; ++p) {
             const uint32_t a = __float_as_uint(x), b = __float_as_uint(y);
-            if (p + 1 < GP) {
-                w[p][e] = __builtin_amdgcn_perm(b, a, 0x07060302u);
-                x -= __uint_as_float(a & 0xFFFF0000u);
-                y -= __uint_as_float(b & 0xFFFF0000u);
-            } else {
-                w[p][e] = bf16_rn(x) | bf16_rn(y) << 16;
-            }
+            w[p][e] = p == 1 && GP == 2 ? pack_bf16(x, y)
+                                        : __builtin_amdgcn_perm(b, a, 0x07060302u);
+            x -= __uint_as_float(a & 0xFFFF0000u);
+            y -= __uint_as_float(b & 0xFFFF0000u);
         }
     }
 #pragma unroll
@@ -429,6 +433,15 @@ __device__ __forceinline__ void grad_tile(const uint4* a, const float (&g)[16],
 
 __device__ __forceinline__ int reg_row(int i, int h) { return 8 * (i >> 2) + 4 * h + (i & 3); }
 
+// kGone where the bits (shifted right by 4 h) say so.  The empty asm keeps the compiler from taking
+// the selects out of their branch: 48 instructions for every tile against 200 for the tile itself.
+__device__ __forceinline__ void mask_tile(f32x16& c, uint32_t bits) {
+    asm volatile("");
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+        if (bits >> reg_row(i, 0) & 1u) c[i] = kGone;
+}
+
 // ------------------------------------------------------------------ forward
 // Waves of a block: as many as the registers of two blocks' waves per SIMD allow, since the block
 // shares each streamed tile.
@@ -451,7 +464,9 @@ __global__ __launch_bounds__((forward_waves<T, KT>() * 64)) void softmax_forward
     const int lane = threadIdx.x & 63, h = lane >> 5, wave = threadIdx.x >> 6;
     const int split = blockIdx.x % j.splits;
     const int64_t ut = (int64_t)(blockIdx.x / j.splits) * WAVES + wave;
-    const bool mine = ut < j.u.tiles;  // the others only help to stage
+    // A wave behind the last tile of users does tile 0's work and drops it: a branch around the work
+    // costs the others more (the accumulators change registers at it).
+    const bool mine = ut < j.u.tiles;  // as in the forward pass
     const int64_t row = (mine ? ut : 0) * 32 + (lane & 31);
     uint4 b[PS][KT];
 #pragma unroll
@@ -476,7 +491,6 @@ __global__ __launch_bounds__((forward_waves<T, KT>() * 64)) void softmax_forward
     for (int ts = t0, at = 0; ts < t1; ts += TPS, at ^= 1) {
         stage_wait();
         if (ts + TPS < t1) load(ts + TPS, at ^ 1);
-        if (!mine) continue;
         for (int x = 0; x < TPS && ts + x < t1; ++x) {
             const int tl = ts + x;
             const uint32_t bits = next_bits >> (4 * h);
@@ -489,11 +503,7 @@ __global__ __launch_bounds__((forward_waves<T, KT>() * 64)) void softmax_forward
                 for (int e = 0; e < 4; ++e) c[4 * q + e] = v[e];
             }
             c = score_tile<T, KT>(buf[at] + x * PS * KT * 64, b, c, lane);
-            if (__any(bits & 0x0F0F0F0Fu)) {
-#pragma unroll
-                for (int i = 0; i < 16; ++i)
-                    if (bits >> reg_row(i, 0) & 1u) c[i] = kGone;
-            }
+            if (__any(bits & 0x0F0F0F0Fu)) mask_tile(c, bits);
             float mt = c[0];
 #pragma unroll
             for (int i = 1; i < 16; ++i) mt = fmaxf(mt, c[i]);
@@ -504,7 +514,7 @@ __global__ __launch_bounds__((forward_waves<T, KT>() * 64)) void softmax_forward
                     const int first = max(t0, tl & ~31);
                     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
                     const int col = lane & 31;
-                    const bool in = col >= (first & 31) && col <= (tl & 31);
+                    const bool in = mine && col >= (first & 31) && col <= (tl & 31);
                     for (int r = h; r < 32; r += 2)
                         if (in)
                             j.cmax[(ut * 32 + r) * j.cpad + (tl & ~31) + col] =
@@ -819,7 +829,7 @@ __global__ __launch_bounds__(grad_waves<KT>() * 64) void softmax_grad_users_kern
     const int lane = threadIdx.x & 63, h = lane >> 5, wave = threadIdx.x >> 6;
     const int split = blockIdx.x % j.splits;
     const int64_t ut = (int64_t)(blockIdx.x / j.splits) * WAVES + wave;
-    const bool mine = ut < j.u.tiles;
+    const bool mine = ut < j.u.tiles;  // as in the forward pass
     const int64_t row = (mine ? ut : 0) * 32 + (lane & 31);
     uint4 b[PS][KT];
 #pragma unroll
@@ -846,29 +856,23 @@ __global__ __launch_bounds__(grad_waves<KT>() * 64) void softmax_grad_users_kern
         stage_wait();
         stage<WAVES>(j.v.trans + (int64_t)tl * NT * 64, tbuf, NT);
         float g[16];
-        if (mine) {
-            f32x16 c;
+        f32x16 c;
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                const f32x4 v = bias[tl & 1][2 * q + h];
+        for (int q = 0; q < 4; ++q) {
+            const f32x4 v = bias[tl & 1][2 * q + h];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) c[4 * q + e] = v[e];
-            }
-            c = score_tile<T, KT>(sbuf, b, c, lane);
-            if (__any(bits & 0x0F0F0F0Fu)) {
+            for (int e = 0; e < 4; ++e) c[4 * q + e] = v[e];
+        }
+        c = score_tile<T, KT>(sbuf, b, c, lane);
+        if (__any(bits & 0x0F0F0F0Fu)) mask_tile(c, bits);
 #pragma unroll
-                for (int i = 0; i < 16; ++i)
-                    if (bits >> reg_row(i, 0) & 1u) c[i] = kGone;
-            }
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                const float x = fmaf(c[i], kLog2e, -mr.lse2);
-                g[i] = -__builtin_amdgcn_exp2f(x) * fmaf(mr.c1, x, mr.c0);
-            }
+        for (int i = 0; i < 16; ++i) {
+            const float x = fmaf(c[i], kLog2e, -mr.lse2);
+            g[i] = -__builtin_amdgcn_exp2f(x) * fmaf(mr.c1, x, mr.c0);
         }
         stage_wait();
         if (tl + 1 < t1) load(tl + 1);
-        if (mine) grad_tile<T, KT>(tbuf, g, acc, lane);
+        grad_tile<T, KT>(tbuf, g, acc, lane);
     }
     if (!mine) return;
     float* out = j.du_part + ((int64_t)split * j.rows_pad + row) * KP;
@@ -920,37 +924,36 @@ __global__ __launch_bounds__(grad_waves<KT>() * 64) void softmax_grad_items_kern
         stage_wait();
         stage<WAVES>(j.u.trans + (int64_t)tl * NT * 64, tbuf, NT);
         float g[16];
-        if (mine) {
-            f32x16 c;
+        f32x16 c;
 #pragma unroll
-            for (int i = 0; i < 16; ++i) c[i] = bias;
-            c = score_tile<T, KT>(sbuf, b, c, lane);
-            const RowMeta* meta = (const RowMeta*)mbuf[tl & 1];
-            if (__any(word)) {
+        for (int i = 0; i < 16; ++i) c[i] = bias;
+        c = score_tile<T, KT>(sbuf, b, c, lane);
+        const RowMeta* meta = (const RowMeta*)mbuf[tl & 1];
+        if (__any(word)) {
+            asm volatile("");  // as in mask_tile
 #pragma unroll
-                for (int i = 0; i < 16; ++i)
-                    if (__shfl((int)word, reg_row(i, h)) >> (lane & 31) & 1) c[i] = kGone;
-            }
-            float sum = 0.0f;
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                const RowMeta mr = meta[reg_row(i, h)];
-                const float x = fmaf(c[i], kLog2e, -mr.lse2);
-                g[i] = -__builtin_amdgcn_exp2f(x) * fmaf(mr.c1, x, mr.c0);
-            }
-            if (__any(meta[lane & 31].t >> 5 == (int32_t)vt)) {
-#pragma unroll
-                for (int i = 0; i < 16; ++i)
-                    if (meta[reg_row(i, h)].t == (int32_t)item)
-                        g[i] += j.w[tl * 32 + reg_row(i, h)];
-            }
-#pragma unroll
-            for (int i = 0; i < 16; ++i) sum += g[i];
-            db += sum;
+            for (int i = 0; i < 16; ++i)
+                if (__shfl((int)word, reg_row(i, h)) >> (lane & 31) & 1) c[i] = kGone;
         }
+        float sum = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const RowMeta mr = meta[reg_row(i, h)];
+            const float x = fmaf(c[i], kLog2e, -mr.lse2);
+            g[i] = -__builtin_amdgcn_exp2f(x) * fmaf(mr.c1, x, mr.c0);
+        }
+        if (__any(meta[lane & 31].t >> 5 == (int32_t)vt)) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+                if (meta[reg_row(i, h)].t == (int32_t)item)
+                    g[i] += j.w[tl * 32 + reg_row(i, h)];
+        }
+#pragma unroll
+        for (int i = 0; i < 16; ++i) sum += g[i];
+        db += sum;
         stage_wait();
         if (tl + 1 < t1) load(tl + 1);
-        if (mine) grad_tile<T, KT>(tbuf, g, acc, lane);
+        grad_tile<T, KT>(tbuf, g, acc, lane);
     }
     if (!mine) return;
     const int64_t items_pad = (int64_t)j.v.tiles * 32;
