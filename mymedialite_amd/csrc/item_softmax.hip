@@ -10,13 +10,17 @@
 // The R x N matrices s, p and G are never stored: 32 x 32 tiles of s are made on the matrix cores,
 // used in registers and dropped (flash style: a running maximum m, sum l and sum of e y).
 //
-// f32 factors run on the bf16 matrix cores at f32 accuracy: every value is split into three bf16
-// planes (8 significant bits each) and a product takes the six plane products a b with
-// plane(a) + plane(b) <= 2, accumulated in f32; the dropped ones are below 2^-23 of |a b|.
-// v_mfma_f32_32x32x16_bf16 does 1,024 flops per cycle and SIMD against 64 of the f32 form, so six
-// products are 2.7 times as fast.  bf16 factors are one plane; f16 factors one f16 plane for the
-// scores and two bf16 planes (exact: 11 bits) for the gradient products.  G is split into three
-// (f32) or two (bf16, f16: 16 bits, against outputs of 8 and 11 bits) planes.
+// f32 factors run on the f16 matrix cores at close to f32 accuracy: a value x, scaled by a power of
+// two common to its matrix (largest magnitude just under 2^13), is hi + lo with hi = f16(x) and
+// lo = f16(x - hi), 22 significant bits down to 2^-16 of the matrix' largest value and 2^-38 of it
+// below; a product takes lo hi + hi lo + hi hi, accumulated in f32 (the dropped lo lo is below 2^-22
+// of |a b|).  v_mfma_f32_32x32x16_f16 does 1,024 flops per cycle and SIMD against 64 of the f32
+// form, so three products are 5 times as fast, and twice as fast as the six products that three bf16
+// planes take -- which counts doubly, since the matrix cores run into the power limit first
+// (1.6 PFLOP/s on random data against 2.3 on constants).  f16 factors are one f16 plane, bf16
+// factors one bf16 plane.  G is split into two planes as well: f16 under a power of two that every
+// kept row adapts to the largest |G| it has met (the sums are scaled along, as a running maximum's
+// are), or bf16 for bf16 factors (16 bits against the result's 8).
 //
 // Tile layout.  v_mfma_f32_32x32x16: A (32 x 16), lane l holds row l % 32, k = 8 (l / 32) .. + 7;
 // B (16 x 32) the same with the column; C: lane l holds column l % 32, register i row
@@ -47,27 +51,22 @@ using f16x8 = __attribute__((ext_vector_type(8))) _Float16;
 
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr float kLn2 = 0.69314718055994530942f;
-// The score of an excluded item.  Finite, so that e * y below is 0 * finite = 0 and not 0 * inf.
+// A bias of this or less excludes its item; the score of an excluded item where scores are not scaled.
+// Finite, so that e * y below is 0 * finite = 0 and not 0 * inf.
 constexpr float kGone = -1e30f;
-// Where the running maximum starts: above kGone, so that an excluded item's e is 0 before the first
-// score too (a row whose scores are all below it counts as empty).
-constexpr float kFloor = -1e28f;
 constexpr int kMaxTop = 128;
 
-// Planes of a factor type: PS of the score product, PG of the gradient product's factors, GP of G.
+// Planes of a factor type: PS of the score product, PG of the gradient product's factors, GP of G;
+// HALF: the planes are f16 (else bf16).
 template <int T>
-struct Planes;
+struct Planes {  // bf16 and f16 factors
+    static constexpr int PS = 1, PG = 1, GP = 2;
+    static constexpr bool HALF = T == MML_DTYPE_F16;
+};
 template <>
 struct Planes<MML_DTYPE_F32> {
-    static constexpr int PS = 3, PG = 3, GP = 3;
-};
-template <>
-struct Planes<MML_DTYPE_BF16> {
-    static constexpr int PS = 1, PG = 1, GP = 2;
-};
-template <>
-struct Planes<MML_DTYPE_F16> {
-    static constexpr int PS = 1, PG = 2, GP = 2;
+    static constexpr int PS = 2, PG = 2, GP = 2;
+    static constexpr bool HALF = true;
 };
 
 template <int T>
@@ -130,11 +129,25 @@ struct RowMeta {  // per row of the users' side, gradient only
 
 static_assert(sizeof(RowMeta) == 16, "staged 16 bytes per lane");
 
+// Powers of two that the planes are scaled by (f32 factors; otherwise 1), so scores come out of the
+// matrix cores as s 2^(eu + ev), and what follows from them.  Written by the preparation.
+struct Scale {
+    float kappa;  // log2 e / 2^(eu + ev)
+    float unit;   // 2^-(eu + ev)
+    float gone;   // the score of an excluded item: below every other
+    float floor;  // where a running maximum starts: above gone, so that an excluded item's e is 0
+                  // before the first score too (a row whose scores are all below it counts as empty)
+    int32_t eu, ev;
+};
+constexpr int kMaxParts = 512, kUserParts = 64;  // partial maxima of softmax_max_kernel
+
 struct Job {
     Side u, v;
+    float* parts;   // [kMaxParts]: largest |factor| each: kUserParts of the users', then the items'
+    Scale* scale;
     const float* bias;   // items (nullptr: 0)
-    float* vbias;        // [v.tiles * 32]: bias, kGone for an excluded or padding item, NaN where
-                         // the factors are not finite
+    float* vbias;        // [v.tiles * 32]: bias 2^(eu + ev), scale->gone for an excluded or padding
+                         // item, NaN where the factors are not finite
     uint8_t* ubad;       // [u.tiles * 32]: 1 = factors not finite, 2 = unknown user
     uint32_t* mask;      // [v.tiles][rows_pad]: bit i of word (tile, r): item 32 tile + i excluded
     int64_t rows_pad;    // u.tiles * 32
@@ -175,6 +188,20 @@ __device__ __forceinline__ int64_t source_row(const Side& s, int64_t x) {  // -1
 }
 
 // ------------------------------------------------------------------ preparation
+// The next plane of v, to nearest; v becomes what is left
+template <int T>
+__device__ __forceinline__ uint32_t take_plane(float& v) {
+    if constexpr (Planes<T>::HALF) {
+        const _Float16 h = (_Float16)v;
+        v -= (float)h;
+        return (uint32_t)__builtin_bit_cast(uint16_t, h);
+    } else {
+        const uint32_t b = bf16_rn(v);
+        v -= __uint_as_float(b << 16);
+        return b;
+    }
+}
+
 __global__ __launch_bounds__(256) void softmax_clear_kernel(uint32_t* p, int64_t n) {
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256)
         p[i] = 0;
@@ -196,6 +223,82 @@ __global__ __launch_bounds__(256) void softmax_mask_kernel(Job j) {
     }
 }
 
+// The largest finite magnitude of either matrix (the batch's users only), in kMaxParts parts.
+template <int T>
+__global__ __launch_bounds__(256) void softmax_max_kernel(Job j) {
+    __shared__ float red[4];
+    const bool users = blockIdx.x < kUserParts;
+    const Side& s = users ? j.u : j.v;
+    const int part = users ? blockIdx.x : blockIdx.x - kUserParts;
+    const int parts = users ? kUserParts : kMaxParts - kUserParts;
+    float m = 0.0f;
+    const auto take = [&](float x) {
+        const float a = fabsf(x);
+        if (a < 3e38f) m = fmaxf(m, a);
+    };
+    // a wave per row and turn
+    const int lane = threadIdx.x & 63;
+    if (!s.index && s.ld == j.k && s.vec8) {  // one contiguous array
+        const int64_t n = s.n * j.k / 4;
+        for (int64_t x = (int64_t)part * 256 + threadIdx.x; x < n; x += (int64_t)parts * 256) {
+            const f32x4 v = ((const f32x4*)s.src)[x];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) take(v[e]);
+        }
+        if (part == 0 && threadIdx.x < s.n * j.k % 4) take(((const float*)s.src)[4 * n + threadIdx.x]);
+    } else {
+        for (int64_t r = (int64_t)part * 4 + (threadIdx.x >> 6); r < s.n; r += (int64_t)parts * 4) {
+            const int64_t src = source_row(s, r);
+            if (src < 0) continue;
+            for (int f = lane; f < j.k; f += 64) take(load_factor<T>(s.src, src * s.ld + f));
+        }
+    }
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor(m, d));
+    if (lane == 0) red[threadIdx.x >> 6] = m;
+    __syncthreads();
+    if (threadIdx.x == 0)
+        j.parts[blockIdx.x] = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+}
+
+// The scales from the parts; all 256 threads of a block take part.  A matrix' largest magnitude comes
+// out in [2^12, 2^13), unless that takes an exponent outside [-40, 12] (above 2^53 a plane overflows
+// and the rows become NaN; small values need no more).
+template <int T>
+__device__ __forceinline__ Scale make_scale(const Job& j) {
+    int eu = 0, ev = 0;
+    if constexpr (T == MML_DTYPE_F32) {
+        __shared__ float red[4], first;
+        const int t = threadIdx.x;
+        float v = j.parts[t], u = v;
+        if (t < kUserParts) v = 0.0f;
+        v = fmaxf(v, j.parts[t + 256]);
+#pragma unroll
+        for (int d = 32; d > 0; d >>= 1) {
+            v = fmaxf(v, __shfl_xor(v, d));
+            u = fmaxf(u, __shfl_xor(u, d));
+        }
+        static_assert(kUserParts == 64, "the users' parts are wave 0's");
+        if (t == 0) first = u;
+        if ((t & 63) == 0) red[t >> 6] = v;
+        __syncthreads();
+        u = first;
+        v = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+        // (frexp: x = f 2^e, f in [0.5, 1); of 0 it is 0)
+        eu = max(-40, min(12, 13 - __builtin_amdgcn_frexp_expf(u)));
+        ev = max(-40, min(12, 13 - __builtin_amdgcn_frexp_expf(v)));
+    }
+    Scale c;
+    const int e = eu + ev;
+    c.unit = ldexpf(1.0f, -e);
+    c.kappa = ldexpf(kLog2e, -e);
+    c.gone = -fmaxf(ldexpf(1e30f, min(e, 0)), 1.0995116e12f);  // 2^40: scaled scores are below 2^35
+    c.floor = c.gone * 0.0625f;
+    c.eu = eu;
+    c.ev = ev;
+    return c;
+}
+
 // Fragments of both sides, one block per tile of 32 rows (the users' tiles first).  A row with a
 // value that is not finite is written as zeros and marked, so that 0 * NaN cannot reach the other
 // rows' sums: an item that is not excluded gets the bias NaN, a user the mark in ubad.
@@ -209,6 +312,8 @@ __global__ __launch_bounds__(256) void softmax_prep_kernel(Job j) {
     const Side& s = users ? j.u : j.v;
     const int64_t tl = users ? blockIdx.x : blockIdx.x - j.u.tiles;
     const int t = threadIdx.x;
+    const Scale sc = make_scale<T>(j);
+    if (blockIdx.x == 0 && t == 0) *j.scale = sc;
     if (t < 32)
         bad[t] = users && tl * 32 + t < s.n && source_row(s, tl * 32 + t) < 0 ? 2 : 0;
     __syncthreads();
@@ -254,11 +359,13 @@ __global__ __launch_bounds__(256) void softmax_prep_kernel(Job j) {
             j.ubad[row] = (uint8_t)bad[t];
         } else {
             float b = row < s.n ? (j.bias ? j.bias[row] : 0.0f) : kGone;
-            if (b <= kGone) b = kGone;
-            else if (bad[t] || !(fabsf(b) < 3e38f)) b = __builtin_nanf("");
+            if (b <= kGone) b = sc.gone;
+            else if (bad[t] || !(b < -kGone)) b = __builtin_nanf("");
+            else b = fmaxf(ldexpf(b, sc.eu + sc.ev), sc.gone * 0.5f);
             j.vbias[row] = b;
         }
     }
+    const float mul = ldexpf(1.0f, users ? sc.eu : sc.ev);
     for (int x = t; x < KT * 64; x += 256) {
         const int ks = x >> 6, lane = x & 63, row = lane & 31;
         const f32x4* src = (const f32x4*)&tile[row * LD + ks * 16 + 8 * (lane >> 5)];
@@ -266,16 +373,9 @@ __global__ __launch_bounds__(256) void softmax_prep_kernel(Job j) {
         uint32_t q[P::PS][8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-            float v = bad[row] ? 0.0f : e < 4 ? lo[e & 3] : hi[e & 3];
-            if constexpr (T == MML_DTYPE_F16) {
-                q[0][e] = (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)v);
-            } else {
+            float v = bad[row] ? 0.0f : (e < 4 ? lo[e & 3] : hi[e & 3]) * mul;
 #pragma unroll
-                for (int p = 0; p < P::PS; ++p) {
-                    q[p][e] = bf16_rn(v);
-                    v -= __uint_as_float(q[p][e] << 16);
-                }
-            }
+            for (int p = 0; p < P::PS; ++p) q[p][e] = take_plane<T>(v);
         }
 #pragma unroll
         for (int p = 0; p < P::PS; ++p)
@@ -290,12 +390,9 @@ __global__ __launch_bounds__(256) void softmax_prep_kernel(Job j) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
             const int row = 16 * step + 8 * (e >> 2) + 4 * (lane >> 5) + (e & 3);
-            float v = f < KP && !bad[row] ? tile[row * LD + f] : 0.0f;
+            float v = f < KP && !bad[row] ? tile[row * LD + f] * mul : 0.0f;
 #pragma unroll
-            for (int p = 0; p < P::PG; ++p) {
-                q[p][e] = bf16_rn(v);
-                v -= __uint_as_float(q[p][e] << 16);
-            }
+            for (int p = 0; p < P::PG; ++p) q[p][e] = take_plane<T>(v);
         }
 #pragma unroll
         for (int p = 0; p < P::PG; ++p)
@@ -315,7 +412,7 @@ __global__ __launch_bounds__(256) void softmax_meta_kernel(Job j) {
     if (r < j.n_rows && j.ubad[r] < 2) {
         const float lse = j.in_norm[r], h = j.g_ent ? j.g_ent[r] : 0.0f;
         int32_t t = j.target ? j.target[r] : -1;
-        if (t < 0 || t >= j.n_items || j.vbias[t] <= kGone ||
+        if (t < 0 || t >= j.n_items || j.vbias[t] <= j.scale->gone ||
             (j.mask && (j.mask[(int64_t)(t >> 5) * j.rows_pad + r] >> (t & 31) & 1u)))
             t = -1;
         w = t >= 0 && j.g_lp ? j.g_lp[r] : 0.0f;
@@ -331,16 +428,25 @@ __global__ __launch_bounds__(256) void softmax_meta_kernel(Job j) {
 }
 
 // ------------------------------------------------------------------ staging
-// n KB of fragments into LDS, asynchronously (global_load_lds: 16 bytes per lane, no registers), the
-// 1 KB pieces dealt over the block's waves.  stage_wait: this wave's pieces have landed; with the
-// barrier behind it, everyone's have.
+// One asynchronous copy of 16 bytes per active lane into LDS: lane i's 16 bytes at `from` go to
+// to + 16 i (`to` is the same in all lanes).  Written in assembly, and not as the builtin, because
+// the compiler makes every later LDS read wait for a builtin's copy to land, the reads of the other
+// buffer too; stage_wait is the wait, and a __shared__ array filled here is only read behind one.
+// (An SALU write of m0 needs a wait state before its use; nothing else here uses m0.)
+__device__ __forceinline__ void copy_to_lds(const void* from, void* to) {
+    const uint32_t at = __builtin_amdgcn_readfirstlane(
+        (uint32_t)(uintptr_t)(__attribute__((address_space(3))) void*)to);
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off"
+                 :
+                 : "s"(at), "v"(from)
+                 : "memory");
+}
+// n KB of fragments, the 1 KB pieces dealt over the block's waves.  stage_wait: this wave's copies
+// have landed; with the barrier behind it, everyone's have.
 template <int WAVES>
 __device__ __forceinline__ void stage(const uint4* __restrict__ src, uint4* dst, int n) {
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    for (int c = wave; c < n; c += WAVES)
-        __builtin_amdgcn_global_load_lds(
-            (const __attribute__((address_space(1))) void*)(src + c * 64 + lane),
-            (__attribute__((address_space(3))) void*)(dst + c * 64), 16, 0, 0);
+    for (int c = wave; c < n; c += WAVES) copy_to_lds(src + c * 64 + lane, dst + c * 64);
 }
 __device__ __forceinline__ void stage_wait() {
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -348,6 +454,21 @@ __device__ __forceinline__ void stage_wait() {
 }
 
 // ------------------------------------------------------------------ tiles
+template <int T>
+__device__ __forceinline__ f32x16 mfma(uint4 a, uint4 b, f32x16 c) {
+    if constexpr (Planes<T>::HALF)
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a),
+                                                      __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a),
+                                                       __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+// The larger of the two values in lanes l and l + 32, in both
+__device__ __forceinline__ float both_max(float x) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false,
+                                                    false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
 // c + A B over the PS planes of KT steps (smallest products first).  A: fragments in LDS.
 template <int T, int KT>
 __device__ __forceinline__ f32x16 score_tile(const uint4* a,
@@ -359,49 +480,75 @@ __device__ __forceinline__ f32x16 score_tile(const uint4* a,
         uint4 x[PS];
 #pragma unroll
         for (int p = 0; p < PS; ++p) x[p] = a[(p * KT + ks) * 64 + lane];
-        if constexpr (T == MML_DTYPE_F16) {
-            c = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, x[0]),
-                                                       __builtin_bit_cast(f16x8, b[0][ks]), c, 0, 0,
-                                                       0);
-        } else {
 #pragma unroll
-            for (int sum = PS - 1; sum >= 0; --sum)
+        for (int sum = PS - 1; sum >= 0; --sum)
 #pragma unroll
-                for (int p = sum; p >= 0; --p)
-                    c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
-                        __builtin_bit_cast(bf16x8, x[p]), __builtin_bit_cast(bf16x8, b[sum - p][ks]),
-                        c, 0, 0, 0);
-        }
+            for (int p = sum; p >= 0; --p) c = mfma<T>(x[p], b[sum - p][ks], c);
     }
     return c;
 }
 
-// Two values as bf16, to nearest even (v_cvt_pk_bf16_f32)
-__device__ __forceinline__ uint32_t pack_bf16(float x, float y) {
+// The planes of G's registers 8 s .. 8 s + 7 as B operands.  bf16: the first plane is cut off, so
+// the second starts from the exact rest; the second is rounded to nearest.  f16: both rounded to
+// nearest.
+template <int T>
+__device__ __forceinline__ void split_g(const float (&g)[16], int step, uint4 (&q)[2]) {
     using f32x2 = __attribute__((ext_vector_type(2))) float;
     using bf16x2 = __attribute__((ext_vector_type(2))) __bf16;
-    return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{x, y}), bf16x2));
-}
-// The planes of G's registers 8 s .. 8 s + 7 as B operands.  The leading planes are cut off, so the
-// next holds the rest exactly; of three planes the last has its 8 bits left and is cut too, of two
-// it is rounded to nearest.
-template <int GP>
-__device__ __forceinline__ void split_g(const float (&g)[16], int step, uint4 (&q)[GP]) {
-    uint32_t w[GP][4];
+    using f16x2 = __attribute__((ext_vector_type(2))) _Float16;
+    uint32_t w[2][4];
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-        float x = g[8 * step + 2 * e], y = g[8 * step + 2 * e + 1];
-#pragma unroll
-        for (int p = 0; p < GP; ++p) {
-            const uint32_t a = __float_as_uint(x), b = __float_as_uint(y);
-            w[p][e] = p == 1 && GP == 2 ? pack_bf16(x, y)
-                                        : __builtin_amdgcn_perm(b, a, 0x07060302u);
-            x -= __uint_as_float(a & 0xFFFF0000u);
-            y -= __uint_as_float(b & 0xFFFF0000u);
+        const f32x2 x = {g[8 * step + 2 * e], g[8 * step + 2 * e + 1]};
+        if constexpr (Planes<T>::HALF) {
+            const f16x2 hi = __builtin_convertvector(x, f16x2);
+            const f32x2 rest = {x[0] - (float)hi[0], x[1] - (float)hi[1]};
+            w[0][e] = __builtin_bit_cast(uint32_t, hi);
+            w[1][e] = __builtin_bit_cast(uint32_t, __builtin_convertvector(rest, f16x2));
+        } else {
+            const uint32_t a = __float_as_uint(x[0]), b = __float_as_uint(x[1]);
+            const f32x2 rest = {x[0] - __uint_as_float(a & 0xFFFF0000u),
+                                x[1] - __uint_as_float(b & 0xFFFF0000u)};
+            w[0][e] = __builtin_amdgcn_perm(b, a, 0x07060302u);
+            w[1][e] = __builtin_bit_cast(uint32_t, __builtin_convertvector(rest, bf16x2));
         }
     }
 #pragma unroll
-    for (int p = 0; p < GP; ++p) q[p] = make_uint4(w[p][0], w[p][1], w[p][2], w[p][3]);
+    for (int p = 0; p < 2; ++p) q[p] = make_uint4(w[p][0], w[p][1], w[p][2], w[p][3]);
+}
+
+// The power of two that a kept row's G and sums carry (f16 planes): |G| 2^e stays under 2^15.  Where
+// a larger |G| comes, the exponent drops to bring it into [2^13, 2^14) and the sums follow, exactly.
+// Both lanes of a row hold the same.
+struct Shift {
+    int32_t e = 100;
+    float f = 1.2676506e30f;  // 2^e
+};
+template <int T, int MT>
+__device__ __forceinline__ void scale_g(float (&g)[16], f32x16 (&acc)[MT], Shift& sh) {
+    if constexpr (Planes<T>::HALF) {
+        float most = fabsf(g[0]);
+#pragma unroll
+        for (int i = 1; i < 16; ++i) most = fmaxf(most, fabsf(g[i]));
+        most = both_max(most);
+        if (__any(most * sh.f > 32768.0f)) {
+            const int e = most * sh.f > 32768.0f ? 14 - __builtin_amdgcn_frexp_expf(most) : sh.e;
+            const float down = ldexpf(1.0f, max(e - sh.e, -126));
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) acc[mt][i] *= down;
+            sh.e = e;
+            sh.f = ldexpf(1.0f, e);
+        }
+#pragma unroll
+        for (int i = 0; i < 16; ++i) g[i] *= sh.f;
+    }
+}
+// What a sum is multiplied by in the end: the planes' scale 2^ex and G's undone
+template <int T>
+__device__ __forceinline__ float unscale(float x, const Shift& sh, int ex) {
+    return Planes<T>::HALF ? ldexpf(x, -sh.e - ex) : x;
 }
 
 // acc[mt] += A B for the MT tiles of 32 factors: A the transposed fragments, B the planes of G
@@ -413,7 +560,7 @@ __device__ __forceinline__ void grad_tile(const uint4* a, const float (&g)[16],
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
         uint4 q[P::GP];
-        split_g<P::GP>(g, s, q);
+        split_g<T>(g, s, q);
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt) {
             uint4 x[P::PG];
@@ -423,23 +570,22 @@ __device__ __forceinline__ void grad_tile(const uint4* a, const float (&g)[16],
             for (int sum = MAXSUM; sum >= 0; --sum)
 #pragma unroll
                 for (int p = P::PG - 1; p >= 0; --p)
-                    if (sum - p >= 0 && sum - p < P::GP)
-                        acc[mt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
-                            __builtin_bit_cast(bf16x8, x[p]), __builtin_bit_cast(bf16x8, q[sum - p]),
-                            acc[mt], 0, 0, 0);
+                    if (sum - p >= 0 && sum - p < P::GP) acc[mt] = mfma<T>(x[p], q[sum - p], acc[mt]);
         }
     }
 }
 
 __device__ __forceinline__ int reg_row(int i, int h) { return 8 * (i >> 2) + 4 * h + (i & 3); }
 
-// kGone where the bits (shifted right by 4 h) say so.  The empty asm keeps the compiler from taking
-// the selects out of their branch: 48 instructions for every tile against 200 for the tile itself.
-__device__ __forceinline__ void mask_tile(f32x16& c, uint32_t bits) {
+// `gone` where the bits (shifted right by 4 h) say so.  The empty asm keeps the compiler from taking
+// the selects out of their branch: 32 instructions for every tile against 110 for the tile itself.
+__device__ __forceinline__ void mask_tile(f32x16& c, uint32_t bits, float gone) {
     asm volatile("");
 #pragma unroll
-    for (int i = 0; i < 16; ++i)
-        if (bits >> reg_row(i, 0) & 1u) c[i] = kGone;
+    for (int i = 0; i < 16; ++i) {
+        const uint32_t on = (uint32_t)((int32_t)(bits << (31 - reg_row(i, 0))) >> 31);
+        c[i] = __uint_as_float((on & __float_as_uint(gone)) | (~on & __float_as_uint(c[i])));
+    }
 }
 
 // ------------------------------------------------------------------ forward
@@ -447,26 +593,33 @@ __device__ __forceinline__ void mask_tile(f32x16& c, uint32_t bits) {
 // shares each streamed tile.
 template <int T, int KT>
 constexpr int forward_waves() {
-    return Planes<T>::PS * KT > 24 ? 4 : 8;
+    return Planes<T>::PS * KT > 16 ? 4 : 8;
 }
+
+// Tiles staged at a time: up to 8 in 32 KB.  Fewer barriers, and between two of them the waves
+// drift apart, so that one's matrix work runs under another's exponentials.
+template <int T, int KT>
+constexpr int forward_tiles() {
+    constexpr int n = 32 / (Planes<T>::PS * KT);
+    return n >= 8 ? 8 : n >= 4 ? 4 : n >= 2 ? 2 : 1;
+}
+constexpr int kTileGroup = 8;  // the streamed items are padded to a multiple of so many tiles
 
 // A block's waves keep 32 users each and stream the item tiles of a split through LDS, TPS tiles a
 // turn in two buffers: the next turn's tiles are on the way while this one's are used.  Lane l: user
-// l % 32, 16 of a tile's 32 items.  m, l, w: the running maximum, sum of e = exp(s - m) and of e y,
-// y = log2 e.  The tiles' maxima gather in LDS and leave 32 at a time, a row's 128 bytes together.
+// l % 32, 16 of a tile's 32 items.  m, l, w: the running maximum (of scaled scores), the sum of
+// e = exp(s - m) and of e y, y = log2 e.
 template <int T, int KT, bool TOP>
 __global__ __launch_bounds__((forward_waves<T, KT>() * 64)) void softmax_forward_kernel(Job j) {
-    constexpr int PS = Planes<T>::PS, WAVES = forward_waves<T, KT>();
-    constexpr int TPS = PS * KT < 8 ? 8 / (PS * KT) : 1;
+    constexpr int PS = Planes<T>::PS, WAVES = forward_waves<T, KT>(), TPS = forward_tiles<T, KT>();
     __shared__ uint4 buf[2][TPS * PS * KT * 64];
     __shared__ f32x4 bias[2][TPS * 8];
-    __shared__ float tmax[TOP ? WAVES : 1][TOP ? 32 * 33 : 1];
     const int lane = threadIdx.x & 63, h = lane >> 5, wave = threadIdx.x >> 6;
     const int split = blockIdx.x % j.splits;
     const int64_t ut = (int64_t)(blockIdx.x / j.splits) * WAVES + wave;
     // A wave behind the last tile of users does tile 0's work and drops it: a branch around the work
     // costs the others more (the accumulators change registers at it).
-    const bool mine = ut < j.u.tiles;  // as in the forward pass
+    const bool mine = ut < j.u.tiles;
     const int64_t row = (mine ? ut : 0) * 32 + (lane & 31);
     uint4 b[PS][KT];
 #pragma unroll
@@ -474,27 +627,52 @@ __global__ __launch_bounds__((forward_waves<T, KT>() * 64)) void softmax_forward
 #pragma unroll
         for (int ks = 0; ks < KT; ++ks)
             b[p][ks] = j.u.frag[(((mine ? ut : 0) * PS + p) * KT + ks) * 64 + lane];
-    const int t0 = (int)((int64_t)j.v.tiles * split / j.splits);
-    const int t1 = (int)((int64_t)j.v.tiles * (split + 1) / j.splits);
+    const int t0 = (int)((int64_t)(j.v.tiles / TPS) * split / j.splits) * TPS;
+    const int t1 = (int)((int64_t)(j.v.tiles / TPS) * (split + 1) / j.splits) * TPS;
     const auto load = [&](int tl, int at) {
-        const int n = min(TPS, t1 - tl);
-        stage<WAVES>(j.v.frag + (int64_t)tl * PS * KT * 64, buf[at], n * PS * KT);
-        if (wave == WAVES - 1 && lane < n * 8)  // n * 32 floats
-            __builtin_amdgcn_global_load_lds(
-                (const __attribute__((address_space(1))) void*)((const f32x4*)j.vbias + tl * 8 +
-                                                                lane),
-                (__attribute__((address_space(3))) void*)bias[at], 16, 0, 0);
+        stage<WAVES>(j.v.frag + (int64_t)tl * PS * KT * 64, buf[at], TPS * PS * KT);
+        if (wave == WAVES - 1 && lane < TPS * 8)  // TPS * 32 floats
+            copy_to_lds((const f32x4*)j.vbias + tl * 8 + lane, bias[at]);
     };
-    float m = kFloor, l = 0.0f, w = 0.0f;
-    uint32_t next_bits = j.mask && t0 < t1 ? j.mask[(int64_t)t0 * j.rows_pad + row] : 0;
-    if (t0 < t1) load(t0, 0);
+    const Scale sc = *j.scale;
+    float m = sc.floor, l = 0.0f, w = 0.0f, mx[TPS];
+    uint32_t bits[TPS] = {}, next[TPS] = {};
+    const auto load_bits = [&](int tl) {
+#pragma unroll
+        for (int x = 0; x < TPS; ++x) next[x] = j.mask[(int64_t)(tl + x) * j.rows_pad + row];
+    };
+    // a turn's maxima leave in the next turn, so that no wait meets the stores
+    const auto store_max = [&](int tl) {
+        if (!TOP || h || !mine) return;
+        float* p = j.cmax + row * j.cpad + tl;
+        if constexpr (TPS >= 4) {
+#pragma unroll
+            for (int x = 0; x < TPS; x += 4)
+                *(f32x4*)(p + x) = f32x4{mx[x], mx[x + 1], mx[x + 2], mx[x + 3]};
+        } else {
+#pragma unroll
+            for (int x = 0; x < TPS; ++x) p[x] = mx[x];
+        }
+    };
+    if (t0 < t1) {
+        load(t0, 0);
+        if (j.mask) load_bits(t0);
+    }
     for (int ts = t0, at = 0; ts < t1; ts += TPS, at ^= 1) {
         stage_wait();
-        if (ts + TPS < t1) load(ts + TPS, at ^ 1);
-        for (int x = 0; x < TPS && ts + x < t1; ++x) {
-            const int tl = ts + x;
-            const uint32_t bits = next_bits >> (4 * h);
-            if (j.mask && tl + 1 < t1) next_bits = j.mask[(int64_t)(tl + 1) * j.rows_pad + row];
+#pragma unroll
+        for (int x = 0; x < TPS; ++x) {
+            // the wait for this load belongs before the next copies, not behind them
+            asm volatile("" : "+v"(next[x]));
+            bits[x] = next[x] >> (4 * h);
+        }
+        if (ts + TPS < t1) {
+            load(ts + TPS, at ^ 1);
+            if (j.mask) load_bits(ts + TPS);
+        }
+        if (ts > t0) store_max(ts - TPS);
+#pragma unroll
+        for (int x = 0; x < TPS; ++x) {
             f32x16 c;
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
@@ -503,37 +681,23 @@ __global__ __launch_bounds__((forward_waves<T, KT>() * 64)) void softmax_forward
                 for (int e = 0; e < 4; ++e) c[4 * q + e] = v[e];
             }
             c = score_tile<T, KT>(buf[at] + x * PS * KT * 64, b, c, lane);
-            if (__any(bits & 0x0F0F0F0Fu)) mask_tile(c, bits);
+            if (__any(bits[x] & 0x0F0F0F0Fu)) mask_tile(c, bits[x], sc.gone);
             float mt = c[0];
 #pragma unroll
             for (int i = 1; i < 16; ++i) mt = fmaxf(mt, c[i]);
-            if constexpr (TOP) {
-                const float both = fmaxf(mt, __shfl_xor(mt, 32));
-                if (h == 0) tmax[wave][lane * 33 + (tl & 31)] = both;
-                if ((tl & 31) == 31 || tl + 1 == t1) {  // 32 tiles, or the split's ends
-                    const int first = max(t0, tl & ~31);
-                    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-                    const int col = lane & 31;
-                    const bool in = mine && col >= (first & 31) && col <= (tl & 31);
-                    for (int r = h; r < 32; r += 2)
-                        if (in)
-                            j.cmax[(ut * 32 + r) * j.cpad + (tl & ~31) + col] =
-                                tmax[wave][r * 33 + col];
-                    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-                }
-            }
+            if constexpr (TOP) mx[x] = both_max(mt);
             if (__any(mt > m)) {
-                const float mn = fmaxf(m, mt), d = (m - mn) * kLog2e;
+                const float mn = fmaxf(m, mt), d = (m - mn) * sc.kappa;
                 const float f = __builtin_amdgcn_exp2f(d);
                 w = f * fmaf(l, d, w);
                 l *= f;
                 m = mn;
             }
-            const float m2 = m * kLog2e;
+            const float m2 = m * sc.kappa;
             float sl = 0.0f, sw = 0.0f;
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
-                const float y = fmaf(c[i], kLog2e, -m2), e = __builtin_amdgcn_exp2f(y);
+                const float y = fmaf(c[i], sc.kappa, -m2), e = __builtin_amdgcn_exp2f(y);
                 sl += e;
                 sw = fmaf(e, y, sw);
             }
@@ -541,9 +705,10 @@ __global__ __launch_bounds__((forward_waves<T, KT>() * 64)) void softmax_forward
             w += sw;
         }
     }
+    if (t0 < t1) store_max(t1 - TPS);
     if (!mine) return;
     // the halves' states joined: lanes l and l + 32 hold the same user
-    const float mo = __shfl_xor(m, 32), mn = fmaxf(m, mo), d = (m - mn) * kLog2e;
+    const float mn = both_max(m), d = (m - mn) * sc.kappa;
     const float f = __builtin_amdgcn_exp2f(d);
     w = f * fmaf(l, d, w);
     l *= f;
@@ -591,7 +756,7 @@ __device__ __forceinline__ double exact_score(const Job& j, const float* u, int6
     return a + (j.bias ? (double)j.bias[i] : 0.0);
 }
 __device__ __forceinline__ bool is_excluded(const Job& j, int64_t r, int64_t i) {
-    return j.vbias[i] <= kGone ||
+    return j.vbias[i] <= j.scale->gone ||
            (j.mask && (j.mask[(i >> 5) * j.rows_pad + r] >> (i & 31) & 1u));
 }
 // A double as an unsigned key in the same order (-inf is the smallest that occurs)
@@ -697,7 +862,8 @@ __global__ __launch_bounds__(TOP ? 256 : 64) void softmax_finish_kernel(Job j) {
     const int64_t u = source_row(j.u, r);
     for (int f = t; f < j.k; f += NT)
         urow[f] = u >= 0 ? load_factor<T>(j.u.src, u * j.u.ld + f) : 0.0f;
-    float m = kFloor;
+    const Scale sc = *j.scale;
+    float m = sc.floor;
     for (int s = t; s < j.splits; s += NT) m = fmaxf(m, j.part[(int64_t)s * 3 * j.rows_pad + r]);
 #pragma unroll
     for (int d = 32; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor(m, d));
@@ -709,7 +875,7 @@ __global__ __launch_bounds__(TOP ? 256 : 64) void softmax_finish_kernel(Job j) {
     double l = 0.0, w = 0.0;
     for (int s = t; s < j.splits; s += NT) {
         const float* p = j.part + (int64_t)s * 3 * j.rows_pad + r;
-        const double d = ((double)p[0] - m) * 1.4426950408889634;
+        const double d = ((double)p[0] - m) * sc.unit * 1.4426950408889634;
         const double f = exp2(d);
         w += f * ((double)p[2 * j.rows_pad] + (double)p[j.rows_pad] * d);
         l += f * p[j.rows_pad];
@@ -727,8 +893,8 @@ __global__ __launch_bounds__(TOP ? 256 : 64) void softmax_finish_kernel(Job j) {
     } else {
         __syncthreads();
     }
-    const bool empty = m <= kFloor && l == l;
-    double lse = (double)m + log(l), H = log(l) - 0.69314718055994531 * w / l;
+    const bool empty = m <= sc.floor && l == l;
+    double lse = (double)m * sc.unit + log(l), H = log(l) - 0.69314718055994531 * w / l;
     if (empty) lse = -INFINITY, H = 0.0;
     if (j.ubad[r]) lse = H = __builtin_nan("");
     if (t < 64) {
@@ -838,16 +1004,15 @@ __global__ __launch_bounds__(grad_waves<KT>() * 64) void softmax_grad_users_kern
         for (int ks = 0; ks < KT; ++ks)
             b[p][ks] = j.u.frag[(((mine ? ut : 0) * PS + p) * KT + ks) * 64 + lane];
     const RowMeta mr = j.meta[row];
+    const Scale sc = *j.scale;
+    Shift sh;
     f32x16 acc[MT] = {};
     const int t0 = (int)((int64_t)j.v.tiles * split / j.splits);
     const int t1 = (int)((int64_t)j.v.tiles * (split + 1) / j.splits);
     const auto load = [&](int tl) {
         stage<WAVES>(j.v.frag + (int64_t)tl * NS * 64, sbuf, NS);
         if (wave == WAVES - 1 && lane < 8)
-            __builtin_amdgcn_global_load_lds(
-                (const __attribute__((address_space(1))) void*)((const f32x4*)j.vbias + tl * 8 +
-                                                                lane),
-                (__attribute__((address_space(3))) void*)bias[tl & 1], 16, 0, 0);
+            copy_to_lds((const f32x4*)j.vbias + tl * 8 + lane, bias[tl & 1]);
     };
     if (t0 < t1) load(t0);
     for (int tl = t0; tl < t1; ++tl) {
@@ -864,17 +1029,22 @@ __global__ __launch_bounds__(grad_waves<KT>() * 64) void softmax_grad_users_kern
             for (int e = 0; e < 4; ++e) c[4 * q + e] = v[e];
         }
         c = score_tile<T, KT>(sbuf, b, c, lane);
-        if (__any(bits & 0x0F0F0F0Fu)) mask_tile(c, bits);
+        if (__any(bits & 0x0F0F0F0Fu)) mask_tile(c, bits, sc.gone);
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-            const float x = fmaf(c[i], kLog2e, -mr.lse2);
+            const float x = fmaf(c[i], sc.kappa, -mr.lse2);
             g[i] = -__builtin_amdgcn_exp2f(x) * fmaf(mr.c1, x, mr.c0);
         }
         stage_wait();
         if (tl + 1 < t1) load(tl + 1);
+        scale_g<T, MT>(g, acc, sh);
         grad_tile<T, KT>(tbuf, g, acc, lane);
     }
     if (!mine) return;
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) acc[mt][i] = unscale<T>(acc[mt][i], sh, sc.ev);
     float* out = j.du_part + ((int64_t)split * j.rows_pad + row) * KP;
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt)
@@ -905,6 +1075,8 @@ __global__ __launch_bounds__(grad_waves<KT>() * 64) void softmax_grad_items_kern
         for (int ks = 0; ks < KT; ++ks)
             b[p][ks] = j.v.frag[(((mine ? vt : 0) * PS + p) * KT + ks) * 64 + lane];
     const float bias = j.vbias[item];
+    const Scale sc = *j.scale;
+    Shift sh;
     f32x16 acc[MT] = {};
     float db = 0.0f;
     const int t0 = (int)((int64_t)j.u.tiles * split / j.vsplits);
@@ -912,10 +1084,7 @@ __global__ __launch_bounds__(grad_waves<KT>() * 64) void softmax_grad_items_kern
     const auto load = [&](int tl) {
         stage<WAVES>(j.u.frag + (int64_t)tl * NS * 64, sbuf, NS);
         if (wave == WAVES - 1 && lane < 32)
-            __builtin_amdgcn_global_load_lds(
-                (const __attribute__((address_space(1))) void*)((const uint4*)j.meta + tl * 32 +
-                                                                lane),
-                (__attribute__((address_space(3))) void*)mbuf[tl & 1], 16, 0, 0);
+            copy_to_lds((const uint4*)j.meta + tl * 32 + lane, mbuf[tl & 1]);
     };
     if (t0 < t1) load(t0);
     for (int tl = t0; tl < t1; ++tl) {
@@ -933,13 +1102,13 @@ __global__ __launch_bounds__(grad_waves<KT>() * 64) void softmax_grad_items_kern
             asm volatile("");  // as in mask_tile
 #pragma unroll
             for (int i = 0; i < 16; ++i)
-                if (__shfl((int)word, reg_row(i, h)) >> (lane & 31) & 1) c[i] = kGone;
+                if (__shfl((int)word, reg_row(i, h)) >> (lane & 31) & 1) c[i] = sc.gone;
         }
         float sum = 0.0f;
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
             const RowMeta mr = meta[reg_row(i, h)];
-            const float x = fmaf(c[i], kLog2e, -mr.lse2);
+            const float x = fmaf(c[i], sc.kappa, -mr.lse2);
             g[i] = -__builtin_amdgcn_exp2f(x) * fmaf(mr.c1, x, mr.c0);
         }
         if (__any(meta[lane & 31].t >> 5 == (int32_t)vt)) {
@@ -953,11 +1122,16 @@ __global__ __launch_bounds__(grad_waves<KT>() * 64) void softmax_grad_items_kern
         db += sum;
         stage_wait();
         if (tl + 1 < t1) load(tl + 1);
+        scale_g<T, MT>(g, acc, sh);
         grad_tile<T, KT>(tbuf, g, acc, lane);
     }
     if (!mine) return;
     const int64_t items_pad = (int64_t)j.v.tiles * 32;
     db += __shfl_xor(db, 32);
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) acc[mt][i] = unscale<T>(acc[mt][i], sh, sc.eu);
     if (j.vsplits == 1) {  // nothing to join: the result itself
         if (item >= j.n_items) return;
         if (h == 0) j.gb[item] = db;
@@ -1046,8 +1220,7 @@ void check_args(const mml_item_softmax_args* a) {
 // The launch's numbers and its arrays in the workspace at `base` (nullptr: sizes only).
 int64_t plan(const mml_item_softmax_args* a, bool grad, void* base, Job& j) {
     const int T = a->dtype, kt = steps_of(a->num_factors), mt = kt > 1 ? kt / 2 : 1;
-    const int ps = T == MML_DTYPE_F32 ? 3 : 1;
-    const int pg = T == MML_DTYPE_F32 ? 3 : T == MML_DTYPE_F16 ? 2 : 1;
+    const int ps = T == MML_DTYPE_F32 ? 2 : 1, pg = ps;
     j = Job{};
     j.k = a->num_factors;
     j.n_items = a->n_items;
@@ -1056,7 +1229,9 @@ int64_t plan(const mml_item_softmax_args* a, bool grad, void* base, Job& j) {
     j.u = Side{a->user_factors, a->ld_users, a->users, a->n_users, a->n_rows,
                (int32_t)((a->n_rows + 31) / 32), nullptr, nullptr, 0};
     j.v = Side{a->item_factors, a->ld_items, nullptr, a->n_items, a->n_items,
-               (int32_t)(((int64_t)a->n_items + 31) / 32), nullptr, nullptr, 0};
+               (int32_t)(((int64_t)a->n_items + 32 * kTileGroup - 1) / (32 * kTileGroup) *
+                         kTileGroup),
+               nullptr, nullptr, 0};
     const int size = T == MML_DTYPE_F32 ? 4 : 2;
     j.u.vec8 = (uintptr_t)a->user_factors % 16 == 0 && a->ld_users * size % 16 == 0;
     j.v.vec8 = (uintptr_t)a->item_factors % 16 == 0 && a->ld_items * size % 16 == 0;
@@ -1080,6 +1255,8 @@ int64_t plan(const mml_item_softmax_args* a, bool grad, void* base, Job& j) {
     j.splits = splits(j.u.tiles, j.v.tiles);
     j.vsplits = splits(j.v.tiles, j.u.tiles);
     Carve c{(char*)base};
+    j.scale = c.take<Scale>(1);
+    if (T == MML_DTYPE_F32) j.parts = c.take<float>(kMaxParts);
     j.u.frag = c.take<uint4>((int64_t)j.u.tiles * ps * kt * 64);
     j.v.frag = c.take<uint4>((int64_t)j.v.tiles * ps * kt * 64);
     j.vbias = c.take<float>(items_pad);
@@ -1087,7 +1264,7 @@ int64_t plan(const mml_item_softmax_args* a, bool grad, void* base, Job& j) {
     if (a->exclude_offsets) j.mask = c.take<uint32_t>((int64_t)j.v.tiles * j.rows_pad);
     if (!grad) {
         j.part = c.take<float>((int64_t)j.splits * 3 * j.rows_pad);
-        j.cpad = (j.v.tiles + 31) / 32 * 32;
+        j.cpad = j.v.tiles;
         if (j.n_top) j.cmax = c.take<float>(j.rows_pad * j.cpad);
     } else {
         j.u.trans = c.take<uint4>((int64_t)j.u.tiles * pg * mt * 128);
@@ -1133,6 +1310,7 @@ void mask_and_prep(const Job& j, int T, hipStream_t st) {
             j.mask, words);
         softmax_mask_kernel<<<grid_of((j.n_rows + 3) / 4), 256, 0, st>>>(j);
     }
+    if (T == MML_DTYPE_F32) softmax_max_kernel<MML_DTYPE_F32><<<kMaxParts, 256, 0, st>>>(j);
     dispatch(T, steps_of(j.k), [&](auto tt, auto kt) {
         softmax_prep_kernel<decltype(tt)::value, decltype(kt)::value>
             <<<grid_of((int64_t)j.u.tiles + j.v.tiles), 256, 0, st>>>(j);

@@ -2,14 +2,18 @@
 bits.
 
 Tolerances.  With A_r = max_j (sum_f |u_f v_jf| + |b_j|) a score is off by at most
-(4 + 12 KT + 8) 2^-24 A_r: 4 for the three-plane split of both factors and the dropped products, two
-roundings for each of the 6 KT accumulations (KT = steps of 16 factors), 8 for the bias and the
-product with log2 e.  The log normaliser adds the roundings of the exponents (|y| <= 64 where e
+(12 + 12 KT + 8) 2^-24 A_r: f32 factors are split into two f16 planes, hi off by 2^-11, lo (below
+2^-11 of the value) by 2^-11 of itself, so a factor is off by 2^-22 = 4 units of 2^-24, two factors by
+8, the dropped lo lo is 4 more; two roundings for each of at most 6 KT accumulations (KT = steps of 16
+factors); 8 for the bias and the product with log2 e.  The planes are scaled to a largest magnitude
+of 2^12 at least and end at 2^-25 (half the smallest f16): 2^-37 of the matrix' largest value, for each
+of the k products and both factors, is lost below.  The log normaliser adds the roundings of the exponents (|y| <= 64 where e
 counts) and of the sum (one per tile and 16 within).  Half-precision factors are exact operands, so
 the bound holds for them too.  An entropy moves by 2 d (H + 1) for a change d of every log p, and
 its sum rounds as the normaliser's: 4 d (H + 1).
 Gradients: G is off by 4 d |G|-like terms (G's parts taken with their magnitudes), each product's
-split by 4 x 2^-24 (f32) or 2^-16 (G in two planes), and every accumulated step rounds twice.  What
+split by 12 x 2^-24 as above (f32) or 2^-16 (G in two planes), every accumulated step rounds twice, and
+G's planes lose 2^-37 of the largest |G| of the kept row, for each element of the sum.  What
 is returned in half precision is off by half a step, finfo.eps / 2, more.
 """
 import numpy as np
@@ -106,15 +110,17 @@ def reference(d, n_top=0, g_lp=None, g_ent=None):
         mag = np.abs(delta) + np.abs(w)[:, None] * p + np.abs(h)[:, None] * p * (
             np.abs(lz) + H[:, None] + 1)
         out.update(gu=G @ Vz, gv=G.T @ u, gb=G.sum(0), mag=mag, magu=mag @ np.abs(Vz),
-                   magv=mag.T @ np.abs(u), magb=mag.sum(0))
+                   magv=mag.T @ np.abs(u), magb=mag.sum(0),
+                   sumv=np.abs(Vz).sum(0), sumu=np.abs(np.where(np.isfinite(u), u, 0)).sum(0))
     return out
 
 
 def tol_score(d, ref):
     k, n = d["V"].shape[1], d["V"].shape[0]
     tiles = -(-n // 32)
-    return EPS * ((4 + 12 * steps(k) + 8) * ref["A"] + 64 + tiles + 16
-                  + 4 * np.abs(np.where(np.isfinite(ref["lse"]), ref["lse"], 0)))
+    top = lambda x: float(x[torch.isfinite(x).all(1)].abs().max().double())
+    return EPS * ((12 + 12 * steps(k) + 8) * ref["A"] + 64 + tiles + 16
+                  + 2 * 2.0 ** -13 * k * top(d["U"]) * top(d["V"]) + 4 * np.abs(np.where(np.isfinite(ref["lse"]), ref["lse"], 0)))
 
 
 def to_gpu(d):
@@ -157,7 +163,7 @@ def check_forward(d, r, n_top=0, ref=None):
 def check_backward(d, got, ref):
     k, n, R = d["V"].shape[1], d["V"].shape[0], len(ref["lse"])
     tol = tol_score(d, ref)
-    split = 4 * EPS if d["U"].dtype == F32 else 2.0 ** -16
+    split = 12 * EPS if d["U"].dtype == F32 else 2.0 ** -16
     half = 0.0 if d["U"].dtype == F32 else torch.finfo(d["U"].dtype).eps / 2
     tiny = 0.0 if d["U"].dtype != F16 else 2.0 ** -25  # half the smallest f16
     gu, gv, gb = got
@@ -168,11 +174,14 @@ def check_backward(d, got, ref):
     lost = 2.0 ** -118
     lost_u = lost * n * float(d["V"][torch.isfinite(d["V"]).all(1)].abs().max().double())
     lost_v = lost * R * float(d["U"].abs().max().double())
+    fine = 2.0 ** -37 * ref["mag"]
+    below_u = fine.max(1)[:, None] * ref["sumv"]
+    below_v = fine.max(0)[:, None] * ref["sumu"]
     acc = lambda m: 24 * -(-m // 32) * EPS  # 2 steps x 6 products x 2 roundings per tile
     near(gu, ref["gu"], ref["magu"] * (4 * tol[:, None] + split + acc(n) + 64 * EPS)
-         + half * np.abs(ref["gu"]) + tiny + lost_u)
+         + half * np.abs(ref["gu"]) + tiny + lost_u + below_u)
     near(gv, ref["gv"], ref["magv"] * (4 * tol.max() + split + acc(R) + 64 * EPS)
-         + half * np.abs(ref["gv"]) + tiny + lost_v)
+         + half * np.abs(ref["gv"]) + tiny + lost_v + below_v)
     near(gb, ref["gb"], ref["magb"] * (4 * tol.max() + (R + 64) * EPS) + lost * R)
 
 
