@@ -121,13 +121,11 @@ struct Side {  // one factor matrix as fragments
     int32_t vec8;          // the rows begin at multiples of 16 bytes
 };
 
-struct RowMeta {  // per row of the users' side, gradient only
-    float lse2;   // lse * log2 e; 1e30 for a row without a gradient (p = 0)
-    float c0, c1; // G = -p (c0 + c1 x) + [j = t] w,  x = log2 p
-    int32_t t;    // the given item, -1: none
+struct RowMeta {  // per tile of the users' side, gradient only
+    float lse2[32];   // lse * log2 e; 1e30 for a row without a gradient (p = 0)
+    float c0[32], c1[32];  // G = p (c0 + c1 x) + [j = t] w,  x = log2 p
+    int32_t t[32];    // the given item, -1: none
 };
-
-static_assert(sizeof(RowMeta) == 16, "staged 16 bytes per lane");
 
 // Powers of two that the planes are scaled by (f32 factors; otherwise 1), so scores come out of the
 // matrix cores as s 2^(eu + ev), and what follows from them.  Written by the preparation.
@@ -168,7 +166,7 @@ struct Job {
     int32_t* top_items;
     // gradient
     const float *in_norm, *in_entropy, *g_lp, *g_ent;
-    RowMeta* meta;  // [rows_pad]
+    RowMeta* meta;  // [u.tiles]
     float* w;       // [rows_pad]
     float *du_part, *dv_part, *db_part;
     int32_t vsplits;
@@ -407,7 +405,8 @@ __global__ __launch_bounds__(256) void softmax_prep_kernel(Job j) {
 __global__ __launch_bounds__(256) void softmax_meta_kernel(Job j) {
     const int64_t r = (int64_t)blockIdx.x * 256 + threadIdx.x;
     if (r >= j.rows_pad) return;
-    RowMeta m{1e30f, 0.0f, 0.0f, -1};
+    float lse2 = 1e30f, c0 = 0.0f, c1 = 0.0f;
+    int32_t given = -1;
     float w = 0.0f;
     if (r < j.n_rows && j.ubad[r] < 2) {
         const float lse = j.in_norm[r], h = j.g_ent ? j.g_ent[r] : 0.0f;
@@ -418,12 +417,19 @@ __global__ __launch_bounds__(256) void softmax_meta_kernel(Job j) {
         w = t >= 0 && j.g_lp ? j.g_lp[r] : 0.0f;
         if ((w != 0.0f || h != 0.0f) && lse != -INFINITY) {
             const float H = h != 0.0f ? j.in_entropy[r] : 0.0f;
-            m = RowMeta{j.ubad[r] ? __builtin_nanf("") : lse * kLog2e, w + h * H, h * kLn2, t};
+            lse2 = j.ubad[r] ? __builtin_nanf("") : lse * kLog2e;
+            c0 = -(w + h * H);
+            c1 = -h * kLn2;
+            given = t;
         } else {
             w = 0.0f;
         }
     }
-    j.meta[r] = m;
+    RowMeta& m = j.meta[r >> 5];
+    m.lse2[r & 31] = lse2;
+    m.c0[r & 31] = c0;
+    m.c1[r & 31] = c1;
+    m.t[r & 31] = given;
     j.w[r] = w;
 }
 
@@ -469,23 +475,45 @@ __device__ __forceinline__ float both_max(float x) {
                                                     false);
     return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
 }
-// c + A B over the PS planes of KT steps (smallest products first).  A: fragments in LDS.
-template <int T, int KT>
+// c + A B over the PS planes of KT steps (smallest products first).  A: fragments in LDS; B: the kept
+// side's fragments in registers, the last LK steps' in LDS.
+template <int T, int KT, int LK>
 __device__ __forceinline__ f32x16 score_tile(const uint4* a,
-                                             const uint4 (&b)[Planes<T>::PS][KT], f32x16 c,
-                                             int lane) {
+                                             const uint4 (&b)[Planes<T>::PS][KT - LK],
+                                             const uint4* kept, f32x16 c, int lane) {
     constexpr int PS = Planes<T>::PS;
 #pragma unroll
     for (int ks = 0; ks < KT; ++ks) {
-        uint4 x[PS];
+        uint4 x[PS], y[PS];
 #pragma unroll
-        for (int p = 0; p < PS; ++p) x[p] = a[(p * KT + ks) * 64 + lane];
+        for (int p = 0; p < PS; ++p) {
+            x[p] = a[(p * KT + ks) * 64 + lane];
+            y[p] = ks < KT - LK ? b[p][ks < KT - LK ? ks : 0]
+                                : kept[(p * LK + ks - (KT - LK)) * 64 + lane];
+        }
 #pragma unroll
         for (int sum = PS - 1; sum >= 0; --sum)
 #pragma unroll
-            for (int p = sum; p >= 0; --p) c = mfma<T>(x[p], b[sum - p][ks], c);
+            for (int p = sum; p >= 0; --p) c = mfma<T>(x[p], y[sum - p], c);
     }
     return c;
+}
+// The kept side's fragments of tile `tl`
+template <int T, int KT, int LK>
+__device__ __forceinline__ void load_kept(const uint4* __restrict__ frag, int64_t tl,
+                                          uint4 (&b)[Planes<T>::PS][KT - LK], uint4* kept,
+                                          int lane) {
+    constexpr int PS = Planes<T>::PS;
+#pragma unroll
+    for (int p = 0; p < PS; ++p)
+#pragma unroll
+        for (int ks = 0; ks < KT; ++ks) {
+            const uint4 x = frag[((tl * PS + p) * KT + ks) * 64 + lane];
+            if (ks < KT - LK)
+                b[p][ks < KT - LK ? ks : 0] = x;
+            else
+                kept[(p * LK + ks - (KT - LK)) * 64 + lane] = x;
+        }
 }
 
 // The planes of G's registers 8 s .. 8 s + 7 as B operands.  bf16: the first plane is cut off, so
@@ -497,12 +525,14 @@ __device__ __forceinline__ void split_g(const float (&g)[16], int step, uint4 (&
     using bf16x2 = __attribute__((ext_vector_type(2))) __bf16;
     using f16x2 = __attribute__((ext_vector_type(2))) _Float16;
     uint32_t w[2][4];
+    float minus = -1.0f;  // unknown to the compiler, so that x - hi is one v_fma_mix_f32
+    asm("" : "+s"(minus));
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
         const f32x2 x = {g[8 * step + 2 * e], g[8 * step + 2 * e + 1]};
         if constexpr (Planes<T>::HALF) {
             const f16x2 hi = __builtin_convertvector(x, f16x2);
-            const f32x2 rest = {x[0] - (float)hi[0], x[1] - (float)hi[1]};
+            const f32x2 rest = {fmaf((float)hi[0], minus, x[0]), fmaf((float)hi[1], minus, x[1])};
             w[0][e] = __builtin_bit_cast(uint32_t, hi);
             w[1][e] = __builtin_bit_cast(uint32_t, __builtin_convertvector(rest, f16x2));
         } else {
@@ -622,11 +652,7 @@ __global__ __launch_bounds__((forward_waves<T, KT>() * 64)) void softmax_forward
     const bool mine = ut < j.u.tiles;
     const int64_t row = (mine ? ut : 0) * 32 + (lane & 31);
     uint4 b[PS][KT];
-#pragma unroll
-    for (int p = 0; p < PS; ++p)
-#pragma unroll
-        for (int ks = 0; ks < KT; ++ks)
-            b[p][ks] = j.u.frag[(((mine ? ut : 0) * PS + p) * KT + ks) * 64 + lane];
+    load_kept<T, KT, 0>(j.u.frag, mine ? ut : 0, b, nullptr, lane);
     const int t0 = (int)((int64_t)(j.v.tiles / TPS) * split / j.splits) * TPS;
     const int t1 = (int)((int64_t)(j.v.tiles / TPS) * (split + 1) / j.splits) * TPS;
     const auto load = [&](int tl, int at) {
@@ -680,7 +706,7 @@ __global__ __launch_bounds__((forward_waves<T, KT>() * 64)) void softmax_forward
 #pragma unroll
                 for (int e = 0; e < 4; ++e) c[4 * q + e] = v[e];
             }
-            c = score_tile<T, KT>(buf[at] + x * PS * KT * 64, b, c, lane);
+            c = score_tile<T, KT, 0>(buf[at] + x * PS * KT * 64, b, nullptr, c, lane);
             if (__any(bits[x] & 0x0F0F0F0Fu)) mask_tile(c, bits[x], sc.gone);
             float mt = c[0];
 #pragma unroll
@@ -977,33 +1003,54 @@ __global__ __launch_bounds__(TOP ? 256 : 64) void softmax_finish_kernel(Job j) {
 
 // ------------------------------------------------------------------ gradient
 // Both kernels stage a tile's score fragments in one LDS buffer and its transposed ones in another:
-// while one is used, the other is on the way, with a barrier between.  Waves of a block: 4 where
-// the accumulators (8 x 16) and the kept side fill half of the registers.
-template <int KT>
-constexpr int grad_waves() {
-    return KT > 8 ? 4 : 8;
+// while one is used, the other is on the way, with a barrier between.  A block's waves share the
+// streamed tile, and other blocks' waves fill the time at the barriers.  Waves of a block and waves
+// per SIMD that the registers are held down to, measured (2048 x 100k, k = 64 f32; 1001 x 30k, k = 100
+// f16; 1024 x 500k, k = 256 bf16): users 156 us with 8 and 4 against 199 with 8 and 2; items 206 with
+// 4 and 3 against 236 with 8 and 4, which spills (a reload waits for the copies on the way); k > 128:
+// users 729 with 4 and 2 against 1,221 with 4 and 1.
+template <int T, int KT>
+constexpr int users_waves() {
+    return KT > 4 ? 4 : 8;
+}
+template <int T, int KT>
+constexpr int users_per_simd() {
+    return KT <= 4 ? 4 : KT <= 8 || T != MML_DTYPE_F32 ? 2 : 1;
+}
+// Steps of the kept fragments that stay in LDS, so that nothing is spilled at those waves per SIMD
+template <int T, int KT>
+constexpr int users_in_lds() {
+    return KT == 4 && T == MML_DTYPE_F32 ? 1 : KT == 16 && T == MML_DTYPE_F16 ? 4 : 0;
+}
+constexpr int kItemsWaves = 4;
+template <int T, int KT>
+constexpr int items_per_simd() {
+    return KT <= 4 || (KT == 8 && T != MML_DTYPE_F32) ? 3 : KT == 8 || T != MML_DTYPE_F32 ? 2 : 1;
+}
+template <int T, int KT>
+constexpr int items_in_lds() {
+    return T == MML_DTYPE_F32 ? 0 : KT == 8 ? 3 : KT == 16 ? (T == MML_DTYPE_F16 ? 8 : 6) : 0;
 }
 
 // Users' side: as the forward pass, G in place of the softmax state, dU += G V.
 template <int T, int KT>
-__global__ __launch_bounds__(grad_waves<KT>() * 64) void softmax_grad_users_kernel(Job j) {
+__global__ __launch_bounds__((users_waves<T, KT>() * 64), (users_per_simd<T, KT>())) void
+softmax_grad_users_kernel(Job j) {
     using P = Planes<T>;
-    constexpr int PS = P::PS, MT = KT > 1 ? KT / 2 : 1, KP = MT * 32, WAVES = grad_waves<KT>();
+    constexpr int PS = P::PS, MT = KT > 1 ? KT / 2 : 1, KP = MT * 32, WAVES = users_waves<T, KT>();
     constexpr int NS = PS * KT, NT = P::PG * MT * 2;  // KB of score and of transposed fragments
-    __shared__ uint4 sbuf[NS * 64], tbuf[NT * 64];
+    constexpr int LK = users_in_lds<T, KT>();
+    __shared__ uint4 sbuf[NS * 64], tbuf[NT * 64], kept[WAVES][LK ? PS * LK * 64 : 1];
     __shared__ f32x4 bias[2][8];
     const int lane = threadIdx.x & 63, h = lane >> 5, wave = threadIdx.x >> 6;
     const int split = blockIdx.x % j.splits;
     const int64_t ut = (int64_t)(blockIdx.x / j.splits) * WAVES + wave;
     const bool mine = ut < j.u.tiles;  // as in the forward pass
     const int64_t row = (mine ? ut : 0) * 32 + (lane & 31);
-    uint4 b[PS][KT];
-#pragma unroll
-    for (int p = 0; p < PS; ++p)
-#pragma unroll
-        for (int ks = 0; ks < KT; ++ks)
-            b[p][ks] = j.u.frag[(((mine ? ut : 0) * PS + p) * KT + ks) * 64 + lane];
-    const RowMeta mr = j.meta[row];
+    uint4 b[PS][KT - LK], *mykept = kept[wave];
+    load_kept<T, KT, LK>(j.u.frag, mine ? ut : 0, b, mykept, lane);
+    const RowMeta& meta = j.meta[mine ? ut : 0];
+    const float lse2 = meta.lse2[lane & 31], c0 = meta.c0[lane & 31], c1 = meta.c1[lane & 31];
     const Scale sc = *j.scale;
     Shift sh;
     f32x16 acc[MT] = {};
@@ -1028,12 +1075,12 @@ __global__ __launch_bounds__(grad_waves<KT>() * 64) void softmax_grad_users_kern
 #pragma unroll
             for (int e = 0; e < 4; ++e) c[4 * q + e] = v[e];
         }
-        c = score_tile<T, KT>(sbuf, b, c, lane);
+        c = score_tile<T, KT, LK>(sbuf, b, mykept, c, lane);
         if (__any(bits & 0x0F0F0F0Fu)) mask_tile(c, bits, sc.gone);
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-            const float x = fmaf(c[i], sc.kappa, -mr.lse2);
-            g[i] = -__builtin_amdgcn_exp2f(x) * fmaf(mr.c1, x, mr.c0);
+            const float x = fmaf(c[i], sc.kappa, -lse2);
+            g[i] = __builtin_amdgcn_exp2f(x) * fmaf(c1, x, c0);
         }
         stage_wait();
         if (tl + 1 < t1) load(tl + 1);
@@ -1057,23 +1104,21 @@ __global__ __launch_bounds__(grad_waves<KT>() * 64) void softmax_grad_users_kern
 // Items' side: a wave keeps 32 items and streams the user tiles of its split; dV += G^T U,
 // db = the sum of G.  The given items add w to G's element here.
 template <int T, int KT>
-__global__ __launch_bounds__(grad_waves<KT>() * 64) void softmax_grad_items_kernel(Job j) {
+__global__ __launch_bounds__((kItemsWaves * 64), (items_per_simd<T, KT>())) void
+softmax_grad_items_kernel(Job j) {
     using P = Planes<T>;
-    constexpr int PS = P::PS, MT = KT > 1 ? KT / 2 : 1, KP = MT * 32, WAVES = grad_waves<KT>();
+    constexpr int PS = P::PS, MT = KT > 1 ? KT / 2 : 1, KP = MT * 32, WAVES = kItemsWaves;
     constexpr int NS = PS * KT, NT = P::PG * MT * 2;
-    __shared__ uint4 sbuf[NS * 64], tbuf[NT * 64];
-    __shared__ uint4 mbuf[2][32];  // the tile's RowMeta
+    constexpr int LK = items_in_lds<T, KT>();
+    __shared__ uint4 sbuf[NS * 64], tbuf[NT * 64], kept[WAVES][LK ? PS * LK * 64 : 1];
+    __shared__ __align__(16) RowMeta mbuf[2];
     const int lane = threadIdx.x & 63, h = lane >> 5, wave = threadIdx.x >> 6;
     const int split = blockIdx.x % j.vsplits;
     const int64_t vt = (int64_t)(blockIdx.x / j.vsplits) * WAVES + wave;
     const bool mine = vt < j.v.tiles;
     const int64_t item = (mine ? vt : 0) * 32 + (lane & 31);
-    uint4 b[PS][KT];
-#pragma unroll
-    for (int p = 0; p < PS; ++p)
-#pragma unroll
-        for (int ks = 0; ks < KT; ++ks)
-            b[p][ks] = j.v.frag[(((mine ? vt : 0) * PS + p) * KT + ks) * 64 + lane];
+    uint4 b[PS][KT - LK], *mykept = kept[wave];
+    load_kept<T, KT, LK>(j.v.frag, mine ? vt : 0, b, mykept, lane);
     const float bias = j.vbias[item];
     const Scale sc = *j.scale;
     Shift sh;
@@ -1084,7 +1129,7 @@ __global__ __launch_bounds__(grad_waves<KT>() * 64) void softmax_grad_items_kern
     const auto load = [&](int tl) {
         stage<WAVES>(j.u.frag + (int64_t)tl * NS * 64, sbuf, NS);
         if (wave == WAVES - 1 && lane < 32)
-            copy_to_lds((const uint4*)j.meta + tl * 32 + lane, mbuf[tl & 1]);
+            copy_to_lds((const uint4*)(j.meta + tl) + lane, &mbuf[tl & 1]);
     };
     if (t0 < t1) load(t0);
     for (int tl = t0; tl < t1; ++tl) {
@@ -1096,26 +1141,38 @@ __global__ __launch_bounds__(grad_waves<KT>() * 64) void softmax_grad_items_kern
         f32x16 c;
 #pragma unroll
         for (int i = 0; i < 16; ++i) c[i] = bias;
-        c = score_tile<T, KT>(sbuf, b, c, lane);
-        const RowMeta* meta = (const RowMeta*)mbuf[tl & 1];
+        c = score_tile<T, KT, LK>(sbuf, b, mykept, c, lane);
+        const RowMeta& meta = mbuf[tl & 1];
         if (__any(word)) {
             asm volatile("");  // as in mask_tile
 #pragma unroll
-            for (int i = 0; i < 16; ++i)
-                if (__shfl((int)word, reg_row(i, h)) >> (lane & 31) & 1) c[i] = sc.gone;
+            for (int i = 0; i < 16; ++i) {  // the rows of register i in the lower and upper lanes
+                const uint64_t lo = (uint32_t)__builtin_amdgcn_readlane((int)word, reg_row(i, 0));
+                const uint64_t hi = (uint32_t)__builtin_amdgcn_readlane((int)word, reg_row(i, 1));
+                if (__builtin_amdgcn_inverse_ballot_w64(lo | hi << 32)) c[i] = sc.gone;
+            }
         }
         float sum = 0.0f;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            const RowMeta mr = meta[reg_row(i, h)];
-            const float x = fmaf(c[i], sc.kappa, -mr.lse2);
-            g[i] = -__builtin_amdgcn_exp2f(x) * fmaf(mr.c1, x, mr.c0);
-        }
-        if (__any(meta[lane & 31].t >> 5 == (int32_t)vt)) {
+        for (int q = 0; q < 4; ++q) {
+            const f32x4 lse2 = *(const f32x4*)&meta.lse2[8 * q + 4 * h];
+            const f32x4 c0 = *(const f32x4*)&meta.c0[8 * q + 4 * h];
+            const f32x4 c1 = *(const f32x4*)&meta.c1[8 * q + 4 * h];
 #pragma unroll
-            for (int i = 0; i < 16; ++i)
-                if (meta[reg_row(i, h)].t == (int32_t)item)
-                    g[i] += j.w[tl * 32 + reg_row(i, h)];
+            for (int e = 0; e < 4; ++e) {
+                const float x = fmaf(c[4 * q + e], sc.kappa, -lse2[e]);
+                g[4 * q + e] = __builtin_amdgcn_exp2f(x) * fmaf(c1[e], x, c0[e]);
+            }
+        }
+        const int32_t given = meta.t[lane & 31];
+        uint32_t hits = (uint32_t)__ballot(given >> 5 == (int32_t)vt);
+        while (hits) {  // a given item of the tile's rows among this wave's: rarely
+            const int r = __builtin_ctz(hits);
+            hits &= hits - 1;
+            const bool here = (int32_t)item == __builtin_amdgcn_readlane(given, r);
+            const float add = here ? j.w[tl * 32 + r] : 0.0f;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) g[i] += r - 4 * h == reg_row(i, 0) ? add : 0.0f;
         }
 #pragma unroll
         for (int i = 0; i < 16; ++i) sum += g[i];
@@ -1163,7 +1220,7 @@ __global__ __launch_bounds__(256) void softmax_join_users_kernel(Job j, int32_t 
     const int f = (int)(x % j.k);
     float a = 0.0f;
     for (int s = 0; s < j.splits; ++s) a += j.du_part[((int64_t)s * j.rows_pad + r) * kp + f];
-    const int32_t t = j.meta[r].t;
+    const int32_t t = j.meta[r >> 5].t[r & 31];
     if (t >= 0) a = fmaf(j.w[r], load_factor<T>(j.v.src, (int64_t)t * j.v.ld + f), a);
     store_factor<T>(j.gu, r * j.ld_gu + f, a);
 }
@@ -1269,7 +1326,7 @@ int64_t plan(const mml_item_softmax_args* a, bool grad, void* base, Job& j) {
     } else {
         j.u.trans = c.take<uint4>((int64_t)j.u.tiles * pg * mt * 128);
         j.v.trans = c.take<uint4>((int64_t)j.v.tiles * pg * mt * 128);
-        j.meta = c.take<RowMeta>(j.rows_pad);
+        j.meta = c.take<RowMeta>(j.u.tiles);
         j.w = c.take<float>(j.rows_pad);
         j.du_part = c.take<float>((int64_t)j.splits * j.rows_pad * mt * 32);
         if (j.vsplits > 1) {
@@ -1409,14 +1466,15 @@ void item_log_probs_grad(const mml_item_softmax_args* a, const float* log_norm,
     const uint32_t ju = grid_of((j.n_rows * j.k + 255) / 256);
     const uint32_t ji = grid_of(((int64_t)j.n_items * j.k + 255) / 256);
     dispatch(a->dtype, kt0, [&](auto tt, auto kt) {
-        constexpr int T = decltype(tt)::value, KT = decltype(kt)::value, W = grad_waves<KT>();
-        const uint32_t ub = grid_of((int64_t)((j.u.tiles + W - 1) / W) * j.splits);
-        const uint32_t vb = grid_of((int64_t)((j.v.tiles + W - 1) / W) * j.vsplits);
+        constexpr int T = decltype(tt)::value, KT = decltype(kt)::value, UW = users_waves<T, KT>();
+        constexpr int IW = kItemsWaves;
+        const uint32_t ub = grid_of((int64_t)((j.u.tiles + UW - 1) / UW) * j.splits);
+        const uint32_t vb = grid_of((int64_t)((j.v.tiles + IW - 1) / IW) * j.vsplits);
         if (j.n_rows > 0) {
-            softmax_grad_users_kernel<T, KT><<<ub, W * 64, 0, st>>>(j);
+            softmax_grad_users_kernel<T, KT><<<ub, UW * 64, 0, st>>>(j);
             softmax_join_users_kernel<T><<<ju, 256, 0, st>>>(j, kp);
         }
-        softmax_grad_items_kernel<T, KT><<<vb, W * 64, 0, st>>>(j);
+        softmax_grad_items_kernel<T, KT><<<vb, IW * 64, 0, st>>>(j);
         if (j.vsplits > 1) softmax_join_items_kernel<T><<<ji, 256, 0, st>>>(j, kp);
     });
     MML_HIP(hipGetLastError());
