@@ -172,7 +172,7 @@ struct Job {
     int32_t vsplits;
     void *gu, *gv;
     int64_t ld_gu, ld_gv;
-    int32_t gv_vec4;
+    int32_t gu_vec4, gv_vec4;
     float* gb;
 };
 
@@ -626,6 +626,11 @@ constexpr int forward_waves() {
     return Planes<T>::PS * KT > 16 ? 4 : 8;
 }
 
+template <int T, int KT>
+constexpr int forward_per_simd() {
+    return Planes<T>::PS * KT > 16 ? 2 : 4;
+}
+
 // Tiles staged at a time: up to 8 in 32 KB.  Fewer barriers, and between two of them the waves
 // drift apart, so that one's matrix work runs under another's exponentials.
 template <int T, int KT>
@@ -640,7 +645,8 @@ constexpr int kTileGroup = 8;  // the streamed items are padded to a multiple of
 // l % 32, 16 of a tile's 32 items.  m, l, w: the running maximum (of scaled scores), the sum of
 // e = exp(s - m) and of e y, y = log2 e.
 template <int T, int KT, bool TOP>
-__global__ __launch_bounds__((forward_waves<T, KT>() * 64)) void softmax_forward_kernel(Job j) {
+__global__ __launch_bounds__((forward_waves<T, KT>() * 64), (forward_per_simd<T, KT>())) void
+softmax_forward_kernel(Job j) {
     constexpr int PS = Planes<T>::PS, WAVES = forward_waves<T, KT>(), TPS = forward_tiles<T, KT>();
     __shared__ uint4 buf[2][TPS * PS * KT * 64];
     __shared__ f32x4 bias[2][TPS * 8];
@@ -1020,7 +1026,7 @@ constexpr int users_per_simd() {
 // Steps of the kept fragments that stay in LDS, so that nothing is spilled at those waves per SIMD
 template <int T, int KT>
 constexpr int users_in_lds() {
-    return KT == 4 && T == MML_DTYPE_F32 ? 1 : KT == 16 && T == MML_DTYPE_F16 ? 4 : 0;
+    return KT == 16 && T == MML_DTYPE_F16 ? 4 : 0;
 }
 constexpr int kItemsWaves = 4;
 template <int T, int KT>
@@ -1211,34 +1217,54 @@ softmax_grad_items_kernel(Job j) {
     if (h == 0) j.db_part[split * items_pad + item] = db;
 }
 
-// The splits' sums in split order (the same result every time), the users' rows with w V_t added.
+// Four factors of a row summed over the splits: kJoin neighbouring threads take every kJoin-th split
+// and are joined in order, so the result is the same every time.
+constexpr int kJoin = 8;
+__device__ __forceinline__ f32x4 join_splits(const float* __restrict__ part, int64_t stride,
+                                             int splits) {
+    const int g = threadIdx.x % kJoin;
+    f32x4 a = {};
+#pragma unroll 4
+    for (int s = g; s < splits; s += kJoin) a += *(const f32x4*)(part + s * stride);
+#pragma unroll
+    for (int d = 1; d < kJoin; d <<= 1)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) a[e] += __shfl_xor(a[e], d);
+    return a;
+}
+// The users' rows with w V_t added
 template <int T>
 __global__ __launch_bounds__(256) void softmax_join_users_kernel(Job j, int32_t kp) {
-    const int64_t x = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (x >= j.n_rows * j.k) return;
-    const int64_t r = x / j.k;
-    const int f = (int)(x % j.k);
-    float a = 0.0f;
-    for (int s = 0; s < j.splits; ++s) a += j.du_part[((int64_t)s * j.rows_pad + r) * kp + f];
+    const int64_t x = ((int64_t)blockIdx.x * 256 + threadIdx.x) / kJoin;
+    const int quads = (j.k + 3) / 4;
+    const bool in = x < j.n_rows * quads;  // (all lanes take part in the join)
+    const int64_t r = in ? x / quads : 0;
+    const int f = in ? 4 * (int)(x % quads) : 0;
+    f32x4 a = join_splits(j.du_part + r * kp + f, j.rows_pad * kp, j.splits);
+    if (!in || threadIdx.x % kJoin) return;
     const int32_t t = j.meta[r >> 5].t[r & 31];
-    if (t >= 0) a = fmaf(j.w[r], load_factor<T>(j.v.src, (int64_t)t * j.v.ld + f), a);
-    store_factor<T>(j.gu, r * j.ld_gu + f, a);
+    if (t >= 0)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (f + e < j.k)
+                a[e] = fmaf(j.w[r], load_factor<T>(j.v.src, (int64_t)t * j.v.ld + f + e), a[e]);
+    store_factors<T>(j.gu, r * j.ld_gu, f, j.k, j.gu_vec4, a);
 }
 template <int T>
 __global__ __launch_bounds__(256) void softmax_join_items_kernel(Job j, int32_t kp) {
-    const int64_t x = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    const int64_t x = ((int64_t)blockIdx.x * 256 + threadIdx.x) / kJoin;
     const int64_t items_pad = (int64_t)j.v.tiles * 32;
-    if (x < (int64_t)j.n_items * j.k) {
-        const int64_t i = x / j.k;
-        const int f = (int)(x % j.k);
-        float a = 0.0f;
-        for (int s = 0; s < j.vsplits; ++s) a += j.dv_part[((int64_t)s * items_pad + i) * kp + f];
-        store_factor<T>(j.gv, i * j.ld_gv + f, a);
-    }
-    if (x < j.n_items) {
-        float a = 0.0f;
-        for (int s = 0; s < j.vsplits; ++s) a += j.db_part[s * items_pad + x];
-        j.gb[x] = a;
+    const int quads = (j.k + 3) / 4;
+    const bool in = x < (int64_t)j.n_items * quads;
+    const int64_t i = in ? x / quads : 0;
+    const int f = in ? 4 * (int)(x % quads) : 0;
+    const f32x4 a = join_splits(j.dv_part + i * kp + f, items_pad * kp, j.vsplits);
+    if (!in || threadIdx.x % kJoin) return;
+    store_factors<T>(j.gv, i * j.ld_gv, f, j.k, j.gv_vec4, a);
+    if (f == 0) {
+        float b = 0.0f;
+        for (int s = 0; s < j.vsplits; ++s) b += j.db_part[s * items_pad + i];
+        j.gb[i] = b;
     }
 }
 
@@ -1247,6 +1273,51 @@ int steps_of(int32_t k) {  // KT: the factors padded to 16, 32, 64, 128 or 256
     int kt = 1;
     while (kt * 16 < k) kt *= 2;
     return kt;
+}
+
+template <class F>
+void dispatch(int T, int kt, F&& f) {
+#define MML_KT(TT)                                                       \
+    switch (kt) {                                                        \
+        case 1: return f(std::integral_constant<int, TT>{}, std::integral_constant<int, 1>{});   \
+        case 2: return f(std::integral_constant<int, TT>{}, std::integral_constant<int, 2>{});   \
+        case 4: return f(std::integral_constant<int, TT>{}, std::integral_constant<int, 4>{});   \
+        case 8: return f(std::integral_constant<int, TT>{}, std::integral_constant<int, 8>{});   \
+        default: return f(std::integral_constant<int, TT>{}, std::integral_constant<int, 16>{}); \
+    }
+    switch (T) {
+        case MML_DTYPE_F32: MML_KT(MML_DTYPE_F32)
+        case MML_DTYPE_BF16: MML_KT(MML_DTYPE_BF16)
+        default: MML_KT(MML_DTYPE_F16)
+    }
+#undef MML_KT
+}
+
+// How many splits of the streamed side: enough blocks to fill the 256 CUs with as many waves as fit,
+// and short ones, so that the last blocks leave little idle; against a fixed cost per block (its kept
+// fragments, the first tile) and the join of the splits' results.  kept / streamed: tiles of either
+// side; matrix instructions per pair of tiles; bytes a split leaves per kept tile.  In cycles: a wave's
+// tile takes 32 per matrix instruction and 500 besides; w waves on a SIMD take (w + 1.5) / 2.5 times as
+// long as one (measured: 1.6 times the throughput from one to two, 1.2 from two to four); a block 6,000
+// to start; results are written and read back at 2 KB a cycle.  Above 8, a multiple of the 8 XCDs:
+// block b runs on XCD b mod 8, so a split's blocks share an L2.
+int32_t choose_splits(int64_t kept, int64_t streamed, int waves, int per_simd, int instructions,
+                      double bytes) {
+    const int64_t row_blocks = std::max<int64_t>(1, (kept + waves - 1) / waves);
+    const int64_t most_per_cu = std::max(1, per_simd * 4 / waves);
+    double best = 0.0;
+    int32_t chosen = 1;
+    for (int64_t s = 1; s <= 1024 && s <= streamed; s += s < 8 ? 1 : 8) {
+        const int64_t blocks = row_blocks * s;
+        const int64_t per_cu = std::min(most_per_cu, (blocks + 255) / 256);
+        const double tile = (per_cu * waves / 4.0 + 1.5) / 2.5 * (instructions * 32.0 + 500.0);
+        const double one = tile * ((streamed + s - 1) / s) + 6000.0;
+        const double fill = (double)blocks / (256.0 * per_cu);
+        const double cost = (fill <= 1.0 ? 1.0 : fill + 0.35) * one +
+                            (s > 1 ? s * kept * bytes / 1024.0 : 0.0);
+        if (s == 1 || cost < best) best = cost, chosen = (int32_t)s;
+    }
+    return chosen;
 }
 
 struct Carve {  // a workspace cut into arrays of 256-byte alignment (base null: sizes only)
@@ -1301,16 +1372,24 @@ int64_t plan(const mml_item_softmax_args* a, bool grad, void* base, Job& j) {
     j.ex_off = a->exclude_offsets;
     j.ex_items = a->exclude_items;
     j.n_ex = a->n_exclude;
-    // about 4,096 waves, a split not under 4 tiles; a multiple of the 8 XCDs where there are more,
-    // so that the blocks of one split share an L2 (block b runs on XCD b mod 8)
-    const auto splits = [](int64_t kept, int64_t streamed) {
-        int64_t s = std::min<int64_t>((4096 + kept - 1) / std::max<int64_t>(kept, 1),
-                                      (streamed + 3) / 4);
-        if (s > 8) s &= ~(int64_t)7;
-        return (int32_t)std::max<int64_t>(1, s);
-    };
-    j.splits = splits(j.u.tiles, j.v.tiles);
-    j.vsplits = splits(j.v.tiles, j.u.tiles);
+    if (grad) {
+        dispatch(T, kt, [&](auto tt, auto k) {
+            constexpr int TT = decltype(tt)::value, KT = decltype(k)::value;
+            constexpr int M = Planes<TT>::PS == 2 ? 6 * KT : 3 * KT;
+            j.splits = choose_splits(j.u.tiles, j.v.tiles, users_waves<TT, KT>(),
+                                     users_per_simd<TT, KT>(), M, mt * 4096.0);
+            j.vsplits = choose_splits(j.v.tiles, j.u.tiles, kItemsWaves, items_per_simd<TT, KT>(),
+                                      M, mt * 4096.0);
+        });
+    } else {
+        dispatch(T, kt, [&](auto tt, auto k) {
+            constexpr int TT = decltype(tt)::value, KT = decltype(k)::value;
+            constexpr int M = Planes<TT>::PS == 2 ? 3 * KT : KT;
+            j.splits = choose_splits(j.u.tiles, j.v.tiles / forward_tiles<TT, KT>(),
+                                     forward_waves<TT, KT>(), forward_per_simd<TT, KT>(),
+                                     M * forward_tiles<TT, KT>(), 384.0);
+        });
+    }
     Carve c{(char*)base};
     j.scale = c.take<Scale>(1);
     if (T == MML_DTYPE_F32) j.parts = c.take<float>(kMaxParts);
@@ -1335,24 +1414,6 @@ int64_t plan(const mml_item_softmax_args* a, bool grad, void* base, Job& j) {
         }
     }
     return c.used;
-}
-
-template <class F>
-void dispatch(int T, int kt, F&& f) {
-#define MML_KT(TT)                                                       \
-    switch (kt) {                                                        \
-        case 1: return f(std::integral_constant<int, TT>{}, std::integral_constant<int, 1>{});   \
-        case 2: return f(std::integral_constant<int, TT>{}, std::integral_constant<int, 2>{});   \
-        case 4: return f(std::integral_constant<int, TT>{}, std::integral_constant<int, 4>{});   \
-        case 8: return f(std::integral_constant<int, TT>{}, std::integral_constant<int, 8>{});   \
-        default: return f(std::integral_constant<int, TT>{}, std::integral_constant<int, 16>{}); \
-    }
-    switch (T) {
-        case MML_DTYPE_F32: MML_KT(MML_DTYPE_F32)
-        case MML_DTYPE_BF16: MML_KT(MML_DTYPE_BF16)
-        default: MML_KT(MML_DTYPE_F16)
-    }
-#undef MML_KT
 }
 
 uint32_t grid_of(int64_t n) {
@@ -1457,14 +1518,16 @@ void item_log_probs_grad(const mml_item_softmax_args* a, const float* log_norm,
     j.ld_gv = ld_gv;
     j.gb = gb;
     const int size = a->dtype == MML_DTYPE_F32 ? 4 : 2;
+    j.gu_vec4 = j.k % 4 == 0 && ld_gu % 4 == 0 && (uintptr_t)gu % (4 * size) == 0;
     j.gv_vec4 = j.k % 4 == 0 && ld_gv % 4 == 0 && (uintptr_t)gv % (4 * size) == 0;
     const int kt0 = steps_of(j.k), kp = std::max(32, kt0 * 16);
     if (a->n_rows > 0) {
         mask_and_prep(j, a->dtype, st);
         softmax_meta_kernel<<<grid_of((j.rows_pad + 255) / 256), 256, 0, st>>>(j);
     }
-    const uint32_t ju = grid_of((j.n_rows * j.k + 255) / 256);
-    const uint32_t ji = grid_of(((int64_t)j.n_items * j.k + 255) / 256);
+    const int64_t quads = (j.k + 3) / 4;
+    const uint32_t ju = grid_of((j.n_rows * quads * kJoin + 255) / 256);
+    const uint32_t ji = grid_of(((int64_t)j.n_items * quads * kJoin + 255) / 256);
     dispatch(a->dtype, kt0, [&](auto tt, auto kt) {
         constexpr int T = decltype(tt)::value, KT = decltype(kt)::value, UW = users_waves<T, KT>();
         constexpr int IW = kItemsWaves;

@@ -38,6 +38,13 @@ def test_bad_sizes(bad, text):
 def test_workspace_sizes():
     with pytest.raises(N.MMLError, match="args is null"):
         workspace(None)
+    for grad in (0, 1):
+        assert workspace(args(n_rows=0), grad) > 0  # no rows are a call too
+        for rows in (1, 31, 32, 33, 5000):
+            for items in (1, 255, 257, 70_000):
+                for k in (1, 16, 17, 64, 256):
+                    assert workspace(args(n_rows=rows, n_users=rows, n_items=items, num_factors=k,
+                                          ld_users=k, ld_items=k, n_top=5 * (1 - grad)), grad) > 0
     small, large = workspace(args()), workspace(args(n_rows=4, n_items=500))
     assert 0 < small < large
     assert workspace(args(n_top=5)) > small
