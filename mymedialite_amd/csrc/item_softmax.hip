@@ -1008,8 +1008,10 @@ __global__ __launch_bounds__(TOP ? 256 : 64) void softmax_finish_kernel(Job j) {
 }
 
 // ------------------------------------------------------------------ gradient
-// Both kernels stage a tile's score fragments in one LDS buffer and its transposed ones in another:
-// while one is used, the other is on the way, with a barrier between.  A block's waves share the
+// Both kernels stage a tile's score fragments and its transposed ones.  Where two tiles' fit next to
+// other blocks (k <= 128), in two buffers of both: the next tile's are on the way while this one's
+// are used, one barrier a tile.  Else in one buffer of each: while the score fragments are used the
+// transposed ones are on the way, and the other way round.  A block's waves share the
 // streamed tile, and other blocks' waves fill the time at the barriers.  Waves of a block and waves
 // per SIMD that the registers are held down to, measured (2048 x 100k, k = 64 f32; 1001 x 30k, k = 100
 // f16; 1024 x 500k, k = 256 bf16): users 156 us with 8 and 4 against 199 with 8 and 2; items 206 with
@@ -1022,6 +1024,10 @@ constexpr int users_waves() {
 template <int T, int KT>
 constexpr int users_per_simd() {
     return KT <= 4 ? 4 : KT <= 8 || T != MML_DTYPE_F32 ? 2 : 1;
+}
+template <int KT>
+constexpr int tile_buffers() {
+    return KT <= 8 ? 2 : 1;
 }
 // Steps of the kept fragments that stay in LDS, so that nothing is spilled at those waves per SIMD
 template <int T, int KT>
@@ -1046,7 +1052,8 @@ softmax_grad_users_kernel(Job j) {
     constexpr int PS = P::PS, MT = KT > 1 ? KT / 2 : 1, KP = MT * 32, WAVES = users_waves<T, KT>();
     constexpr int NS = PS * KT, NT = P::PG * MT * 2;  // KB of score and of transposed fragments
     constexpr int LK = users_in_lds<T, KT>();
-    __shared__ uint4 sbuf[NS * 64], tbuf[NT * 64], kept[WAVES][LK ? PS * LK * 64 : 1];
+    constexpr int NB = tile_buffers<KT>();
+    __shared__ uint4 sbuf[NB][NS * 64], tbuf[NB][NT * 64], kept[WAVES][LK ? PS * LK * 64 : 1];
     __shared__ f32x4 bias[2][8];
     const int lane = threadIdx.x & 63, h = lane >> 5, wave = threadIdx.x >> 6;
     const int split = blockIdx.x % j.splits;
@@ -1062,17 +1069,24 @@ softmax_grad_users_kernel(Job j) {
     f32x16 acc[MT] = {};
     const int t0 = (int)((int64_t)j.v.tiles * split / j.splits);
     const int t1 = (int)((int64_t)j.v.tiles * (split + 1) / j.splits);
-    const auto load = [&](int tl) {
-        stage<WAVES>(j.v.frag + (int64_t)tl * NS * 64, sbuf, NS);
+    uint32_t word = 0;
+    const auto load_trans = [&](int tl, int at) {
+        stage<WAVES>(j.v.trans + (int64_t)tl * NT * 64, tbuf[at], NT);
+    };
+    const auto load = [&](int tl, int at) {
+        stage<WAVES>(j.v.frag + (int64_t)tl * NS * 64, sbuf[at], NS);
         if (wave == WAVES - 1 && lane < 8)
             copy_to_lds((const f32x4*)j.vbias + tl * 8 + lane, bias[tl & 1]);
+        if (NB == 2) load_trans(tl, at);
+        if (j.mask) word = j.mask[(int64_t)tl * j.rows_pad + row];
     };
-    if (t0 < t1) load(t0);
-    for (int tl = t0; tl < t1; ++tl) {
-        const uint32_t bits =
-            j.mask ? j.mask[(int64_t)tl * j.rows_pad + row] >> (4 * h) : 0;
+    if (t0 < t1) load(t0, 0);
+    for (int tl = t0, at = 0; tl < t1; ++tl, at ^= NB - 1) {
         stage_wait();
-        stage<WAVES>(j.v.trans + (int64_t)tl * NT * 64, tbuf, NT);
+        asm volatile("" : "+v"(word));  // the wait for this load belongs before the next copies
+        const uint32_t bits = word >> (4 * h);
+        if (NB == 1) load_trans(tl, 0);
+        else if (tl + 1 < t1) load(tl + 1, at ^ 1);
         float g[16];
         f32x16 c;
 #pragma unroll
@@ -1081,17 +1095,19 @@ softmax_grad_users_kernel(Job j) {
 #pragma unroll
             for (int e = 0; e < 4; ++e) c[4 * q + e] = v[e];
         }
-        c = score_tile<T, KT, LK>(sbuf, b, mykept, c, lane);
+        c = score_tile<T, KT, LK>(sbuf[at], b, mykept, c, lane);
         if (__any(bits & 0x0F0F0F0Fu)) mask_tile(c, bits, sc.gone);
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
             const float x = fmaf(c[i], sc.kappa, -lse2);
             g[i] = __builtin_amdgcn_exp2f(x) * fmaf(c1, x, c0);
         }
-        stage_wait();
-        if (tl + 1 < t1) load(tl + 1);
+        if (NB == 1) {
+            stage_wait();
+            if (tl + 1 < t1) load(tl + 1, 0);
+        }
         scale_g<T, MT>(g, acc, sh);
-        grad_tile<T, KT>(tbuf, g, acc, lane);
+        grad_tile<T, KT>(tbuf[at], g, acc, lane);
     }
     if (!mine) return;
 #pragma unroll
@@ -1116,7 +1132,8 @@ softmax_grad_items_kernel(Job j) {
     constexpr int PS = P::PS, MT = KT > 1 ? KT / 2 : 1, KP = MT * 32, WAVES = kItemsWaves;
     constexpr int NS = PS * KT, NT = P::PG * MT * 2;
     constexpr int LK = items_in_lds<T, KT>();
-    __shared__ uint4 sbuf[NS * 64], tbuf[NT * 64], kept[WAVES][LK ? PS * LK * 64 : 1];
+    constexpr int NB = tile_buffers<KT>();
+    __shared__ uint4 sbuf[NB][NS * 64], tbuf[NB][NT * 64], kept[WAVES][LK ? PS * LK * 64 : 1];
     __shared__ __align__(16) RowMeta mbuf[2];
     const int lane = threadIdx.x & 63, h = lane >> 5, wave = threadIdx.x >> 6;
     const int split = blockIdx.x % j.vsplits;
@@ -1132,22 +1149,29 @@ softmax_grad_items_kernel(Job j) {
     float db = 0.0f;
     const int t0 = (int)((int64_t)j.u.tiles * split / j.vsplits);
     const int t1 = (int)((int64_t)j.u.tiles * (split + 1) / j.vsplits);
-    const auto load = [&](int tl) {
-        stage<WAVES>(j.u.frag + (int64_t)tl * NS * 64, sbuf, NS);
+    uint32_t next = 0;
+    const auto load_trans = [&](int tl, int at) {
+        stage<WAVES>(j.u.trans + (int64_t)tl * NT * 64, tbuf[at], NT);
+    };
+    const auto load = [&](int tl, int at) {
+        stage<WAVES>(j.u.frag + (int64_t)tl * NS * 64, sbuf[at], NS);
         if (wave == WAVES - 1 && lane < 32)
             copy_to_lds((const uint4*)(j.meta + tl) + lane, &mbuf[tl & 1]);
+        if (NB == 2) load_trans(tl, at);
+        if (j.mask) next = j.mask[(mine ? vt : 0) * j.rows_pad + tl * 32 + (lane & 31)];
     };
-    if (t0 < t1) load(t0);
-    for (int tl = t0; tl < t1; ++tl) {
-        const uint32_t word =
-            j.mask ? j.mask[(mine ? vt : 0) * j.rows_pad + tl * 32 + (lane & 31)] : 0;
+    if (t0 < t1) load(t0, 0);
+    for (int tl = t0, at = 0; tl < t1; ++tl, at ^= NB - 1) {
         stage_wait();
-        stage<WAVES>(j.u.trans + (int64_t)tl * NT * 64, tbuf, NT);
+        asm volatile("" : "+v"(next));
+        const uint32_t word = next;
+        if (NB == 1) load_trans(tl, 0);
+        else if (tl + 1 < t1) load(tl + 1, at ^ 1);
         float g[16];
         f32x16 c;
 #pragma unroll
         for (int i = 0; i < 16; ++i) c[i] = bias;
-        c = score_tile<T, KT, LK>(sbuf, b, mykept, c, lane);
+        c = score_tile<T, KT, LK>(sbuf[at], b, mykept, c, lane);
         const RowMeta& meta = mbuf[tl & 1];
         if (__any(word)) {
             asm volatile("");  // as in mask_tile
@@ -1183,10 +1207,12 @@ softmax_grad_items_kernel(Job j) {
 #pragma unroll
         for (int i = 0; i < 16; ++i) sum += g[i];
         db += sum;
-        stage_wait();
-        if (tl + 1 < t1) load(tl + 1);
+        if (NB == 1) {
+            stage_wait();
+            if (tl + 1 < t1) load(tl + 1, 0);
+        }
         scale_g<T, MT>(g, acc, sh);
-        grad_tile<T, KT>(tbuf, g, acc, lane);
+        grad_tile<T, KT>(tbuf[at], g, acc, lane);
     }
     if (!mine) return;
     const int64_t items_pad = (int64_t)j.v.tiles * 32;
