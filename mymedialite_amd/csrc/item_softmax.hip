@@ -75,6 +75,25 @@ __device__ __forceinline__ float load_factor(const void* p, int64_t i) {
     if constexpr (T == MML_DTYPE_BF16) return __uint_as_float((uint32_t)((const uint16_t*)p)[i] << 16);
     if constexpr (T == MML_DTYPE_F16) return (float)((const _Float16*)p)[i];
 }
+// Factors at .. at + 7 (16-byte aligned)
+template <int T>
+__device__ __forceinline__ void load_factors(const void* p, int64_t at, float (&v)[8]) {
+    if constexpr (T == MML_DTYPE_F32) {
+        const f32x4 lo = *(const f32x4*)((const float*)p + at);
+        const f32x4 hi = *(const f32x4*)((const float*)p + at + 4);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = lo[e], v[4 + e] = hi[e];
+    } else {
+        const uint4 q = *(const uint4*)((const uint16_t*)p + at);
+        const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const uint16_t b = (uint16_t)(w[e >> 1] >> (16 * (e & 1)));
+            v[e] = T == MML_DTYPE_F16 ? (float)__builtin_bit_cast(_Float16, b)
+                                      : __uint_as_float((uint32_t)b << 16);
+        }
+    }
+}
 __device__ __forceinline__ uint32_t bf16_rn(float x) {
     const uint32_t b = __float_as_uint(x);
     return (b + 0x7FFFu + ((b >> 16) & 1u)) >> 16;
@@ -137,6 +156,9 @@ struct Scale {
                   // before the first score too (a row whose scores are all below it counts as empty)
     int32_t eu, ev;
 };
+__device__ __forceinline__ Scale plain_scale() {
+    return Scale{kLog2e, 1.0f, kGone, kGone * 0.0625f, 0, 0};
+}
 constexpr int kMaxParts = 512, kUserParts = 64;  // partial maxima of softmax_max_kernel
 
 struct Job {
@@ -156,12 +178,13 @@ struct Job {
     int32_t k, n_items;
     int64_t n_rows;
     int32_t splits;
+    int32_t bias_vec4;  // the bias can be loaded 4 at a time
+    int32_t direct;  // at most kDirectRows rows, forward: no preparation
     // forward
-    float* part;    // [splits][3][rows_pad]: m, l, w
+    float* part;    // [3][rows_pad][splits]: m, l, w
     float* cmax;    // [rows_pad][cpad]: every tile's largest score (n_top > 0)
     int64_t cpad;
     int32_t n_top;
-    int32_t vec4;   // the items' rows can be loaded 4 factors at a time
     float *log_probs, *log_norm, *entropy, *top_lp;
     int32_t* top_items;
     // gradient
@@ -322,21 +345,7 @@ __global__ __launch_bounds__(256) void softmax_prep_kernel(Job j) {
         if (src >= 0) {
             const int64_t at = src * s.ld + f;
             if (s.vec8 && f + 8 <= j.k) {
-                if constexpr (T == MML_DTYPE_F32) {
-                    const f32x4 lo = *(const f32x4*)((const float*)s.src + at);
-                    const f32x4 hi = *(const f32x4*)((const float*)s.src + at + 4);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) v[e] = lo[e], v[4 + e] = hi[e];
-                } else {
-                    const uint4 q = *(const uint4*)((const uint16_t*)s.src + at);
-                    const uint32_t w[4] = {q.x, q.y, q.z, q.w};
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        const uint16_t b = (uint16_t)(w[e >> 1] >> (16 * (e & 1)));
-                        v[e] = T == MML_DTYPE_F16 ? (float)__builtin_bit_cast(_Float16, b)
-                                                  : __uint_as_float((uint32_t)b << 16);
-                    }
-                }
+                load_factors<T>(s.src, at, v);
             } else {
 #pragma unroll
                 for (int e = 0; e < 8; ++e)
@@ -623,12 +632,12 @@ __device__ __forceinline__ void mask_tile(f32x16& c, uint32_t bits, float gone) 
 // shares each streamed tile.
 template <int T, int KT>
 constexpr int forward_waves() {
-    return Planes<T>::PS * KT > 16 ? 4 : 8;
+    return Planes<T>::PS * KT > 16 || (T == MML_DTYPE_F32 && KT == 8) ? 4 : 8;
 }
 
 template <int T, int KT>
 constexpr int forward_per_simd() {
-    return Planes<T>::PS * KT > 16 ? 2 : 4;
+    return Planes<T>::PS * KT > 16 || (T == MML_DTYPE_F32 && KT == 8) ? 2 : 4;
 }
 
 // Tiles staged at a time: up to 8 in 32 KB.  Fewer barriers, and between two of them the waves
@@ -747,48 +756,215 @@ softmax_forward_kernel(Job j) {
     w += __shfl_xor(w, 32);
     l += __shfl_xor(l, 32);
     if (h == 0) {
-        float* p = j.part + (int64_t)split * 3 * j.rows_pad + row;
+        float* p = j.part + row * j.splits + split;
+        const int64_t next = j.rows_pad * j.splits;
         p[0] = mn;
-        p[j.rows_pad] = l;
-        p[2 * j.rows_pad] = w;
+        p[next] = l;
+        p[2 * next] = w;
+    }
+}
+
+// The forward pass for at most 32 rows: every item is used by one tile of users, so there is nothing
+// to share and nothing to prepare.  A wave makes its fragments from the factors themselves, both
+// sides', and the catalogue is read once.  f32: every tile of items has a scale of its own, 2^ev, and
+// the scores are brought back before the bias is added (one instruction more per score, which the
+// memory's pace hides: 25.6 MB of factors take about 5 us at the rate of a large copy).  m, l, w as in
+// the forward pass, in true units; the block's waves are joined before they are written.
+constexpr int kDirectRows = 32, kDirectWaves = 4;
+
+// Fragments of 32 rows from their source: row `row` of src in lanes l and l + 32.  Returns the
+// exponent of the f32 planes' scale; finite: whether this lane's values are
+template <int T, int KT>
+__device__ __forceinline__ void load_rows(const Side& s, int64_t src, int k, int h,
+                                          float (&v)[KT][8]) {
+#pragma unroll
+    for (int ks = 0; ks < KT; ++ks) {
+        const int f = 16 * ks + 8 * h;
+        if (src >= 0 && s.vec8 && f + 8 <= k) {
+            load_factors<T>(s.src, src * s.ld + f, v[ks]);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                v[ks][e] = src >= 0 && f + e < k ? load_factor<T>(s.src, src * s.ld + f + e) : 0.0f;
+        }
+    }
+}
+template <int T, int KT>
+__device__ __forceinline__ int make_planes(float (&v)[KT][8], uint4 (&q)[Planes<T>::PS][KT],
+                                           bool& finite) {
+    using P = Planes<T>;
+    float most = 0.0f;
+    finite = true;
+#pragma unroll
+    for (int ks = 0; ks < KT; ++ks)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const float a = fabsf(v[ks][e]);
+            finite = finite && a < 3e38f;
+            if (T == MML_DTYPE_F32) most = fmaxf(most, a < 3e38f ? a : 0.0f);
+        }
+    int ex = 0;
+    float mul = 1.0f;
+    if constexpr (T == MML_DTYPE_F32) {
+#pragma unroll
+        for (int d = 32; d > 0; d >>= 1) most = fmaxf(most, __shfl_xor(most, d));
+        ex = max(-40, min(12, 13 - __builtin_amdgcn_frexp_expf(most)));
+        mul = ldexpf(1.0f, ex);
+    }
+#pragma unroll
+    for (int ks = 0; ks < KT; ++ks) {
+        uint32_t w[P::PS][8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            float x = finite ? v[ks][e] * mul : 0.0f;
+#pragma unroll
+            for (int p = 0; p < P::PS; ++p) w[p][e] = take_plane<T>(x);
+        }
+#pragma unroll
+        for (int p = 0; p < P::PS; ++p)
+            q[p][ks] = make_uint4(w[p][0] | w[p][1] << 16, w[p][2] | w[p][3] << 16,
+                                  w[p][4] | w[p][5] << 16, w[p][6] | w[p][7] << 16);
+    }
+    return ex;
+}
+
+template <int T, int KT, bool TOP>
+__global__ __launch_bounds__(kDirectWaves * 64) void softmax_direct_kernel(Job j) {
+    constexpr int PS = Planes<T>::PS, W = kDirectWaves;
+    __shared__ float state[W][3][32];
+    const int lane = threadIdx.x & 63, h = lane >> 5, wave = threadIdx.x >> 6, row = lane & 31;
+    const int ways = j.splits * W, way = blockIdx.x * W + wave;
+    const int t0 = (int)((int64_t)j.v.tiles * way / ways);
+    const int t1 = (int)((int64_t)j.v.tiles * (way + 1) / ways);
+    // a tile's factors are on the way while the one before is used (up to k = 128: registers)
+    constexpr bool AHEAD = KT <= 8;
+    float v[KT][8], u[KT][8];
+    uint4 b[PS][KT];
+    bool finite;
+    load_rows<T, KT>(j.u, source_row(j.u, row), j.k, h, u);
+    if (AHEAD && t0 < t1) load_rows<T, KT>(j.v, source_row(j.v, (int64_t)t0 * 32 + row), j.k, h, v);
+    const int eu = make_planes<T, KT>(u, b, finite);
+    const Scale sc = plain_scale();
+    float m = sc.floor, l = 0.0f, w = 0.0f;
+    for (int tl = t0; tl < t1; ++tl) {
+        float bias[16];
+        const bool whole = j.bias && j.bias_vec4 && tl * 32 + 32 <= j.n_items;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const int64_t item = (int64_t)tl * 32 + 8 * q + 4 * h;
+            if (whole) {
+                const f32x4 x = *(const f32x4*)&j.bias[item];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) bias[4 * q + e] = x[e];
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    bias[4 * q + e] =
+                        item + e < j.n_items ? (j.bias ? j.bias[item + e] : 0.0f) : kGone;
+            }
+        }
+        const uint32_t bits =
+            j.mask ? j.mask[(int64_t)tl * j.rows_pad + row] >> (4 * h) : 0;
+        uint4 a[PS][KT];
+        if (!AHEAD) load_rows<T, KT>(j.v, source_row(j.v, (int64_t)tl * 32 + row), j.k, h, v);
+        const int ev = make_planes<T, KT>(v, a, finite);
+        const uint64_t odd = __ballot(!finite);  // rows with a value that is not finite
+        if (AHEAD && tl + 1 < t1)
+            load_rows<T, KT>(j.v, source_row(j.v, (int64_t)(tl + 1) * 32 + row), j.k, h, v);
+        f32x16 c = {};
+#pragma unroll
+        for (int ks = 0; ks < KT; ++ks)
+#pragma unroll
+            for (int sum = PS - 1; sum >= 0; --sum)
+#pragma unroll
+                for (int p = sum; p >= 0; --p) c = mfma<T>(a[p][ks], b[sum - p][ks], c);
+        const float unit = ldexpf(1.0f, -eu - ev);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            c[i] = fmaf(c[i], unit, bias[i]);
+            if (!(bias[i] < -kGone)) c[i] = __builtin_nanf("");  // not finite
+        }
+        if (odd) {
+            const uint32_t rows = (uint32_t)odd | (uint32_t)(odd >> 32);
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+                if (rows >> reg_row(i, h) & 1u) c[i] = __builtin_nanf("");
+        }
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+            if (bias[i] <= kGone) c[i] = sc.gone;
+        if (__any(bits & 0x0F0F0F0Fu)) mask_tile(c, bits, sc.gone);
+        float mt = c[0];
+#pragma unroll
+        for (int i = 1; i < 16; ++i) mt = fmaxf(mt, c[i]);
+        if constexpr (TOP) {
+            const float most = both_max(mt);
+            if (lane < j.n_rows) j.cmax[row * j.cpad + tl] = most;  // (at most 32 rows)
+        }
+        const float mn = fmaxf(m, mt), d = (m - mn) * kLog2e, f = __builtin_amdgcn_exp2f(d);
+        w = f * fmaf(l, d, w);
+        l *= f;
+        m = mn;
+        const float m2 = m * kLog2e;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const float y = fmaf(c[i], kLog2e, -m2), e = __builtin_amdgcn_exp2f(y);
+            l += e;
+            w = fmaf(e, y, w);
+        }
+    }
+    {
+        const float mn = both_max(m), d = (m - mn) * kLog2e, f = __builtin_amdgcn_exp2f(d);
+        w = f * fmaf(l, d, w);
+        l *= f;
+        w += __shfl_xor(w, 32);
+        l += __shfl_xor(l, 32);
+        if (h == 0) state[wave][0][row] = mn, state[wave][1][row] = l, state[wave][2][row] = w;
+    }
+    __syncthreads();
+    if (threadIdx.x < 32) {
+        m = state[0][0][row];
+#pragma unroll
+        for (int x = 1; x < W; ++x) m = fmaxf(m, state[x][0][row]);
+        l = w = 0.0f;
+#pragma unroll
+        for (int x = 0; x < W; ++x) {
+            const float d = (state[x][0][row] - m) * kLog2e, f = __builtin_amdgcn_exp2f(d);
+            w += f * fmaf(state[x][1][row], d, state[x][2][row]);
+            l += f * state[x][1][row];
+        }
+        float* p = j.part + row * j.splits + blockIdx.x;
+        const int64_t next = j.rows_pad * j.splits;
+        p[0] = m;
+        p[next] = l;
+        p[2 * next] = w;
     }
 }
 
 // s_rj in 64 bits for the given and the top items: exact products, f64 sums.  LANES neighbouring
 // lanes share an item (every lane gets the sum); u: the user's row in LDS.
 template <int T, int LANES>
-__device__ __forceinline__ double exact_score(const Job& j, const float* u, int64_t i, int lane) {
+__device__ __forceinline__ double exact_score(const Job& j, const double* u, int64_t i, int lane) {
     double a = 0.0;
     const int64_t at = i * j.v.ld;
-    if (j.vec4) {  // rows of whole groups of 4 factors, aligned: one load per group
-        for (int f = 4 * lane; f < j.k; f += 4 * LANES) {
-            float x[4];
-            if constexpr (T == MML_DTYPE_F32) {
-                const f32x4 v = *(const f32x4*)((const float*)j.v.src + at + f);
-                x[0] = v[0], x[1] = v[1], x[2] = v[2], x[3] = v[3];
-            } else {
-                const uint2 v = *(const uint2*)((const uint16_t*)j.v.src + at + f);
-                const uint32_t w[2] = {v.x, v.y};
+    if (j.v.vec8 && j.k % 8 == 0) {  // whole groups of 8 factors in loads of 16 bytes
+#pragma unroll 4
+        for (int f = 8 * lane; f < j.k; f += 8 * LANES) {
+            float x[8];
+            load_factors<T>(j.v.src, at + f, x);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const uint16_t b = (uint16_t)(w[e >> 1] >> (16 * (e & 1)));
-                    x[e] = T == MML_DTYPE_F16 ? (float)__builtin_bit_cast(_Float16, b)
-                                              : __uint_as_float((uint32_t)b << 16);
-                }
-            }
-#pragma unroll
-            for (int e = 0; e < 4; ++e) a = fma((double)u[f + e], (double)x[e], a);
+            for (int e = 0; e < 8; ++e) a = fma(u[f + e], (double)x[e], a);
         }
     } else {
         for (int f = lane; f < j.k; f += LANES)
-            a = fma((double)u[f], (double)load_factor<T>(j.v.src, at + f), a);
+            a = fma(u[f], (double)load_factor<T>(j.v.src, at + f), a);
     }
 #pragma unroll
     for (int d = 1; d < LANES; d <<= 1) a += __shfl_xor(a, d);
     return a + (j.bias ? (double)j.bias[i] : 0.0);
 }
 __device__ __forceinline__ bool is_excluded(const Job& j, int64_t r, int64_t i) {
-    return j.vbias[i] <= j.scale->gone ||
+    return (j.bias && j.bias[i] <= kGone) ||
            (j.mask && (j.mask[(i >> 5) * j.rows_pad + r] >> (i & 31) & 1u));
 }
 // A double as an unsigned key in the same order (-inf is the smallest that occurs)
@@ -809,39 +985,62 @@ __device__ __forceinline__ uint32_t key_of(float x) {
 
 constexpr int kListed = 1024;  // tiles that the selection below lists at most
 
-// The `want` tiles with the largest maxima cm[0 .. tiles), ordered, the lower tile first among
-// equals.  The want-th largest of the 256 threads' own maxima is a lower bound of the want-th
-// largest maximum, so few tiles are at or above it; they are listed and ranked by counting.  Where
-// more than kListed are (many equal maxima), they are taken one after another.
-__device__ __forceinline__ void select_tiles(const float* __restrict__ cm, int tiles, int want,
-                                             int32_t* chosen, uint32_t* key, int32_t* index) {
-    __shared__ int32_t count;
-    __shared__ uint32_t bound;
-    const int t = threadIdx.x;
+// A bound that at least `want` of the 256 keys reach and few more: the want-th largest key with its
+// low bits cut off, found bit by bit.  One wave, four keys a lane.
+__device__ __forceinline__ uint32_t bound_of(const uint32_t* key, int want) {
+    uint32_t k[4], b = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) k[i] = key[(threadIdx.x & 63) + 64 * i];
+#pragma unroll 1
+    for (int bit = 31; bit >= 12; --bit) {
+        const uint32_t c = b | 1u << bit;
+        int n = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) n += __builtin_popcountll(__ballot(k[i] >= c));
+        if (n >= want) b = c;
+    }
+    return b;
+}
+// The largest of this thread's share of the tiles' maxima (the tiles are a multiple of 8)
+template <int NT>
+__device__ __forceinline__ uint32_t largest_of(const float* __restrict__ cm, int tiles) {
     uint32_t mine = 0;
-    for (int x = t; x < tiles; x += 256) mine = max(mine, key_of(cm[x]));
-    key[t] = mine;
-    if (t == 0) count = 0;
-    __syncthreads();
-    int rank = 0;
-    for (int x = 0; x < 256; ++x) rank += before(key[x], x, mine, t);
-    if (rank == want - 1) bound = mine;
-    __syncthreads();
-    const uint32_t least = bound;
-    for (int x = t; x < tiles; x += 256) {
-        const uint32_t v = key_of(cm[x]);
-        if (v >= least) {
-            const int at = atomicAdd(&count, 1);
-            if (at < kListed) {
-                key[at] = v;
-                index[at] = x;
+#pragma unroll 4
+    for (int x = 4 * threadIdx.x; x < tiles; x += 4 * NT) {
+        const f32x4 v = *(const f32x4*)(cm + x);
+        mine = max(mine, key_of(fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3]))));
+    }
+    return mine;
+}
+
+// The `want` tiles with the largest maxima cm[0 .. tiles), ordered, the lower tile first among
+// equals.  `least` is under the want-th largest of 256 partial maxima, which is a lower
+// bound of the want-th largest maximum, so few tiles are at or above it: they are listed and ranked
+// by counting.  Where more than kListed are (many equal maxima), they are taken one after another.
+template <int NT>
+__device__ __forceinline__ void select_tiles(const float* __restrict__ cm, int tiles, int want,
+                                             uint32_t least, int32_t* chosen, uint32_t* key,
+                                             int32_t* index, int32_t& count) {
+    const int t = threadIdx.x;
+#pragma unroll 4
+    for (int x = 4 * t; x < tiles; x += 4 * NT) {
+        const f32x4 q = *(const f32x4*)(cm + x);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const uint32_t v = key_of(q[e]);
+            if (v >= least) {
+                const int at = atomicAdd(&count, 1);
+                if (at < kListed) {
+                    key[at] = v;
+                    index[at] = x + e;
+                }
             }
         }
     }
     __syncthreads();
     const int n = count;
     if (n <= kListed) {
-        for (int x = t; x < n; x += 256) {
+        for (int x = t; x < n; x += NT) {
             const uint32_t v = key[x];
             const int32_t i = index[x];
             int r = 0;
@@ -856,7 +1055,7 @@ __device__ __forceinline__ void select_tiles(const float* __restrict__ cm, int t
     for (int c = 0; c < want; ++c) {
         uint32_t bv = 0;
         int32_t bi = 0x7FFFFFFF;
-        for (int x = t; x < tiles; x += 256) {
+        for (int x = t; x < tiles; x += NT) {
             const uint32_t v = key_of(cm[x]);
             if (before(lv, li, v, x) && before(v, x, bv, bi)) bv = v, bi = x;
         }
@@ -870,7 +1069,7 @@ __device__ __forceinline__ void select_tiles(const float* __restrict__ cm, int t
         if ((t & 63) == 0) key[t >> 6] = bv, index[t >> 6] = bi;
         __syncthreads();
         bv = key[0], bi = index[0];
-        for (int w = 1; w < 4; ++w)
+        for (int w = 1; w < NT / 64; ++w)
             if (before(key[w], index[w], bv, bi)) bv = key[w], bi = index[w];
         lv = bv, li = bi;
         if (t == 0) chosen[c] = bi;
@@ -878,64 +1077,72 @@ __device__ __forceinline__ void select_tiles(const float* __restrict__ cm, int t
     __syncthreads();
 }
 
-// One block per row (256 threads with top items, 64 without): the splits' states joined, the
+// One block per row (64 threads; with top items 256, or 1,024 where the rows are too few to fill the
+// GPU): the splits' states joined, the
 // outputs, and the top items.  The n best items lie in the n tiles with the largest maxima (lower
 // tile first among equals); two more tiles cover the rounding of the maxima.  Their items are
 // scored again in 64 bits, so the order is that of the exact scores.  The n-th largest of the tiles'
 // exact maxima bounds the n-th best score from below: the items at or above it are ranked by
 // counting.  Dynamic LDS: the candidates' keys, 8 bytes each.
-template <int T, bool TOP>
-__global__ __launch_bounds__(TOP ? 256 : 64) void softmax_finish_kernel(Job j) {
-    constexpr int NT = TOP ? 256 : 64;
-    __shared__ float urow[256];
-    __shared__ double join[3][NT / 64];
+template <int T, int NT>
+__global__ __launch_bounds__(NT) void softmax_finish_kernel(Job j) {
+    constexpr bool TOP = NT > 64;
+    __shared__ double urow[256], joined[2];
+    __shared__ uint32_t key[TOP ? kListed : 1], least_tile;
     const int64_t r = blockIdx.x;
     const int t = threadIdx.x;
     const int64_t u = source_row(j.u, r);
-    for (int f = t; f < j.k; f += NT)
-        urow[f] = u >= 0 ? load_factor<T>(j.u.src, u * j.u.ld + f) : 0.0f;
-    const Scale sc = *j.scale;
-    float m = sc.floor;
-    for (int s = t; s < j.splits; s += NT) m = fmaxf(m, j.part[(int64_t)s * 3 * j.rows_pad + r]);
-#pragma unroll
-    for (int d = 32; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor(m, d));
+    uint32_t mine = 0;
     if (TOP) {
-        if ((t & 63) == 0) join[0][t >> 6] = m;
-        __syncthreads();
-        for (int w = 0; w < NT / 64; ++w) m = fmaxf(m, (float)join[0][w]);
+        mine = largest_of<NT>(j.cmax + r * j.cpad, j.v.tiles);
+        if (t < 256) key[t] = mine;
     }
-    double l = 0.0, w = 0.0;
-    for (int s = t; s < j.splits; s += NT) {
-        const float* p = j.part + (int64_t)s * 3 * j.rows_pad + r;
-        const double d = ((double)p[0] - m) * sc.unit * 1.4426950408889634;
-        const double f = exp2(d);
-        w += f * ((double)p[2 * j.rows_pad] + (double)p[j.rows_pad] * d);
-        l += f * p[j.rows_pad];
+    bool bad = u < 0;  // an unknown user, or factors that are not finite
+    for (int f = t & 63; f < j.k; f += 64) {  // every wave checks the whole row, wave 0 keeps it
+        const float x = u >= 0 ? load_factor<T>(j.u.src, u * j.u.ld + f) : 0.0f;
+        bad = bad || !(fabsf(x) < 3e38f);
+        if (t < 64) urow[f] = (double)x;
     }
+    bad = __any(bad);
+    if (t < 64) {  // the splits' states
+        const Scale sc = j.scale ? *j.scale : plain_scale();
+        const float* part = j.part + r * j.splits;
+        const int64_t next = j.rows_pad * j.splits;
+        float m = sc.floor;
+        for (int s = t; s < j.splits; s += 64) m = fmaxf(m, part[s]);
 #pragma unroll
-    for (int d = 32; d > 0; d >>= 1) {
-        l += __shfl_xor(l, d);
-        w += __shfl_xor(w, d);
+        for (int d = 32; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor(m, d));
+        double l = 0.0, w = 0.0;
+        for (int s = t; s < j.splits; s += 64) {
+            const double d = ((double)part[s] - m) * sc.unit * 1.4426950408889634;
+            const double f = __builtin_amdgcn_exp2f((float)d), ls = part[s + next];
+            w += f * ((double)part[s + 2 * next] + ls * d);
+            l += f * ls;
+        }
+#pragma unroll
+        for (int d = 32; d > 0; d >>= 1) {
+            l += __shfl_xor(l, d);
+            w += __shfl_xor(w, d);
+        }
+        double lse = (double)m * sc.unit + log(l), H = log(l) - 0.69314718055994531 * w / l;
+        if (m <= sc.floor && l == l) lse = -INFINITY, H = 0.0;  // no item left
+        if (bad) lse = H = __builtin_nan("");
+        if (t == 0) joined[0] = lse, joined[1] = H;
     }
-    if (TOP) {
-        if ((t & 63) == 0) join[1][t >> 6] = l, join[2][t >> 6] = w;
-        __syncthreads();
-        l = w = 0.0;
-        for (int x = 0; x < NT / 64; ++x) l += join[1][x], w += join[2][x];
-    } else {
+    __syncthreads();
+    if (NT > 256) {
+        if (t >= 256) atomicMax(&key[t & 255], mine);
         __syncthreads();
     }
-    const bool empty = m <= sc.floor && l == l;
-    double lse = (double)m * sc.unit + log(l), H = log(l) - 0.69314718055994531 * w / l;
-    if (empty) lse = -INFINITY, H = 0.0;
-    if (j.ubad[r]) lse = H = __builtin_nan("");
-    if (t < 64) {
+    const double lse = joined[0];
+    if (t >= NT - 64) {  // the last wave
         const int32_t g = j.target ? j.target[r] : -1;
         double lp = 0.0;
         if (lse != lse) lp = lse;
         else if (g >= 0 && g < j.n_items)
-            lp = is_excluded(j, r, g) ? -INFINITY : exact_score<T, 64>(j, urow, g, t) - lse;
-        if (t == 0) {
+            lp = is_excluded(j, r, g) ? -INFINITY : exact_score<T, 64>(j, urow, g, t & 63) - lse;
+        if (t == NT - 1) {
+            const double H = joined[1];
             j.log_probs[r] = (float)lp;
             j.log_norm[r] = (float)lse;
             j.entropy[r] = (float)(H < 0.0 ? 0.0 : H);
@@ -943,23 +1150,28 @@ __global__ __launch_bounds__(TOP ? 256 : 64) void softmax_finish_kernel(Job j) {
     }
     if constexpr (TOP) {
         extern __shared__ uint64_t cand[];
-        __shared__ uint32_t key[kListed];
-        __shared__ int32_t index[kListed], chosen[kMaxTop + 2], count;
+        __shared__ int32_t index[kListed], chosen[kMaxTop + 2], count, found_tiles;
         __shared__ unsigned long long tmax[kMaxTop + 2], bound;
         const int n = j.n_top;
-        if (lse != lse || empty) {
-            for (int x = t; x < n; x += 256) {
+        if (lse != lse || lse == -INFINITY) {
+            for (int x = t; x < n; x += NT) {
                 j.top_items[r * n + x] = -1;
-                j.top_lp[r * n + x] = (float)(empty ? -INFINITY : lse);
+                j.top_lp[r * n + x] = (float)lse;
             }
             return;
         }
         const int want = min(n + 2, j.v.tiles);
+        if (t < 64) {
+            const uint32_t b = bound_of(key, want);
+            if (t == 0) least_tile = b;
+        }
         if (t < want) tmax[t] = 0;
-        if (t == 0) count = 0, bound = 0;
-        select_tiles(j.cmax + r * j.cpad, j.v.tiles, want, chosen, key, index);
+        if (t == 0) count = found_tiles = 0, bound = 0;
+        __syncthreads();
+        select_tiles<NT>(j.cmax + r * j.cpad, j.v.tiles, want, least_tile, chosen, key, index,
+                     found_tiles);
         const uint64_t none = key_of(-INFINITY);
-        for (int x = t >> 2; x < want * 32; x += 64) {
+        for (int x = t >> 2; x < want * 32; x += NT / 4) {
             const int64_t i = (int64_t)chosen[x >> 5] * 32 + (x & 31);
             uint64_t k = none;
             if (i < j.n_items && !is_excluded(j, r, i))
@@ -977,7 +1189,7 @@ __global__ __launch_bounds__(TOP ? 256 : 64) void softmax_finish_kernel(Job j) {
         }
         __syncthreads();
         const uint64_t least = max((uint64_t)bound, none + 1);
-        for (int x = t; x < want * 32; x += 256)
+        for (int x = t; x < want * 32; x += NT)
             if (cand[x] >= least) {
                 const int at = atomicAdd(&count, 1);
                 if (at < kListed) index[at] = x;
@@ -985,7 +1197,7 @@ __global__ __launch_bounds__(TOP ? 256 : 64) void softmax_finish_kernel(Job j) {
         __syncthreads();
         const int found = count;
         const bool listed = found <= kListed;
-        for (int y = t; y < (listed ? found : want * 32); y += 256) {
+        for (int y = t; y < (listed ? found : want * 32); y += NT) {
             const int x = listed ? index[y] : y;
             const uint64_t v = cand[x];
             if (v < least) continue;
@@ -1000,7 +1212,7 @@ __global__ __launch_bounds__(TOP ? 256 : 64) void softmax_finish_kernel(Job j) {
                 j.top_lp[r * n + rank] = (float)(value_of(v) - lse);
             }
         }
-        for (int x = found + t; x < n; x += 256) {
+        for (int x = found + t; x < n; x += NT) {
             j.top_items[r * n + x] = -1;
             j.top_lp[r * n + x] = -INFINITY;
         }
@@ -1041,7 +1253,7 @@ constexpr int items_per_simd() {
 }
 template <int T, int KT>
 constexpr int items_in_lds() {
-    return T == MML_DTYPE_F32 ? 0 : KT == 8 ? 3 : KT == 16 ? (T == MML_DTYPE_F16 ? 8 : 6) : 0;
+    return T == MML_DTYPE_F32 ? 0 : KT == 8 ? 4 : KT == 16 ? (T == MML_DTYPE_F16 ? 8 : 6) : 0;
 }
 
 // Users' side: as the forward pass, G in place of the softmax state, dU += G V.
@@ -1392,9 +1604,8 @@ int64_t plan(const mml_item_softmax_args* a, bool grad, void* base, Job& j) {
     j.rows_pad = (int64_t)j.u.tiles * 32;
     const int64_t items_pad = (int64_t)j.v.tiles * 32;
     j.bias = a->item_bias;
+    j.bias_vec4 = (uintptr_t)a->item_bias % 16 == 0;
     j.target = a->items;
-    j.vec4 = a->num_factors % 4 == 0 && a->ld_items % 4 == 0 &&
-             (uintptr_t)a->item_factors % (4 * size) == 0;
     j.ex_off = a->exclude_offsets;
     j.ex_items = a->exclude_items;
     j.n_ex = a->n_exclude;
@@ -1407,6 +1618,11 @@ int64_t plan(const mml_item_softmax_args* a, bool grad, void* base, Job& j) {
             j.vsplits = choose_splits(j.v.tiles, j.u.tiles, kItemsWaves, items_per_simd<TT, KT>(),
                                       M, mt * 4096.0);
         });
+    } else if (a->n_rows <= kDirectRows) {
+        // two tiles or more a wave, up to 8 waves a SIMD
+        j.direct = 1;
+        j.splits = (int32_t)std::max<int64_t>(
+            1, std::min<int64_t>((j.v.tiles + 2 * kDirectWaves - 1) / (2 * kDirectWaves), 2048));
     } else {
         dispatch(T, kt, [&](auto tt, auto k) {
             constexpr int TT = decltype(tt)::value, KT = decltype(k)::value;
@@ -1417,12 +1633,14 @@ int64_t plan(const mml_item_softmax_args* a, bool grad, void* base, Job& j) {
         });
     }
     Carve c{(char*)base};
-    j.scale = c.take<Scale>(1);
-    if (T == MML_DTYPE_F32) j.parts = c.take<float>(kMaxParts);
-    j.u.frag = c.take<uint4>((int64_t)j.u.tiles * ps * kt * 64);
-    j.v.frag = c.take<uint4>((int64_t)j.v.tiles * ps * kt * 64);
-    j.vbias = c.take<float>(items_pad);
-    j.ubad = c.take<uint8_t>(j.rows_pad);
+    if (!j.direct) {
+        j.scale = c.take<Scale>(1);
+        if (T == MML_DTYPE_F32) j.parts = c.take<float>(kMaxParts);
+        j.u.frag = c.take<uint4>((int64_t)j.u.tiles * ps * kt * 64);
+        j.v.frag = c.take<uint4>((int64_t)j.v.tiles * ps * kt * 64);
+        j.vbias = c.take<float>(items_pad);
+        j.ubad = c.take<uint8_t>(j.rows_pad);
+    }
     if (a->exclude_offsets) j.mask = c.take<uint32_t>((int64_t)j.v.tiles * j.rows_pad);
     if (!grad) {
         j.part = c.take<float>((int64_t)j.splits * 3 * j.rows_pad);
@@ -1439,7 +1657,7 @@ int64_t plan(const mml_item_softmax_args* a, bool grad, void* base, Job& j) {
             j.db_part = c.take<float>((int64_t)j.vsplits * items_pad);
         }
     }
-    return c.used;
+    return std::max<int64_t>(c.used, 256);
 }
 
 uint32_t grid_of(int64_t n) {
@@ -1447,13 +1665,14 @@ uint32_t grid_of(int64_t n) {
     return (uint32_t)n;
 }
 
-void mask_and_prep(const Job& j, int T, hipStream_t st) {
-    if (j.mask) {
-        const int64_t words = (int64_t)j.v.tiles * j.rows_pad;
-        softmax_clear_kernel<<<(uint32_t)std::min<int64_t>((words + 255) / 256, 8192), 256, 0, st>>>(
-            j.mask, words);
-        softmax_mask_kernel<<<grid_of((j.n_rows + 3) / 4), 256, 0, st>>>(j);
-    }
+void make_mask(const Job& j, hipStream_t st) {
+    if (!j.mask) return;
+    const int64_t words = (int64_t)j.v.tiles * j.rows_pad;
+    softmax_clear_kernel<<<(uint32_t)std::min<int64_t>((words + 255) / 256, 8192), 256, 0, st>>>(
+        j.mask, words);
+    softmax_mask_kernel<<<grid_of((j.n_rows + 3) / 4), 256, 0, st>>>(j);
+}
+void prepare(const Job& j, int T, hipStream_t st) {
     if (T == MML_DTYPE_F32) softmax_max_kernel<MML_DTYPE_F32><<<kMaxParts, 256, 0, st>>>(j);
     dispatch(T, steps_of(j.k), [&](auto tt, auto kt) {
         softmax_prep_kernel<decltype(tt)::value, decltype(kt)::value>
@@ -1489,10 +1708,18 @@ void item_log_probs(const mml_item_softmax_args* a, float* log_probs, float* log
     j.entropy = entropy;
     j.top_items = top_items;
     j.top_lp = top_log_probs;
-    mask_and_prep(j, a->dtype, st);
+    make_mask(j, st);
+    if (!j.direct) prepare(j, a->dtype, st);
     dispatch(a->dtype, steps_of(j.k), [&](auto tt, auto kt) {
         constexpr int T = decltype(tt)::value, KT = decltype(kt)::value;
         constexpr int W = forward_waves<T, KT>();
+        if (j.direct) {
+            if (j.n_top)
+                softmax_direct_kernel<T, KT, true><<<j.splits, kDirectWaves * 64, 0, st>>>(j);
+            else
+                softmax_direct_kernel<T, KT, false><<<j.splits, kDirectWaves * 64, 0, st>>>(j);
+            return;
+        }
         const uint32_t blocks = grid_of((int64_t)((j.u.tiles + W - 1) / W) * j.splits);
         if (j.n_top)
             softmax_forward_kernel<T, KT, true><<<blocks, W * 64, 0, st>>>(j);
@@ -1502,10 +1729,12 @@ void item_log_probs(const mml_item_softmax_args* a, float* log_probs, float* log
     const uint32_t lds = std::min(j.n_top + 2, j.v.tiles) * 32 * sizeof(uint64_t);
     dispatch(a->dtype, 1, [&](auto tt, auto) {
         constexpr int T = decltype(tt)::value;
-        if (j.n_top)
-            softmax_finish_kernel<T, true><<<grid_of(j.n_rows), 256, lds, st>>>(j);
+        if (!j.n_top)
+            softmax_finish_kernel<T, 64><<<grid_of(j.n_rows), 64, 0, st>>>(j);
+        else if (j.n_rows <= 512)
+            softmax_finish_kernel<T, 1024><<<grid_of(j.n_rows), 1024, lds, st>>>(j);
         else
-            softmax_finish_kernel<T, false><<<grid_of(j.n_rows), 64, 0, st>>>(j);
+            softmax_finish_kernel<T, 256><<<grid_of(j.n_rows), 256, lds, st>>>(j);
     });
     MML_HIP(hipGetLastError());
 }
@@ -1548,7 +1777,8 @@ void item_log_probs_grad(const mml_item_softmax_args* a, const float* log_norm,
     j.gv_vec4 = j.k % 4 == 0 && ld_gv % 4 == 0 && (uintptr_t)gv % (4 * size) == 0;
     const int kt0 = steps_of(j.k), kp = std::max(32, kt0 * 16);
     if (a->n_rows > 0) {
-        mask_and_prep(j, a->dtype, st);
+        make_mask(j, st);
+        prepare(j, a->dtype, st);
         softmax_meta_kernel<<<grid_of((j.rows_pad + 255) / 256), 256, 0, st>>>(j);
     }
     const int64_t quads = (j.k + 3) / 4;
