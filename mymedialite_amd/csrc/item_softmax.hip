@@ -48,6 +48,9 @@ using f32x4 = __attribute__((ext_vector_type(4))) float;
 using u32x4 = __attribute__((ext_vector_type(4))) uint32_t;
 using bf16x8 = __attribute__((ext_vector_type(8))) __bf16;
 using f16x8 = __attribute__((ext_vector_type(8))) _Float16;
+using f32x2 = __attribute__((ext_vector_type(2))) float;
+using bf16x2 = __attribute__((ext_vector_type(2))) __bf16;
+using f16x2 = __attribute__((ext_vector_type(2))) _Float16;
 
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr float kLn2 = 0.69314718055994530942f;
@@ -169,7 +172,7 @@ struct Job {
     float* vbias;        // [v.tiles * 32]: bias 2^(eu + ev), scale->gone for an excluded or padding
                          // item, NaN where the factors are not finite
     uint8_t* ubad;       // [u.tiles * 32]: 1 = factors not finite, 2 = unknown user
-    uint32_t* mask;      // [v.tiles][rows_pad]: bit i of word (tile, r): item 32 tile + i excluded
+    uint32_t* mask;      // [rows_pad][v.tiles]: bit i of word (r, tile): item 32 tile + i excluded
     int64_t rows_pad;    // u.tiles * 32
     const int64_t* ex_off;
     const int32_t* ex_items;
@@ -223,25 +226,29 @@ __device__ __forceinline__ uint32_t take_plane(float& v) {
     }
 }
 
-__global__ __launch_bounds__(256) void softmax_clear_kernel(uint32_t* p, int64_t n) {
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256)
-        p[i] = 0;
-}
-
-// One wave per row sets the bits of its user's exclusion list.  The lists may be unsorted and may
-// repeat an item (an OR of bits does not depend on the order); ids outside the catalogue and
-// offsets outside the array are skipped.
+// The exclusion lists as bits: a block makes up to kMaskWords words of a row in LDS and writes them.  The
+// lists may be unsorted and may repeat an item (an OR of bits does not depend on the order); ids
+// outside the catalogue and offsets outside the array are skipped.
+constexpr int kMaskWords = 16384;
 __global__ __launch_bounds__(256) void softmax_mask_kernel(Job j) {
-    const int64_t r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (r >= j.n_rows) return;
+    extern __shared__ uint32_t words[];
+    const int parts = (j.v.tiles + kMaskWords - 1) / kMaskWords;
+    const int64_t r = blockIdx.x / parts;
+    const int w0 = (int)(blockIdx.x % parts) * kMaskWords, n = min(kMaskWords, j.v.tiles - w0);
+    for (int x = threadIdx.x; x < n; x += 256) words[x] = 0;
     const int64_t u = source_row(j.u, r);
-    if (u < 0) return;
-    const int64_t b = clamp64(j.ex_off[u], 0, j.n_ex), e = clamp64(j.ex_off[u + 1], 0, j.n_ex);
-    for (int64_t x = b + (threadIdx.x & 63); x < e; x += 64) {
+    int64_t b = 0, e = 0;
+    if (u >= 0) b = clamp64(j.ex_off[u], 0, j.n_ex), e = clamp64(j.ex_off[u + 1], 0, j.n_ex);
+    __syncthreads();
+    for (int64_t x = b + threadIdx.x; x < e; x += 256) {
         const int32_t i = j.ex_items[x];
-        if (i >= 0 && i < j.n_items)
-            atomicOr(&j.mask[(int64_t)(i >> 5) * j.rows_pad + r], 1u << (i & 31));
+        const int at = (i >> 5) - w0;
+        if (i >= 0 && i < j.n_items && at >= 0 && at < n) atomicOr(&words[at], 1u << (i & 31));
     }
+    __syncthreads();
+    uint32_t* out = j.mask + r * j.v.tiles + w0;
+    for (int x = 4 * threadIdx.x; x < n; x += 1024)  // (the tiles are a multiple of 8)
+        *(uint4*)(out + x) = *(const uint4*)(words + x);
 }
 
 // The largest finite magnitude of either matrix (the batch's users only), in kMaxParts parts.
@@ -421,7 +428,7 @@ __global__ __launch_bounds__(256) void softmax_meta_kernel(Job j) {
         const float lse = j.in_norm[r], h = j.g_ent ? j.g_ent[r] : 0.0f;
         int32_t t = j.target ? j.target[r] : -1;
         if (t < 0 || t >= j.n_items || j.vbias[t] <= j.scale->gone ||
-            (j.mask && (j.mask[(int64_t)(t >> 5) * j.rows_pad + r] >> (t & 31) & 1u)))
+            (j.mask && (j.mask[r * j.v.tiles + (t >> 5)] >> (t & 31) & 1u)))
             t = -1;
         w = t >= 0 && j.g_lp ? j.g_lp[r] : 0.0f;
         if ((w != 0.0f || h != 0.0f) && lse != -INFINITY) {
@@ -525,25 +532,26 @@ __device__ __forceinline__ void load_kept(const uint4* __restrict__ frag, int64_
         }
 }
 
+// Two values as two f16 planes, both rounded to nearest
+__device__ __forceinline__ void split_pair(float x, float y, uint32_t& hi, uint32_t& lo) {
+    float minus = -1.0f;  // unknown to the compiler, so that x - hi is one v_fma_mix_f32
+    asm("" : "+s"(minus));
+    const f16x2 h = __builtin_convertvector((f32x2{x, y}), f16x2);
+    const f32x2 rest = {fmaf((float)h[0], minus, x), fmaf((float)h[1], minus, y)};
+    hi = __builtin_bit_cast(uint32_t, h);
+    lo = __builtin_bit_cast(uint32_t, __builtin_convertvector(rest, f16x2));
+}
 // The planes of G's registers 8 s .. 8 s + 7 as B operands.  bf16: the first plane is cut off, so
 // the second starts from the exact rest; the second is rounded to nearest.  f16: both rounded to
 // nearest.
 template <int T>
 __device__ __forceinline__ void split_g(const float (&g)[16], int step, uint4 (&q)[2]) {
-    using f32x2 = __attribute__((ext_vector_type(2))) float;
-    using bf16x2 = __attribute__((ext_vector_type(2))) __bf16;
-    using f16x2 = __attribute__((ext_vector_type(2))) _Float16;
     uint32_t w[2][4];
-    float minus = -1.0f;  // unknown to the compiler, so that x - hi is one v_fma_mix_f32
-    asm("" : "+s"(minus));
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
         const f32x2 x = {g[8 * step + 2 * e], g[8 * step + 2 * e + 1]};
         if constexpr (Planes<T>::HALF) {
-            const f16x2 hi = __builtin_convertvector(x, f16x2);
-            const f32x2 rest = {fmaf((float)hi[0], minus, x[0]), fmaf((float)hi[1], minus, x[1])};
-            w[0][e] = __builtin_bit_cast(uint32_t, hi);
-            w[1][e] = __builtin_bit_cast(uint32_t, __builtin_convertvector(rest, f16x2));
+            split_pair(x[0], x[1], w[0][e], w[1][e]);
         } else {
             const uint32_t a = __float_as_uint(x[0]), b = __float_as_uint(x[1]);
             const f32x2 rest = {x[0] - __uint_as_float(a & 0xFFFF0000u),
@@ -680,7 +688,7 @@ softmax_forward_kernel(Job j) {
     uint32_t bits[TPS] = {}, next[TPS] = {};
     const auto load_bits = [&](int tl) {
 #pragma unroll
-        for (int x = 0; x < TPS; ++x) next[x] = j.mask[(int64_t)(tl + x) * j.rows_pad + row];
+        for (int x = 0; x < TPS; ++x) next[x] = j.mask[row * j.v.tiles + tl + x];
     };
     // a turn's maxima leave in the next turn, so that no wait meets the stores
     const auto store_max = [&](int tl) {
@@ -789,23 +797,24 @@ __device__ __forceinline__ void load_rows(const Side& s, int64_t src, int k, int
         }
     }
 }
+// (What a row holds reaches its own scores only, so values that are not finite need no zeros here.)
 template <int T, int KT>
-__device__ __forceinline__ int make_planes(float (&v)[KT][8], uint4 (&q)[Planes<T>::PS][KT],
+__device__ __forceinline__ int make_planes(const float (&v)[KT][8], uint4 (&q)[Planes<T>::PS][KT],
                                            bool& finite) {
     using P = Planes<T>;
-    float most = 0.0f;
-    finite = true;
+    float most = 0.0f, zero = 0.0f;
 #pragma unroll
     for (int ks = 0; ks < KT; ++ks)
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-            const float a = fabsf(v[ks][e]);
-            finite = finite && a < 3e38f;
-            if (T == MML_DTYPE_F32) most = fmaxf(most, a < 3e38f ? a : 0.0f);
+            zero = fmaf(v[ks][e], 0.0f, zero);  // NaN from the first value that is not finite on
+            if (T == MML_DTYPE_F32) most = fmaxf(most, fabsf(v[ks][e]));
         }
+    finite = zero == 0.0f && most < 3e38f;
     int ex = 0;
     float mul = 1.0f;
     if constexpr (T == MML_DTYPE_F32) {
+        if (!finite) most = 0.0f;
 #pragma unroll
         for (int d = 32; d > 0; d >>= 1) most = fmaxf(most, __shfl_xor(most, d));
         ex = max(-40, min(12, 13 - __builtin_amdgcn_frexp_expf(most)));
@@ -813,17 +822,20 @@ __device__ __forceinline__ int make_planes(float (&v)[KT][8], uint4 (&q)[Planes<
     }
 #pragma unroll
     for (int ks = 0; ks < KT; ++ks) {
-        uint32_t w[P::PS][8];
+        uint32_t w[P::PS][4];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            float x = finite ? v[ks][e] * mul : 0.0f;
-#pragma unroll
-            for (int p = 0; p < P::PS; ++p) w[p][e] = take_plane<T>(x);
+        for (int e = 0; e < 4; ++e) {
+            const float x = v[ks][2 * e], y = v[ks][2 * e + 1];
+            if constexpr (T == MML_DTYPE_F32) {
+                split_pair(x * mul, y * mul, w[0][e], w[P::PS - 1][e]);
+            } else if constexpr (T == MML_DTYPE_F16) {
+                w[0][e] = __builtin_bit_cast(uint32_t, f16x2{(_Float16)x, (_Float16)y});
+            } else {
+                w[0][e] = __float_as_uint(x) >> 16 | (__float_as_uint(y) & 0xFFFF0000u);
+            }
         }
 #pragma unroll
-        for (int p = 0; p < P::PS; ++p)
-            q[p][ks] = make_uint4(w[p][0] | w[p][1] << 16, w[p][2] | w[p][3] << 16,
-                                  w[p][4] | w[p][5] << 16, w[p][6] | w[p][7] << 16);
+        for (int p = 0; p < P::PS; ++p) q[p][ks] = make_uint4(w[p][0], w[p][1], w[p][2], w[p][3]);
     }
     return ex;
 }
@@ -864,7 +876,7 @@ __global__ __launch_bounds__(kDirectWaves * 64) void softmax_direct_kernel(Job j
             }
         }
         const uint32_t bits =
-            j.mask ? j.mask[(int64_t)tl * j.rows_pad + row] >> (4 * h) : 0;
+            j.mask ? j.mask[row * (int64_t)j.v.tiles + tl] >> (4 * h) : 0;
         uint4 a[PS][KT];
         if (!AHEAD) load_rows<T, KT>(j.v, source_row(j.v, (int64_t)tl * 32 + row), j.k, h, v);
         const int ev = make_planes<T, KT>(v, a, finite);
@@ -879,20 +891,21 @@ __global__ __launch_bounds__(kDirectWaves * 64) void softmax_direct_kernel(Job j
 #pragma unroll
                 for (int p = sum; p >= 0; --p) c = mfma<T>(a[p][ks], b[sum - p][ks], c);
         const float unit = ldexpf(1.0f, -eu - ev);
+        bool strange = odd != 0;  // a factor or a bias that is not finite: rarely
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-            c[i] = fmaf(c[i], unit, bias[i]);
-            if (!(bias[i] < -kGone)) c[i] = __builtin_nanf("");  // not finite
+            strange = strange || !(bias[i] < -kGone);
+            c[i] = fmaxf(fmaf(c[i], unit, bias[i]), sc.gone);  // (an excluded item's bias is below)
         }
-        if (odd) {
+        if (__any(strange)) {
+            asm volatile("");
             const uint32_t rows = (uint32_t)odd | (uint32_t)(odd >> 32);
 #pragma unroll
-            for (int i = 0; i < 16; ++i)
-                if (rows >> reg_row(i, h) & 1u) c[i] = __builtin_nanf("");
+            for (int i = 0; i < 16; ++i) {
+                if (!(bias[i] < -kGone) || rows >> reg_row(i, h) & 1u) c[i] = __builtin_nanf("");
+                if (bias[i] <= kGone) c[i] = sc.gone;
+            }
         }
-#pragma unroll
-        for (int i = 0; i < 16; ++i)
-            if (bias[i] <= kGone) c[i] = sc.gone;
         if (__any(bits & 0x0F0F0F0Fu)) mask_tile(c, bits, sc.gone);
         float mt = c[0];
 #pragma unroll
@@ -965,7 +978,7 @@ __device__ __forceinline__ double exact_score(const Job& j, const double* u, int
 }
 __device__ __forceinline__ bool is_excluded(const Job& j, int64_t r, int64_t i) {
     return (j.bias && j.bias[i] <= kGone) ||
-           (j.mask && (j.mask[(i >> 5) * j.rows_pad + r] >> (i & 31) & 1u));
+           (j.mask && (j.mask[r * j.v.tiles + (i >> 5)] >> (i & 31) & 1u));
 }
 // A double as an unsigned key in the same order (-inf is the smallest that occurs)
 __device__ __forceinline__ uint64_t key_of(double x) {
@@ -1290,7 +1303,7 @@ softmax_grad_users_kernel(Job j) {
         if (wave == WAVES - 1 && lane < 8)
             copy_to_lds((const f32x4*)j.vbias + tl * 8 + lane, bias[tl & 1]);
         if (NB == 2) load_trans(tl, at);
-        if (j.mask) word = j.mask[(int64_t)tl * j.rows_pad + row];
+        if (j.mask) word = j.mask[row * j.v.tiles + tl];
     };
     if (t0 < t1) load(t0, 0);
     for (int tl = t0, at = 0; tl < t1; ++tl, at ^= NB - 1) {
@@ -1370,7 +1383,7 @@ softmax_grad_items_kernel(Job j) {
         if (wave == WAVES - 1 && lane < 32)
             copy_to_lds((const uint4*)(j.meta + tl) + lane, &mbuf[tl & 1]);
         if (NB == 2) load_trans(tl, at);
-        if (j.mask) next = j.mask[(mine ? vt : 0) * j.rows_pad + tl * 32 + (lane & 31)];
+        if (j.mask) next = j.mask[(tl * 32 + (lane & 31)) * (int64_t)j.v.tiles + (mine ? vt : 0)];
     };
     if (t0 < t1) load(t0, 0);
     for (int tl = t0, at = 0; tl < t1; ++tl, at ^= NB - 1) {
@@ -1667,10 +1680,9 @@ uint32_t grid_of(int64_t n) {
 
 void make_mask(const Job& j, hipStream_t st) {
     if (!j.mask) return;
-    const int64_t words = (int64_t)j.v.tiles * j.rows_pad;
-    softmax_clear_kernel<<<(uint32_t)std::min<int64_t>((words + 255) / 256, 8192), 256, 0, st>>>(
-        j.mask, words);
-    softmax_mask_kernel<<<grid_of((j.n_rows + 3) / 4), 256, 0, st>>>(j);
+    const int64_t parts = (j.v.tiles + kMaskWords - 1) / kMaskWords;
+    softmax_mask_kernel<<<grid_of(j.rows_pad * parts), 256,
+                          std::min(j.v.tiles, kMaskWords) * sizeof(uint32_t), st>>>(j);
 }
 void prepare(const Job& j, int T, hipStream_t st) {
     if (T == MML_DTYPE_F32) softmax_max_kernel<MML_DTYPE_F32><<<kMaxParts, 256, 0, st>>>(j);
