@@ -785,16 +785,28 @@ constexpr int kDirectRows = 32, kDirectWaves = 4;
 template <int T, int KT>
 __device__ __forceinline__ void load_rows(const Side& s, int64_t src, int k, int h,
                                           float (&v)[KT][8]) {
+    if (s.vec8 && k % 8 == 0) {
+        // whole groups: every lane loads (a lane without a group row 0's), so that all loads are on
+        // the way together
 #pragma unroll
-    for (int ks = 0; ks < KT; ++ks) {
-        const int f = 16 * ks + 8 * h;
-        if (src >= 0 && s.vec8 && f + 8 <= k) {
-            load_factors<T>(s.src, src * s.ld + f, v[ks]);
-        } else {
-#pragma unroll
-            for (int e = 0; e < 8; ++e)
-                v[ks][e] = src >= 0 && f + e < k ? load_factor<T>(s.src, src * s.ld + f + e) : 0.0f;
+        for (int ks = 0; ks < KT; ++ks) {
+            const int f = 16 * ks + 8 * h;
+            load_factors<T>(s.src, src >= 0 && f < k ? src * s.ld + f : 0, v[ks]);
         }
+#pragma unroll
+        for (int ks = 0; ks < KT; ++ks) {
+            const bool in = src >= 0 && 16 * ks + 8 * h < k;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[ks][e] = in ? v[ks][e] : 0.0f;
+        }
+    } else {
+#pragma unroll
+        for (int ks = 0; ks < KT; ++ks)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const int f = 16 * ks + 8 * h + e;
+                v[ks][e] = src >= 0 && f < k ? load_factor<T>(s.src, src * s.ld + f) : 0.0f;
+            }
     }
 }
 // (What a row holds reaches its own scores only, so values that are not finite need no zeros here.)
@@ -1587,7 +1599,7 @@ void check_args(const mml_item_softmax_args* a) {
     MML_REQUIRE(a->dtype >= MML_DTYPE_F32 && a->dtype <= MML_DTYPE_F16, "unknown dtype");
     MML_REQUIRE(a->num_factors >= 1 && a->num_factors <= 256, "num_factors must be in [1, 256]");
     MML_REQUIRE(a->n_rows >= 0 && a->n_rows <= (int64_t)1 << 30, "bad n_rows");
-    MML_REQUIRE(a->n_users >= 0 && a->n_items >= 1, "bad n_users or n_items");
+    MML_REQUIRE((a->n_users >= 1 || a->n_rows == 0) && a->n_items >= 1, "bad n_users or n_items");
     MML_REQUIRE(a->n_items <= 0x7FFFFF00, "n_items too large");
     MML_REQUIRE(a->users || a->n_rows <= a->n_users, "more rows than users");
     MML_REQUIRE(a->ld_users >= a->num_factors && a->ld_items >= a->num_factors,

@@ -25,7 +25,7 @@ def workspace(a, grad=0):
 @pytest.mark.parametrize("bad,text", [
     (dict(dtype=3), "dtype"), (dict(dtype=-1), "dtype"), (dict(num_factors=0), "num_factors"),
     (dict(num_factors=257, ld_users=257, ld_items=257), "num_factors"), (dict(n_rows=-1), "n_rows"),
-    (dict(n_rows=5), "more rows"), (dict(n_items=0), "n_items"), (dict(ld_users=7), "stride"),
+    (dict(n_rows=5), "more rows"), (dict(n_items=0), "n_items"), (dict(n_users=0, users=256), "n_users"), (dict(ld_users=7), "stride"),
     (dict(ld_items=7), "stride"), (dict(n_top=129), "n_top"), (dict(n_top=-1), "n_top"),
     (dict(n_exclude=-1), "n_exclude")])
 def test_bad_sizes(bad, text):
