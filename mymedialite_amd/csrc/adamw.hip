@@ -27,7 +27,7 @@ namespace {
 
 constexpr int kBlock = MML_ADAMW_BLOCK;  // values per scale
 constexpr int kChunk = 2048;             // values per block of threads and turn
-constexpr int kMaxTensors = 40;          // 72 bytes each: under the 4 KB of kernel arguments
+constexpr int kMaxTensors = 48;          // 72 bytes each: under the 4 KB of kernel arguments
 constexpr float kPerMax = 1.0f / 448.0f;   // the largest e4m3 value
 constexpr float kE4m3Min = 0.001953125f;   // the smallest that is not zero, 2^-9
 
@@ -38,7 +38,8 @@ struct Tensor {
     float *ms, *vs;
     int64_t n;
     int64_t chunk0;  // the tensor's first chunk in the launch
-    int32_t p_type, g_type;
+    int16_t p_type, g_type;
+    int32_t vec4;    // every array can be read and written 4 values at a time
 };
 
 struct Step {
@@ -46,6 +47,7 @@ struct Step {
     int64_t chunks;
     int32_t n_tensors, last;  // last: this launch ends the step (counts it)
     double lr, beta1, beta2, eps, decay;
+    double log1, log2;  // log2 of the betas
     int32_t* state;  // [0] steps done, [1] blocks that are through
 };
 static_assert(sizeof(Step) <= 4096, "kernel arguments");
@@ -64,6 +66,31 @@ __device__ __forceinline__ void store_as(void* p, int type, int64_t i, float x) 
     } else {
         ((_Float16*)p)[i] = (_Float16)x;
     }
+}
+
+using f32x4 = __attribute__((ext_vector_type(4))) float;
+// Four values at i (a multiple of 4 from an aligned start)
+__device__ __forceinline__ f32x4 load4(const void* p, int type, int64_t i) {
+    if (type == MML_DTYPE_F32) return *(const f32x4*)((const float*)p + i);
+    const uint2 q = *(const uint2*)((const uint16_t*)p + i);
+    const uint32_t w[4] = {q.x & 0xFFFFu, q.x >> 16, q.y & 0xFFFFu, q.y >> 16};
+    f32x4 x;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+        x[e] = type == MML_DTYPE_BF16 ? __uint_as_float(w[e] << 16)
+                                      : (float)__builtin_bit_cast(_Float16, (uint16_t)w[e]);
+    return x;
+}
+__device__ __forceinline__ void store4(void* p, int type, int64_t i, f32x4 x) {
+    if (type == MML_DTYPE_F32) {
+        *(f32x4*)((float*)p + i) = x;
+        return;
+    }
+    uint16_t w[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) store_as(w, type, e, x[e]);
+    *(uint2*)((uint16_t*)p + i) =
+        make_uint2(w[0] | (uint32_t)w[1] << 16, w[2] | (uint32_t)w[3] << 16);
 }
 
 // The update of one value; m and v come and go in f32.
@@ -92,6 +119,39 @@ __device__ __forceinline__ float finite_abs(float x) {
     return a < INFINITY ? a : 0.0f;  // (NaN too)
 }
 
+// The largest of a wave's values, in every lane: within rows of 16 by DPP, across them by the swaps
+__device__ __forceinline__ float wave_max(float x) {
+    const auto dpp = [](float v, auto ctrl) {
+        return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), decltype(ctrl)::value,
+                                                          0xF, 0xF, true));
+    };
+    x = fmaxf(x, dpp(x, std::integral_constant<int, 0xB1>{}));   // quad_perm 1 0 3 2
+    x = fmaxf(x, dpp(x, std::integral_constant<int, 0x4E>{}));   // quad_perm 2 3 0 1
+    x = fmaxf(x, dpp(x, std::integral_constant<int, 0x141>{}));  // row_half_mirror
+    x = fmaxf(x, dpp(x, std::integral_constant<int, 0x140>{}));  // row_mirror
+    const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+    const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+// Four finite values / scale as codes.  The quotients are rounded as a division rounds them: one
+// division for the block's reciprocal y, then q = x y corrected by its remainder (Markstein 1990).
+// Scales under 2^-100 are divided by.
+__device__ __forceinline__ uint32_t encode4(const f32x4 x, float scale, float y) {
+    f32x4 q;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        const float z = x[e] * y;
+        q[e] = fmaf(fmaf(-z, scale, x[e]), y, z);
+    }
+    int w = __builtin_amdgcn_cvt_pk_fp8_f32(q[0], q[1], 0, false);
+    return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(q[2], q[3], w, true);
+}
+__device__ __forceinline__ f32x4 decode4(uint32_t w) {
+    return f32x4{__builtin_amdgcn_cvt_f32_fp8((int)w, 0), __builtin_amdgcn_cvt_f32_fp8((int)w, 1),
+                 __builtin_amdgcn_cvt_f32_fp8((int)w, 2), __builtin_amdgcn_cvt_f32_fp8((int)w, 3)};
+}
+
 template <int BITS>
 __global__ __launch_bounds__(256) void adamw_kernel(Step s) {
     const int t = threadIdx.x;
@@ -99,8 +159,8 @@ __global__ __launch_bounds__(256) void adamw_kernel(Step s) {
     Factors f;
     {
         // in 64 bits: 1 - beta and 1 - beta^t cancel for a beta near 1
-        const double c1 = 1.0 - pow(s.beta1, (double)step);
-        const double c2 = 1.0 - pow(s.beta2, (double)step);
+        const double c1 = 1.0 - exp2(s.log1 * step);
+        const double c2 = 1.0 - exp2(s.log2 * step);
         f.beta1 = (float)s.beta1;
         f.one1 = (float)(1.0 - s.beta1);
         f.beta2 = (float)s.beta2;
@@ -115,7 +175,92 @@ __global__ __launch_bounds__(256) void adamw_kernel(Step s) {
         while (at + 1 < s.n_tensors && c >= s.t[at + 1].chunk0) ++at;
         const Tensor& q = s.t[at];
         const int64_t base = (c - q.chunk0) * kChunk;
-        if constexpr (BITS == 32) {
+        if (q.vec4 && base + kChunk <= q.n) {  // a whole chunk: 2 groups of 4 values a thread
+            f32x4 p[2], g[2], m[2], v[2];
+            int64_t at[2];
+            uint32_t mq[2], vq[2];
+            float ms[2], vs[2];
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                // 8 bits: a wave's 256 values are a block; waves take blocks 2 w, 2 w + 1
+                at[u] = base + (BITS == 32 ? u * 1024 + 4 * t
+                                           : ((t >> 6) * 2 + u) * kBlock + 4 * (t & 63));
+                p[u] = load4(q.p, q.p_type, at[u]);
+                g[u] = load4(q.g, q.g_type, at[u]);
+                if constexpr (BITS == 32) {
+                    m[u] = *(const f32x4*)((const float*)q.m + at[u]);
+                    v[u] = *(const f32x4*)((const float*)q.v + at[u]);
+                } else {
+                    mq[u] = *(const uint32_t*)((const uint8_t*)q.m + at[u]);
+                    vq[u] = *(const uint32_t*)((const uint8_t*)q.v + at[u]);
+                    ms[u] = q.ms[at[u] / kBlock];
+                    vs[u] = q.vs[at[u] / kBlock];
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                f32x4 r;
+                if constexpr (BITS == 8) {
+                    m[u] = decode4(mq[u]) * ms[u];
+                    const f32x4 root = decode4(vq[u]) * vs[u];
+                    v[u] = root * root;
+                }
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    float me = m[u][e], ve = v[u][e], re;
+                    p[u][e] = update(f, p[u][e], g[u][e], me, ve, re);
+                    m[u][e] = me;
+                    v[u][e] = ve;
+                    r[e] = re;
+                }
+                store4(q.p, q.p_type, at[u], p[u]);
+                if constexpr (BITS == 32) {
+                    *(f32x4*)((float*)q.m + at[u]) = m[u];
+                    *(f32x4*)((float*)q.v + at[u]) = v[u];
+                } else {
+                    float am = 0.0f, ar = 0.0f;
+                    bool odd = false;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        am = fmaxf(am, fabsf(m[u][e]));
+                        ar = fmaxf(ar, r[e]);
+                        odd = odd || !(fabsf(m[u][e]) < INFINITY) || !(r[e] < INFINITY);
+                    }
+                    if (__any(odd)) {  // the largest of the finite values
+                        am = ar = 0.0f;
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            am = fmaxf(am, finite_abs(m[u][e]));
+                            ar = fmaxf(ar, finite_abs(r[e]));
+                        }
+                        odd = true;
+                    }
+                    const float nm = wave_max(am) * kPerMax, nr = wave_max(ar) * kPerMax;
+                    const float least = kE4m3Min * nr;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        r[e] = r[e] > 0.0f && r[e] < least ? least : r[e];
+                    uint32_t cm, cv;
+                    if (__any(odd) || !(nm > 0x1p-100f) || !(nr > 0x1p-100f)) {
+                        cm = cv = 0;
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            cm |= (uint32_t)encode(m[u][e], nm) << (8 * e);
+                            cv |= (uint32_t)encode(r[e], nr) << (8 * e);
+                        }
+                    } else {
+                        cm = encode4(m[u], nm, 1.0f / nm);
+                        cv = encode4(r, nr, 1.0f / nr);
+                    }
+                    *(uint32_t*)((uint8_t*)q.m + at[u]) = cm;
+                    *(uint32_t*)((uint8_t*)q.v + at[u]) = cv;
+                    if ((t & 63) == 0) {
+                        q.ms[at[u] / kBlock] = nm;
+                        q.vs[at[u] / kBlock] = nr;
+                    }
+                }
+            }
+        } else if constexpr (BITS == 32) {
             for (int x = t; x < kChunk; x += 256) {
                 const int64_t i = base + x;
                 if (i >= q.n) break;
@@ -171,15 +316,15 @@ __global__ __launch_bounds__(256) void adamw_kernel(Step s) {
             }
         }
     }
-    // The last block through counts the step: every block has read the count by then.
+    // The last block through counts the step: every block has read the count by then, which is all the
+    // order there is, so the arrivals are relaxed (a fence here would write the XCD's L2 back once a
+    // block: 80 us of 105 at 7 M values).
     if (!s.last) return;
     __syncthreads();
-    if (t == 0) {
-        __threadfence();
-        if (atomicAdd(&s.state[1], 1) == (int)gridDim.x - 1) {
-            s.state[0] = step;
-            s.state[1] = 0;
-        }
+    if (t == 0 && __hip_atomic_fetch_add(&s.state[1], 1, __ATOMIC_RELAXED,
+                                         __HIP_MEMORY_SCOPE_AGENT) == (int)gridDim.x - 1) {
+        s.state[0] = step;
+        s.state[1] = 0;
     }
 }
 
@@ -217,6 +362,8 @@ extern "C" mml_status mml_adamw_step_device(const mml_adamw_tensor* tensors, int
         s.beta2 = a.beta2;
         s.eps = a.epsilon;
         s.decay = a.weight_decay;
+        s.log1 = std::log2(a.beta1);
+        s.log2 = std::log2(a.beta2);
         s.state = step_state;
         int32_t i = 0;
         do {
@@ -225,8 +372,16 @@ extern "C" mml_status mml_adamw_step_device(const mml_adamw_tensor* tensors, int
             for (; i < n_tensors && s.n_tensors < kMaxTensors; ++i) {
                 const mml_adamw_tensor& x = tensors[i];
                 if (x.n == 0) continue;
+                const auto aligned = [](const void* q, size_t bytes) {
+                    return (uintptr_t)q % bytes == 0;
+                };
+                const size_t moment = a.state_bits == 32 ? 16 : 4;
+                const bool vec4 = aligned(x.param, x.param_dtype == MML_DTYPE_F32 ? 16 : 8) &&
+                                  aligned(x.grad, x.grad_dtype == MML_DTYPE_F32 ? 16 : 8) &&
+                                  aligned(x.m, moment) && aligned(x.v, moment);
                 s.t[s.n_tensors++] = Tensor{x.param, x.grad, x.m, x.v, x.m_scale, x.v_scale, x.n,
-                                            s.chunks, x.param_dtype, x.grad_dtype};
+                                            s.chunks, (int16_t)x.param_dtype,
+                                            (int16_t)x.grad_dtype, vec4};
                 s.chunks += (x.n + kChunk - 1) / kChunk;
             }
             s.last = i == n_tensors;
