@@ -86,11 +86,12 @@ __device__ __forceinline__ void store4(void* p, int type, int64_t i, f32x4 x) {
         *(f32x4*)((float*)p + i) = x;
         return;
     }
-    uint16_t w[4];
-#pragma unroll
-    for (int e = 0; e < 4; ++e) store_as(w, type, e, x[e]);
+    // one rounding each, to nearest even, two at a time
+    using bf16x4 = __attribute__((ext_vector_type(4))) __bf16;
+    using f16x4 = __attribute__((ext_vector_type(4))) _Float16;
     *(uint2*)((uint16_t*)p + i) =
-        make_uint2(w[0] | (uint32_t)w[1] << 16, w[2] | (uint32_t)w[3] << 16);
+        type == MML_DTYPE_BF16 ? __builtin_bit_cast(uint2, __builtin_convertvector(x, bf16x4))
+                               : __builtin_bit_cast(uint2, __builtin_convertvector(x, f16x4));
 }
 
 // The update of one value; m and v come and go in f32.
@@ -102,7 +103,8 @@ __device__ __forceinline__ float update(const Factors& f, float p, float g, floa
     m = fmaf(f.one1, g, f.beta1 * m);
     v = fmaf(f.one2, g * g, f.beta2 * v);
     root = sqrtf(v);
-    return fmaf(-f.rate, m / fmaf(root, f.root2, f.eps), p * f.shrink);
+    // (the reciprocal is off by one unit in the last place of the step, which p rounds away)
+    return fmaf(-f.rate, m * __builtin_amdgcn_rcpf(fmaf(root, f.root2, f.eps)), p * f.shrink);
 }
 
 __device__ __forceinline__ float decode(uint8_t c) {
@@ -157,7 +159,10 @@ __global__ __launch_bounds__(256) void adamw_kernel(Step s) {
     const int t = threadIdx.x;
     const int32_t step = s.state[0] + 1;
     Factors f;
-    {
+    bool ready = false;
+    const auto prepare = [&] {  // behind the first chunk's loads
+        if (ready) return;
+        ready = true;
         // in 64 bits: 1 - beta and 1 - beta^t cancel for a beta near 1
         const double c1 = 1.0 - exp2(s.log1 * step);
         const double c2 = 1.0 - exp2(s.log2 * step);
@@ -169,7 +174,7 @@ __global__ __launch_bounds__(256) void adamw_kernel(Step s) {
         f.rate = (float)(s.lr / c1);
         f.root2 = (float)(1.0 / sqrt(c2));
         f.eps = (float)s.eps;
-    }
+    };
     int at = 0;
     for (int64_t c = blockIdx.x; c < s.chunks; c += gridDim.x) {
         while (at + 1 < s.n_tensors && c >= s.t[at + 1].chunk0) ++at;
@@ -193,10 +198,14 @@ __global__ __launch_bounds__(256) void adamw_kernel(Step s) {
                 } else {
                     mq[u] = *(const uint32_t*)((const uint8_t*)q.m + at[u]);
                     vq[u] = *(const uint32_t*)((const uint8_t*)q.v + at[u]);
-                    ms[u] = q.ms[at[u] / kBlock];
-                    vs[u] = q.vs[at[u] / kBlock];
+                    // (the same in all lanes: a scalar load)
+                    const int64_t b = base / kBlock +
+                                      __builtin_amdgcn_readfirstlane((t >> 6) * 2 + u);
+                    ms[u] = q.ms[b];
+                    vs[u] = q.vs[b];
                 }
             }
+            prepare();
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
                 f32x4 r;
@@ -261,6 +270,7 @@ __global__ __launch_bounds__(256) void adamw_kernel(Step s) {
                 }
             }
         } else if constexpr (BITS == 32) {
+            prepare();
             for (int x = t; x < kChunk; x += 256) {
                 const int64_t i = base + x;
                 if (i >= q.n) break;
@@ -272,6 +282,7 @@ __global__ __launch_bounds__(256) void adamw_kernel(Step s) {
                 store_as(q.p, q.p_type, i, p);
             }
         } else {
+            prepare();
             // a wave per block of 256: lane l holds values l, l + 64, l + 128, l + 192
             for (int blk = t >> 6; blk < kChunk / kBlock; blk += 4) {
                 const int64_t b0 = base + blk * kBlock;
