@@ -98,11 +98,21 @@ __device__ __forceinline__ void store4(void* p, int type, int64_t i, f32x4 x) {
 struct Factors {
     float beta1, one1, beta2, one2, shrink, rate, root2, eps;
 };
-__device__ __forceinline__ float update(const Factors& f, float p, float g, float& m, float& v,
-                                        float& root) {
+__device__ __forceinline__ void moments(const Factors& f, float g, float& m, float& v) {
     m = fmaf(f.one1, g, f.beta1 * m);
     v = fmaf(f.one2, g * g, f.beta2 * v);
-    root = sqrtf(v);
+}
+// A square root rounded as sqrtf's from the reciprocal root in fewer instructions: one step for both
+// sqrt(v) and 1 / (2 sqrt(v)), then the remainder.  For v from 2^-96 on (no term underflows).
+__device__ __forceinline__ float normal_root(float v) {
+    const float y = __builtin_amdgcn_rsqf(v);
+    float g = v * y, h = 0.5f * y;
+    const float r = fmaf(-h, g, 0.5f);
+    g = fmaf(g, r, g);
+    h = fmaf(h, r, h);
+    return fmaf(fmaf(-g, g, v), h, g);
+}
+__device__ __forceinline__ float step_of(const Factors& f, float p, float m, float root) {
     // (the reciprocal is off by one unit in the last place of the step, which p rounds away)
     return fmaf(-f.rate, m * __builtin_amdgcn_rcpf(fmaf(root, f.root2, f.eps)), p * f.shrink);
 }
@@ -121,21 +131,23 @@ __device__ __forceinline__ float finite_abs(float x) {
     return a < INFINITY ? a : 0.0f;  // (NaN too)
 }
 
-// The largest of a wave's values, in every lane: within rows of 16 by DPP, across them by the swaps
-__device__ __forceinline__ float wave_max(float x) {
-    const auto dpp = [](float v, auto ctrl) {
-        return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), decltype(ctrl)::value,
-                                                          0xF, 0xF, true));
+// The largest of a wave's values, in every lane: within rows of 16 by DPP, across them by the swaps.
+// Magnitudes as their bits, which order as they do, with infinity and the NaNs above.
+__device__ __forceinline__ uint32_t wave_max(uint32_t x) {
+    const auto dpp = [](uint32_t v, auto ctrl) {
+        return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, decltype(ctrl)::value, 0xF, 0xF, true);
     };
-    x = fmaxf(x, dpp(x, std::integral_constant<int, 0xB1>{}));   // quad_perm 1 0 3 2
-    x = fmaxf(x, dpp(x, std::integral_constant<int, 0x4E>{}));   // quad_perm 2 3 0 1
-    x = fmaxf(x, dpp(x, std::integral_constant<int, 0x141>{}));  // row_half_mirror
-    x = fmaxf(x, dpp(x, std::integral_constant<int, 0x140>{}));  // row_mirror
-    const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-    x = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
-    const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-    return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+    x = max(x, dpp(x, std::integral_constant<int, 0xB1>{}));   // quad_perm 1 0 3 2
+    x = max(x, dpp(x, std::integral_constant<int, 0x4E>{}));   // quad_perm 2 3 0 1
+    x = max(x, dpp(x, std::integral_constant<int, 0x141>{}));  // row_half_mirror
+    x = max(x, dpp(x, std::integral_constant<int, 0x140>{}));  // row_mirror
+    const auto a = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+    x = max(a[0], a[1]);
+    const auto b = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+    return max(b[0], b[1]);
 }
+__device__ __forceinline__ uint32_t magnitude(float x) { return __float_as_uint(x) & 0x7FFFFFFFu; }
+constexpr uint32_t kInfinity = 0x7F800000u;
 // Four finite values / scale as codes.  The quotients are rounded as a division rounds them: one
 // division for the block's reciprocal y, then q = x y corrected by its remainder (Markstein 1990).
 // Scales under 2^-100 are divided by.
@@ -214,52 +226,67 @@ __global__ __launch_bounds__(256) void adamw_kernel(Step s) {
                     const f32x4 root = decode4(vq[u]) * vs[u];
                     v[u] = root * root;
                 }
+                bool small = false;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    float me = m[u][e], ve = v[u][e], re;
-                    p[u][e] = update(f, p[u][e], g[u][e], me, ve, re);
+                    float me = m[u][e], ve = v[u][e];
+                    moments(f, g[u][e], me, ve);
                     m[u][e] = me;
                     v[u][e] = ve;
-                    r[e] = re;
+                    small = small || !(ve >= 0x1p-96f && ve < INFINITY);
                 }
+                if (__any(small)) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) r[e] = sqrtf(v[u][e]);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) r[e] = normal_root(v[u][e]);
+                }
+#pragma unroll
+                for (int e = 0; e < 4; ++e) p[u][e] = step_of(f, p[u][e], m[u][e], r[e]);
                 store4(q.p, q.p_type, at[u], p[u]);
                 if constexpr (BITS == 32) {
                     *(f32x4*)((float*)q.m + at[u]) = m[u];
                     *(f32x4*)((float*)q.v + at[u]) = v[u];
                 } else {
-                    float am = 0.0f, ar = 0.0f;
-                    bool odd = false;
+                    uint32_t am = 0, ar = 0;
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        am = fmaxf(am, fabsf(m[u][e]));
-                        ar = fmaxf(ar, r[e]);
-                        odd = odd || !(fabsf(m[u][e]) < INFINITY) || !(r[e] < INFINITY);
+                        am = max(am, magnitude(m[u][e]));
+                        ar = max(ar, magnitude(r[e]));
                     }
-                    if (__any(odd)) {  // the largest of the finite values
-                        am = ar = 0.0f;
+                    am = wave_max(am);
+                    ar = wave_max(ar);
+                    const bool odd = am >= kInfinity || ar >= kInfinity;  // in all lanes
+                    if (odd) {  // the largest of the finite values
+                        am = ar = 0;
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
-                            am = fmaxf(am, finite_abs(m[u][e]));
-                            ar = fmaxf(ar, finite_abs(r[e]));
+                            am = max(am, magnitude(finite_abs(m[u][e])));
+                            ar = max(ar, magnitude(finite_abs(r[e])));
                         }
-                        odd = true;
+                        am = wave_max(am);
+                        ar = wave_max(ar);
                     }
-                    const float nm = wave_max(am) * kPerMax, nr = wave_max(ar) * kPerMax;
-                    const float least = kE4m3Min * nr;
-#pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        r[e] = r[e] > 0.0f && r[e] < least ? least : r[e];
+                    const float nm = __uint_as_float(am) * kPerMax, nr = __uint_as_float(ar) * kPerMax;
                     uint32_t cm, cv;
-                    if (__any(odd) || !(nm > 0x1p-100f) || !(nr > 0x1p-100f)) {
+                    if (odd || !(nm > 0x1p-100f) || !(nr > 0x1p-100f)) {
+                        const float least = kE4m3Min * nr;
                         cm = cv = 0;
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
+                            const float root = r[e] > 0.0f && r[e] < least ? least : r[e];
                             cm |= (uint32_t)encode(m[u][e], nm) << (8 * e);
-                            cv |= (uint32_t)encode(r[e], nr) << (8 * e);
+                            cv |= (uint32_t)encode(root, nr) << (8 * e);
                         }
                     } else {
                         cm = encode4(m[u], nm, 1.0f / nm);
-                        cv = encode4(r, nr, 1.0f / nr);
+                        // code 1 at least for a root that is not zero (the codes of roots are < 128)
+                        const uint32_t c = encode4(r, nr, 1.0f / nr);
+                        cv = 0;
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            cv |= max(c >> (8 * e) & 0xFFu, r[e] > 0.0f ? 1u : 0u) << (8 * e);
                     }
                     *(uint32_t*)((uint8_t*)q.m + at[u]) = cm;
                     *(uint32_t*)((uint8_t*)q.v + at[u]) = cv;
@@ -275,8 +302,9 @@ __global__ __launch_bounds__(256) void adamw_kernel(Step s) {
                 const int64_t i = base + x;
                 if (i >= q.n) break;
                 float m = ((float*)q.m)[i], v = ((float*)q.v)[i], root;
-                const float p = update(f, load_as(q.p, q.p_type, i), load_as(q.g, q.g_type, i), m, v,
-                                       root);
+                moments(f, load_as(q.g, q.g_type, i), m, v);
+                root = sqrtf(v);
+                const float p = step_of(f, load_as(q.p, q.p_type, i), m, root);
                 ((float*)q.m)[i] = m;
                 ((float*)q.v)[i] = v;
                 store_as(q.p, q.p_type, i, p);
@@ -298,8 +326,9 @@ __global__ __launch_bounds__(256) void adamw_kernel(Step s) {
                         m[e] = decode(((uint8_t*)q.m)[i]) * ms;
                         const float root = decode(((uint8_t*)q.v)[i]) * vs;
                         float v = root * root;
-                        const float p = update(f, load_as(q.p, q.p_type, i),
-                                               load_as(q.g, q.g_type, i), m[e], v, r[e]);
+                        moments(f, load_as(q.g, q.g_type, i), m[e], v);
+                        r[e] = sqrtf(v);
+                        const float p = step_of(f, load_as(q.p, q.p_type, i), m[e], r[e]);
                         store_as(q.p, q.p_type, i, p);
                         am = fmaxf(am, finite_abs(m[e]));
                         ar = fmaxf(ar, finite_abs(r[e]));
