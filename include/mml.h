@@ -671,9 +671,9 @@ mml_status mml_item_log_probs_grad_device(const mml_item_softmax_args* args, con
  * and no other's.  All zero is the start of
  * both forms.  Stream-ordered like mml_item_log_probs_device, nothing allocated or read back; a
  * captured step counts on at every replay (learn_rate is replayed as captured).  step_state:
- * int32_t[2] on the device, {steps done, 0}; one step at a time may use it.  Tensors must not
+ * int32_t[MML_ADAMW_STATE] on the device, {steps done, 0, ..., 0}; one step at a time may use it.  Tensors must not
  * overlap. */
-enum { MML_ADAMW_BLOCK = 256 };
+enum { MML_ADAMW_BLOCK = 256, MML_ADAMW_STATE = 1056 };
 typedef struct {
     void* param;
     const void* grad;

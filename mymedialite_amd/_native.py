@@ -83,7 +83,7 @@ class ItemSoftmaxArgs(ctypes.Structure):
 
 
 
-ADAMW_BLOCK = 256
+ADAMW_BLOCK, ADAMW_STATE = 256, 1056
 
 
 class AdamwTensor(ctypes.Structure):

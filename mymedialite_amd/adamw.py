@@ -68,8 +68,8 @@ class AdamW:
                                      "parameters' (scales: blocks') shapes on their device")
             setattr(self, name, x)
         self._names = names
-        self._count = torch.tensor([int(s.get("step", 0)), 0], dtype=torch.int32,
-                                   device=self._device)
+        self._count = torch.zeros(N.ADAMW_STATE, dtype=torch.int32, device=self._device)
+        self._count[0] = int(s.get("step", 0))
         n = len(self.params)
         self._tensors = (N.AdamwTensor * max(n, 1))()
         for i, p in enumerate(self.params):
