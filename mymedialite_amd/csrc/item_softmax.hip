@@ -182,7 +182,7 @@ struct Job {
     int64_t n_rows;
     int32_t splits;
     int32_t bias_vec4;  // the bias can be loaded 4 at a time
-    int32_t direct;  // at most kDirectRows rows, forward: no preparation
+    int32_t direct;  // forward: no preparation
     // forward
     float* part;    // [3][rows_pad][splits]: m, l, w
     float* cmax;    // [rows_pad][cpad]: every tile's largest score (n_top > 0)
@@ -772,13 +772,13 @@ softmax_forward_kernel(Job j) {
     }
 }
 
-// The forward pass for at most 32 rows: every item is used by one tile of users, so there is nothing
-// to share and nothing to prepare.  A wave makes its fragments from the factors themselves, both
-// sides', and the catalogue is read once.  f32: every tile of items has a scale of its own, 2^ev, and
+// The forward pass for at most 32 rows, or for so little work that launches cost more: with one tile
+// of users there is nothing to share and nothing to prepare.  A wave makes its fragments from the
+// factors themselves, both sides', and the catalogue is read once (per tile of users).  f32: every tile of items has a scale of its own, 2^ev, and
 // the scores are brought back before the bias is added (one instruction more per score, which the
 // memory's pace hides: 25.6 MB of factors take about 5 us at the rate of a large copy).  m, l, w as in
 // the forward pass, in true units; the block's waves are joined before they are written.
-constexpr int kDirectRows = 32, kDirectWaves = 4;
+constexpr int kDirectWaves = 4;
 
 // Fragments of 32 rows from their source: row `row` of src in lanes l and l + 32.  Returns the
 // exponent of the f32 planes' scale; finite: whether this lane's values are
@@ -856,8 +856,10 @@ template <int T, int KT, bool TOP>
 __global__ __launch_bounds__(kDirectWaves * 64) void softmax_direct_kernel(Job j) {
     constexpr int PS = Planes<T>::PS, W = kDirectWaves;
     __shared__ float state[W][3][32];
-    const int lane = threadIdx.x & 63, h = lane >> 5, wave = threadIdx.x >> 6, row = lane & 31;
-    const int ways = j.splits * W, way = blockIdx.x * W + wave;
+    const int lane = threadIdx.x & 63, h = lane >> 5, wave = threadIdx.x >> 6, col = lane & 31;
+    const int split = blockIdx.x % j.splits;
+    const int64_t row = (int64_t)(blockIdx.x / j.splits) * 32 + col;
+    const int ways = j.splits * W, way = split * W + wave;
     const int t0 = (int)((int64_t)j.v.tiles * way / ways);
     const int t1 = (int)((int64_t)j.v.tiles * (way + 1) / ways);
     // a tile's factors are on the way while the one before is used (up to k = 128: registers)
@@ -866,7 +868,7 @@ __global__ __launch_bounds__(kDirectWaves * 64) void softmax_direct_kernel(Job j
     uint4 b[PS][KT];
     bool finite;
     load_rows<T, KT>(j.u, source_row(j.u, row), j.k, h, u);
-    if (AHEAD && t0 < t1) load_rows<T, KT>(j.v, source_row(j.v, (int64_t)t0 * 32 + row), j.k, h, v);
+    if (AHEAD && t0 < t1) load_rows<T, KT>(j.v, source_row(j.v, (int64_t)t0 * 32 + col), j.k, h, v);
     const int eu = make_planes<T, KT>(u, b, finite);
     const Scale sc = plain_scale();
     float m = sc.floor, l = 0.0f, w = 0.0f;
@@ -890,11 +892,11 @@ __global__ __launch_bounds__(kDirectWaves * 64) void softmax_direct_kernel(Job j
         const uint32_t bits =
             j.mask ? j.mask[row * (int64_t)j.v.tiles + tl] >> (4 * h) : 0;
         uint4 a[PS][KT];
-        if (!AHEAD) load_rows<T, KT>(j.v, source_row(j.v, (int64_t)tl * 32 + row), j.k, h, v);
+        if (!AHEAD) load_rows<T, KT>(j.v, source_row(j.v, (int64_t)tl * 32 + col), j.k, h, v);
         const int ev = make_planes<T, KT>(v, a, finite);
         const uint64_t odd = __ballot(!finite);  // rows with a value that is not finite
         if (AHEAD && tl + 1 < t1)
-            load_rows<T, KT>(j.v, source_row(j.v, (int64_t)(tl + 1) * 32 + row), j.k, h, v);
+            load_rows<T, KT>(j.v, source_row(j.v, (int64_t)(tl + 1) * 32 + col), j.k, h, v);
         f32x16 c = {};
 #pragma unroll
         for (int ks = 0; ks < KT; ++ks)
@@ -924,7 +926,7 @@ __global__ __launch_bounds__(kDirectWaves * 64) void softmax_direct_kernel(Job j
         for (int i = 1; i < 16; ++i) mt = fmaxf(mt, c[i]);
         if constexpr (TOP) {
             const float most = both_max(mt);
-            if (lane < j.n_rows) j.cmax[row * j.cpad + tl] = most;  // (at most 32 rows)
+            if (h == 0 && row < j.n_rows) j.cmax[row * j.cpad + tl] = most;
         }
         const float mn = fmaxf(m, mt), d = (m - mn) * kLog2e, f = __builtin_amdgcn_exp2f(d);
         w = f * fmaf(l, d, w);
@@ -944,21 +946,21 @@ __global__ __launch_bounds__(kDirectWaves * 64) void softmax_direct_kernel(Job j
         l *= f;
         w += __shfl_xor(w, 32);
         l += __shfl_xor(l, 32);
-        if (h == 0) state[wave][0][row] = mn, state[wave][1][row] = l, state[wave][2][row] = w;
+        if (h == 0) state[wave][0][col] = mn, state[wave][1][col] = l, state[wave][2][col] = w;
     }
     __syncthreads();
     if (threadIdx.x < 32) {
-        m = state[0][0][row];
+        m = state[0][0][col];
 #pragma unroll
-        for (int x = 1; x < W; ++x) m = fmaxf(m, state[x][0][row]);
+        for (int x = 1; x < W; ++x) m = fmaxf(m, state[x][0][col]);
         l = w = 0.0f;
 #pragma unroll
         for (int x = 0; x < W; ++x) {
-            const float d = (state[x][0][row] - m) * kLog2e, f = __builtin_amdgcn_exp2f(d);
-            w += f * fmaf(state[x][1][row], d, state[x][2][row]);
-            l += f * state[x][1][row];
+            const float d = (state[x][0][col] - m) * kLog2e, f = __builtin_amdgcn_exp2f(d);
+            w += f * fmaf(state[x][1][col], d, state[x][2][col]);
+            l += f * state[x][1][col];
         }
-        float* p = j.part + row * j.splits + blockIdx.x;
+        float* p = j.part + row * j.splits + split;
         const int64_t next = j.rows_pad * j.splits;
         p[0] = m;
         p[next] = l;
@@ -1643,8 +1645,9 @@ int64_t plan(const mml_item_softmax_args* a, bool grad, void* base, Job& j) {
             j.vsplits = choose_splits(j.v.tiles, j.u.tiles, kItemsWaves, items_per_simd<TT, KT>(),
                                       M, mt * 4096.0);
         });
-    } else if (a->n_rows <= kDirectRows) {
-        // two tiles or more a wave, up to 8 waves a SIMD
+    } else if (j.u.tiles <= 1 || (int64_t)j.u.tiles * j.v.tiles * kt <= 16384) {
+        // no preparation: one tile of users, or as little work as 100 k items at k = 64 with one (37
+        // users, 1,682 items, k = 10: 24 us a call against 36).  Two tiles of items or more a wave.
         j.direct = 1;
         j.splits = (int32_t)std::max<int64_t>(
             1, std::min<int64_t>((j.v.tiles + 2 * kDirectWaves - 1) / (2 * kDirectWaves), 2048));
@@ -1733,15 +1736,16 @@ void item_log_probs(const mml_item_softmax_args* a, float* log_probs, float* log
     j.top_items = top_items;
     j.top_lp = top_log_probs;
     make_mask(j, st);
+    const uint32_t direct_blocks = grid_of((int64_t)j.u.tiles * j.splits);
     if (!j.direct) prepare(j, a->dtype, st);
     dispatch(a->dtype, steps_of(j.k), [&](auto tt, auto kt) {
         constexpr int T = decltype(tt)::value, KT = decltype(kt)::value;
         constexpr int W = forward_waves<T, KT>();
         if (j.direct) {
             if (j.n_top)
-                softmax_direct_kernel<T, KT, true><<<j.splits, kDirectWaves * 64, 0, st>>>(j);
+                softmax_direct_kernel<T, KT, true><<<direct_blocks, kDirectWaves * 64, 0, st>>>(j);
             else
-                softmax_direct_kernel<T, KT, false><<<j.splits, kDirectWaves * 64, 0, st>>>(j);
+                softmax_direct_kernel<T, KT, false><<<direct_blocks, kDirectWaves * 64, 0, st>>>(j);
             return;
         }
         const uint32_t blocks = grid_of((int64_t)((j.u.tiles + W - 1) / W) * j.splits);
