@@ -483,6 +483,16 @@ mml_status mml_bpr_set_rows(mml_bpr* h, int32_t side, int32_t n_rows, const int3
 /* BPRMF.Predict (:425-431), batched: float.MinValue for ids beyond the model. */
 mml_status mml_bpr_predict(mml_bpr* h, const int32_t* users, const int32_t* items, int64_t n,
                            float* out);
+/* The softmax over the catalogue for users[n] (repeats allowed), on host arrays: the results of
+ * mml_item_log_probs_device (its definitions, below) for this model's factors and biases.  items[n]:
+ * the given items, NULL for none (-1: none for that row); n_top 0 .. 128; exclude_training != 0: each
+ * user's training items are excluded.  log_probs, log_norm, entropy [n], top_items and top_log_probs
+ * [n x n_top] (NULL only with n_top 0).  On a multi-device context each user's row is computed on the
+ * device that holds it. */
+mml_status mml_bpr_log_probs(mml_bpr* h, const int32_t* users, const int32_t* items, int64_t n,
+                             int32_t n_top, int32_t exclude_training, float* log_probs,
+                             float* log_norm, float* entropy, int32_t* top_items,
+                             float* top_log_probs);
 /* out[0] = the last epoch's device time (ms), out[1] = its update kernel alone (the rest is the
  * triple sampler; with mml_bpr_set_next_seed, the part of the next epoch's sampling that the
  * update did not cover) */
@@ -579,6 +589,11 @@ mml_status mml_wrmf_retrain(mml_wrmf* h, int32_t side, int32_t n_rows, const int
 /* MF.Predict (MF.cs:151-157): float.MinValue for ids beyond the model. */
 mml_status mml_wrmf_predict(mml_wrmf* h, const int32_t* users, const int32_t* items, int64_t n,
                             float* out);
+/* As mml_bpr_log_probs for the WRMF (MF.Predict) scorer. */
+mml_status mml_wrmf_log_probs(mml_wrmf* h, const int32_t* users, const int32_t* items, int64_t n,
+                              int32_t n_top, int32_t exclude_training, float* log_probs,
+                              float* log_norm, float* entropy, int32_t* top_items,
+                              float* top_log_probs);
 mml_status mml_wrmf_last_timing(mml_wrmf* h, float* out);
 /* Device time of the last mml_wrmf_iterate's two row-shard all-gathers (ABI 10; U after the user
  * half, V after the item half; the slowest shard on a multi-device context); 0 on one rank. */

@@ -8,6 +8,7 @@ from .data import (DeviceRatingFile, IdentityMapping, Mapping, PosOnlyFeedback, 
 from .random import Random, SystemRandom
 from .recommender import (create_item_recommender, create_rating_predictor, create_recommender,
                           list_recommenders)
+from ._native import ItemLogProbs
 from .item_recommendation import (BPRMF, WRMF, MultiCoreBPRMF, SoftMarginRankingMF,
                                   WeightedBPRMF)
 from .rating_prediction import (BiasedMatrixFactorization, MatrixFactorization,
@@ -19,7 +20,7 @@ from .rating_prediction import (BiasedMatrixFactorization, MatrixFactorization,
 
 def __getattr__(name):
     """The operators on torch tensors, loaded on first use: the recommenders need no torch."""
-    if name in ("item_log_probs", "item_log_probs_grad", "ItemLogProbs"):
+    if name in ("item_log_probs", "item_log_probs_grad"):
         from . import item_softmax
         return getattr(item_softmax, name)
     if name == "AdamW":

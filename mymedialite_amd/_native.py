@@ -7,6 +7,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+from typing import NamedTuple
 
 import numpy as np
 
@@ -81,6 +82,15 @@ class ItemSoftmaxArgs(ctypes.Structure):
                 ("users", _vp), ("items", _vp), ("exclude_offsets", _vp), ("exclude_items", _vp),
                 ("n_exclude", ctypes.c_int64), ("n_top", ctypes.c_int32)]
 
+
+class ItemLogProbs(NamedTuple):
+    """The softmax over the catalogue: torch tensors from item_log_probs, numpy arrays from a
+    recommender's log_probs."""
+    log_probs: object      # [rows] f32
+    log_norm: object       # [rows] f32
+    entropy: object        # [rows] f32
+    top_items: object      # [rows, n_top] int32 (None without n_top)
+    top_log_probs: object  # [rows, n_top] f32 (None without n_top)
 
 
 ADAMW_BLOCK, ADAMW_STATE = 256, 1056
@@ -177,6 +187,8 @@ SIGNATURES = {
     "mml_bpr_iterate": (_st, [_vp, ctypes.c_uint64]),
     "mml_bpr_set_next_seed": (_st, [_vp, ctypes.c_uint64]),
     "mml_bpr_predict": (_st, [_vp, _i32p, _i32p, ctypes.c_int64, _f32p]),
+    "mml_bpr_log_probs": (_st, [_vp, _i32p, _i32p, ctypes.c_int64, ctypes.c_int32, ctypes.c_int32,
+                            _f32p, _f32p, _f32p, _i32p, _f32p]),
     "mml_bpr_apply_triples": (_st, [_vp, _i32p, _i32p, _i32p, ctypes.c_int64]),
     "mml_bpr_last_timing": (_st, [_vp, _f32p]),
     "mml_bpr_last_kernel": (_st, [_vp, ctypes.c_char_p, ctypes.c_int32]),
@@ -213,6 +225,8 @@ SIGNATURES = {
     "mml_wrmf_get_model": (_st, [_vp, _f32p, _f32p]),
     "mml_wrmf_iterate": (_st, [_vp]),
     "mml_wrmf_predict": (_st, [_vp, _i32p, _i32p, ctypes.c_int64, _f32p]),
+    "mml_wrmf_log_probs": (_st, [_vp, _i32p, _i32p, ctypes.c_int64, ctypes.c_int32, ctypes.c_int32,
+                             _f32p, _f32p, _f32p, _i32p, _f32p]),
     "mml_wrmf_last_timing": (_st, [_vp, _f32p]),
     "mml_wrmf_last_refine_passes": (_st, [_vp, _i32p, _f32p]),
     "mml_wrmf_auc": (_st, [_vp, _i32p, ctypes.c_int32, _i32p, ctypes.c_int32, _i64p, _i32p,

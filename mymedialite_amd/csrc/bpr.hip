@@ -755,6 +755,7 @@ struct mml_bpr {
     mml::DeviceArray<float> U, V, bias, ev_out;
     mml::DeviceArray<int64_t> off;
     mml::DeviceArray<int32_t> cols, eligible, ev_u, ev_i, q_u, q_i;
+    mml::LogProbsWork lp_work;
     // the epoch's triples (two-phase epoch) in two sets, so that the next epoch's can be drawn
     // beside this epoch's update (mml_bpr_set_next_seed); cur = the last epoch's set
     BprTriples tb[2];
@@ -2122,6 +2123,64 @@ extern "C" mml_status mml_bpr_predict(mml_bpr* h, const int32_t* users, const in
         MML_HIP(hipMemcpyAsync(out, h->ev_out.get(), sizeof(float) * n, hipMemcpyDeviceToHost,
                                st));
         MML_HIP(hipStreamSynchronize(st));
+    });
+}
+
+extern "C" mml_status mml_bpr_log_probs(mml_bpr* h, const int32_t* users, const int32_t* items,
+                                        int64_t n, int32_t n_top, int32_t exclude_training,
+                                        float* log_probs, float* log_norm, float* entropy,
+                                        int32_t* top_items, float* top_log_probs) {
+    return guard([&] {
+        MML_REQUIRE(h && h->ctx, "null handle");
+        mml::check_model_log_probs(users, n, n_top, log_probs, log_norm, entropy, top_items,
+                                   top_log_probs);
+        MML_REQUIRE(h->has_model, "no model");
+        MML_REQUIRE(!exclude_training || h->has_data, "no training data to exclude");
+        if (n == 0) return;
+        if (h->ctx->multi()) {  // each user on the device that holds its row
+            const auto r = bpr_route(h, users, n);
+            mml::on_devices(h->ctx, [&](int32_t d) {
+                const auto& ix = r[d];
+                if (ix.empty()) return (mml_status)MML_OK;
+                const size_t m = ix.size(), t = (size_t)n_top;
+                std::vector<int32_t> u(m), i(items ? m : 0), ti(m * t);
+                std::vector<float> o(3 * m), tl(m * t);
+                for (size_t x = 0; x < m; ++x) {
+                    u[x] = users[ix[x]];
+                    if (items) i[x] = items[ix[x]];
+                }
+                const mml_status st = mml_bpr_log_probs(
+                    h->shards[d], u.data(), items ? i.data() : nullptr, (int64_t)m, n_top,
+                    exclude_training, o.data(), o.data() + m, o.data() + 2 * m, ti.data(),
+                    tl.data());
+                for (size_t x = 0; st == MML_OK && x < m; ++x) {
+                    log_probs[ix[x]] = o[x];
+                    log_norm[ix[x]] = o[m + x];
+                    entropy[ix[x]] = o[2 * m + x];
+                    std::copy_n(ti.data() + x * t, t, top_items + ix[x] * t);
+                    std::copy_n(tl.data() + x * t, t, top_log_probs + ix[x] * t);
+                }
+                return st;
+            });
+            return;
+        }
+        h->ctx->activate();
+        mml_item_softmax_args a{};
+        a.dtype = MML_DTYPE_F32;
+        a.num_factors = h->k;
+        a.n_users = h->n_users;
+        a.n_items = h->n_items;
+        a.user_factors = h->U.get();
+        a.item_factors = h->V.get();
+        a.ld_users = a.ld_items = h->ld;
+        a.item_bias = h->bias.get();
+        if (exclude_training) {
+            a.exclude_offsets = h->off.get();
+            a.exclude_items = h->cols.get();
+            a.n_exclude = (int64_t)h->cols.count;
+        }
+        mml::model_log_probs(h->ctx->stream, a, h->lp_work, users, items, n, n_top, log_probs,
+                             log_norm, entropy, top_items, top_log_probs);
     });
 }
 

@@ -1647,7 +1647,7 @@ int64_t plan(const mml_item_softmax_args* a, bool grad, void* base, Job& j) {
         });
     } else if (j.u.tiles <= 1 || (int64_t)j.u.tiles * j.v.tiles * kt <= 16384) {
         // no preparation: one tile of users, or as little work as 100 k items at k = 64 with one (37
-        // users, 1,682 items, k = 10: 24 us a call against 36).  Two tiles of items or more a wave.
+        // users, 1,682 items, k = 10: 30 us a call against 36).  Two tiles of items or more a wave.
         j.direct = 1;
         j.splits = (int32_t)std::max<int64_t>(
             1, std::min<int64_t>((j.v.tiles + 2 * kDirectWaves - 1) / (2 * kDirectWaves), 2048));
@@ -1825,6 +1825,55 @@ void item_log_probs_grad(const mml_item_softmax_args* a, const float* log_norm,
         if (j.vsplits > 1) softmax_join_items_kernel<T><<<ji, 256, 0, st>>>(j, kp);
     });
     MML_HIP(hipGetLastError());
+}
+
+void check_model_log_probs(const int32_t* users, int64_t n, int32_t n_top, const float* log_probs,
+                           const float* log_norm, const float* entropy, const int32_t* top_items,
+                           const float* top_log_probs) {
+    MML_REQUIRE(n >= 0 && n <= (int64_t)1 << 30, "bad n");
+    MML_REQUIRE(n_top >= 0 && n_top <= kMaxTop, "n_top must be in [0, 128]");
+    MML_REQUIRE(n == 0 || users, "null users");
+    MML_REQUIRE(n == 0 || (log_probs && log_norm && entropy), "null output");
+    MML_REQUIRE(n == 0 || n_top == 0 || (top_items && top_log_probs), "n_top without its outputs");
+}
+
+void model_log_probs(hipStream_t st, mml_item_softmax_args a, LogProbsWork& w, const int32_t* users,
+                     const int32_t* items, int64_t n, int32_t n_top, float* log_probs,
+                     float* log_norm, float* entropy, int32_t* top_items, float* top_log_probs) {
+    int64_t rows = n;
+    a.n_top = n_top;
+    a.users = users;  // (only whether there are any matters to the size)
+    a.items = items;
+    for (;; rows = (rows / 2 + 31) / 32 * 32) {
+        a.n_rows = rows;
+        if (rows <= 32 || item_log_probs_workspace(&a, false) <= (int64_t)1 << 30) break;
+    }
+    w.ids.reserve(2 * rows);
+    w.out.reserve((3 + 2 * (int64_t)n_top) * rows);
+    for (int64_t r = 0; r < n; r += rows) {
+        const int64_t m = std::min(rows, n - r);
+        a.n_rows = m;
+        const int64_t need = item_log_probs_workspace(&a, false);
+        w.ws.reserve(need);
+        float* out = w.out.get();
+        int32_t* top = reinterpret_cast<int32_t*>(out + 3 * m);
+        float* top_lp = out + (3 + n_top) * m;
+        MML_HIP(hipMemcpyAsync(w.ids.get(), users + r, 4 * m, hipMemcpyHostToDevice, st));
+        if (items)
+            MML_HIP(hipMemcpyAsync(w.ids.get() + m, items + r, 4 * m, hipMemcpyHostToDevice, st));
+        a.users = w.ids.get();
+        a.items = items ? w.ids.get() + m : nullptr;
+        item_log_probs(&a, out, out + m, out + 2 * m, top, top_lp, w.ws.get(), need, st);
+        const auto copy = [&](void* to, const void* from, int64_t words) {
+            if (words > 0) MML_HIP(hipMemcpyAsync(to, from, 4 * words, hipMemcpyDeviceToHost, st));
+        };
+        copy(log_probs + r, out, m);
+        copy(log_norm + r, out + m, m);
+        copy(entropy + r, out + 2 * m, m);
+        copy(top_items + r * n_top, top, m * n_top);
+        copy(top_log_probs + r * n_top, top_lp, m * n_top);
+        MML_HIP(hipStreamSynchronize(st));
+    }
 }
 
 }  // namespace mml

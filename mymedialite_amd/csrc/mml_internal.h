@@ -165,6 +165,23 @@ void item_log_probs_grad(const mml_item_softmax_args* a, const float* log_norm,
                          int64_t ws_bytes, hipStream_t st);
 int64_t item_log_probs_workspace(const mml_item_softmax_args* a, bool grad);
 
+// A model's device arrays as `args` (without rows), and the device memory that its host-array calls
+// keep between them (mml_bpr_log_probs, mml_wrmf_log_probs): the rows in ranges whose workspace stays
+// under 1 GiB, results copied out, the stream idle at the end.
+struct LogProbsWork {
+    DeviceArray<uint8_t> ws;
+    DeviceArray<int32_t> ids;  // users, items
+    DeviceArray<float> out;    // log_probs, log_norm, entropy, top items, top log probs
+};
+void model_log_probs(hipStream_t st, mml_item_softmax_args args, LogProbsWork& w,
+                     const int32_t* users, const int32_t* items, int64_t n, int32_t n_top,
+                     float* log_probs, float* log_norm, float* entropy, int32_t* top_items,
+                     float* top_log_probs);
+// The checks of those calls that need no device.
+void check_model_log_probs(const int32_t* users, int64_t n, int32_t n_top, const float* log_probs,
+                           const float* log_norm, const float* entropy, const int32_t* top_items,
+                           const float* top_log_probs);
+
 // contiguous row shards with balanced work (weight deg + k/2), bounds[parts + 1] (mml_core.cpp)
 std::vector<int64_t> balanced_rows(const std::vector<int64_t>& deg, int32_t k, int32_t parts);
 

@@ -532,6 +532,7 @@ struct mml_wrmf {
     mml::DeviceArray<float> U, V, q_out;
     mml::DeviceArray<int64_t> uoff, ioff;
     mml::DeviceArray<int32_t> ucols, icols, q_u, q_i;
+    mml::LogProbsWork lp_work;
     mml::DeviceArray<double> HH, partial;
     bool has_data = false, has_model = false;
     float last_ms = 0.0f;
@@ -1223,6 +1224,42 @@ extern "C" mml_status mml_wrmf_predict(mml_wrmf* h, const int32_t* users, const 
         MML_HIP(hipMemcpyAsync(out, h->q_out.get(), sizeof(float) * n, hipMemcpyDeviceToHost,
                                st));
         MML_HIP(hipStreamSynchronize(st));
+    });
+}
+
+extern "C" mml_status mml_wrmf_log_probs(mml_wrmf* h, const int32_t* users, const int32_t* items,
+                                         int64_t n, int32_t n_top, int32_t exclude_training,
+                                         float* log_probs, float* log_norm, float* entropy,
+                                         int32_t* top_items, float* top_log_probs) {
+    return guard([&] {
+        MML_REQUIRE(h && h->ctx, "null handle");
+        if (h->ctx->multi()) return (void)mml::on_devices(h->ctx, [&](int32_t d) {
+            return d == 0 ? mml_wrmf_log_probs(h->shards[0], users, items, n, n_top,
+                                               exclude_training, log_probs, log_norm, entropy,
+                                               top_items, top_log_probs)
+                          : (mml_status)MML_OK;
+        });
+        mml::check_model_log_probs(users, n, n_top, log_probs, log_norm, entropy, top_items,
+                                   top_log_probs);
+        MML_REQUIRE(h->has_model, "no model");
+        MML_REQUIRE(!exclude_training || h->has_data, "no training data to exclude");
+        if (n == 0) return;
+        h->ctx->activate();
+        mml_item_softmax_args a{};
+        a.dtype = MML_DTYPE_F32;
+        a.num_factors = h->k;
+        a.n_users = h->n_users;
+        a.n_items = h->n_items;
+        a.user_factors = h->U.get();
+        a.item_factors = h->V.get();
+        a.ld_users = a.ld_items = h->k;
+        if (exclude_training) {
+            a.exclude_offsets = h->uoff.get();
+            a.exclude_items = h->ucols.get();
+            a.n_exclude = (int64_t)h->ucols.count;
+        }
+        mml::model_log_probs(h->ctx->stream, a, h->lp_work, users, items, n, n_top, log_probs,
+                             log_norm, entropy, top_items, top_log_probs);
     });
 }
 

@@ -61,6 +61,9 @@ class _MFBase(Recommender):
     def _auc_symbol(self):
         raise NotImplementedError
 
+    def _log_probs_symbol(self):
+        raise NotImplementedError
+
     # SaveModel / LoadModel (MF.cs:160-195, BPRMF.cs:434-479): IO/Model.cs text format
     TYPE_NAME = ""
 
@@ -147,6 +150,28 @@ class _MFBase(Recommender):
         return {"AUC": float(np.float32(acc / np.float32(n))) if n else 0.0, "num_users": n,
                 "num_items": int(len(cand)), "per_user": out}
 
+    def log_probs(self, users, items=None, n_top=0, exclude_training=False) -> N.ItemLogProbs:
+        """The softmax over the catalogue's scores for every user of ``users`` (repeats allowed), as
+        numpy arrays: the log probability of ``items`` (one per user, -1 or None: none), the log
+        normaliser, the entropy and the ``n_top`` (<= 128) likeliest items; exclude_training: without
+        the user's training items.  mymedialite_amd.item_log_probs is the same on torch tensors."""
+        if self._h is None:
+            raise RuntimeError("model not initialised: call train()/init_model() first")
+        u = N.i32(np.atleast_1d(users))
+        i = None if items is None else N.i32(np.atleast_1d(items))
+        if u.ndim != 1 or (i is not None and i.shape != u.shape):
+            raise ValueError("users and items must be 1-D and of one length")
+        n, n_top = len(u), int(n_top)
+        out = np.empty((3, n), np.float32)
+        ids = lp = None
+        if n_top > 0:
+            ids = np.empty((n, n_top), np.int32)
+            lp = np.empty((n, n_top), np.float32)
+        N.check(getattr(N.lib(), self._log_probs_symbol())(
+            self._h, N.ptr(u, N._i32p), N.ptr(i, N._i32p), n, n_top, int(bool(exclude_training)),
+            *(N.ptr(x, N._f32p) for x in out), N.ptr(ids, N._i32p), N.ptr(lp, N._f32p)))
+        return N.ItemLogProbs(out[0], out[1], out[2], ids, lp)
+
     def _release(self):
         raise NotImplementedError
 
@@ -195,6 +220,9 @@ class BPRMF(_MFBase):
     def _auc_symbol(self):
         return "mml_bpr_auc"
 
+    def _log_probs_symbol(self):
+        return "mml_bpr_log_probs"
+
     TYPE_NAME = "MyMediaLite.ItemRecommendation.BPRMF"
 
     def _has_bias(self) -> bool:
@@ -231,6 +259,54 @@ class BPRMF(_MFBase):
         N.check(N.lib().mml_bpr_apply_triples(self._h, N.ptr(u, N._i32p), N.ptr(i, N._i32p),
                                               N.ptr(j, N._i32p), len(u)))
         self._host = None
+
+    def apply_softmax(self, users, items, BatchSize=4096, state=None, **hyper):
+        """One pass over the given events by AdamW steps on the softmax's loss, the mean of
+        -log_probs(users, items) over BatchSize events at a time, in order: apply_triples' counterpart
+        for a loss over the whole catalogue (item_log_probs, item_log_probs_grad, AdamW).  hyper: AdamW's
+        LearnRate, Beta1, Beta2, Epsilon, WeightDecay and StateBits.  Returns (the steps' losses,
+        float32; the optimizer's state, to go on from with state=).  Steps are dense: a user or item
+        without an event moves by its moments and the weight decay.  The model changes at the end of
+        the pass."""
+        import torch
+        from .adamw import AdamW
+        from .item_softmax import item_log_probs, item_log_probs_grad
+        if self._h is None:
+            raise RuntimeError("model not initialised: call train()/init_model() first")
+        _single_device_only(self)
+        u, i = N.i32(users), N.i32(items)
+        batch = int(BatchSize)
+        if u.ndim != 1 or u.shape != i.shape:
+            raise ValueError("users and items must be 1-D and of one length")
+        if batch < 1:
+            raise ValueError("BatchSize must be at least 1")
+        if len(u) and (u.min() < 0 or u.max() > self.MaxUserID or i.min() < 0
+                       or i.max() > self.MaxItemID):
+            raise ValueError("user or item id beyond the model")
+        dev = torch.device("cuda", self._ctx.device)
+        m = self.get_model()
+        with torch.cuda.device(dev):
+            model = [torch.tensor(m[x], device=dev) for x in ("U", "V", "bias")]
+            U, V, bias = model
+            opt = AdamW(model, state=state, **hyper)
+            tu, ti = torch.tensor(u, device=dev), torch.tensor(i, device=dev)
+            losses = []
+            for a in range(0, len(u), batch):
+                bu, bi = tu[a:a + batch], ti[a:a + batch]
+                r = item_log_probs(U, V, bias, bi, bu)
+                w = torch.full_like(r.log_probs, -1.0 / len(bu))
+                gu, gv, gb = item_log_probs_grad(U, V, bias, bi, log_norm=r.log_norm,
+                                                 grad_log_probs=w, users=bu)
+                # a user's rows added up in the order of the events (accumulate=True sorts them)
+                gU = torch.zeros_like(U).index_put_((bu.long(),), gu, accumulate=True)
+                opt.step([gU, gv, gb])
+                losses.append(-r.log_probs.mean())
+            if losses:
+                new = [x.cpu().numpy() for x in model]
+                N.check(N.lib().mml_bpr_set_model(self._h, *(N.ptr(x, N._f32p) for x in new)))
+                self._host = dict(zip(("U", "V", "bias"), new))
+            loss = torch.stack(losses).cpu().numpy() if losses else np.zeros(0, np.float32)
+            return loss, opt.state()
 
     # ------------------------------------------------------------------ incremental updates
     UpdateUsers = True  # IncrementalItemRecommender.UpdateUsers / UpdateItems
@@ -635,6 +711,9 @@ class WRMF(_MFBase):
 
     def _auc_symbol(self):
         return "mml_wrmf_auc"
+
+    def _log_probs_symbol(self):
+        return "mml_wrmf_log_probs"
 
     TYPE_NAME = "MyMediaLite.ItemRecommendation.WRMF"
 

@@ -9,21 +9,13 @@ trained recommender, on host arrays.)
 from __future__ import annotations
 
 import ctypes
-from typing import NamedTuple
 
 import torch
 
 from . import _native as N
+from ._native import ItemLogProbs
 
 _DTYPES = {torch.float32: N.DTYPE_F32, torch.bfloat16: N.DTYPE_BF16, torch.float16: N.DTYPE_F16}
-
-
-class ItemLogProbs(NamedTuple):
-    log_probs: torch.Tensor            # [rows] f32
-    log_norm: torch.Tensor             # [rows] f32
-    entropy: torch.Tensor              # [rows] f32
-    top_items: torch.Tensor | None     # [rows, n_top] int32
-    top_log_probs: torch.Tensor | None  # [rows, n_top] f32
 
 
 def _factors(x, name):
