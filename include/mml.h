@@ -629,8 +629,13 @@ mml_status mml_wrmf_auc(mml_wrmf* h, const int32_t* candidates, int32_t n_candid
  * catalogue skipped), and for every row the items whose bias is -1e30 or lower (-inf included);
  * what their factors hold does not matter.  A row with no item left has log_norm -inf, entropy 0,
  * log_probs -inf, top_items -1 and no gradient.  A user id outside [0, n_users) gives NaN (top
- * items -1) and no gradient; a factor or bias that is not finite (or above 3e38) and not excluded
- * makes its rows NaN. */
+ * items -1, top_log_probs NaN) and no gradient.  A factor that is not finite (above 3e38) and a bias
+ * of 1e30 or more, not excluded, make their rows NaN.  Scores have to lie within +-1e28 (rows beyond
+ * are NaN, or empty where all their scores are under it).
+ *
+ * Accuracy: f32 factors are held to 2^-22 of their value, and to 2^-37 of their matrix' largest at
+ * least (the batch's users; the items that no bias excludes); half-precision factors exactly.  Sums
+ * are f32 within a tile and a split and f64 between them. */
 enum { MML_DTYPE_F32 = 0, MML_DTYPE_BF16 = 1, MML_DTYPE_F16 = 2 };
 typedef struct {
     int32_t dtype;                  /* MML_DTYPE_* of both factor matrices */
@@ -655,7 +660,9 @@ mml_status mml_item_log_probs_workspace(const mml_item_softmax_args* args, int32
 /* log_probs[r] = log p_r(items[r]) (0 without one, -inf for an excluded one), log_norm[r] =
  * log sum_j exp(s_rj), entropy[r] = -sum_j p_rj log p_rj, top_items / top_log_probs [n_rows x n_top]:
  * the n_top likeliest items and their log p, ordered by the exact score (64-bit sums), the lower
- * id first among equals, -1 / -inf behind the last item. */
+ * id first among equals, -1 / -inf behind the last item.  (The items scored again are those of the
+ * n_top + 2 groups of 32 with the largest maxima in the accuracy above: where more groups than that
+ * come as close to the last place, which of them is named is within that accuracy.) */
 mml_status mml_item_log_probs_device(const mml_item_softmax_args* args, float* log_probs,
                                      float* log_norm, float* entropy, int32_t* top_items,
                                      float* top_log_probs, void* workspace,
@@ -683,11 +690,11 @@ mml_status mml_item_log_probs_grad_device(const mml_item_softmax_args* args, con
  * of its MML_ADAMW_BLOCK consecutive values, scale = largest magnitude / 448 (float[ceil(n / 256)]);
  * v's codes hold sqrt(v), and one that is not zero never gets code 0.  A gradient that is not
  * finite (8 bits: or whose square is not) makes that value's parameter and moments NaN or infinite
- * and no other's.  All zero is the start of
- * both forms.  Stream-ordered like mml_item_log_probs_device, nothing allocated or read back; a
- * captured step counts on at every replay (learn_rate is replayed as captured).  step_state:
- * int32_t[MML_ADAMW_STATE] on the device, {steps done, 0, ..., 0}; one step at a time may use it.  Tensors must not
- * overlap. */
+ * and no other's.  All zero is the start of both forms.
+ * Stream-ordered like mml_item_log_probs_device, nothing allocated or read back; a captured step
+ * counts on at every replay (learn_rate is replayed as captured).  step_state:
+ * int32_t[MML_ADAMW_STATE] on the device, {steps done, 0, ..., 0}; one step at a time may use it.
+ * Tensors must not overlap. */
 enum { MML_ADAMW_BLOCK = 256, MML_ADAMW_STATE = 1056 };
 typedef struct {
     void* param;

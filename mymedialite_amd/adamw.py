@@ -37,9 +37,10 @@ class AdamW:
                 raise ValueError("parameters must be on one device")
             if not p.is_contiguous():
                 raise ValueError("parameters must be contiguous: they are updated in place")
-        starts = [p.data_ptr() for p in self.params if p.numel()]
-        if len(set(starts)) != len(starts):
-            raise ValueError("a parameter is listed twice")
+        spans = sorted((p.data_ptr(), p.data_ptr() + p.numel() * p.element_size())
+                       for p in self.params if p.numel())
+        if any(x[1] > y[0] for x, y in zip(spans, spans[1:])):
+            raise ValueError("a parameter is listed twice, or two overlap")
         self._device = self.params[0].device if self.params else torch.device("cuda", 0)
         blocks = [-(-p.numel() // N.ADAMW_BLOCK) for p in self.params]
         kind = torch.float32 if StateBits == 32 else torch.float8_e4m3fn
@@ -97,6 +98,8 @@ class AdamW:
                 g = g.contiguous()
                 keep.append(g)
             t = self._tensors[i]
+            if p.data_ptr() != (t.param or 0):
+                raise ValueError(f"parameter {i} is in other memory than at the start")
             t.grad, t.grad_dtype = g.data_ptr(), _DTYPES[g.dtype]
         a = N.AdamwParams(self.LearnRate, self.Beta1, self.Beta2, self.Epsilon, self.WeightDecay,
                           self._bits)

@@ -8,7 +8,7 @@
 //   G_rj = dL / ds_rj = w_r ([j = t_r] - p_rj) - h_r p_rj (log p_rj + H_r),
 //   dL/dU = G V,  dL/dV = G^T U,  dL/db_j = sum_r G_rj.
 // The R x N matrices s, p and G are never stored: 32 x 32 tiles of s are made on the matrix cores,
-// used in registers and dropped (flash style: a running maximum m, sum l and sum of e y).
+// used in registers and dropped (one pass with a running maximum m, sum l and sum of e y).
 //
 // f32 factors run on the f16 matrix cores at close to f32 accuracy: a value x, scaled by a power of
 // two common to its matrix (largest magnitude just under 2^13), is hi + lo with hi = f16(x) and
@@ -157,11 +157,15 @@ struct Scale {
     float gone;   // the score of an excluded item: below every other
     float floor;  // where a running maximum starts: above gone, so that an excluded item's e is 0
                   // before the first score too (a row whose scores are all below it counts as empty)
-    int32_t eu, ev;
+    int32_t eu, ev;  // of the score's planes
+    int32_t gu, gv;  // of the gradient products' (transposed) planes
 };
 __device__ __forceinline__ Scale plain_scale() {
-    return Scale{kLog2e, 1.0f, kGone, kGone * 0.0625f, 0, 0};
+    return Scale{kLog2e, 1.0f, kGone, kGone * 0.0625f, 0, 0, 0, 0};
 }
+// 2^86: scaled scores are below 2^35, so products beyond are far outside f32; and an excluded item's
+// score times kappa, 2^40 2^86, is still finite.
+constexpr int kLeastExponent = -86;
 constexpr int kMaxParts = 512, kUserParts = 64;  // partial maxima of softmax_max_kernel
 
 struct Job {
@@ -251,7 +255,8 @@ __global__ __launch_bounds__(256) void softmax_mask_kernel(Job j) {
         *(uint4*)(out + x) = *(const uint4*)(words + x);
 }
 
-// The largest finite magnitude of either matrix (the batch's users only), in kMaxParts parts.
+// The largest finite magnitude of either matrix (the batch's users only, without the items that their
+// bias excludes), in kMaxParts parts.
 template <int T>
 __global__ __launch_bounds__(256) void softmax_max_kernel(Job j) {
     __shared__ float red[4];
@@ -264,20 +269,24 @@ __global__ __launch_bounds__(256) void softmax_max_kernel(Job j) {
         const float a = fabsf(x);
         if (a < 3e38f) m = fmaxf(m, a);
     };
-    // a wave per row and turn
     const int lane = threadIdx.x & 63;
-    if (!s.index && s.ld == j.k && s.vec8) {  // one contiguous array
-        const int64_t n = s.n * j.k / 4;
+    const float* bias = users ? nullptr : j.bias;
+    if (s.vec8 && j.k % 4 == 0) {  // 4 factors a thread and turn
+        const uint32_t quads = (uint32_t)j.k / 4;
+        const int64_t n = s.n * quads;
         for (int64_t x = (int64_t)part * 256 + threadIdx.x; x < n; x += (int64_t)parts * 256) {
-            const f32x4 v = ((const f32x4*)s.src)[x];
+            const int64_t r = n >> 32 ? x / quads : (int64_t)((uint32_t)x / quads);
+            const int64_t src = source_row(s, r);
+            if (src < 0) continue;
+            const f32x4 v = *(const f32x4*)((const float*)s.src + src * s.ld + 4 * (x - r * quads));
+            if (bias && bias[r] <= kGone) continue;
 #pragma unroll
             for (int e = 0; e < 4; ++e) take(v[e]);
         }
-        if (part == 0 && threadIdx.x < s.n * j.k % 4) take(((const float*)s.src)[4 * n + threadIdx.x]);
-    } else {
+    } else {  // a wave per row and turn
         for (int64_t r = (int64_t)part * 4 + (threadIdx.x >> 6); r < s.n; r += (int64_t)parts * 4) {
             const int64_t src = source_row(s, r);
-            if (src < 0) continue;
+            if (src < 0 || (bias && bias[r] <= kGone)) continue;
             for (int f = lane; f < j.k; f += 64) take(load_factor<T>(s.src, src * s.ld + f));
         }
     }
@@ -290,11 +299,11 @@ __global__ __launch_bounds__(256) void softmax_max_kernel(Job j) {
 }
 
 // The scales from the parts; all 256 threads of a block take part.  A matrix' largest magnitude comes
-// out in [2^12, 2^13), unless that takes an exponent outside [-40, 12] (above 2^53 a plane overflows
-// and the rows become NaN; small values need no more).
+// out in [2^12, 2^13) -- for the scores only while eu + ev <= 24, so that biases of any size stay in f32
+// when they are scaled along: what is lost of the smaller matrix then is below 2^-36 of a score of 1.
 template <int T>
 __device__ __forceinline__ Scale make_scale(const Job& j) {
-    int eu = 0, ev = 0;
+    int eu = 0, ev = 0, gu = 0, gv = 0;
     if constexpr (T == MML_DTYPE_F32) {
         __shared__ float red[4], first;
         const int t = threadIdx.x;
@@ -313,8 +322,13 @@ __device__ __forceinline__ Scale make_scale(const Job& j) {
         u = first;
         v = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
         // (frexp: x = f 2^e, f in [0.5, 1); of 0 it is 0)
-        eu = max(-40, min(12, 13 - __builtin_amdgcn_frexp_expf(u)));
-        ev = max(-40, min(12, 13 - __builtin_amdgcn_frexp_expf(v)));
+        eu = gu = 13 - __builtin_amdgcn_frexp_expf(u);
+        ev = gv = 13 - __builtin_amdgcn_frexp_expf(v);
+        if (eu + ev > 24) {
+            if (eu > 12 && ev > 12) eu = ev = 12;
+            else if (eu > 12) eu = 24 - ev;
+            else ev = 24 - eu;
+        }
     }
     Scale c;
     const int e = eu + ev;
@@ -322,14 +336,18 @@ __device__ __forceinline__ Scale make_scale(const Job& j) {
     c.kappa = ldexpf(kLog2e, -e);
     c.gone = -fmaxf(ldexpf(1e30f, min(e, 0)), 1.0995116e12f);  // 2^40: scaled scores are below 2^35
     c.floor = c.gone * 0.0625f;
+    if (e < kLeastExponent) c.unit = c.kappa = __builtin_nanf("");
     c.eu = eu;
     c.ev = ev;
+    c.gu = gu;
+    c.gv = gv;
     return c;
 }
 
 // Fragments of both sides, one block per tile of 32 rows (the users' tiles first).  A row with a
 // value that is not finite is written as zeros and marked, so that 0 * NaN cannot reach the other
-// rows' sums: an item that is not excluded gets the bias NaN, a user the mark in ubad.
+// rows' sums: an item that is not excluded gets the bias NaN, a user the mark in ubad.  So is an item
+// that its bias excludes, whose factors the scale does not count.
 template <int T, int KT>
 __global__ __launch_bounds__(256) void softmax_prep_kernel(Job j) {
     using P = Planes<T>;
@@ -342,8 +360,11 @@ __global__ __launch_bounds__(256) void softmax_prep_kernel(Job j) {
     const int t = threadIdx.x;
     const Scale sc = make_scale<T>(j);
     if (blockIdx.x == 0 && t == 0) *j.scale = sc;
-    if (t < 32)
-        bad[t] = users && tl * 32 + t < s.n && source_row(s, tl * 32 + t) < 0 ? 2 : 0;
+    if (t < 32) {
+        const int64_t row = tl * 32 + t;
+        bad[t] = row >= s.n ? 0 : users ? 2 * (source_row(s, row) < 0)
+                                        : 4 * (j.bias && j.bias[row] <= kGone);
+    }
     __syncthreads();
     for (int x = t; x < 64 * KT; x += 256) {  // 8 factors each
         const int row = x / (2 * KT), f = 8 * (x % (2 * KT));
@@ -379,7 +400,7 @@ __global__ __launch_bounds__(256) void softmax_prep_kernel(Job j) {
             j.vbias[row] = b;
         }
     }
-    const float mul = ldexpf(1.0f, users ? sc.eu : sc.ev);
+    const int ex = users ? sc.eu : sc.ev, gx = users ? sc.gu : sc.gv;
     for (int x = t; x < KT * 64; x += 256) {
         const int ks = x >> 6, lane = x & 63, row = lane & 31;
         const f32x4* src = (const f32x4*)&tile[row * LD + ks * 16 + 8 * (lane >> 5)];
@@ -387,7 +408,7 @@ __global__ __launch_bounds__(256) void softmax_prep_kernel(Job j) {
         uint32_t q[P::PS][8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-            float v = bad[row] ? 0.0f : (e < 4 ? lo[e & 3] : hi[e & 3]) * mul;
+            float v = bad[row] ? 0.0f : ldexpf(e < 4 ? lo[e & 3] : hi[e & 3], ex);
 #pragma unroll
             for (int p = 0; p < P::PS; ++p) q[p][e] = take_plane<T>(v);
         }
@@ -404,7 +425,7 @@ __global__ __launch_bounds__(256) void softmax_prep_kernel(Job j) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
             const int row = 16 * step + 8 * (e >> 2) + 4 * (lane >> 5) + (e & 3);
-            float v = f < KP && !bad[row] ? tile[row * LD + f] * mul : 0.0f;
+            float v = f < KP && !bad[row] ? ldexpf(tile[row * LD + f], gx) : 0.0f;
 #pragma unroll
             for (int p = 0; p < P::PG; ++p) q[p][e] = take_plane<T>(v);
         }
@@ -829,7 +850,7 @@ __device__ __forceinline__ int make_planes(const float (&v)[KT][8], uint4 (&q)[P
         if (!finite) most = 0.0f;
 #pragma unroll
         for (int d = 32; d > 0; d >>= 1) most = fmaxf(most, __shfl_xor(most, d));
-        ex = max(-40, min(12, 13 - __builtin_amdgcn_frexp_expf(most)));
+        ex = min(100, 13 - __builtin_amdgcn_frexp_expf(most));  // (100: mul is finite)
         mul = ldexpf(1.0f, ex);
     }
 #pragma unroll
@@ -891,10 +912,21 @@ __global__ __launch_bounds__(kDirectWaves * 64) void softmax_direct_kernel(Job j
         }
         const uint32_t bits =
             j.mask ? j.mask[row * (int64_t)j.v.tiles + tl] >> (4 * h) : 0;
+        const int64_t own = (int64_t)tl * 32 + col;
+        const bool off = j.bias && own < j.n_items && j.bias[own] <= kGone;
         uint4 a[PS][KT];
         if (!AHEAD) load_rows<T, KT>(j.v, source_row(j.v, (int64_t)tl * 32 + col), j.k, h, v);
+        // an item that its bias excludes: its factors do not matter
+        if (__any(off)) {
+            asm volatile("");  // as in mask_tile
+#pragma unroll
+            for (int ks = 0; ks < KT; ++ks)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[ks][e] = off ? 0.0f : v[ks][e];
+        }
         const int ev = make_planes<T, KT>(v, a, finite);
-        const uint64_t odd = __ballot(!finite);  // rows with a value that is not finite
+        uint64_t odd = __ballot(!finite);  // rows with a value that is not finite
+        if (eu + ev < kLeastExponent) odd = ~0ull;
         if (AHEAD && tl + 1 < t1)
             load_rows<T, KT>(j.v, source_row(j.v, (int64_t)(tl + 1) * 32 + col), j.k, h, v);
         f32x16 c = {};
@@ -1352,7 +1384,7 @@ softmax_grad_users_kernel(Job j) {
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) acc[mt][i] = unscale<T>(acc[mt][i], sh, sc.ev);
+        for (int i = 0; i < 16; ++i) acc[mt][i] = unscale<T>(acc[mt][i], sh, sc.gv);
     float* out = j.du_part + ((int64_t)split * j.rows_pad + row) * KP;
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt)
@@ -1459,7 +1491,7 @@ softmax_grad_items_kernel(Job j) {
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) acc[mt][i] = unscale<T>(acc[mt][i], sh, sc.eu);
+        for (int i = 0; i < 16; ++i) acc[mt][i] = unscale<T>(acc[mt][i], sh, sc.gu);
     if (j.vsplits == 1) {  // nothing to join: the result itself
         if (item >= j.n_items) return;
         if (h == 0) j.gb[item] = db;

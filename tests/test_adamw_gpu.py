@@ -277,3 +277,16 @@ def test_refusals():
         with pytest.raises(N.MMLError):
             o.step([g])
         assert o.state()["step"] == 0
+
+
+def test_overlapping_and_moved_parameters_are_refused():
+    x = torch.zeros(10, device="cuda")
+    with pytest.raises(ValueError, match="overlap"):
+        AdamW([x[:6], x[5:]])
+    a, b, none = x[:5], x[5:], torch.zeros(0, device="cuda")
+    o = AdamW([a, b, none])
+    o.step([torch.ones(5, device="cuda"), torch.ones(5, device="cuda"), none])
+    a.data = torch.zeros(5, device="cuda")
+    with pytest.raises(ValueError, match="parameter 0 is in other memory"):
+        o.step([torch.ones(5, device="cuda"), torch.ones(5, device="cuda"), none])
+    assert o.state()["step"] == 1

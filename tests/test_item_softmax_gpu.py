@@ -495,3 +495,50 @@ def test_refusals():
     with pytest.raises(ValueError, match="log_norm is required"):
         item_log_probs_grad(**ok, log_norm=None)
     check_forward(d, forward(c))  # and the next call is unharmed
+
+
+@pytest.mark.parametrize("rows,n_items", [(5, 333), (300, 30_001)], ids=["few", "many"])
+@pytest.mark.parametrize("up,vp", [(60, -60), (-60, 60), (-30, -30), (-100, 0), (0, -100), (-24, 13)])
+def test_factors_of_any_magnitude(rows, n_items, up, vp):
+    """f32 factors times 2^up and 2^vp: what is held of them does not depend on their size."""
+    d = make(rows, n_items, 17, F32, seed=8)
+    d["U"] *= 2.0 ** up
+    d["V"] *= 2.0 ** vp
+    c = to_gpu(d)
+    r = forward(c, 3)
+    g_lp, g_ent = torch.full((rows,), -1.0 / rows), torch.full((rows,), 0.1 / rows)
+    ref = reference(d, 3, g_lp, g_ent)
+    check_forward(d, r, 3, ref)
+    check_backward(d, backward(c, r, g_lp, g_ent), ref)
+
+
+@pytest.mark.parametrize("dtype,huge", [(F32, 1e20), (F32, 2e38), (F32, float("inf")), (BF16, 1e38),
+                                        (F16, 6e4)])
+@pytest.mark.parametrize("rows,n_items", [(5, 333), (300, 30_001)], ids=["few", "many"])
+def test_excluded_items_factors_do_not_matter(rows, n_items, dtype, huge):
+    """Items that their bias excludes, with factors of any size: every result is the one of zeros."""
+    d = make(rows, n_items, 17, dtype, seed=9)
+    out = torch.arange(0, n_items, 11)
+    d["b"][out] = torch.tensor([-np.inf, -1e30, -3e38], dtype=F32).repeat(len(out))[:len(out)]
+    d["V"][out] = 0
+    clean = dict(d, V=d["V"].clone())
+    d["V"][out] = torch.randn(len(out), 17).sign().mul(huge).to(dtype)
+    c = to_gpu(d)
+    r = forward(c, 3)
+    g_lp, g_ent = torch.full((rows,), -1.0 / rows), torch.full((rows,), 0.1 / rows)
+    ref = reference(clean, 3, g_lp, g_ent)
+    check_forward(clean, r, 3, ref)
+    got = backward(c, r, g_lp, g_ent)
+    check_backward(clean, got, ref)
+    assert (got[1][out.cuda()] == 0).all() and (got[2][out.cuda()] == 0).all()
+
+
+def test_products_beyond_f32_are_nan():
+    """Factors whose products leave f32 (2^121) give NaN, not a number of the wrong size."""
+    for rows, n_items in ((5, 333), (300, 30_001)):
+        d = make(rows, n_items, 17, F32, seed=10)
+        d["U"] *= 2.0 ** 62
+        d["V"] *= 2.0 ** 62
+        r = forward(to_gpu(d), 2)
+        assert torch.isnan(r.log_norm).all() and torch.isnan(r.log_probs).all()
+        assert (r.top_items == -1).all()
