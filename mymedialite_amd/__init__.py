@@ -21,12 +21,13 @@ from .rating_prediction import (BiasedMatrixFactorization, MatrixFactorization,
 def __getattr__(name):
     """The operators on torch tensors, loaded on first use: the recommenders need no torch."""
     if name in ("item_log_probs", "item_log_probs_grad"):
-        from . import item_softmax
-        return getattr(item_softmax, name)
-    if name == "AdamW":
-        from .adamw import AdamW
-        return AdamW
-    raise AttributeError(f"module {__name__!r} has no attribute {name!r}")
+        from . import item_softmax as module
+    elif name == "AdamW":
+        from . import adamw as module
+    else:
+        raise AttributeError(f"module {__name__!r} has no attribute {name!r}")
+    value = globals()[name] = getattr(module, name)
+    return value
 
 
 __all__ = ["BiasedMatrixFactorization", "MatrixFactorization", "SocialMF",

@@ -105,7 +105,7 @@ class AdamW:
                           self._bits)
         N.check(N.lib().mml_adamw_step_device(
             self._tensors, len(self.params), ctypes.byref(a), self._count.data_ptr(),
-            self._device.index, torch.cuda.current_stream(self._device).cuda_stream))
+            self._device.index, torch._C._cuda_getCurrentRawStream(self._device.index)))
 
     def state(self):
         """{"step", "m", "v"} and with 8 bits {"m_scale", "v_scale"}: the optimizer's own tensors

@@ -274,14 +274,16 @@ __global__ __launch_bounds__(256) void softmax_max_kernel(Job j) {
     if (s.vec8 && j.k % 4 == 0) {  // 4 factors a thread and turn
         const uint32_t quads = (uint32_t)j.k / 4;
         const int64_t n = s.n * quads;
-        for (int64_t x = (int64_t)part * 256 + threadIdx.x; x < n; x += (int64_t)parts * 256) {
-            const int64_t r = n >> 32 ? x / quads : (int64_t)((uint32_t)x / quads);
+        const int64_t at = (int64_t)part * 256 + threadIdx.x, turn = (int64_t)parts * 256;
+#pragma unroll 4
+        for (int64_t x = at; x < n; x += turn) {
+            const int64_t r = n >> 31 ? x / quads : (int64_t)((uint32_t)x / quads);
             const int64_t src = source_row(s, r);
-            if (src < 0) continue;
-            const f32x4 v = *(const f32x4*)((const float*)s.src + src * s.ld + 4 * (x - r * quads));
-            if (bias && bias[r] <= kGone) continue;
+            const f32x4 v = *(const f32x4*)((const float*)s.src + max(src, (int64_t)0) * s.ld +
+                                            4 * (x - r * quads));
+            const bool counts = src >= 0 && !(bias && bias[r] <= kGone);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) take(v[e]);
+            for (int e = 0; e < 4; ++e) take(counts ? v[e] : 0.0f);
         }
     } else {  // a wave per row and turn
         for (int64_t r = (int64_t)part * 4 + (threadIdx.x >> 6); r < s.n; r += (int64_t)parts * 4) {

@@ -18,6 +18,11 @@ from ._native import ItemLogProbs
 _DTYPES = {torch.float32: N.DTYPE_F32, torch.bfloat16: N.DTYPE_BF16, torch.float16: N.DTYPE_F16}
 
 
+def _stream(index):
+    """torch's current stream of device `index` as a pointer"""
+    return torch._C._cuda_getCurrentRawStream(index)
+
+
 def _factors(x, name):
     if not isinstance(x, torch.Tensor) or x.dim() != 2:
         raise ValueError(f"{name} must be a 2-D tensor")
@@ -26,49 +31,49 @@ def _factors(x, name):
     if not x.is_cuda:
         raise ValueError(f"{name} must be on the GPU")
     # a row stride under a row's length (an expanded tensor) is laid out
-    return x if x.stride(1) == 1 and x.stride(0) >= x.shape[1] else x.contiguous()
+    row, step = x.stride()
+    return x if step == 1 and row >= x.shape[1] else x.contiguous()
 
 
-def _vector(x, name, dtype, n, device):
+def _vector(x, name, dtype, n, index):
+    """x and its address"""
     if x is None:
-        return None
+        return None, None
     if not isinstance(x, torch.Tensor) or x.dim() != 1 or x.dtype != dtype:
         raise ValueError(f"{name} must be a 1-D {dtype} tensor")
     if n is not None and x.shape[0] != n:
         raise ValueError(f"{name} has {x.shape[0]} entries, expected {n}")
-    if x.device != device:
-        raise ValueError(f"{name} is on {x.device}, the factors are on {device}")
-    return x if x.stride(0) == 1 or x.numel() < 2 else x.contiguous()
-
-
-def _ptr(x):
-    return None if x is None else x.data_ptr()
+    if x.get_device() != index:
+        raise ValueError(f"{name} is on {x.device}, the factors are on cuda:{index}")
+    if x.stride(0) != 1 and x.shape[0] > 1:
+        x = x.contiguous()
+    return x, x.data_ptr()
 
 
 def _arguments(user_factors, item_factors, item_bias, items, users, exclude, n_top):
-    """(mml_item_softmax_args, the tensors that it points to)"""
+    """(mml_item_softmax_args, the device's index, the tensors that the arguments point to)"""
     U, V = _factors(user_factors, "user_factors"), _factors(item_factors, "item_factors")
     if U.dtype != V.dtype:
         raise ValueError("user_factors and item_factors must have one dtype")
-    if U.device != V.device:
+    index = U.get_device()
+    if index != V.get_device():
         raise ValueError("user_factors and item_factors must be on one device")
-    if U.shape[1] != V.shape[1]:
-        raise ValueError(f"{U.shape[1]} user factors, {V.shape[1]} item factors")
-    dev = U.device
-    bias = _vector(item_bias, "item_bias", torch.float32, V.shape[0], dev)
-    users = _vector(users, "users", torch.int32, None, dev)
-    rows = U.shape[0] if users is None else users.shape[0]
-    items = _vector(items, "items", torch.int32, rows, dev)
-    off = ex = None
+    (n_users, k), (n_items, kv) = U.shape, V.shape
+    if k != kv:
+        raise ValueError(f"{k} user factors, {kv} item factors")
+    bias, bias_at = _vector(item_bias, "item_bias", torch.float32, n_items, index)
+    users, users_at = _vector(users, "users", torch.int32, None, index)
+    rows = n_users if users is None else users.shape[0]
+    items, items_at = _vector(items, "items", torch.int32, rows, index)
+    off = ex = off_at = ex_at = None
     if exclude is not None:
-        off = _vector(exclude[0], "exclude[0]", torch.int64, U.shape[0] + 1, dev)
-        ex = _vector(exclude[1], "exclude[1]", torch.int32, None, dev)
-    n_top = int(n_top)
+        off, off_at = _vector(exclude[0], "exclude[0]", torch.int64, n_users + 1, index)
+        ex, ex_at = _vector(exclude[1], "exclude[1]", torch.int32, None, index)
     a = N.ItemSoftmaxArgs(
-        _DTYPES[U.dtype], U.shape[1], rows, U.shape[0], V.shape[0], U.data_ptr(), V.data_ptr(),
-        max(U.stride(0), U.shape[1]), max(V.stride(0), V.shape[1]), _ptr(bias), _ptr(users),
-        _ptr(items), _ptr(off), _ptr(ex), 0 if ex is None else ex.shape[0], n_top)
-    return a, (U, V, bias, users, items, off, ex)
+        _DTYPES[U.dtype], k, rows, n_users, n_items, U.data_ptr(), V.data_ptr(),
+        max(U.stride(0), k), max(V.stride(0), k), bias_at, users_at, items_at, off_at, ex_at,
+        0 if ex is None else ex.shape[0], int(n_top))
+    return a, index, (U, V, bias, users, items, off, ex)
 
 
 def _workspace(a, grad, device):
@@ -85,19 +90,20 @@ def item_log_probs(user_factors, item_factors, item_bias=None, items=None, users
     item_bias [n_items] float32; users [rows] int32: the rows' users (default: all, in order);
     items [rows] int32: the given items, -1 for none; exclude: (offsets [n_users + 1] int64, items
     int32), the CSR of every user's excluded items (Feedback.user_matrix); n_top <= 128."""
-    a, keep = _arguments(user_factors, item_factors, item_bias, items, users, exclude, n_top)
+    a, index, keep = _arguments(user_factors, item_factors, item_bias, items, users, exclude, n_top)
     dev, rows, n_top = keep[0].device, a.n_rows, a.n_top
     ws = _workspace(a, 0, dev)
-    out = torch.empty((3, rows), dtype=torch.float32, device=dev)
-    ids = lp = None
+    log_probs, log_norm, entropy = torch.empty((3, rows), dtype=torch.float32, device=dev).unbind()
+    p = log_probs.data_ptr()
+    ids = lp = ids_at = lp_at = None
     if n_top:
         ids = torch.empty((rows, n_top), dtype=torch.int32, device=dev)
         lp = torch.empty((rows, n_top), dtype=torch.float32, device=dev)
-    p = out.data_ptr()
+        ids_at, lp_at = ids.data_ptr(), lp.data_ptr()
     N.check(N.lib().mml_item_log_probs_device(
-        ctypes.byref(a), p, p + 4 * rows, p + 8 * rows, _ptr(ids), _ptr(lp), ws.data_ptr(),
-        ws.numel(), dev.index, torch.cuda.current_stream(dev).cuda_stream))
-    return ItemLogProbs(out[0], out[1], out[2], ids, lp)
+        ctypes.byref(a), p, p + 4 * rows, p + 8 * rows, ids_at, lp_at, ws.data_ptr(), ws.shape[0],
+        index, _stream(index)))
+    return ItemLogProbs(log_probs, log_norm, entropy, ids, lp)
 
 
 def item_log_probs_grad(user_factors, item_factors, item_bias=None, items=None, *, log_norm,
@@ -107,21 +113,21 @@ def item_log_probs_grad(user_factors, item_factors, item_bias=None, items=None, 
     by item_log_probs' log_probs and entropy (mml_item_log_probs_grad_device).  The first seven
     arguments are those of that call, log_norm and entropy its results.  dL/dU has one row per row
     of the batch; the factors' gradients have the factors' type, dL/db is float32."""
-    a, keep = _arguments(user_factors, item_factors, item_bias, items, users, exclude, 0)
+    a, index, keep = _arguments(user_factors, item_factors, item_bias, items, users, exclude, 0)
     U, V = keep[0], keep[1]
-    dev, rows = U.device, a.n_rows
-    vec = [_vector(x, n, torch.float32, rows, dev) for x, n in (
-        (log_norm, "log_norm"), (entropy, "entropy"), (grad_log_probs, "grad_log_probs"),
-        (grad_entropy, "grad_entropy"))]
-    if vec[0] is None:
+    dev, rows, k = U.device, a.n_rows, a.num_factors
+    if log_norm is None:
         raise ValueError("log_norm is required")
+    f32 = torch.float32
+    log_norm, norm_at = _vector(log_norm, "log_norm", f32, rows, index)
+    entropy, entropy_at = _vector(entropy, "entropy", f32, rows, index)
+    grad_log_probs, glp_at = _vector(grad_log_probs, "grad_log_probs", f32, rows, index)
+    grad_entropy, gent_at = _vector(grad_entropy, "grad_entropy", f32, rows, index)
     ws = _workspace(a, 1, dev)
-    k = a.num_factors
     gu = torch.empty((rows, k), dtype=U.dtype, device=dev)
-    gv = torch.empty((V.shape[0], k), dtype=U.dtype, device=dev)
-    gb = torch.empty(V.shape[0], dtype=torch.float32, device=dev)
+    gv = torch.empty((a.n_items, k), dtype=U.dtype, device=dev)
+    gb = torch.empty(a.n_items, dtype=f32, device=dev)
     N.check(N.lib().mml_item_log_probs_grad_device(
-        ctypes.byref(a), *(_ptr(x) for x in vec), gu.data_ptr(), k, gv.data_ptr(), k,
-        gb.data_ptr(), ws.data_ptr(), ws.numel(), dev.index,
-        torch.cuda.current_stream(dev).cuda_stream))
+        ctypes.byref(a), norm_at, entropy_at, glp_at, gent_at, gu.data_ptr(), k, gv.data_ptr(), k,
+        gb.data_ptr(), ws.data_ptr(), ws.shape[0], index, _stream(index)))
     return gu, gv, gb
