@@ -166,7 +166,7 @@ __device__ __forceinline__ Scale plain_scale() {
 // 2^86: scaled scores are below 2^35, so products beyond are far outside f32; and an excluded item's
 // score times kappa, 2^40 2^86, is still finite.
 constexpr int kLeastExponent = -86;
-constexpr int kMaxParts = 512, kUserParts = 64;  // partial maxima of softmax_max_kernel
+constexpr int kMaxParts = 512, kUserParts = 64;  // partial maxima of largest_factors
 
 struct Job {
     Side u, v;
@@ -234,11 +234,11 @@ __device__ __forceinline__ uint32_t take_plane(float& v) {
 // lists may be unsorted and may repeat an item (an OR of bits does not depend on the order); ids
 // outside the catalogue and offsets outside the array are skipped.
 constexpr int kMaskWords = 16384;
-__global__ __launch_bounds__(256) void softmax_mask_kernel(Job j) {
+__device__ __forceinline__ void make_mask(const Job& j, uint32_t block) {
     extern __shared__ uint32_t words[];
     const int parts = (j.v.tiles + kMaskWords - 1) / kMaskWords;
-    const int64_t r = blockIdx.x / parts;
-    const int w0 = (int)(blockIdx.x % parts) * kMaskWords, n = min(kMaskWords, j.v.tiles - w0);
+    const int64_t r = block / parts;
+    const int w0 = (int)(block % parts) * kMaskWords, n = min(kMaskWords, j.v.tiles - w0);
     for (int x = threadIdx.x; x < n; x += 256) words[x] = 0;
     const int64_t u = source_row(j.u, r);
     int64_t b = 0, e = 0;
@@ -258,11 +258,11 @@ __global__ __launch_bounds__(256) void softmax_mask_kernel(Job j) {
 // The largest finite magnitude of either matrix (the batch's users only, without the items that their
 // bias excludes), in kMaxParts parts.
 template <int T>
-__global__ __launch_bounds__(256) void softmax_max_kernel(Job j) {
+__device__ __forceinline__ void largest_factors(const Job& j, int block) {
     __shared__ float red[4];
-    const bool users = blockIdx.x < kUserParts;
+    const bool users = block < kUserParts;
     const Side& s = users ? j.u : j.v;
-    const int part = users ? blockIdx.x : blockIdx.x - kUserParts;
+    const int part = users ? block : block - kUserParts;
     const int parts = users ? kUserParts : kMaxParts - kUserParts;
     float m = 0.0f;
     const auto take = [&](float x) {
@@ -297,7 +297,19 @@ __global__ __launch_bounds__(256) void softmax_max_kernel(Job j) {
     if (lane == 0) red[threadIdx.x >> 6] = m;
     __syncthreads();
     if (threadIdx.x == 0)
-        j.parts[blockIdx.x] = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+        j.parts[block] = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+}
+// Both in one launch: kMaxParts blocks for the magnitudes (where j.parts is set), then the mask's.
+template <int T>
+__global__ __launch_bounds__(256) void softmax_start_kernel(Job j) {
+    uint32_t block = blockIdx.x;
+    if constexpr (T == MML_DTYPE_F32) {
+        if (j.parts) {
+            if (block < kMaxParts) return largest_factors<T>(j, (int)block);
+            block -= kMaxParts;
+        }
+    }
+    make_mask(j, block);
 }
 
 // The scales from the parts; all 256 threads of a block take part.  A matrix' largest magnitude comes
@@ -344,6 +356,38 @@ __device__ __forceinline__ Scale make_scale(const Job& j) {
     c.gu = gu;
     c.gv = gv;
     return c;
+}
+
+// The rows' constants of the gradient (thread t < 32 of a users' block: row r; bad as ubad).  A row
+// without one -- both coefficients 0, no items left, an unknown user -- gets lse2 = 1e30, so that its
+// p are 0.
+__device__ __forceinline__ void make_meta(const Job& j, int64_t r, int bad) {
+    float lse2 = 1e30f, c0 = 0.0f, c1 = 0.0f;
+    int32_t given = -1;
+    float w = 0.0f;
+    if (r < j.n_rows && bad < 2) {
+        const float lse = j.in_norm[r], h = j.g_ent ? j.g_ent[r] : 0.0f;
+        int32_t t = j.target ? j.target[r] : -1;
+        if (t < 0 || t >= j.n_items || (j.bias && j.bias[t] <= kGone) ||
+            (j.mask && (j.mask[r * j.v.tiles + (t >> 5)] >> (t & 31) & 1u)))
+            t = -1;
+        w = t >= 0 && j.g_lp ? j.g_lp[r] : 0.0f;
+        if ((w != 0.0f || h != 0.0f) && lse != -INFINITY) {
+            const float H = h != 0.0f ? j.in_entropy[r] : 0.0f;
+            lse2 = bad ? __builtin_nanf("") : lse * kLog2e;
+            c0 = -(w + h * H);
+            c1 = -h * kLn2;
+            given = t;
+        } else {
+            w = 0.0f;
+        }
+    }
+    RowMeta& m = j.meta[r >> 5];
+    m.lse2[r & 31] = lse2;
+    m.c0[r & 31] = c0;
+    m.c1[r & 31] = c1;
+    m.t[r & 31] = given;
+    j.w[r] = w;
 }
 
 // Fragments of both sides, one block per tile of 32 rows (the users' tiles first).  A row with a
@@ -394,6 +438,7 @@ __global__ __launch_bounds__(256) void softmax_prep_kernel(Job j) {
         const int64_t row = tl * 32 + t;
         if (users) {
             j.ubad[row] = (uint8_t)bad[t];
+            if (j.meta) make_meta(j, row, bad[t]);
         } else {
             float b = row < s.n ? (j.bias ? j.bias[row] : 0.0f) : kGone;
             if (b <= kGone) b = sc.gone;
@@ -437,39 +482,6 @@ __global__ __launch_bounds__(256) void softmax_prep_kernel(Job j) {
                 make_uint4(q[p][0] | q[p][1] << 16, q[p][2] | q[p][3] << 16,
                            q[p][4] | q[p][5] << 16, q[p][6] | q[p][7] << 16);
     }
-}
-
-// The rows' constants of the gradient.  A row without one -- both coefficients 0, no items left, an
-// unknown user -- gets lse2 = 1e30, so that its p are 0.
-__global__ __launch_bounds__(256) void softmax_meta_kernel(Job j) {
-    const int64_t r = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (r >= j.rows_pad) return;
-    float lse2 = 1e30f, c0 = 0.0f, c1 = 0.0f;
-    int32_t given = -1;
-    float w = 0.0f;
-    if (r < j.n_rows && j.ubad[r] < 2) {
-        const float lse = j.in_norm[r], h = j.g_ent ? j.g_ent[r] : 0.0f;
-        int32_t t = j.target ? j.target[r] : -1;
-        if (t < 0 || t >= j.n_items || j.vbias[t] <= j.scale->gone ||
-            (j.mask && (j.mask[r * j.v.tiles + (t >> 5)] >> (t & 31) & 1u)))
-            t = -1;
-        w = t >= 0 && j.g_lp ? j.g_lp[r] : 0.0f;
-        if ((w != 0.0f || h != 0.0f) && lse != -INFINITY) {
-            const float H = h != 0.0f ? j.in_entropy[r] : 0.0f;
-            lse2 = j.ubad[r] ? __builtin_nanf("") : lse * kLog2e;
-            c0 = -(w + h * H);
-            c1 = -h * kLn2;
-            given = t;
-        } else {
-            w = 0.0f;
-        }
-    }
-    RowMeta& m = j.meta[r >> 5];
-    m.lse2[r & 31] = lse2;
-    m.c0[r & 31] = c0;
-    m.c1[r & 31] = c1;
-    m.t[r & 31] = given;
-    j.w[r] = w;
 }
 
 // ------------------------------------------------------------------ staging
@@ -645,6 +657,9 @@ __device__ __forceinline__ void grad_tile(const uint4* a, const float (&g)[16],
     }
 }
 
+// The larger, or NaN if either is: what the instruction does without quieting its operands first
+__device__ __forceinline__ float largest(float a, float b) { return __builtin_elementwise_maximum(a, b); }
+
 __device__ __forceinline__ int reg_row(int i, int h) { return 8 * (i >> 2) + 4 * h + (i & 3); }
 
 // `gone` where the bits (shifted right by 4 h) say so.  The empty asm keeps the compiler from taking
@@ -707,23 +722,33 @@ softmax_forward_kernel(Job j) {
             copy_to_lds((const f32x4*)j.vbias + tl * 8 + lane, bias[at]);
     };
     const Scale sc = *j.scale;
-    float m = sc.floor, l = 0.0f, w = 0.0f, mx[TPS];
+    float m = sc.floor, m2 = m * sc.kappa, l = 0.0f, w = 0.0f, mx[TPS];
     uint32_t bits[TPS] = {}, next[TPS] = {};
     const auto load_bits = [&](int tl) {
 #pragma unroll
         for (int x = 0; x < TPS; ++x) next[x] = j.mask[row * j.v.tiles + tl + x];
     };
-    // a turn's maxima leave in the next turn, so that no wait meets the stores
+    // A turn's maxima leave in the next turn, so that no wait meets the stores.  mx: of this lane's 16
+    // items each; a swap joins the halves of two tiles, the first in the lower lanes.
     const auto store_max = [&](int tl) {
-        if (!TOP || h || !mine) return;
+        if (!TOP || !mine) return;
         float* p = j.cmax + row * j.cpad + tl;
-        if constexpr (TPS >= 4) {
-#pragma unroll
-            for (int x = 0; x < TPS; x += 4)
-                *(f32x4*)(p + x) = f32x4{mx[x], mx[x + 1], mx[x + 2], mx[x + 3]};
+        if constexpr (TPS == 1) {
+            const float most = both_max(mx[0]);
+            if (h == 0) *p = most;
         } else {
+            constexpr int N = TPS / 2;
+            float q[N];
 #pragma unroll
-            for (int x = 0; x < TPS; ++x) p[x] = mx[x];
+            for (int x = 0; x < N; ++x) {
+                const auto s = __builtin_amdgcn_permlane32_swap(
+                    __float_as_uint(mx[x]), __float_as_uint(mx[x + N]), false, false);
+                q[x] = largest(__uint_as_float(s[0]), __uint_as_float(s[1]));
+            }
+            p += N * h;
+            if constexpr (N == 4) *(f32x4*)p = f32x4{q[0], q[1], q[2], q[3]};
+            else if constexpr (N == 2) *(f32x2*)p = f32x2{q[0], q[1]};
+            else *p = q[0];
         }
     };
     if (t0 < t1) {
@@ -736,7 +761,7 @@ softmax_forward_kernel(Job j) {
         for (int x = 0; x < TPS; ++x) {
             // the wait for this load belongs before the next copies, not behind them
             asm volatile("" : "+v"(next[x]));
-            bits[x] = next[x] >> (4 * h);
+            bits[x] = next[x];
         }
         if (ts + TPS < t1) {
             load(ts + TPS, at ^ 1);
@@ -753,25 +778,25 @@ softmax_forward_kernel(Job j) {
                 for (int e = 0; e < 4; ++e) c[4 * q + e] = v[e];
             }
             c = score_tile<T, KT, 0>(buf[at] + x * PS * KT * 64, b, nullptr, c, lane);
-            if (__any(bits[x] & 0x0F0F0F0Fu)) mask_tile(c, bits[x], sc.gone);
+            if (__any(bits[x])) mask_tile(c, bits[x] >> (4 * h), sc.gone);
             float mt = c[0];
 #pragma unroll
-            for (int i = 1; i < 16; ++i) mt = fmaxf(mt, c[i]);
-            if constexpr (TOP) mx[x] = both_max(mt);
+            for (int i = 1; i < 16; ++i) mt = largest(mt, c[i]);
+            mx[x] = mt;
             if (__any(mt > m)) {
                 const float mn = fmaxf(m, mt), d = (m - mn) * sc.kappa;
                 const float f = __builtin_amdgcn_exp2f(d);
                 w = f * fmaf(l, d, w);
                 l *= f;
                 m = mn;
+                m2 = m * sc.kappa;
             }
-            const float m2 = m * sc.kappa;
-            float sl = 0.0f, sw = 0.0f;
+            float sl, sw;
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
                 const float y = fmaf(c[i], sc.kappa, -m2), e = __builtin_amdgcn_exp2f(y);
-                sl += e;
-                sw = fmaf(e, y, sw);
+                sl = i ? sl + e : e;
+                sw = i ? fmaf(e, y, sw) : e * y;
             }
             l += sl;
             w += sw;
@@ -1533,8 +1558,8 @@ __device__ __forceinline__ f32x4 join_splits(const float* __restrict__ part, int
 }
 // The users' rows with w V_t added
 template <int T>
-__global__ __launch_bounds__(256) void softmax_join_users_kernel(Job j, int32_t kp) {
-    const int64_t x = ((int64_t)blockIdx.x * 256 + threadIdx.x) / kJoin;
+__device__ __forceinline__ void join_users(const Job& j, int32_t kp, uint32_t block) {
+    const int64_t x = ((int64_t)block * 256 + threadIdx.x) / kJoin;
     const int quads = (j.k + 3) / 4;
     const bool in = x < j.n_rows * quads;  // (all lanes take part in the join)
     const int64_t r = in ? x / quads : 0;
@@ -1550,8 +1575,8 @@ __global__ __launch_bounds__(256) void softmax_join_users_kernel(Job j, int32_t 
     store_factors<T>(j.gu, r * j.ld_gu, f, j.k, j.gu_vec4, a);
 }
 template <int T>
-__global__ __launch_bounds__(256) void softmax_join_items_kernel(Job j, int32_t kp) {
-    const int64_t x = ((int64_t)blockIdx.x * 256 + threadIdx.x) / kJoin;
+__device__ __forceinline__ void join_items(const Job& j, int32_t kp, uint32_t block) {
+    const int64_t x = ((int64_t)block * 256 + threadIdx.x) / kJoin;
     const int64_t items_pad = (int64_t)j.v.tiles * 32;
     const int quads = (j.k + 3) / 4;
     const bool in = x < (int64_t)j.n_items * quads;
@@ -1565,6 +1590,12 @@ __global__ __launch_bounds__(256) void softmax_join_items_kernel(Job j, int32_t 
         for (int s = 0; s < j.vsplits; ++s) b += j.db_part[s * items_pad + i];
         j.gb[i] = b;
     }
+}
+// Both in one launch: `users` blocks for the users' rows, then the items' (vsplits > 1).
+template <int T>
+__global__ __launch_bounds__(256) void softmax_join_kernel(Job j, int32_t kp, uint32_t users) {
+    if (blockIdx.x < users) join_users<T>(j, kp, blockIdx.x);
+    else join_items<T>(j, kp, blockIdx.x - users);
 }
 
 // ------------------------------------------------------------------ host side
@@ -1727,14 +1758,16 @@ uint32_t grid_of(int64_t n) {
     return (uint32_t)n;
 }
 
-void make_mask(const Job& j, hipStream_t st) {
-    if (!j.mask) return;
-    const int64_t parts = (j.v.tiles + kMaskWords - 1) / kMaskWords;
-    softmax_mask_kernel<<<grid_of(j.rows_pad * parts), 256,
-                          std::min(j.v.tiles, kMaskWords) * sizeof(uint32_t), st>>>(j);
-}
+// The mask, the scales and the fragments (direct: the mask only)
 void prepare(const Job& j, int T, hipStream_t st) {
-    if (T == MML_DTYPE_F32) softmax_max_kernel<MML_DTYPE_F32><<<kMaxParts, 256, 0, st>>>(j);
+    dispatch(T, 1, [&](auto tt, auto) {
+        const int64_t parts = (j.v.tiles + kMaskWords - 1) / kMaskWords;
+        const int64_t blocks = (j.parts ? kMaxParts : 0) + (j.mask ? j.rows_pad * parts : 0);
+        const size_t lds = j.mask ? std::min(j.v.tiles, kMaskWords) * sizeof(uint32_t) : 0;
+        if (blocks)
+            softmax_start_kernel<decltype(tt)::value><<<grid_of(blocks), 256, lds, st>>>(j);
+    });
+    if (j.direct) return;
     dispatch(T, steps_of(j.k), [&](auto tt, auto kt) {
         softmax_prep_kernel<decltype(tt)::value, decltype(kt)::value>
             <<<grid_of((int64_t)j.u.tiles + j.v.tiles), 256, 0, st>>>(j);
@@ -1769,9 +1802,8 @@ void item_log_probs(const mml_item_softmax_args* a, float* log_probs, float* log
     j.entropy = entropy;
     j.top_items = top_items;
     j.top_lp = top_log_probs;
-    make_mask(j, st);
+    prepare(j, a->dtype, st);
     const uint32_t direct_blocks = grid_of((int64_t)j.u.tiles * j.splits);
-    if (!j.direct) prepare(j, a->dtype, st);
     dispatch(a->dtype, steps_of(j.k), [&](auto tt, auto kt) {
         constexpr int T = decltype(tt)::value, KT = decltype(kt)::value;
         constexpr int W = forward_waves<T, KT>();
@@ -1838,25 +1870,19 @@ void item_log_probs_grad(const mml_item_softmax_args* a, const float* log_norm,
     j.gu_vec4 = j.k % 4 == 0 && ld_gu % 4 == 0 && (uintptr_t)gu % (4 * size) == 0;
     j.gv_vec4 = j.k % 4 == 0 && ld_gv % 4 == 0 && (uintptr_t)gv % (4 * size) == 0;
     const int kt0 = steps_of(j.k), kp = std::max(32, kt0 * 16);
-    if (a->n_rows > 0) {
-        make_mask(j, st);
-        prepare(j, a->dtype, st);
-        softmax_meta_kernel<<<grid_of((j.rows_pad + 255) / 256), 256, 0, st>>>(j);
-    }
+    if (a->n_rows > 0) prepare(j, a->dtype, st);
     const int64_t quads = (j.k + 3) / 4;
     const uint32_t ju = grid_of((j.n_rows * quads * kJoin + 255) / 256);
-    const uint32_t ji = grid_of(((int64_t)j.n_items * quads * kJoin + 255) / 256);
+    const uint32_t ji =
+        j.vsplits > 1 ? grid_of(((int64_t)j.n_items * quads * kJoin + 255) / 256) : 0;
     dispatch(a->dtype, kt0, [&](auto tt, auto kt) {
         constexpr int T = decltype(tt)::value, KT = decltype(kt)::value, UW = users_waves<T, KT>();
         constexpr int IW = kItemsWaves;
         const uint32_t ub = grid_of((int64_t)((j.u.tiles + UW - 1) / UW) * j.splits);
         const uint32_t vb = grid_of((int64_t)((j.v.tiles + IW - 1) / IW) * j.vsplits);
-        if (j.n_rows > 0) {
-            softmax_grad_users_kernel<T, KT><<<ub, UW * 64, 0, st>>>(j);
-            softmax_join_users_kernel<T><<<ju, 256, 0, st>>>(j, kp);
-        }
+        if (j.n_rows > 0) softmax_grad_users_kernel<T, KT><<<ub, UW * 64, 0, st>>>(j);
         softmax_grad_items_kernel<T, KT><<<vb, IW * 64, 0, st>>>(j);
-        if (j.vsplits > 1) softmax_join_items_kernel<T><<<ji, 256, 0, st>>>(j, kp);
+        if (ju + ji) softmax_join_kernel<T><<<grid_of((int64_t)ju + ji), 256, 0, st>>>(j, kp, ju);
     });
     MML_HIP(hipGetLastError());
 }
