@@ -199,7 +199,8 @@ struct Job {
     RowMeta* meta;  // [u.tiles]
     float* w;       // [rows_pad]
     float *du_part, *dv_part, *db_part;
-    int32_t vsplits;
+    int32_t vsplits;  // of the item tiles from vwhole on; those before have one block each
+    int32_t vwhole;
     void *gu, *gv;
     int64_t ld_gu, ld_gv;
     int32_t gu_vec4, gv_vec4;
@@ -1454,8 +1455,9 @@ softmax_grad_items_kernel(Job j) {
     __shared__ uint4 sbuf[NB][NS * 64], tbuf[NB][NT * 64], kept[WAVES][LK ? PS * LK * 64 : 1];
     __shared__ __align__(16) RowMeta mbuf[2];
     const int lane = threadIdx.x & 63, h = lane >> 5, wave = threadIdx.x >> 6;
-    const int split = blockIdx.x % j.vsplits;
-    const int64_t vt = (int64_t)(blockIdx.x / j.vsplits) * WAVES + wave;
+    const int whole = j.vwhole / WAVES, rest = (int)blockIdx.x - whole;
+    const int splits = rest < 0 ? 1 : j.vsplits, split = rest < 0 ? 0 : rest % splits;
+    const int64_t vt = (int64_t)(rest < 0 ? (int)blockIdx.x : whole + rest / splits) * WAVES + wave;
     const bool mine = vt < j.v.tiles;
     const int64_t item = (mine ? vt : 0) * 32 + (lane & 31);
     uint4 b[PS][KT - LK], *mykept = kept[wave];
@@ -1465,8 +1467,8 @@ softmax_grad_items_kernel(Job j) {
     Shift sh;
     f32x16 acc[MT] = {};
     float db = 0.0f;
-    const int t0 = (int)((int64_t)j.u.tiles * split / j.vsplits);
-    const int t1 = (int)((int64_t)j.u.tiles * (split + 1) / j.vsplits);
+    const int t0 = (int)((int64_t)j.u.tiles * split / splits);
+    const int t1 = (int)((int64_t)j.u.tiles * (split + 1) / splits);
     uint32_t next = 0;
     const auto load_trans = [&](int tl, int at) {
         stage<WAVES>(j.u.trans + (int64_t)tl * NT * 64, tbuf[at], NT);
@@ -1539,7 +1541,7 @@ softmax_grad_items_kernel(Job j) {
     for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
         for (int i = 0; i < 16; ++i) acc[mt][i] = unscale<T>(acc[mt][i], sh, sc.gu);
-    if (j.vsplits == 1) {  // nothing to join: the result itself
+    if (splits == 1) {  // nothing to join: the result itself
         if (item >= j.n_items) return;
         if (h == 0) j.gb[item] = db;
 #pragma unroll
@@ -1551,14 +1553,15 @@ softmax_grad_items_kernel(Job j) {
                                        acc[mt][4 * q + 3]});
         return;
     }
-    float* out = j.dv_part + ((int64_t)split * items_pad + item) * KP;
+    const int64_t first = (int64_t)j.vwhole * 32, parted = items_pad - first;
+    float* out = j.dv_part + ((int64_t)split * parted + item - first) * KP;
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
         for (int q = 0; q < 4; ++q)
             *(f32x4*)&out[32 * mt + 8 * q + 4 * h] =
                 f32x4{acc[mt][4 * q], acc[mt][4 * q + 1], acc[mt][4 * q + 2], acc[mt][4 * q + 3]};
-    if (h == 0) j.db_part[split * items_pad + item] = db;
+    if (h == 0) j.db_part[split * parted + item - first] = db;
 }
 
 // Four factors of a row summed over the splits: kJoin neighbouring threads take every kJoin-th split
@@ -1597,18 +1600,18 @@ __device__ __forceinline__ void join_users(const Job& j, int32_t kp, uint32_t bl
 template <int T>
 __device__ __forceinline__ void join_items(const Job& j, int32_t kp, uint32_t block) {
     const int64_t x = ((int64_t)block * 256 + threadIdx.x) / kJoin;
-    const int64_t items_pad = (int64_t)j.v.tiles * 32;
+    const int64_t first = (int64_t)j.vwhole * 32, parted = (int64_t)j.v.tiles * 32 - first;
     const int quads = (j.k + 3) / 4;
-    const bool in = x < (int64_t)j.n_items * quads;
-    const int64_t i = in ? x / quads : 0;
+    const bool in = x < (j.n_items - first) * quads;
+    const int64_t i = in ? x / quads : 0;  // (from the first item in parts on)
     const int f = in ? 4 * (int)(x % quads) : 0;
-    const f32x4 a = join_splits(j.dv_part + i * kp + f, items_pad * kp, j.vsplits);
+    const f32x4 a = join_splits(j.dv_part + i * kp + f, parted * kp, j.vsplits);
     if (!in || threadIdx.x % kJoin) return;
-    store_factors<T>(j.gv, i * j.ld_gv, f, j.k, j.gv_vec4, a);
+    store_factors<T>(j.gv, (first + i) * j.ld_gv, f, j.k, j.gv_vec4, a);
     if (f == 0) {
         float b = 0.0f;
-        for (int s = 0; s < j.vsplits; ++s) b += j.db_part[s * items_pad + i];
-        j.gb[i] = b;
+        for (int s = 0; s < j.vsplits; ++s) b += j.db_part[s * parted + i];
+        j.gb[first + i] = b;
     }
 }
 // Both in one launch: `users` blocks for the users' rows, then the items' (vsplits > 1).
@@ -1651,23 +1654,43 @@ void dispatch(int T, int kt, F&& f) {
 // long as one (measured: 1.6 times the throughput from one to two, 1.2 from two to four); a block 6,000
 // to start; results are written and read back at 2 KB a cycle.  Above 8, a multiple of the 8 XCDs:
 // block b runs on XCD b mod 8, so a split's blocks share an L2.
-int32_t choose_splits(int64_t kept, int64_t streamed, int waves, int per_simd, int instructions,
-                      double bytes) {
+struct Splits {
+    int32_t n = 1, whole = 0;  // kept tiles from `whole` on are split n ways, those before are not
+    double cost = 0.0;
+};
+double block_time(int64_t per_cu, int waves, int instructions, int64_t tiles) {
+    return (per_cu * waves / 4.0 + 1.5) / 2.5 * (instructions * 32.0 + 500.0) * tiles + 6000.0;
+}
+Splits choose_splits(int64_t kept, int64_t streamed, int waves, int per_simd, int instructions,
+                     double bytes) {
     const int64_t row_blocks = std::max<int64_t>(1, (kept + waves - 1) / waves);
     const int64_t most_per_cu = std::max(1, per_simd * 4 / waves);
-    double best = 0.0;
-    int32_t chosen = 1;
-    for (int64_t s = 1; s <= 1024 && s <= streamed; s += s < 8 ? 1 : 8) {
+    Splits best;
+    for (int64_t s = 1; s <= 1024 && s <= std::max<int64_t>(1, streamed); s += s < 8 ? 1 : 8) {
         const int64_t blocks = row_blocks * s;
         const int64_t per_cu = std::min(most_per_cu, (blocks + 255) / 256);
-        const double tile = (per_cu * waves / 4.0 + 1.5) / 2.5 * (instructions * 32.0 + 500.0);
-        const double one = tile * ((streamed + s - 1) / s) + 6000.0;
+        const double one = block_time(per_cu, waves, instructions, (streamed + s - 1) / s);
         const double fill = (double)blocks / (256.0 * per_cu);
         const double cost = (fill <= 1.0 ? 1.0 : fill + 0.35) * one +
                             (s > 1 ? s * kept * bytes / 1024.0 : 0.0);
-        if (s == 1 || cost < best) best = cost, chosen = (int32_t)s;
+        if (s == 1 || cost < best.cost) best.cost = cost, best.n = (int32_t)s;
     }
-    return chosen;
+    return best;
+}
+// The same with the kept tiles that fill the CUs a whole number of times left in one piece: a few
+// blocks more than fit run alone at the end, and only they are split (2,048 x 100 k, k = 64, 782
+// blocks in 768 places: 234 us for the items' gradient, 187 so).
+Splits choose_splits_of_rest(int64_t kept, int64_t streamed, int waves, int per_simd,
+                             int instructions, double bytes) {
+    const Splits all = choose_splits(kept, streamed, waves, per_simd, instructions, bytes);
+    const int64_t per_cu = std::max(1, per_simd * 4 / waves);
+    const int64_t rounds = kept / waves / (256 * per_cu), whole = rounds * 256 * per_cu * waves;
+    if (rounds == 0 || whole == kept) return all;
+    Splits rest =
+        choose_splits(kept - whole, streamed, waves, per_simd, instructions, bytes);
+    rest.cost += rounds * block_time(per_cu, waves, instructions, streamed);
+    rest.whole = (int32_t)whole;
+    return rest.n > 1 && rest.cost < all.cost ? rest : all;
 }
 
 struct Carve {  // a workspace cut into arrays of 256-byte alignment (base null: sizes only)
@@ -1726,9 +1749,11 @@ int64_t plan(const mml_item_softmax_args* a, bool grad, void* base, Job& j) {
             constexpr int TT = decltype(tt)::value, KT = decltype(k)::value;
             constexpr int M = Planes<TT>::PS == 2 ? 6 * KT : 3 * KT;
             j.splits = choose_splits(j.u.tiles, j.v.tiles, users_waves<TT, KT>(),
-                                     users_per_simd<TT, KT>(), M, mt * 4096.0);
-            j.vsplits = choose_splits(j.v.tiles, j.u.tiles, kItemsWaves, items_per_simd<TT, KT>(),
-                                      M, mt * 4096.0);
+                                     users_per_simd<TT, KT>(), M, mt * 4096.0).n;
+            const Splits v = choose_splits_of_rest(j.v.tiles, j.u.tiles, kItemsWaves,
+                                                   items_per_simd<TT, KT>(), M, mt * 4096.0);
+            j.vsplits = v.n;
+            j.vwhole = v.whole;
         });
     } else if (j.u.tiles <= 1 || (int64_t)j.u.tiles * j.v.tiles * kt <= 16384) {
         // no preparation: one tile of users, or as little work as 100 k items at k = 64 with one (37
@@ -1742,7 +1767,7 @@ int64_t plan(const mml_item_softmax_args* a, bool grad, void* base, Job& j) {
             constexpr int M = Planes<TT>::PS == 2 ? 3 * KT : KT;
             j.splits = choose_splits(j.u.tiles, j.v.tiles / forward_tiles<TT, KT>(),
                                      forward_waves<TT, KT>(), forward_per_simd<TT, KT>(),
-                                     M * forward_tiles<TT, KT>(), 384.0);
+                                     M * forward_tiles<TT, KT>(), 384.0).n;
         });
     }
     Carve c{(char*)base};
@@ -1766,8 +1791,9 @@ int64_t plan(const mml_item_softmax_args* a, bool grad, void* base, Job& j) {
         j.w = c.take<float>(j.rows_pad);
         j.du_part = c.take<float>((int64_t)j.splits * j.rows_pad * mt * 32);
         if (j.vsplits > 1) {
-            j.dv_part = c.take<float>((int64_t)j.vsplits * items_pad * mt * 32);
-            j.db_part = c.take<float>((int64_t)j.vsplits * items_pad);
+            const int64_t parted = items_pad - (int64_t)j.vwhole * 32;
+            j.dv_part = c.take<float>(j.vsplits * parted * mt * 32);
+            j.db_part = c.take<float>(j.vsplits * parted);
         }
     }
     return std::max<int64_t>(c.used, 256);
@@ -1894,12 +1920,15 @@ void item_log_probs_grad(const mml_item_softmax_args* a, const float* log_norm,
     const int64_t quads = (j.k + 3) / 4;
     const uint32_t ju = grid_of((j.n_rows * quads * kJoin + 255) / 256);
     const uint32_t ji =
-        j.vsplits > 1 ? grid_of(((int64_t)j.n_items * quads * kJoin + 255) / 256) : 0;
+        j.vsplits > 1
+            ? grid_of(((j.n_items - (int64_t)j.vwhole * 32) * quads * kJoin + 255) / 256)
+            : 0;
     dispatch(a->dtype, kt0, [&](auto tt, auto kt) {
         constexpr int T = decltype(tt)::value, KT = decltype(kt)::value, UW = users_waves<T, KT>();
         constexpr int IW = kItemsWaves;
         const uint32_t ub = grid_of((int64_t)((j.u.tiles + UW - 1) / UW) * j.splits);
-        const uint32_t vb = grid_of((int64_t)((j.v.tiles + IW - 1) / IW) * j.vsplits);
+        const uint32_t vb = grid_of(j.vwhole / IW +
+                                    (int64_t)((j.v.tiles - j.vwhole + IW - 1) / IW) * j.vsplits);
         if (j.n_rows > 0) softmax_grad_users_kernel<T, KT><<<ub, UW * 64, 0, st>>>(j);
         softmax_grad_items_kernel<T, KT><<<vb, IW * 64, 0, st>>>(j);
         if (ju + ji) softmax_join_kernel<T><<<grid_of((int64_t)ju + ji), 256, 0, st>>>(j, kp, ju);

@@ -542,3 +542,15 @@ def test_products_beyond_f32_are_nan():
         r = forward(to_gpu(d), 2)
         assert torch.isnan(r.log_norm).all() and torch.isnan(r.log_probs).all()
         assert (r.top_items == -1).all()
+
+
+@pytest.mark.parametrize("dtype,k", [(F32, 5), (BF16, 130)], ids=["f32", "bf16"])
+def test_gradient_with_a_few_items_more_than_fit(dtype, k):
+    """A catalogue just above what the CUs hold at once: the items behind it are split over the rows
+    and joined, the others are not."""
+    rows, n_items = 300, (98_500 if dtype == F32 else 65_700)
+    d = make(rows, n_items, k, dtype, seed=12, seen=3)
+    c = to_gpu(d)
+    r = forward(c)
+    g_lp, g_ent = torch.full((rows,), -1.0 / rows), torch.full((rows,), 0.1 / rows)
+    check_backward(d, backward(c, r, g_lp, g_ent), reference(d, 0, g_lp, g_ent))
