@@ -655,6 +655,14 @@ __device__ __forceinline__ void grad_tile(const uint4* a, const float (&g)[16],
                 for (int p = P::PG - 1; p >= 0; --p)
                     if (sum - p >= 0 && sum - p < P::GP) acc[mt] = mfma<T>(x[p], q[sum - p], acc[mt]);
         }
+        // two tiles' LDS reads (0x100) ahead of their matrix instructions (0x008): 1,024 x 500 k, k = 256
+        // bf16: the users' gradient in 664 us against 683; one or three ahead gain less
+        __builtin_amdgcn_sched_group_barrier(0x100, 2 * P::PG, 0);
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) {
+            __builtin_amdgcn_sched_group_barrier(0x008, P::PG == 2 ? 3 : 2, 0);
+            __builtin_amdgcn_sched_group_barrier(0x100, P::PG, 0);
+        }
     }
 }
 
