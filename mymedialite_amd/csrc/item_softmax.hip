@@ -272,27 +272,32 @@ __device__ __forceinline__ void largest_factors(const Job& j, int block) {
     };
     const int lane = threadIdx.x & 63;
     const float* bias = users ? nullptr : j.bias;
-    if (s.vec8 && j.k % 4 == 0) {  // 4 factors a thread and turn
-        const uint32_t quads = (uint32_t)j.k / 4;
-        const int64_t n = s.n * quads;
+    // the factors 4 at a time where they can be loaded so, else one by one
+    const auto scan = [&](auto width) {
+        constexpr int N = decltype(width)::value;
+        const uint32_t per_row = (uint32_t)j.k / N;
+        const int64_t n = s.n * per_row;
         const int64_t at = (int64_t)part * 256 + threadIdx.x, turn = (int64_t)parts * 256;
 #pragma unroll 4
         for (int64_t x = at; x < n; x += turn) {
-            const int64_t r = n >> 31 ? x / quads : (int64_t)((uint32_t)x / quads);
+            const int64_t r = n >> 31 ? x / per_row : (int64_t)((uint32_t)x / per_row);
             const int64_t src = source_row(s, r);
-            const f32x4 v = *(const f32x4*)((const float*)s.src + max(src, (int64_t)0) * s.ld +
-                                            4 * (x - r * quads));
+            const float* p = (const float*)s.src + max(src, (int64_t)0) * s.ld + N * (x - r * per_row);
+            float v[N];
+            if constexpr (N == 4) {
+                const f32x4 q = *(const f32x4*)p;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[e] = q[e];
+            } else {
+                v[0] = *p;
+            }
             const bool counts = src >= 0 && !(bias && bias[r] <= kGone);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) take(counts ? v[e] : 0.0f);
+            for (int e = 0; e < N; ++e) take(counts ? v[e] : 0.0f);
         }
-    } else {  // a wave per row and turn
-        for (int64_t r = (int64_t)part * 4 + (threadIdx.x >> 6); r < s.n; r += (int64_t)parts * 4) {
-            const int64_t src = source_row(s, r);
-            if (src < 0 || (bias && bias[r] <= kGone)) continue;
-            for (int f = lane; f < j.k; f += 64) take(load_factor<T>(s.src, src * s.ld + f));
-        }
-    }
+    };
+    if (s.vec8 && j.k % 4 == 0) scan(std::integral_constant<int, 4>{});
+    else scan(std::integral_constant<int, 1>{});
 #pragma unroll
     for (int d = 32; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor(m, d));
     if (lane == 0) red[threadIdx.x >> 6] = m;
@@ -717,8 +722,8 @@ softmax_forward_kernel(Job j) {
     const int lane = threadIdx.x & 63, h = lane >> 5, wave = threadIdx.x >> 6;
     const int split = blockIdx.x % j.splits;
     const int64_t ut = (int64_t)(blockIdx.x / j.splits) * WAVES + wave;
-    // A wave behind the last tile of users does tile 0's work and drops it: a branch around the work
-    // costs the others more (the accumulators change registers at it).
+    // A wave behind the last tile of users has a loop of its own: a branch around the work in the common
+    // one costs the others more than the work (the accumulators change registers at it).
     const bool mine = ut < j.u.tiles;
     const int64_t row = (mine ? ut : 0) * 32 + (lane & 31);
     uint4 b[PS][KT];
@@ -740,7 +745,7 @@ softmax_forward_kernel(Job j) {
     // A turn's maxima leave in the next turn, so that no wait meets the stores.  mx: of this lane's 16
     // items each; a swap joins the halves of two tiles, the first in the lower lanes.
     const auto store_max = [&](int tl) {
-        if (!TOP || !mine) return;
+        if (!TOP) return;
         float* p = j.cmax + row * j.cpad + tl;
         if constexpr (TPS == 1) {
             const float most = both_max(mx[0]);
@@ -763,6 +768,13 @@ softmax_forward_kernel(Job j) {
     if (t0 < t1) {
         load(t0, 0);
         if (j.mask) load_bits(t0);
+    }
+    if (!mine) {  // copies its share
+        for (int ts = t0, at = 0; ts < t1; ts += TPS, at ^= 1) {
+            stage_wait();
+            if (ts + TPS < t1) load(ts + TPS, at ^ 1);
+        }
+        return;
     }
     for (int ts = t0, at = 0; ts < t1; ts += TPS, at ^= 1) {
         stage_wait();
@@ -812,7 +824,6 @@ softmax_forward_kernel(Job j) {
         }
     }
     if (t0 < t1) store_max(t1 - TPS);
-    if (!mine) return;
     // the halves' states joined: lanes l and l + 32 hold the same user
     const float mn = both_max(m), d = (m - mn) * sc.kappa;
     const float f = __builtin_amdgcn_exp2f(d);
@@ -1043,7 +1054,7 @@ __device__ __forceinline__ double exact_score(const Job& j, const double* u, int
     double a = 0.0;
     const int64_t at = i * j.v.ld;
     if (j.v.vec8 && j.k % 8 == 0) {  // whole groups of 8 factors in loads of 16 bytes
-#pragma unroll 4
+#pragma unroll 2
         for (int f = 8 * lane; f < j.k; f += 8 * LANES) {
             float x[8];
             load_factors<T>(j.v.src, at + f, x);
@@ -1078,7 +1089,8 @@ __device__ __forceinline__ uint32_t key_of(float x) {
     return b >> 31 ? ~b : b | 1u << 31;
 }
 
-constexpr int kListed = 1024;  // tiles that the selection below lists at most
+constexpr int kListed = 1024;     // tiles that the selection below lists at most
+constexpr int kCandidates = 512;  // and items, in the same memory
 
 // A bound that at least `want` of the 256 keys reach and few more: the want-th largest key with its
 // low bits cut off, found bit by bit.  One wave, four keys a lane.
@@ -1158,6 +1170,7 @@ __device__ __forceinline__ void select_tiles(const Maxima<NT>& maxima, int want,
             const uint32_t v = key[x];
             const int32_t i = index[x];
             int r = 0;
+#pragma unroll 4
             for (int y = 0; y < n; ++y) r += before(key[y], index[y], v, i);
             if (r < want) chosen[r] = i;
         }
@@ -1202,7 +1215,11 @@ template <int T, int NT>
 __global__ __launch_bounds__(NT) void softmax_finish_kernel(Job j) {
     constexpr bool TOP = NT > 64;
     __shared__ double urow[256], joined[2];
-    __shared__ uint32_t key[TOP ? kListed : 1], least_tile;
+    // the tiles' keys, later the candidates' (the listed ones' order is that of a counter: any)
+    __shared__ uint64_t listed_key[TOP ? kCandidates : 1];
+    static_assert(kListed * sizeof(uint32_t) == kCandidates * sizeof(uint64_t), "one array for both");
+    __shared__ uint32_t least_tile;
+    uint32_t* key = reinterpret_cast<uint32_t*>(listed_key);
     const int64_t r = blockIdx.x;
     const int t = threadIdx.x;
     const int64_t u = source_row(j.u, r);
@@ -1286,45 +1303,94 @@ __global__ __launch_bounds__(NT) void softmax_finish_kernel(Job j) {
         __syncthreads();
         select_tiles<NT>(maxima, want, least_tile, chosen, key, index, found_tiles);
         const uint64_t none = key_of(-INFINITY);
-        for (int x = t >> 2; x < want * 32; x += NT / 4) {
-            const int64_t i = (int64_t)chosen[x >> 5] * 32 + (x & 31);
-            uint64_t k = none;
-            if (i < j.n_items && !is_excluded(j, r, i))
-                k = key_of(exact_score<T, 4>(j, urow, i, t & 3));
-            if ((t & 3) == 0) {
-                cand[x] = k;
-                atomicMax(&tmax[x >> 5], (unsigned long long)k);
-            }
+        const auto item_at = [&](int x) { return (int64_t)chosen[x >> 5] * 32 + (x & 31); };
+        const auto keep = [&](int x, int64_t i, double score) {
+            const uint64_t k = i < j.n_items && !is_excluded(j, r, i) ? key_of(score) : none;
+            if ((t & 3) == 0) cand[x] = k;
+            // the 16 items of a wave's turn are half a tile
+            uint64_t most = k;
+#pragma unroll
+            for (int d = 4; d < 64; d <<= 1)
+                most = max(most, (uint64_t)__shfl_xor((unsigned long long)most, d));
+            if ((t & 63) == 0) atomicMax(&tmax[x >> 5], (unsigned long long)most);
+        };
+        // two items a turn, whose loads are on the way together (want * 32 and NT / 4 are multiples of
+        // 32: a wave's lanes stay together)
+        for (int x = t >> 2; x < want * 32; x += NT / 2) {
+            const int y = x + NT / 4;
+            const bool two = y < want * 32;
+            const int64_t i = item_at(x), o = item_at(two ? y : x);
+            const int64_t last = j.n_items - 1;
+            const double a = exact_score<T, 4>(j, urow, min(i, last), t & 3);
+            const double b = exact_score<T, 4>(j, urow, min(o, last), t & 3);
+            keep(x, i, a);
+            if (two) keep(y, o, b);
         }
         __syncthreads();
         if (t < want) {  // the n-th largest of the tiles' maxima (none where there are fewer tiles)
             int rank = 0;
+#pragma unroll 4
             for (int x = 0; x < want; ++x) rank += before(tmax[x], x, tmax[t], t);
             if (rank == n - 1) bound = tmax[t];
         }
         __syncthreads();
-        const uint64_t least = max((uint64_t)bound, none + 1);
-        for (int x = t; x < want * 32; x += NT)
-            if (cand[x] >= least) {
-                const int at = atomicAdd(&count, 1);
-                if (at < kListed) index[at] = x;
+        uint64_t least = max((uint64_t)bound, none + 1);
+        const auto list = [&] {
+            for (int x = t; x < want * 32; x += NT)
+                if (cand[x] >= least) {
+                    const int at = atomicAdd(&count, 1);
+                    if (at < kCandidates) {
+                        listed_key[at] = cand[x];
+                        index[at] = (int32_t)item_at(x);
+                    }
+                }
+            __syncthreads();
+        };
+        list();
+        if (count > kCandidates) {
+            // Few tiles for so many items: the n-th largest key's upper half, bit by bit
+            __shared__ int reach[32];
+            uint32_t upper = 0;
+            __syncthreads();  // (count is read by all)
+            if (t < 32) reach[t] = 0;
+            if (t == 0) count = 0;
+            __syncthreads();
+#pragma unroll 1
+            for (int bit = 31; bit >= 0; --bit) {
+                const uint32_t c = upper | 1u << bit;
+                int mine = 0;
+                for (int x = t; x < want * 32; x += NT)
+                    mine += __builtin_popcountll(__ballot((uint32_t)(cand[x] >> 32) >= c));
+                if ((t & 63) == 0 && mine) atomicAdd(&reach[bit], mine);
+                __syncthreads();
+                if (reach[bit] >= n) upper = c;
             }
-        __syncthreads();
+            least = max(least, (uint64_t)upper << 32);
+            list();
+        }
         const int found = count;
-        const bool listed = found <= kListed;
-        for (int y = t; y < (listed ? found : want * 32); y += NT) {
-            const int x = listed ? index[y] : y;
-            const uint64_t v = cand[x];
-            if (v < least) continue;
-            const int32_t i = chosen[x >> 5] * 32 + (x & 31);
-            int rank = 0;
-            for (int z = 0; z < (listed ? found : want * 32); ++z) {
-                const int o = listed ? index[z] : z;
-                rank += before(cand[o], chosen[o >> 5] * 32 + (o & 31), v, i);
+        const auto place = [&](uint64_t v, int32_t i, int rank) {
+            if (rank >= n) return;
+            j.top_items[r * n + rank] = i;
+            j.top_lp[r * n + rank] = (float)(value_of(v) - lse);
+        };
+        if (found <= kCandidates) {
+            for (int y = t; y < found; y += NT) {
+                const uint64_t v = listed_key[y];
+                const int32_t i = index[y];
+                int rank = 0;
+#pragma unroll 4
+                for (int z = 0; z < found; ++z) rank += before(listed_key[z], index[z], v, i);
+                place(v, i, rank);
             }
-            if (rank < n) {
-                j.top_items[r * n + rank] = i;
-                j.top_lp[r * n + rank] = (float)(value_of(v) - lse);
+        } else {
+            for (int y = t; y < want * 32; y += NT) {
+                const uint64_t v = cand[y];
+                if (v < least) continue;
+                const int32_t i = (int32_t)item_at(y);
+                int rank = 0;
+                for (int z = 0; z < want * 32; ++z) rank += before(cand[z], (int32_t)item_at(z), v, i);
+                place(v, i, rank);
             }
         }
         for (int x = found + t; x < n; x += NT) {
@@ -1408,6 +1474,17 @@ softmax_grad_users_kernel(Job j) {
         if (j.mask) word = j.mask[row * j.v.tiles + tl];
     };
     if (t0 < t1) load(t0, 0);
+    if (!mine) {  // copies its share
+        for (int tl = t0, at = 0; tl < t1; ++tl, at ^= NB - 1) {
+            stage_wait();
+            if (NB == 1) {
+                load_trans(tl, 0);
+                stage_wait();
+            }
+            if (tl + 1 < t1) load(tl + 1, NB == 1 ? 0 : at ^ 1);
+        }
+        return;
+    }
     for (int tl = t0, at = 0; tl < t1; ++tl, at ^= NB - 1) {
         stage_wait();
         asm volatile("" : "+v"(word));  // the wait for this load belongs before the next copies
@@ -1436,7 +1513,6 @@ softmax_grad_users_kernel(Job j) {
         scale_g<T, MT>(g, acc, sh);
         grad_tile<T, KT>(tbuf[at], g, acc, lane);
     }
-    if (!mine) return;
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt)
 #pragma unroll

@@ -554,3 +554,32 @@ def test_gradient_with_a_few_items_more_than_fit(dtype, k):
     r = forward(c)
     g_lp, g_ent = torch.full((rows,), -1.0 / rows), torch.full((rows,), 0.1 / rows)
     check_backward(d, backward(c, r, g_lp, g_ent), reference(d, 0, g_lp, g_ent))
+
+
+@pytest.mark.parametrize("rows,n_items", [(3, 1682), (600, 1682), (520, 4100), (2, 4100), (530, 900)])
+def test_many_top_items_of_few(rows, n_items):
+    """128 top items of a catalogue with few tiles of 32; the last rows tie in all of it."""
+    d = make(rows, n_items, 12, F32, seed=13, seen=40)
+    d["b"][:] = torch.randn(n_items)
+    d["U"][-1] = 0
+    check_forward(d, forward(to_gpu(d), 128), 128)
+    d["b"] = None
+    r = forward(to_gpu(d), 128)
+    check_forward(d, r, 128)
+    ids, off = d["ex"][1].numpy(), d["ex"][0].numpy()
+    rest = np.setdiff1d(np.arange(n_items), ids[off[rows - 1]:off[rows]])
+    np.testing.assert_array_equal(r.top_items[-1].cpu().numpy(), rest[:128])
+
+
+def test_odd_factors_and_idle_waves():
+    """k not a multiple of 4 over one long array (the scale is found one value at a time) and one tile
+    of users more than a block keeps."""
+    d = make(257, 20_011, 19, F32, seed=14, seen=10)
+    d["V"][20_010, 18] = 300.0
+    d["b"][20_010] = -600.0
+    c = to_gpu(d)
+    r = forward(c, 4)
+    g_lp, g_ent = torch.full((257,), -1.0 / 257), torch.full((257,), 0.1 / 257)
+    ref = reference(d, 4, g_lp, g_ent)
+    check_forward(d, r, 4, ref)
+    check_backward(d, backward(c, r, g_lp, g_ent), ref)
