@@ -1047,6 +1047,15 @@ __global__ __launch_bounds__(kDirectWaves * 64) void softmax_direct_kernel(Job j
     }
 }
 
+// x of the lane whose number differs in one of the lowest two bits
+template <int D>
+__device__ __forceinline__ double neighbour(double x) {
+    constexpr int ctrl = D == 1 ? 0xB1 : 0x4E;  // quad_perm 1 0 3 2, 2 3 0 1
+    const uint64_t b = (uint64_t)__double_as_longlong(x);
+    const uint32_t lo = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)b, ctrl, 0xF, 0xF, true);
+    const uint32_t hi = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)(b >> 32), ctrl, 0xF, 0xF, true);
+    return __longlong_as_double((long long)((uint64_t)hi << 32 | lo));
+}
 // s_rj in 64 bits for the given and the top items: exact products, f64 sums.  LANES neighbouring
 // lanes share an item (every lane gets the sum); u: the user's row in LDS.
 template <int T, int LANES>
@@ -1065,8 +1074,10 @@ __device__ __forceinline__ double exact_score(const Job& j, const double* u, int
         for (int f = lane; f < j.k; f += LANES)
             a = fma(u[f], (double)load_factor<T>(j.v.src, at + f), a);
     }
+    if (LANES > 1) a += neighbour<1>(a);
+    if (LANES > 2) a += neighbour<2>(a);
 #pragma unroll
-    for (int d = 1; d < LANES; d <<= 1) a += __shfl_xor(a, d);
+    for (int d = 4; d < LANES; d <<= 1) a += __shfl_xor(a, d);
     return a + (j.bias ? (double)j.bias[i] : 0.0);
 }
 __device__ __forceinline__ bool is_excluded(const Job& j, int64_t r, int64_t i) {
@@ -1304,27 +1315,31 @@ __global__ __launch_bounds__(NT) void softmax_finish_kernel(Job j) {
         select_tiles<NT>(maxima, want, least_tile, chosen, key, index, found_tiles);
         const uint64_t none = key_of(-INFINITY);
         const auto item_at = [&](int x) { return (int64_t)chosen[x >> 5] * 32 + (x & 31); };
-        const auto keep = [&](int x, int64_t i, double score) {
-            const uint64_t k = i < j.n_items && !is_excluded(j, r, i) ? key_of(score) : none;
-            if ((t & 3) == 0) cand[x] = k;
-            // the 16 items of a wave's turn are half a tile
-            uint64_t most = k;
+        // four items a turn, whose loads are on the way together
+        constexpr int kTurn = 4;
+        for (int x0 = t >> 2; x0 < want * 32; x0 += kTurn * NT / 4) {
+            bool in[kTurn];
+            double score[kTurn];
 #pragma unroll
-            for (int d = 4; d < 64; d <<= 1)
-                most = max(most, (uint64_t)__shfl_xor((unsigned long long)most, d));
-            if ((t & 63) == 0) atomicMax(&tmax[x >> 5], (unsigned long long)most);
-        };
-        // two items a turn, whose loads are on the way together (want * 32 and NT / 4 are multiples of
-        // 32: a wave's lanes stay together)
-        for (int x = t >> 2; x < want * 32; x += NT / 2) {
-            const int y = x + NT / 4;
-            const bool two = y < want * 32;
-            const int64_t i = item_at(x), o = item_at(two ? y : x);
-            const int64_t last = j.n_items - 1;
-            const double a = exact_score<T, 4>(j, urow, min(i, last), t & 3);
-            const double b = exact_score<T, 4>(j, urow, min(o, last), t & 3);
-            keep(x, i, a);
-            if (two) keep(y, o, b);
+            for (int e = 0; e < kTurn; ++e) {
+                const int x = min(x0 + e * (NT / 4), want * 32 - 1);
+                const int64_t i = min(item_at(x), (int64_t)j.n_items - 1);
+                in[e] = item_at(x) < j.n_items && !is_excluded(j, r, i);
+                score[e] = exact_score<T, 4>(j, urow, i, t & 3);
+            }
+            if ((t & 3) == 0)
+#pragma unroll
+                for (int e = 0; e < kTurn; ++e) {
+                    const int x = x0 + e * (NT / 4);
+                    if (x < want * 32) cand[x] = in[e] ? key_of(score[e]) : none;
+                }
+        }
+        __syncthreads();
+        for (int x = t; x < want * 4; x += NT) {  // 8 items each
+            uint64_t most = 0;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) most = max(most, cand[8 * x + ((e + x) & 7)]);
+            atomicMax(&tmax[x >> 2], (unsigned long long)most);
         }
         __syncthreads();
         if (t < want) {  // the n-th largest of the tiles' maxima (none where there are fewer tiles)
