@@ -399,7 +399,8 @@ __device__ __forceinline__ void make_meta(const Job& j, int64_t r, int bad) {
 // Fragments of both sides, one block per tile of 32 rows (the users' tiles first).  A row with a
 // value that is not finite is written as zeros and marked, so that 0 * NaN cannot reach the other
 // rows' sums: an item that is not excluded gets the bias NaN, a user the mark in ubad.  So is an item
-// that its bias excludes, whose factors the scale does not count.
+// that its bias excludes, whose factors the scale does not count.  Bound by memory: 1 M items, k = 128
+// bf16 in 98 us (512 MB, 5.2 TB/s), 500 k with k = 256 and the transposed fragments in 152 us (768 MB).
 template <int T, int KT>
 __global__ __launch_bounds__(256) void softmax_prep_kernel(Job j) {
     using P = Planes<T>;
@@ -713,6 +714,9 @@ constexpr int kTileGroup = 8;  // the streamed items are padded to a multiple of
 // turn in two buffers: the next turn's tiles are on the way while this one's are used.  Lane l: user
 // l % 32, 16 of a tile's 32 items.  m, l, w: the running maximum (of scaled scores), the sum of
 // e = exp(s - m) and of e y, y = log2 e.
+// Bound by instructions and power, not memory: 2,048 x 1 M, k = 128 bf16 takes 740 us, where the SIMDs
+// issue 464 cycles of vector instructions a tile (16 exponentials of 8 cycles, 84 others of 4), 64 % of
+// the time, beside 256 of matrix instructions, at 1.95 GHz of 2.4: on zeros the same launch takes 500 us.
 template <int T, int KT, bool TOP>
 __global__ __launch_bounds__((forward_waves<T, KT>() * 64), (forward_per_simd<T, KT>())) void
 softmax_forward_kernel(Job j) {
@@ -844,7 +848,8 @@ softmax_forward_kernel(Job j) {
 // of users there is nothing to share and nothing to prepare.  A wave makes its fragments from the
 // factors themselves, both sides', and the catalogue is read once (per tile of users).  f32: every tile of items has a scale of its own, 2^ev, and
 // the scores are brought back before the bias is added (one instruction more per score, which the
-// memory's pace hides: 25.6 MB of factors take about 5 us at the rate of a large copy).  m, l, w as in
+// memory's pace hides: 25.6 MB of factors, one user, take 12 us, of which 5 are a large copy's rate and
+// the rest the latency of a few loads one behind the other).  m, l, w as in
 // the forward pass, in true units; the block's waves are joined before they are written.
 constexpr int kDirectWaves = 4;
 
@@ -1216,12 +1221,14 @@ __device__ __forceinline__ void select_tiles(const Maxima<NT>& maxima, int want,
 }
 
 // One block per row (64 threads; with top items 256, or 1,024 where the rows are too few to fill the
-// GPU): the splits' states joined, the
-// outputs, and the top items.  The n best items lie in the n tiles with the largest maxima (lower
-// tile first among equals); two more tiles cover the rounding of the maxima.  Their items are
-// scored again in 64 bits, so the order is that of the exact scores.  The n-th largest of the tiles'
-// exact maxima bounds the n-th best score from below: the items at or above it are ranked by
-// counting.  Dynamic LDS: the candidates' keys, 8 bytes each.
+// GPU): the splits' states joined, the outputs, and the top items.  The n best items lie in the n
+// tiles with the largest maxima (lower tile first among equals); two more tiles cover the rounding of
+// the maxima.  Their items are scored again in 64 bits, so the order is that of the exact scores.  The
+// n-th largest of the tiles' exact maxima bounds the n-th best score from below: the items at or above
+// it are ranked by counting.  Dynamic LDS: the candidates' keys, 8 bytes each.
+// Bound by memory: the maxima (2,048 rows of 1 M items: 256 MB, read twice, 104 of 143 us with the top
+// 20) and the candidates' factors, 8 KB a tile at k = 64 (4,096 rows of 100 k items: 403 MB with the top
+// 10, 42 of 84 us, out of the Infinity Cache at 9 TB/s).  Without top items 5 us.
 template <int T, int NT>
 __global__ __launch_bounds__(NT) void softmax_finish_kernel(Job j) {
     constexpr bool TOP = NT > 64;
@@ -1425,6 +1432,9 @@ __global__ __launch_bounds__(NT) void softmax_finish_kernel(Job j) {
 // f16; 1024 x 500k, k = 256 bf16): users 156 us with 8 and 4 against 199 with 8 and 2; items 206 with
 // 4 and 3 against 236 with 8 and 4, which spills (a reload waits for the copies on the way); k > 128:
 // users 729 with 4 and 2 against 1,221 with 4 and 1.
+// Bound by the matrix cores and power: 1024 x 500k, k = 256 bf16 takes 3 products a side (the scores
+// again, G's two planes), 786 Gflop, in 664 us (users) and 750 (items): 1.18 and 1.05 Pflop/s, where a
+// large library product reaches 1.23.
 template <int T, int KT>
 constexpr int users_waves() {
     return KT > 4 ? 4 : 8;
