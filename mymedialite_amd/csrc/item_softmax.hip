@@ -677,13 +677,16 @@ __device__ __forceinline__ float largest(float a, float b) { return __builtin_el
 
 __device__ __forceinline__ int reg_row(int i, int h) { return 8 * (i >> 2) + 4 * h + (i & 3); }
 
-// `gone` where the bits (shifted right by 4 h) say so.  The empty asm keeps the compiler from taking
-// the selects out of their branch: 32 instructions for every tile against 110 for the tile itself.
+// `gone` where the bits (shifted right by 4 h) say so.  The first empty asm keeps the compiler from
+// taking the selects out of their branch: 32 instructions for every tile against 110 for the tile
+// itself.  The other hides that `on` is 0 or -1: a bit field and a bitwise select, 2 instructions a
+// score, instead of a comparison and a conditional move with the waits between them.
 __device__ __forceinline__ void mask_tile(f32x16& c, uint32_t bits, float gone) {
     asm volatile("");
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
-        const uint32_t on = (uint32_t)((int32_t)(bits << (31 - reg_row(i, 0))) >> 31);
+        uint32_t on = (uint32_t)__builtin_amdgcn_sbfe((int)bits, reg_row(i, 0), 1);
+        asm("" : "+v"(on));
         c[i] = __uint_as_float((on & __float_as_uint(gone)) | (~on & __float_as_uint(c[i])));
     }
 }
@@ -1673,17 +1676,18 @@ softmax_grad_items_kernel(Job j) {
     if (h == 0) j.db_part[split * parted + item - first] = db;
 }
 
-// Four factors of a row summed over the splits: kJoin neighbouring threads take every kJoin-th split
-// and are joined in order, so the result is the same every time.
-constexpr int kJoin = 8;
+// Four factors of a row summed over the splits: `threads` neighbouring threads take every threads-th
+// split and are joined in order, so the result is the same every time.
+__host__ __device__ __forceinline__ int join_threads(int splits) {  // 1, 2, 4 or 8
+    return splits >= 8 ? 8 : splits >= 4 ? 4 : splits >= 2 ? 2 : 1;
+}
 __device__ __forceinline__ f32x4 join_splits(const float* __restrict__ part, int64_t stride,
-                                             int splits) {
-    const int g = threadIdx.x % kJoin;
+                                             int splits, int threads) {
+    const int g = threadIdx.x & (threads - 1);
     f32x4 a = {};
 #pragma unroll 4
-    for (int s = g; s < splits; s += kJoin) a += *(const f32x4*)(part + s * stride);
-#pragma unroll
-    for (int d = 1; d < kJoin; d <<= 1)
+    for (int s = g; s < splits; s += threads) a += *(const f32x4*)(part + s * stride);
+    for (int d = 1; d < threads; d <<= 1)
 #pragma unroll
         for (int e = 0; e < 4; ++e) a[e] += __shfl_xor(a[e], d);
     return a;
@@ -1691,13 +1695,14 @@ __device__ __forceinline__ f32x4 join_splits(const float* __restrict__ part, int
 // The users' rows with w V_t added
 template <int T>
 __device__ __forceinline__ void join_users(const Job& j, int32_t kp, uint32_t block) {
-    const int64_t x = ((int64_t)block * 256 + threadIdx.x) / kJoin;
+    const int threads = join_threads(j.splits);
+    const int64_t x = ((int64_t)block * 256 + threadIdx.x) / threads;
     const int quads = (j.k + 3) / 4;
     const bool in = x < j.n_rows * quads;  // (all lanes take part in the join)
     const int64_t r = in ? x / quads : 0;
     const int f = in ? 4 * (int)(x % quads) : 0;
-    f32x4 a = join_splits(j.du_part + r * kp + f, j.rows_pad * kp, j.splits);
-    if (!in || threadIdx.x % kJoin) return;
+    f32x4 a = join_splits(j.du_part + r * kp + f, j.rows_pad * kp, j.splits, threads);
+    if (!in || (threadIdx.x & (threads - 1))) return;
     const int32_t t = j.meta[r >> 5].t[r & 31];
     if (t >= 0)
 #pragma unroll
@@ -1708,14 +1713,15 @@ __device__ __forceinline__ void join_users(const Job& j, int32_t kp, uint32_t bl
 }
 template <int T>
 __device__ __forceinline__ void join_items(const Job& j, int32_t kp, uint32_t block) {
-    const int64_t x = ((int64_t)block * 256 + threadIdx.x) / kJoin;
+    const int threads = join_threads(j.vsplits);
+    const int64_t x = ((int64_t)block * 256 + threadIdx.x) / threads;
     const int64_t first = (int64_t)j.vwhole * 32, parted = (int64_t)j.v.tiles * 32 - first;
     const int quads = (j.k + 3) / 4;
     const bool in = x < (j.n_items - first) * quads;
     const int64_t i = in ? x / quads : 0;  // (from the first item in parts on)
     const int f = in ? 4 * (int)(x % quads) : 0;
-    const f32x4 a = join_splits(j.dv_part + i * kp + f, parted * kp, j.vsplits);
-    if (!in || threadIdx.x % kJoin) return;
+    const f32x4 a = join_splits(j.dv_part + i * kp + f, parted * kp, j.vsplits, threads);
+    if (!in || (threadIdx.x & (threads - 1))) return;
     store_factors<T>(j.gv, (first + i) * j.ld_gv, f, j.k, j.gv_vec4, a);
     if (f == 0) {
         float b = 0.0f;
@@ -2027,10 +2033,10 @@ void item_log_probs_grad(const mml_item_softmax_args* a, const float* log_norm,
     const int kt0 = steps_of(j.k), kp = std::max(32, kt0 * 16);
     if (a->n_rows > 0) prepare(j, a->dtype, st);
     const int64_t quads = (j.k + 3) / 4;
-    const uint32_t ju = grid_of((j.n_rows * quads * kJoin + 255) / 256);
+    const uint32_t ju = grid_of((j.n_rows * quads * join_threads(j.splits) + 255) / 256);
     const uint32_t ji =
         j.vsplits > 1
-            ? grid_of(((j.n_items - (int64_t)j.vwhole * 32) * quads * kJoin + 255) / 256)
+            ? grid_of(((j.n_items - (int64_t)j.vwhole * 32) * quads * join_threads(j.vsplits) + 255) / 256)
             : 0;
     dispatch(a->dtype, kt0, [&](auto tt, auto kt) {
         constexpr int T = decltype(tt)::value, KT = decltype(kt)::value, UW = users_waves<T, KT>();
