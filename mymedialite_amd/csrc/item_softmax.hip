@@ -1767,8 +1767,10 @@ void dispatch(int T, int kt, F&& f) {
 // side; matrix instructions per pair of tiles; bytes a split leaves per kept tile.  In cycles: a wave's
 // tile takes 32 per matrix instruction and 500 besides; w waves on a SIMD take (w + 1.5) / 2.5 times as
 // long as one (measured: 1.6 times the throughput from one to two, 1.2 from two to four); a block 6,000
-// to start; results are written and read back at 2 KB a cycle.  Above 8, a multiple of the 8 XCDs:
-// block b runs on XCD b mod 8, so a split's blocks share an L2.
+// to start; results are written and read back at 8 KB a cycle (in the model's cycles, half the real ones
+// a tile: with 2 KB, 1,001 x 30 k, k = 100 f16 took 118 us with 32 and 1 splits, with 8 KB 105 with 64
+// and 2).  Above 8, a multiple of the 8 XCDs: block b runs on XCD b mod 8, so a split's blocks share an
+// L2.
 struct Splits {
     int32_t n = 1, whole = 0;  // kept tiles from `whole` on are split n ways, those before are not
     double cost = 0.0;
@@ -1787,7 +1789,7 @@ Splits choose_splits(int64_t kept, int64_t streamed, int waves, int per_simd, in
         const double one = block_time(per_cu, waves, instructions, (streamed + s - 1) / s);
         const double fill = (double)blocks / (256.0 * per_cu);
         const double cost = (fill <= 1.0 ? 1.0 : fill + 0.35) * one +
-                            (s > 1 ? s * kept * bytes / 1024.0 : 0.0);
+                            (s > 1 ? s * kept * bytes / 4096.0 : 0.0);
         if (s == 1 || cost < best.cost) best.cost = cost, best.n = (int32_t)s;
     }
     return best;
