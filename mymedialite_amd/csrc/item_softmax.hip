@@ -1444,7 +1444,7 @@ constexpr int users_waves() {
 }
 template <int T, int KT>
 constexpr int users_per_simd() {
-    return KT <= 4 ? 4 : KT <= 8 || T != MML_DTYPE_F32 ? 2 : 1;
+    return KT <= 4 ? 4 : KT == 6 ? (T == MML_DTYPE_F32 ? 3 : 4) : KT <= 8 || T != MML_DTYPE_F32 ? 2 : 1;
 }
 template <int KT>
 constexpr int tile_buffers() {
@@ -1458,7 +1458,7 @@ constexpr int users_in_lds() {
 constexpr int kItemsWaves = 4;
 template <int T, int KT>
 constexpr int items_per_simd() {
-    return KT <= 4 || (KT == 8 && T != MML_DTYPE_F32) ? 3 : KT == 8 || T != MML_DTYPE_F32 ? 2 : 1;
+    return KT <= 4 || (KT <= 8 && T != MML_DTYPE_F32) ? 3 : KT <= 8 || T != MML_DTYPE_F32 ? 2 : 1;
 }
 template <int T, int KT>
 constexpr int items_in_lds() {
@@ -1737,10 +1737,10 @@ __global__ __launch_bounds__(256) void softmax_join_kernel(Job j, int32_t kp, ui
 }
 
 // ------------------------------------------------------------------ host side
-int steps_of(int32_t k) {  // KT: the factors padded to 16, 32, 64, 128 or 256
-    int kt = 1;
-    while (kt * 16 < k) kt *= 2;
-    return kt;
+int steps_of(int32_t k) {  // KT: the factors padded to 16, 32, 64, 96, 128, 192 or 256
+    for (const int kt : {1, 2, 4, 6, 8, 12})
+        if (k <= 16 * kt) return kt;
+    return 16;
 }
 
 template <class F>
@@ -1750,7 +1750,9 @@ void dispatch(int T, int kt, F&& f) {
         case 1: return f(std::integral_constant<int, TT>{}, std::integral_constant<int, 1>{});   \
         case 2: return f(std::integral_constant<int, TT>{}, std::integral_constant<int, 2>{});   \
         case 4: return f(std::integral_constant<int, TT>{}, std::integral_constant<int, 4>{});   \
+        case 6: return f(std::integral_constant<int, TT>{}, std::integral_constant<int, 6>{});   \
         case 8: return f(std::integral_constant<int, TT>{}, std::integral_constant<int, 8>{});   \
+        case 12: return f(std::integral_constant<int, TT>{}, std::integral_constant<int, 12>{}); \
         default: return f(std::integral_constant<int, TT>{}, std::integral_constant<int, 16>{}); \
     }
     switch (T) {

@@ -583,3 +583,18 @@ def test_odd_factors_and_idle_waves():
     ref = reference(d, 4, g_lp, g_ent)
     check_forward(d, r, 4, ref)
     check_backward(d, backward(c, r, g_lp, g_ent), ref)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16], ids=["f32", "bf16", "f16"])
+@pytest.mark.parametrize("shape", [(40, 700, 65, 41), (300, 9000, 96, 300), (5, 333, 90, 9),
+                                   (70, 1100, 129, 70), (290, 6000, 192, 300), (3, 500, 170, 3)],
+                         ids=lambda s: "x".join(map(str, s)))
+def test_factors_between_powers_of_two(shape, dtype):
+    R, n, k, nu = shape
+    d = make(R, n, k, dtype, seed=R + k, n_users=nu, seen=9)
+    g_lp, g_ent = torch.full((R,), -1.0 / R), torch.full((R,), 0.1 / R)
+    c = to_gpu(d)
+    r = forward(c, 5)
+    ref = reference(d, 5, g_lp, g_ent)
+    check_forward(d, r, 5, ref)
+    check_backward(d, backward(c, r, g_lp, g_ent), ref)
