@@ -296,8 +296,28 @@ __device__ __forceinline__ void largest_factors(const Job& j, int block) {
             for (int e = 0; e < N; ++e) take(counts ? v[e] : 0.0f);
         }
     };
-    if (s.vec8 && j.k % 4 == 0) scan(std::integral_constant<int, 4>{});
-    else scan(std::integral_constant<int, 1>{});
+    if (s.vec8 && j.k % 4 == 0) {
+        scan(std::integral_constant<int, 4>{});
+    } else if (!s.index && s.ld == j.k && j.k >= 4 && (uintptr_t)s.src % 16 == 0) {
+        // one array: 4 values belong to two rows at most (100 k x 150: 89 us one by one, 28 so)
+        const float* src = (const float*)s.src;
+        const uint32_t k = (uint32_t)j.k;
+        const int64_t all = s.n * k, turn = (int64_t)parts * 1024;
+        const auto counts = [&](int64_t r) { return !(bias && bias[r] <= kGone); };
+#pragma unroll 4
+        for (int64_t x = ((int64_t)part * 256 + threadIdx.x) * 4; x + 4 <= all; x += turn) {
+            const int64_t r = all >> 31 ? x / k : (int64_t)((uint32_t)x / k), end = (r + 1) * k;
+            const f32x4 v = *(const f32x4*)(src + x);
+            const bool c0 = counts(r), c1 = counts(min(r + 1, s.n - 1));
+#pragma unroll
+            for (int e = 0; e < 4; ++e) take((x + e < end ? c0 : c1) ? v[e] : 0.0f);
+        }
+        const int rest = (int)(all % 4);  // of the last row
+        if (part == 0 && (int)threadIdx.x < rest)
+            take(counts(s.n - 1) ? src[all - rest + threadIdx.x] : 0.0f);
+    } else {
+        scan(std::integral_constant<int, 1>{});
+    }
 #pragma unroll
     for (int d = 32; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor(m, d));
     if (lane == 0) red[threadIdx.x >> 6] = m;

@@ -598,3 +598,28 @@ def test_factors_between_powers_of_two(shape, dtype):
     ref = reference(d, 5, g_lp, g_ent)
     check_forward(d, r, 5, ref)
     check_backward(d, backward(c, r, g_lp, g_ent), ref)
+
+
+@pytest.mark.parametrize("k", [1, 2, 3, 5, 7, 90, 97])
+@pytest.mark.parametrize("where", ["first", "last", "excluded"])
+def test_largest_factor_anywhere(k, where):
+    """The scale counts the first and the last value of one long array, and no excluded item's."""
+    rows, n_items = 300, 20_003
+    d = make(rows, n_items, k, F32, seed=15)
+    d["U"] *= 1e-3
+    big = {"first": (0, 0), "last": (n_items - 1, k - 1), "excluded": (777, 0)}[where]
+    d["V"][big] = 2.0 ** 20
+    clean = d
+    if where == "excluded":  # counted, it would leave the others 2^-37 2^100
+        d["b"][777] = -np.inf
+        clean = dict(d, V=d["V"].clone())
+        clean["V"][777] = 0
+        d["V"][big] = 2.0 ** 100
+    else:
+        d["U"][:, big[1]] *= 1e-4
+    c = to_gpu(d)
+    r = forward(c, 3)
+    g_lp, g_ent = torch.full((rows,), -1.0 / rows), torch.full((rows,), 0.1 / rows)
+    ref = reference(clean, 3, g_lp, g_ent)
+    check_forward(clean, r, 3, ref)
+    check_backward(clean, backward(c, r, g_lp, g_ent), ref)
