@@ -78,17 +78,18 @@ __device__ __forceinline__ float load_factor(const void* p, int64_t i) {
     if constexpr (T == MML_DTYPE_BF16) return __uint_as_float((uint32_t)((const uint16_t*)p)[i] << 16);
     if constexpr (T == MML_DTYPE_F16) return (float)((const _Float16*)p)[i];
 }
-// Factors at .. at + 7 (16-byte aligned)
+// Factors at .. at + 7, in loads of 16 bytes that need no more than an element's alignment
 template <int T>
 __device__ __forceinline__ void load_factors(const void* p, int64_t at, float (&v)[8]) {
+    using f32x4_any = __attribute__((ext_vector_type(4), aligned(4))) float;
+    using u32x4_any = __attribute__((ext_vector_type(4), aligned(2))) uint32_t;
     if constexpr (T == MML_DTYPE_F32) {
-        const f32x4 lo = *(const f32x4*)((const float*)p + at);
-        const f32x4 hi = *(const f32x4*)((const float*)p + at + 4);
+        const f32x4 lo = *(const f32x4_any*)((const float*)p + at);
+        const f32x4 hi = *(const f32x4_any*)((const float*)p + at + 4);
 #pragma unroll
         for (int e = 0; e < 4; ++e) v[e] = lo[e], v[4 + e] = hi[e];
     } else {
-        const uint4 q = *(const uint4*)((const uint16_t*)p + at);
-        const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+        const u32x4 w = *(const u32x4_any*)((const uint16_t*)p + at);
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
             const uint16_t b = (uint16_t)(w[e >> 1] >> (16 * (e & 1)));
@@ -445,7 +446,7 @@ __global__ __launch_bounds__(256) void softmax_prep_kernel(Job j) {
         float v[8] = {};
         if (src >= 0) {
             const int64_t at = src * s.ld + f;
-            if (s.vec8 && f + 8 <= j.k) {
+            if (f + 8 <= j.k) {
                 load_factors<T>(s.src, at, v);
             } else {
 #pragma unroll
@@ -881,7 +882,7 @@ constexpr int kDirectWaves = 4;
 template <int T, int KT>
 __device__ __forceinline__ void load_rows(const Side& s, int64_t src, int k, int h,
                                           float (&v)[KT][8]) {
-    if (s.vec8 && k % 8 == 0) {
+    if (k % 8 == 0) {
         // whole groups: every lane loads (a lane without a group row 0's), so that all loads are on
         // the way together
 #pragma unroll
@@ -897,12 +898,17 @@ __device__ __forceinline__ void load_rows(const Side& s, int64_t src, int k, int
         }
     } else {
 #pragma unroll
-        for (int ks = 0; ks < KT; ++ks)
+        for (int ks = 0; ks < KT; ++ks) {
+            const int f0 = 16 * ks + 8 * h;
+            if (KT > 1 && src >= 0 && f0 + 8 <= k) {
+                load_factors<T>(s.src, src * s.ld + f0, v[ks]);
+            } else {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const int f = 16 * ks + 8 * h + e;
-                v[ks][e] = src >= 0 && f < k ? load_factor<T>(s.src, src * s.ld + f) : 0.0f;
+                for (int e = 0; e < 8; ++e)
+                    v[ks][e] = src >= 0 && f0 + e < k ? load_factor<T>(s.src, src * s.ld + f0 + e)
+                                                      : 0.0f;
             }
+        }
     }
 }
 // (What a row holds reaches its own scores only, so values that are not finite need no zeros here.)
@@ -1090,18 +1096,15 @@ template <int T, int LANES>
 __device__ __forceinline__ double exact_score(const Job& j, const double* u, int64_t i, int lane) {
     double a = 0.0;
     const int64_t at = i * j.v.ld;
-    if (j.v.vec8 && j.k % 8 == 0) {  // whole groups of 8 factors in loads of 16 bytes
 #pragma unroll 2
-        for (int f = 8 * lane; f < j.k; f += 8 * LANES) {
-            float x[8];
-            load_factors<T>(j.v.src, at + f, x);
+    for (int f = 8 * lane; f + 8 <= j.k; f += 8 * LANES) {
+        float x[8];
+        load_factors<T>(j.v.src, at + f, x);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) a = fma(u[f + e], (double)x[e], a);
-        }
-    } else {
-        for (int f = lane; f < j.k; f += LANES)
-            a = fma(u[f], (double)load_factor<T>(j.v.src, at + f), a);
+        for (int e = 0; e < 8; ++e) a = fma(u[f + e], (double)x[e], a);
     }
+    for (int f = (j.k & ~7) + lane; f < j.k; f += LANES)
+        a = fma(u[f], (double)load_factor<T>(j.v.src, at + f), a);
     if (LANES > 1) a += neighbour<1>(a);
     if (LANES > 2) a += neighbour<2>(a);
 #pragma unroll
