@@ -1152,7 +1152,7 @@ __device__ __forceinline__ uint32_t bound_of(const uint32_t* key, int want) {
 }
 // A row's maxima as a block of NT threads reads them, four at a time (the tiles are a multiple of 8):
 // the first groups of a thread stay in registers for the second pass: 256 threads hold 4,096 maxima
-// (131 k items; 4,096 rows of 100 k items, top 10: 84 us against 92 with two reads).  Holding all of
+// (131 k items; 4,096 rows of 100 k items, top 10: 8 us less than with two reads).  Holding all of
 // 1 M items' in 512 threads gained nothing: the registers leave too few blocks to score with.
 template <int NT>
 struct Maxima {
@@ -1252,11 +1252,13 @@ __device__ __forceinline__ void select_tiles(const Maxima<NT>& maxima, int want,
 // the maxima.  Their items are scored again in 64 bits, so the order is that of the exact scores.  The
 // n-th largest of the tiles' exact maxima bounds the n-th best score from below: the items at or above
 // it are ranked by counting.  Dynamic LDS: the candidates' keys, 8 bytes each.
-// Bound by memory: the maxima (2,048 rows of 1 M items: 256 MB, read twice, 104 of 143 us with the top
+// Bound by memory: the maxima (2,048 rows of 1 M items: 256 MB, read twice, 86 of 124 us with the top
 // 20) and the candidates' factors, 8 KB a tile at k = 64 (4,096 rows of 100 k items: 403 MB with the top
-// 10, 42 of 84 us, out of the Infinity Cache at 9 TB/s).  Without top items 5 us.
+// 10, 54 us).  Waves hide its latencies better than loads in flight: 8 a SIMD and one item a turn take
+// those 54 us, 6 and two items 60, 4 and four items 82 (from the top 50 on, where LDS leaves 4 to 6
+// blocks a CU, it is the other way round by a tenth).  Without top items 5 us.
 template <int T, int NT>
-__global__ __launch_bounds__(NT) void softmax_finish_kernel(Job j) {
+__global__ __launch_bounds__(NT, 8) void softmax_finish_kernel(Job j) {
     constexpr bool TOP = NT > 64;
     __shared__ double urow[256], joined[2];
     // the tiles' keys, later the candidates' (the listed ones' order is that of a counter: any)
@@ -1348,24 +1350,11 @@ __global__ __launch_bounds__(NT) void softmax_finish_kernel(Job j) {
         select_tiles<NT>(maxima, want, least_tile, chosen, key, index, found_tiles);
         const uint64_t none = key_of(-INFINITY);
         const auto item_at = [&](int x) { return (int64_t)chosen[x >> 5] * 32 + (x & 31); };
-        // four items a turn, whose loads are on the way together
-        constexpr int kTurn = 4;
-        for (int x0 = t >> 2; x0 < want * 32; x0 += kTurn * NT / 4) {
-            bool in[kTurn];
-            double score[kTurn];
-#pragma unroll
-            for (int e = 0; e < kTurn; ++e) {
-                const int x = min(x0 + e * (NT / 4), want * 32 - 1);
-                const int64_t i = min(item_at(x), (int64_t)j.n_items - 1);
-                in[e] = item_at(x) < j.n_items && !is_excluded(j, r, i);
-                score[e] = exact_score<T, 4>(j, urow, i, t & 3);
-            }
-            if ((t & 3) == 0)
-#pragma unroll
-                for (int e = 0; e < kTurn; ++e) {
-                    const int x = x0 + e * (NT / 4);
-                    if (x < want * 32) cand[x] = in[e] ? key_of(score[e]) : none;
-                }
+        for (int x = t >> 2; x < want * 32; x += NT / 4) {
+            const int64_t i = min(item_at(x), (int64_t)j.n_items - 1);
+            const bool in = item_at(x) < j.n_items && !is_excluded(j, r, i);
+            const double score = exact_score<T, 4>(j, urow, i, t & 3);
+            if ((t & 3) == 0) cand[x] = in ? key_of(score) : none;
         }
         __syncthreads();
         for (int x = t; x < want * 4; x += NT) {  // 8 items each
