@@ -235,9 +235,9 @@ __device__ __forceinline__ uint32_t take_plane(float& v) {
 // The exclusion lists as bits: a block makes up to kMaskWords words of a row in LDS and writes them.  The
 // lists may be unsorted and may repeat an item (an OR of bits does not depend on the order); ids
 // outside the catalogue and offsets outside the array are skipped.
-constexpr int kMaskWords = 16384;
+constexpr int kMaskWords = 16128;  // with the kernel's other 16 bytes under 64 KB
 __device__ __forceinline__ void make_mask(const Job& j, uint32_t block) {
-    extern __shared__ uint32_t words[];
+    extern __shared__ __align__(16) uint32_t words[];
     const int parts = (j.v.tiles + kMaskWords - 1) / kMaskWords;
     const int64_t r = block / parts;
     const int w0 = (int)(block % parts) * kMaskWords, n = min(kMaskWords, j.v.tiles - w0);
@@ -738,7 +738,7 @@ constexpr int kTileGroup = 8;  // the streamed items are padded to a multiple of
 // turn in two buffers: the next turn's tiles are on the way while this one's are used.  Lane l: user
 // l % 32, 16 of a tile's 32 items.  m, l, w: the running maximum (of scaled scores), the sum of
 // e = exp(s - m) and of e y, y = log2 e.
-// Bound by instructions and power, not memory: 2,048 x 1 M, k = 128 bf16 takes 740 us, where the SIMDs
+// Bound by instructions and power, not memory: 2,048 x 1 M, k = 128 bf16 takes 722 us, where the SIMDs
 // issue 464 cycles of vector instructions a tile (16 exponentials of 8 cycles, 84 others of 4), 64 % of
 // the time, beside 256 of matrix instructions, at 1.95 GHz of 2.4: on zeros the same launch takes 500 us.
 template <int T, int KT, bool TOP>
@@ -1448,7 +1448,7 @@ __global__ __launch_bounds__(NT, 8) void softmax_finish_kernel(Job j) {
 // 4 and 3 against 236 with 8 and 4, which spills (a reload waits for the copies on the way); k > 128:
 // users 729 with 4 and 2 against 1,221 with 4 and 1.
 // Bound by the matrix cores and power: 1024 x 500k, k = 256 bf16 takes 3 products a side (the scores
-// again, G's two planes), 786 Gflop, in 664 us (users) and 750 (items): 1.18 and 1.05 Pflop/s, where a
+// again, G's two planes), 786 Gflop, in 654 us (users) and 725 (items): 1.20 and 1.08 Pflop/s, where a
 // large library product reaches 1.23.
 template <int T, int KT>
 constexpr int users_waves() {

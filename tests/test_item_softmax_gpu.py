@@ -623,3 +623,17 @@ def test_largest_factor_anywhere(k, where):
     ref = reference(clean, 3, g_lp, g_ent)
     check_forward(clean, r, 3, ref)
     check_backward(clean, backward(c, r, g_lp, g_ent), ref)
+
+
+@pytest.mark.parametrize("rows", [3, 40], ids=["few", "prepared"])
+def test_exclusions_of_a_catalogue_in_parts(rows):
+    """More items than one block's exclusion bits (516,096), f32, items of every part excluded."""
+    d = make(rows, 1_050_000, 2, F32, seed=16, seen=200)
+    d["items"][1] = int(d["ex"][1][int(d["ex"][0][1])])  # one that user 1 excludes
+    c = to_gpu(d)
+    r = forward(c, 2)
+    g_lp = torch.full((rows,), -1.0 / rows)
+    ref = reference(d, 2, g_lp)
+    check_forward(d, r, 2, ref)
+    assert r.log_probs[1] == -np.inf
+    check_backward(d, backward(c, r, g_lp, None), ref)
