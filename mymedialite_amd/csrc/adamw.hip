@@ -13,7 +13,8 @@
 //
 // Memory-bound: an f32 parameter takes 28 bytes with 32-bit moments (p, m, v read and written, g
 // read), 16.06 with 8-bit ones.  71.5 M f32 values take 397 us with 32-bit moments and 232 with 8-bit
-// ones, 5.0 TB/s both (a large copy: 4.7); small models the 8 us of a launch.  One launch covers up to kMaxTensors tensors, whose addresses are
+// ones, 5.0 TB/s both (a large copy: 4.7); small models the 8 us of a launch.  One launch covers up to
+// kMaxTensors tensors, whose addresses are
 // kernel arguments (a captured graph replays with them); the step count lives on the device, so a
 // replay counts on.
 #include <hip/hip_runtime.h>

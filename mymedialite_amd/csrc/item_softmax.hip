@@ -870,7 +870,8 @@ softmax_forward_kernel(Job j) {
 
 // The forward pass for at most 32 rows, or for so little work that launches cost more: with one tile
 // of users there is nothing to share and nothing to prepare.  A wave makes its fragments from the
-// factors themselves, both sides', and the catalogue is read once (per tile of users).  f32: every tile of items has a scale of its own, 2^ev, and
+// factors themselves, both sides', and the catalogue is read once (per tile of users).  f32: every tile
+// of items has a scale of its own, 2^ev, and
 // the scores are brought back before the bias is added (one instruction more per score, which the
 // memory's pace hides: 25.6 MB of factors, one user, take 12 us, of which 5 are a large copy's rate and
 // the rest the latency of a few loads one behind the other).  m, l, w as in
@@ -1288,10 +1289,12 @@ __global__ __launch_bounds__(NT, 8) void softmax_finish_kernel(Job j) {
         const float* part = j.part + r * j.splits;
         const int64_t next = j.rows_pad * j.splits;
         float m = sc.floor;
+#pragma unroll 4
         for (int s = t; s < j.splits; s += 64) m = fmaxf(m, part[s]);
 #pragma unroll
         for (int d = 32; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor(m, d));
         double l = 0.0, w = 0.0;
+#pragma unroll 4
         for (int s = t; s < j.splits; s += 64) {
             const double d = ((double)part[s] - m) * sc.unit * 1.4426950408889634;
             const double f = __builtin_amdgcn_exp2f((float)d), ls = part[s + next];
