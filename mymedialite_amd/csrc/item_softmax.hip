@@ -699,7 +699,7 @@ __device__ __forceinline__ float largest(float a, float b) { return __builtin_el
 __device__ __forceinline__ int reg_row(int i, int h) { return 8 * (i >> 2) + 4 * h + (i & 3); }
 
 // `gone` where the bits (shifted right by 4 h) say so.  The first empty asm keeps the compiler from
-// taking the selects out of their branch: 32 instructions for every tile against 110 for the tile
+// taking the selects out of their branch: 32 instructions for every tile against 105 for the tile
 // itself.  The other hides that `on` is 0 or -1: a bit field and a bitwise select, 2 instructions a
 // score, instead of a comparison and a conditional move with the waits between them.
 __device__ __forceinline__ void mask_tile(f32x16& c, uint32_t bits, float gone) {
@@ -739,7 +739,7 @@ constexpr int kTileGroup = 8;  // the streamed items are padded to a multiple of
 // l % 32, 16 of a tile's 32 items.  m, l, w: the running maximum (of scaled scores), the sum of
 // e = exp(s - m) and of e y, y = log2 e.
 // Bound by instructions and power, not memory: 2,048 x 1 M, k = 128 bf16 takes 722 us, where the SIMDs
-// issue 464 cycles of vector instructions a tile (16 exponentials of 8 cycles, 84 others of 4), 64 % of
+// issue about 450 cycles of vector instructions a tile (16 exponentials of 8 cycles, 80 others of 4), 64 % of
 // the time, beside 256 of matrix instructions, at 1.95 GHz of 2.4: on zeros the same launch takes 500 us.
 template <int T, int KT, bool TOP>
 __global__ __launch_bounds__((forward_waves<T, KT>() * 64), (forward_per_simd<T, KT>())) void
