@@ -687,7 +687,8 @@ mml_status mml_item_log_probs_grad_device(const mml_item_softmax_args* args, con
  *          - learn_rate m / (1 - beta1^t) / (sqrt(v / (1 - beta2^t)) + epsilon),
  * in f32, a half-precision parameter rounded once to nearest.  state_bits 32: m and v are float[n].
  * 8: m and v are e4m3 codes (uint8_t[n], the OCP format without infinities), value = code x scale
- * of its MML_ADAMW_BLOCK consecutive values, scale = largest magnitude / 448 (float[ceil(n / 256)]);
+ * of its MML_ADAMW_BLOCK consecutive values, scale = largest magnitude / 448 (float[ceil(n / 256)]; 0
+ * for a block of zeros, else 2^-126 at least);
  * v's codes hold sqrt(v), and one that is not zero never gets code 0.  A gradient that is not
  * finite (8 bits: or whose square is not) makes that value's parameter and moments NaN or infinite
  * and no other's.  All zero is the start of both forms.

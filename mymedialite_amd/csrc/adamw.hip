@@ -137,6 +137,12 @@ __device__ __forceinline__ uint8_t encode(float x, float scale) {
     return scale > 0.0f ? (uint8_t)(__builtin_amdgcn_cvt_pk_fp8_f32(x / scale, 0.0f, 0, false) & 0xFF)
                         : 0;
 }
+// A block's scale from its largest magnitude.  Not below the smallest normal number: a subnormal
+// quotient is rounded by up to half of itself, and largest / scale would pass 464, from where on the
+// conversion gives the NaN code.  (A first moment without gradients decays that far in 800 steps.)
+__device__ __forceinline__ float scale_of(float largest) {
+    return largest > 0.0f ? fmaxf(largest * kPerMax, 0x1p-126f) : 0.0f;
+}
 __device__ __forceinline__ float finite_abs(float x) {
     const float a = fabsf(x);
     return a < INFINITY ? a : 0.0f;  // (NaN too)
@@ -280,7 +286,7 @@ __global__ __launch_bounds__(256, BITS == 32 ? 1 : 8) void adamw_kernel(Step s) 
                         am = wave_max(am);
                         ar = wave_max(ar);
                     }
-                    const float nm = __uint_as_float(am) * kPerMax, nr = __uint_as_float(ar) * kPerMax;
+                    const float nm = scale_of(__uint_as_float(am)), nr = scale_of(__uint_as_float(ar));
                     uint32_t cm, cv;
                     if (odd || !(nm > 0x1p-100f) || !(nr > 0x1p-100f)) {
                         const float least = kE4m3Min * nr;
@@ -351,7 +357,7 @@ __global__ __launch_bounds__(256, BITS == 32 ? 1 : 8) void adamw_kernel(Step s) 
                     am = fmaxf(am, __shfl_xor(am, d));
                     ar = fmaxf(ar, __shfl_xor(ar, d));
                 }
-                const float nm = am * kPerMax, nr = ar * kPerMax;
+                const float nm = scale_of(am), nr = scale_of(ar);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     const int64_t i = b0 + e * 64 + (t & 63);
