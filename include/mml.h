@@ -689,7 +689,10 @@ mml_status mml_item_log_probs_grad_device(const mml_item_softmax_args* args, con
  * 8: m and v are e4m3 codes (uint8_t[n], the OCP format without infinities), value = code x scale
  * of its MML_ADAMW_BLOCK consecutive values, scale = largest magnitude / 448 (float[ceil(n / 256)]; 0
  * for a block of zeros, else 2^-126 at least);
- * v's codes hold sqrt(v), and one that is not zero never gets code 0.  A gradient that is not
+ * v's codes hold sqrt(v), and one that is not zero never gets code 0.  A code is the nearest; what it
+ * leaves of its value is kept in `rest` (uint8_t[n], 3 bits for m in sixths of a code's spacing, 5 for
+ * sqrt(v) in thirtieths, rounded with a dither that step and place give; the first 4 steps leave none),
+ * so that moments follow their recurrences though a step changes them by less than half a spacing.  A gradient that is not
  * finite (8 bits: or whose square is not) makes that value's parameter and moments NaN or infinite
  * and no other's.  All zero is the start of both forms.
  * Stream-ordered like mml_item_log_probs_device, nothing allocated or read back; a captured step
@@ -707,6 +710,7 @@ typedef struct {
     int64_t n;
     int32_t param_dtype;     /* MML_DTYPE_* */
     int32_t grad_dtype;
+    uint8_t* rest;           /* 8 bits: [n] */
 } mml_adamw_tensor;
 typedef struct {
     double learn_rate, beta1, beta2, epsilon, weight_decay;

@@ -100,7 +100,7 @@ class AdamwTensor(ctypes.Structure):
     """mml_adamw_tensor (include/mml.h)."""
     _fields_ = [("param", _vp), ("grad", _vp), ("m", _vp), ("v", _vp), ("m_scale", _vp),
                 ("v_scale", _vp), ("n", ctypes.c_int64), ("param_dtype", ctypes.c_int32),
-                ("grad_dtype", ctypes.c_int32)]
+                ("grad_dtype", ctypes.c_int32), ("rest", _vp)]
 
 
 class AdamwParams(ctypes.Structure):

@@ -16,7 +16,8 @@ class AdamW:
     ``step(grads)`` updates the tensors in place on torch's current stream and returns without
     waiting; it may be captured into a graph, and a replay counts its step.  ``StateBits``: 32, or
     8 for moments as e4m3 codes with one scale per 256 values (``m``, ``v`` and ``m_scale``,
-    ``v_scale``; ``v`` then holds the codes of sqrt(v)).  LearnRate, Beta1, Beta2, Epsilon and
+    ``v_scale``; ``v`` then holds the codes of sqrt(v)) and a byte for what both codes leave
+    (``rest``; zeros where a ``state`` has none).  LearnRate, Beta1, Beta2, Epsilon and
     WeightDecay may be changed between steps.  ``state``: the dict that ``state()`` returned (its
     tensors are used, not copied), to go on from there."""
 
@@ -44,28 +45,26 @@ class AdamW:
         self._device = self.params[0].device if self.params else torch.device("cuda", 0)
         blocks = [-(-p.numel() // N.ADAMW_BLOCK) for p in self.params]
         kind = torch.float32 if StateBits == 32 else torch.float8_e4m3fn
-        names = ("m", "v") if StateBits == 32 else ("m", "v", "m_scale", "v_scale")
+        names = ("m", "v") if StateBits == 32 else ("m", "v", "m_scale", "v_scale", "rest")
         s = dict(state) if state is not None else {}
         for name in names:
             scale = name.endswith("scale")
+            dtype = torch.float32 if scale else torch.uint8 if name == "rest" else kind
             if name not in s:
-                if state is not None:
+                if state is not None and name != "rest":
                     raise ValueError(f"state has no {name}")
+                zeros = torch.uint8 if dtype == torch.float8_e4m3fn else dtype
                 s[name] = [torch.zeros(b if scale else p.shape, device=self._device,
-                                       dtype=torch.float32 if scale else torch.uint8
-                                       if StateBits == 8 else kind)
+                                       dtype=zeros).view(dtype)
                            for p, b in zip(self.params, blocks)]
-                if StateBits == 8 and not scale:
-                    s[name] = [x.view(kind) for x in s[name]]
             x = list(s[name])
             if len(x) != len(self.params):
                 raise ValueError(f"state has {len(x)} {name}, expected {len(self.params)}")
             for y, p, b in zip(x, self.params, blocks):
-                want = torch.float32 if scale else kind
                 shape = (b,) if scale else tuple(p.shape)
-                if y.dtype != want or tuple(y.shape) != shape or y.device != self._device \
+                if y.dtype != dtype or tuple(y.shape) != shape or y.device != self._device \
                         or not y.is_contiguous():
-                    raise ValueError(f"state's {name} must be contiguous {want} tensors of the "
+                    raise ValueError(f"state's {name} must be contiguous {dtype} tensors of the "
                                      "parameters' (scales: blocks') shapes on their device")
             setattr(self, name, x)
         self._names = names
@@ -78,6 +77,7 @@ class AdamW:
             t.param, t.m, t.v = p.data_ptr(), self.m[i].data_ptr(), self.v[i].data_ptr()
             if StateBits == 8:
                 t.m_scale, t.v_scale = self.m_scale[i].data_ptr(), self.v_scale[i].data_ptr()
+                t.rest = self.rest[i].data_ptr()
             t.n, t.param_dtype = p.numel(), _DTYPES[p.dtype]
 
     @property
@@ -108,7 +108,7 @@ class AdamW:
             self._device.index, torch._C._cuda_getCurrentRawStream(self._device.index)))
 
     def state(self):
-        """{"step", "m", "v"} and with 8 bits {"m_scale", "v_scale"}: the optimizer's own tensors
+        """{"step", "m", "v"} and with 8 bits {"m_scale", "v_scale", "rest"}: the optimizer's own tensors
         and the number of steps done (waits for the device)."""
         s = {n: getattr(self, n) for n in self._names}
         s["step"] = int(self._count[0])

@@ -64,3 +64,129 @@ def test_first_moments_under_the_smallest_scale(largest):
         assert finite(opt)
     for p in ps:
         assert (p == 1).all()
+
+
+def spacing(code):
+    """of the e4m3 numbers at a code's value (subnormal ones below 2^-6)"""
+    a = np.maximum(np.abs(code), 2.0 ** -6)
+    return 2.0 ** (np.floor(np.log2(a)) - 3)
+
+
+def stored(opt, i):
+    """(m, sqrt(v)) that the state stands for, in 64 bits"""
+    rest = opt.rest[i].cpu().numpy().astype(np.int32)
+    out = []
+    for q, scale, units, r in ((opt.m[i], opt.m_scale[i], 6, (rest << 29) >> 29),
+                               (opt.v[i], opt.v_scale[i], 30, (rest << 24) >> 27)):
+        code = q.cpu().double().numpy()
+        s = np.repeat(scale.cpu().double().numpy(), 256)[:len(code)]
+        assert np.abs(r).max() <= units // 2
+        out.append((code + r * spacing(code) / units) * s)
+    return out
+
+
+HALF = np.arange(1324) % 256 < 128
+PATTERNS = {  # the gradients' sizes at step t, from t = 1
+    "equal": lambda t, rs: np.ones(1324),
+    "log-normal": lambda t, rs: np.exp(np.random.default_rng(1).normal(0, 1, 1324)),
+    "one in fifty": lambda t, rs: rs.random(1324) < 0.02,
+    "rows of 64, one in fifty": lambda t, rs: np.repeat(rs.random(21) < 0.02, 64)[:1324] * 1.0
+    if t > 1 else np.ones(1324),
+    "half falls": lambda t, rs: np.where(HALF & (t > 500), 0.1, 1.0),
+    "half rises": lambda t, rs: np.where(HALF & (t > 500), 10.0, 1.0),
+    "half stops": lambda t, rs: np.where(HALF & (t > 1500), 0.0, 1.0),
+}
+
+
+@pytest.mark.parametrize("steady", [False, True], ids=["noise", "steady"])
+@pytest.mark.parametrize("name", PATTERNS)
+def test_moments_follow_their_definition(name, steady):
+    """3,000 steps against the recurrences in 64 bits (the blocks' values side by side, a whole chunk
+    and a partial one): codes alone are off by factors of 2 to 9 in some of these, since a step's
+    change is lost where it is below half a spacing.
+
+    Tolerance.  A root is rounded once a step to a unit, 1/30 of a spacing (at most 2^-3 of the value):
+    an error under a unit, h <= 2^-3 / 30, of zero mean, with a variance of h^2 / 4 at most (a value's
+    place u between two units: u (1 - u) h^2).  A root's error shrinks by beta2 a step while the root
+    stays, so the sum's variance is under h^2 / 4 / (2 (1 - beta2)) = 125 h^2; a root without gradients
+    shrinks along with it, so its relative errors add up, 1,500 h^2 / 4 more: 22.4 h = 9.4 % as a
+    deviation.  Where the errors are spread as a sum of many, 5 % are beyond two of it: a tenth are
+    allowed, and none beyond six.  A first moment: units of 2^-3 / 6 of the value or of 2^-9 / 6 of the scale below, whose
+    values reach 448, a variance of h^2 / 4 / (1 - 0.81), so 2.4 % of the largest |m| over the last 20
+    steps, of its block for the smallest; six times that."""
+    rs = np.random.default_rng(5)
+    n = 1324
+    opt = AdamW([torch.zeros(n, device="cuda")], StateBits=8, **HYPER)
+    m, v, recent = np.zeros(n), np.zeros(n), np.zeros(n)
+    sign = rs.choice([-1.0, 1.0], n)
+    for t in range(1, 3001):
+        g = (PATTERNS[name](t, rs) * (sign if steady else rs.normal(0, 1, n))).astype(np.float32)
+        opt.step([torch.tensor(g, device="cuda")])
+        m = 0.9 * m + 0.1 * g
+        v = 0.999 * v + 0.001 * g.astype(np.float64) ** 2
+        recent = np.maximum(0.9 ** 0.5 * recent, np.abs(m))
+    got_m, got_root = stored(opt, 0)
+    ratio = got_root[v > 0] / np.sqrt(v[v > 0])
+    sigma = 0.094
+    assert abs(np.median(ratio) - 1) < 0.02, np.median(ratio)
+    assert (np.abs(ratio - 1) <= 6 * sigma).all(), (ratio.min(), ratio.max())
+    assert (np.abs(ratio - 1) <= 2 * sigma).mean() >= 0.9
+    assert (got_root[v == 0] == 0).all()
+    block = np.repeat([recent[b:b + 256].max() for b in range(0, n, 256)], 256)[:n]
+    assert (np.abs(got_m - m) <= 6 * 0.024 * recent + 2.0 ** -9 / 448 * block).all()
+
+
+@pytest.mark.parametrize("at", [0, 1])
+def test_steps_repeat_bit_for_bit(at):
+    """Two runs, one of them resumed from its state and one of them captured, and one whose tensors
+    begin at any byte: the same bits in every tensor of the state."""
+    rs = np.random.default_rng(6)
+    n = 3000
+    gs = [torch.tensor(rs.normal(0, 1, n), dtype=torch.float32, device="cuda") for _ in range(12)]
+    buf = torch.zeros(n + 8, device="cuda")
+    a = AdamW([torch.zeros(n, device="cuda")], StateBits=8, **HYPER)
+    if at:  # a state at odd bytes: the path without vectors
+        u8 = lambda: torch.zeros(n + 8, dtype=torch.uint8, device="cuda")[at:at + n]
+        blocks = -(-n // 256)
+        state = {"step": 0, "rest": [u8()], "m": [u8().view(torch.float8_e4m3fn)],
+                 "v": [u8().view(torch.float8_e4m3fn)],
+                 "m_scale": [torch.zeros(blocks, device="cuda")],
+                 "v_scale": [torch.zeros(blocks, device="cuda")]}
+        b = AdamW([buf[at:at + n]], StateBits=8, state=state, **HYPER)
+    else:
+        b = AdamW([buf[at:at + n]], StateBits=8, **HYPER)
+    for g in gs[:6]:
+        a.step([g])
+        b.step([g])
+    b = AdamW(b.params, StateBits=8, state=b.state(), **HYPER)
+    g = gs[0].clone()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        b.step([g])
+    for x in gs[6:]:
+        a.step([x])
+        g.copy_(x)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert a.state()["step"] == b.state()["step"]
+    assert torch.equal(a.params[0], b.params[0]) and (a.rest[0] != 0).any()
+    for name in ("m", "v", "m_scale", "v_scale", "rest"):
+        x, y = getattr(a, name)[0], getattr(b, name)[0]
+        assert torch.equal(x.view(torch.uint8), y.contiguous().view(torch.uint8)), name
+
+
+def test_states_without_rests_and_refusals():
+    """A state of codes and scales alone goes on from there; rests of another type or size are refused."""
+    p = torch.ones(300, device="cuda")
+    a = AdamW([p], StateBits=8, **HYPER)
+    a.step([torch.full((300,), 0.5, device="cuda")])
+    s = a.state()
+    del s["rest"]
+    b = AdamW([p], StateBits=8, state=s, **HYPER)
+    assert (b.rest[0] == 0).all() and b.rest[0].shape == p.shape
+    for bad in (torch.zeros(300, device="cuda"), torch.zeros(299, dtype=torch.uint8, device="cuda")):
+        with pytest.raises(ValueError, match="state's rest must"):
+            AdamW([p], StateBits=8, state=dict(s, rest=[bad]), **HYPER)
+    with pytest.raises(ValueError, match="1 m, expected 2|state has 1 m"):
+        AdamW([p, p.clone()], StateBits=8, state=s, **HYPER)
