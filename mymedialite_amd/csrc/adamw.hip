@@ -22,8 +22,8 @@
 // within 0.93 and 1.06 of theirs, first moments within 1.5 %.
 //
 // Memory-bound: an f32 parameter takes 28 bytes with 32-bit moments (p, m, v read and written, g
-// read), 18.06 with 8-bit ones.  71.5 M f32 values take 397 us with 32-bit moments and 232 with 8-bit
-// ones, 5.0 TB/s both (a large copy: 4.7); small models the 8 us of a launch.  One launch covers up to
+// read), 18.06 with 8-bit ones.  71.5 M f32 values take 400 us with 32-bit moments and 270 with 8-bit
+// ones, 5.0 and 4.8 TB/s (a large copy: 4.7); small models the 8 us of a launch.  One launch covers up to
 // kMaxTensors tensors, whose addresses are
 // kernel arguments (a captured graph replays with them); the step count lives on the device, so a
 // replay counts on.
@@ -39,8 +39,8 @@ namespace {
 
 constexpr int kBlock = MML_ADAMW_BLOCK;  // values per scale
 // Values per block of threads and turn: 2 groups of 4 a thread with 32-bit moments, 1 with 8-bit
-// ones, whose arithmetic wants the waves instead (8 a SIMD; 64 M bf16 values: 154 us against 187 with
-// 2 groups and 5 waves; 64 M f32 values with 32-bit moments: 354 us with 2 groups, 367 with 1).
+// ones, whose arithmetic wants the waves instead (8 a SIMD; 71.5 M f32 values: 270 us against 320 with
+// 5 to 7 waves, though 7 of a wave's registers are spilled; 64 M f32 values with 32-bit moments: 354 us with 2 groups, 367 with 1).
 template <int BITS>
 constexpr int kGroupsOf4 = BITS == 32 ? 2 : 1;
 template <int BITS>
@@ -204,8 +204,9 @@ __device__ __forceinline__ uint32_t rest_byte(int32_t m, int32_t v) {
 // spacing or more, and codes and scales alone are the state of a run that short.
 constexpr int kBareSteps = 4;
 // Multiples of the golden ratio and of another fraction, as fractions of 2^32
+constexpr uint32_t kPlace = 0x85EBCA6Bu;
 __device__ __forceinline__ uint32_t dither_at(int32_t step, int64_t i) {
-    return (uint32_t)step * 0x9E3779B9u + (uint32_t)i * 0x85EBCA6Bu;
+    return (uint32_t)step * 0x9E3779B9u + (uint32_t)i * kPlace;
 }
 // (under 1, so that what is a code's value exactly, 0 above all, stays it)
 __device__ __forceinline__ float fraction(uint32_t x) { return (float)(x >> 8) * 0x1p-24f; }
@@ -363,9 +364,10 @@ __global__ __launch_bounds__(256, BITS == 32 ? 1 : 8) void adamw_kernel(Step s) 
                     uint32_t rests = 0;
                     if (step > kBareSteps) {
                         const f32x4 dm = decode4(cm), dv = decode4(cv);
+                        const uint32_t first = dither_at(step, at[u]);
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
-                            const float dither = fraction(dither_at(step, at[u] + e));
+                            const float dither = fraction(first + e * kPlace);
                             rests |= rest_byte(rest_of<kUnitsM>(qm[e], dm[e], dither),
                                                rest_of<kUnitsV>(qr[e], dv[e], dither)) << (8 * e);
                         }
