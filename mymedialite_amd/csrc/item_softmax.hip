@@ -1500,6 +1500,7 @@ softmax_grad_users_kernel(Job j) {
     load_kept<T, KT, LK>(j.u.frag, mine ? ut : 0, b, mykept, lane);
     const RowMeta& meta = j.meta[mine ? ut : 0];
     const float lse2 = meta.lse2[lane & 31], c0 = meta.c0[lane & 31], c1 = meta.c1[lane & 31];
+    const int32_t given = meta.t[lane & 31];
     const Scale sc = *j.scale;
     Shift sh;
     f32x16 acc[MT] = {};
@@ -1549,6 +1550,14 @@ softmax_grad_users_kernel(Job j) {
             const float x = fmaf(c[i], sc.kappa, -lse2);
             g[i] = __builtin_amdgcn_exp2f(x) * fmaf(c1, x, c0);
         }
+        // G is whole before it is split: w (1 - p) keeps the planes' bits where p is close to 1, which
+        // -w p in two planes with w V_t added to the sum afterwards does not
+        if (__any(given >> 5 == tl)) {  // a row's given item: rarely
+            asm volatile("");  // as in mask_tile
+            const float add = given >> 5 == tl ? j.w[row] : 0.0f;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) g[i] += (given & 31) - 4 * h == reg_row(i, 0) ? add : 0.0f;
+        }
         if (NB == 1) {
             stage_wait();
             if (tl + 1 < t1) load(tl + 1, 0);
@@ -1570,7 +1579,7 @@ softmax_grad_users_kernel(Job j) {
 }
 
 // Items' side: a wave keeps 32 items and streams the user tiles of its split; dV += G^T U,
-// db = the sum of G.  The given items add w to G's element here.
+// db = the sum of G.
 template <int T, int KT>
 __global__ __launch_bounds__((kItemsWaves * 64), (items_per_simd<T, KT>())) void
 softmax_grad_items_kernel(Job j) {
@@ -1707,7 +1716,7 @@ __device__ __forceinline__ f32x4 join_splits(const float* __restrict__ part, int
         for (int e = 0; e < 4; ++e) a[e] += __shfl_xor(a[e], d);
     return a;
 }
-// The users' rows with w V_t added
+// The users' rows
 template <int T>
 __device__ __forceinline__ void join_users(const Job& j, int32_t kp, uint32_t block) {
     const int threads = join_threads(j.splits);
@@ -1718,12 +1727,6 @@ __device__ __forceinline__ void join_users(const Job& j, int32_t kp, uint32_t bl
     const int f = in ? 4 * (int)(x % quads) : 0;
     f32x4 a = join_splits(j.du_part + r * kp + f, j.rows_pad * kp, j.splits, threads);
     if (!in || (threadIdx.x & (threads - 1))) return;
-    const int32_t t = j.meta[r >> 5].t[r & 31];
-    if (t >= 0)
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-            if (f + e < j.k)
-                a[e] = fmaf(j.w[r], load_factor<T>(j.v.src, (int64_t)t * j.v.ld + f + e), a[e]);
     store_factors<T>(j.gu, r * j.ld_gu, f, j.k, j.gu_vec4, a);
 }
 template <int T>
