@@ -20,7 +20,8 @@
 // (1.6 PFLOP/s on random data against 2.3 on constants).  f16 factors are one f16 plane, bf16
 // factors one bf16 plane.  G is split into two planes as well: f16 under a power of two that every
 // kept row adapts to the largest |G| it has met (the sums are scaled along, as a running maximum's
-// are), or bf16 for bf16 factors (16 bits against the result's 8).
+// are), or bf16 for bf16 factors (17 bits against the result's 8: a result differs
+// from that of G in f32 where the last 2^-18 of it turns a rounding, by one step).
 //
 // Tile layout.  v_mfma_f32_32x32x16: A (32 x 16), lane l holds row l % 32, k = 8 (l / 32) .. + 7;
 // B (16 x 32) the same with the column; C: lane l holds column l % 32, register i row
@@ -604,9 +605,8 @@ __device__ __forceinline__ void split_pair(float x, float y, uint32_t& hi, uint3
     hi = __builtin_bit_cast(uint32_t, h);
     lo = __builtin_bit_cast(uint32_t, __builtin_convertvector(rest, f16x2));
 }
-// The planes of G's registers 8 s .. 8 s + 7 as B operands.  bf16: the first plane is cut off, so
-// the second starts from the exact rest; the second is rounded to nearest.  f16: both rounded to
-// nearest.
+// The planes of G's registers 8 s .. 8 s + 7 as B operands, both rounded to nearest (the rest between
+// them is exact).
 template <int T>
 __device__ __forceinline__ void split_g(const float (&g)[16], int step, uint4 (&q)[2]) {
     uint32_t w[2][4];
@@ -616,10 +616,9 @@ __device__ __forceinline__ void split_g(const float (&g)[16], int step, uint4 (&
         if constexpr (Planes<T>::HALF) {
             split_pair(x[0], x[1], w[0][e], w[1][e]);
         } else {
-            const uint32_t a = __float_as_uint(x[0]), b = __float_as_uint(x[1]);
-            const f32x2 rest = {x[0] - __uint_as_float(a & 0xFFFF0000u),
-                                x[1] - __uint_as_float(b & 0xFFFF0000u)};
-            w[0][e] = __builtin_amdgcn_perm(b, a, 0x07060302u);
+            w[0][e] = __builtin_bit_cast(uint32_t, __builtin_convertvector(x, bf16x2));
+            const f32x2 rest = {x[0] - __uint_as_float(w[0][e] << 16),
+                                x[1] - __uint_as_float(w[0][e] & 0xFFFF0000u)};
             w[1][e] = __builtin_bit_cast(uint32_t, __builtin_convertvector(rest, bf16x2));
         }
     }
