@@ -637,7 +637,8 @@ mml_status mml_wrmf_auc(mml_wrmf* h, const int32_t* candidates, int32_t n_candid
  * least (the batch's users; the items that no bias excludes); half-precision factors exactly.  Sums
  * are f32 within a tile and a split and f64 between them; a gradient's are f32 throughout, of
  * dL/ds held to 2^-22 of itself, and to 2^-37 of its row's or item's largest at least (bf16 factors:
- * to 2^-18 of itself). */
+ * to 2^-18 of itself), whose probabilities are known to 2^-23 of |log_norm| more; a row with a
+ * gradient and a log_norm beyond +-1e6 is NaN. */
 enum { MML_DTYPE_F32 = 0, MML_DTYPE_BF16 = 1, MML_DTYPE_F16 = 2 };
 typedef struct {
     int32_t dtype;                  /* MML_DTYPE_* of both factor matrices */

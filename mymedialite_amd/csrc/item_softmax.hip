@@ -376,7 +376,8 @@ __device__ __forceinline__ Scale make_scale(const Job& j) {
     const int e = eu + ev;
     c.unit = ldexpf(1.0f, -e);
     c.kappa = ldexpf(kLog2e, -e);
-    c.gone = -fmaxf(ldexpf(1e30f, min(e, 0)), 1.0995116e12f);  // 2^40: scaled scores are below 2^35
+    // (e <= 24: 1e30 2^24 is within f32; 2^40: products of scaled factors are below 2^35)
+    c.gone = -fmaxf(ldexpf(1e30f, e), 1.0995116e12f);
     c.floor = c.gone * 0.0625f;
     if (e < kLeastExponent) c.unit = c.kappa = __builtin_nanf("");
     c.eu = eu;
@@ -386,6 +387,9 @@ __device__ __forceinline__ Scale make_scale(const Job& j) {
     return c;
 }
 
+// A probability is 2^(s kappa - lse2), and lse is known to 2^-24 of itself: beyond this norm, where it
+// is off by a tenth and more, a row's gradient is NaN.
+constexpr float kMostNorm = 1e6f;
 // The rows' constants of the gradient (thread t < 32 of a users' block: row r; bad as ubad).  A row
 // without one -- both coefficients 0, no items left, an unknown user -- gets lse2 = 1e30, so that its
 // p are 0.
@@ -402,7 +406,7 @@ __device__ __forceinline__ void make_meta(const Job& j, int64_t r, int bad) {
         w = t >= 0 && j.g_lp ? j.g_lp[r] : 0.0f;
         if ((w != 0.0f || h != 0.0f) && lse != -INFINITY) {
             const float H = h != 0.0f ? j.in_entropy[r] : 0.0f;
-            lse2 = bad ? __builtin_nanf("") : lse * kLog2e;
+            lse2 = bad || !(fabsf(lse) <= kMostNorm) ? __builtin_nanf("") : lse * kLog2e;
             c0 = -(w + h * H);
             c1 = -h * kLn2;
             given = t;
@@ -731,6 +735,10 @@ constexpr int forward_tiles() {
     constexpr int n = 32 / (Planes<T>::PS * KT);
     return n >= 8 ? 8 : n >= 4 ? 4 : n >= 2 ? 2 : 1;
 }
+// Exponents are one fma, s kappa - m2, with m2 = m kappa rounded: off by 2^-24 of |m2|.  From this
+// |m2| on (2^-15 off; from 2^31 on the exponentials would be infinite or 0) the maximum is subtracted
+// first, exactly.
+constexpr float kFar = 1024.0f;
 constexpr int kTileGroup = 8;  // the streamed items are padded to a multiple of so many tiles
 
 // A block's waves keep 32 users each and stream the item tiles of a split through LDS, TPS tiles a
@@ -764,6 +772,7 @@ softmax_forward_kernel(Job j) {
     };
     const Scale sc = *j.scale;
     float m = sc.floor, m2 = m * sc.kappa, l = 0.0f, w = 0.0f, mx[TPS];
+    bool far = false;  // in any lane
     uint32_t bits[TPS] = {}, next[TPS] = {};
     const auto load_bits = [&](int tl) {
 #pragma unroll
@@ -838,11 +847,19 @@ softmax_forward_kernel(Job j) {
                 l *= f;
                 m = mn;
                 m2 = m * sc.kappa;
+                far = __any(fabsf(m2) > kFar && m > sc.floor);
+            }
+            float from = m2;
+            if (far) {
+                asm volatile("");  // as in mask_tile
+                from = 0.0f;
+#pragma unroll
+                for (int i = 0; i < 16; ++i) c[i] -= m;
             }
             float sl, sw;
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
-                const float y = fmaf(c[i], sc.kappa, -m2), e = __builtin_amdgcn_exp2f(y);
+                const float y = fmaf(c[i], sc.kappa, -from), e = __builtin_amdgcn_exp2f(y);
                 sl = i ? sl + e : e;
                 sw = i ? fmaf(e, y, sw) : e * y;
             }
@@ -1045,10 +1062,9 @@ __global__ __launch_bounds__(kDirectWaves * 64) void softmax_direct_kernel(Job j
         w = f * fmaf(l, d, w);
         l *= f;
         m = mn;
-        const float m2 = m * kLog2e;
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-            const float y = fmaf(c[i], kLog2e, -m2), e = __builtin_amdgcn_exp2f(y);
+            const float y = (c[i] - m) * kLog2e, e = __builtin_amdgcn_exp2f(y);
             l += e;
             w = fmaf(e, y, w);
         }
@@ -1321,7 +1337,9 @@ __global__ __launch_bounds__(NT, 8) void softmax_finish_kernel(Job j) {
         double lp = 0.0;
         if (lse != lse) lp = lse;
         else if (g >= 0 && g < j.n_items)
-            lp = is_excluded(j, r, g) ? -INFINITY : exact_score<T, 64>(j, urow, g, t & 63) - lse;
+            lp = lse == -INFINITY || is_excluded(j, r, g)
+                     ? -INFINITY
+                     : exact_score<T, 64>(j, urow, g, t & 63) - lse;
         if (t == NT - 1) {
             const double H = joined[1];
             j.log_probs[r] = (float)lp;
