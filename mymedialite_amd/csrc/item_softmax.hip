@@ -177,7 +177,6 @@ struct Job {
     const float* bias;   // items (nullptr: 0)
     float* vbias;        // [v.tiles * 32]: bias 2^(eu + ev), scale->gone for an excluded or padding
                          // item, NaN where the factors are not finite
-    uint8_t* ubad;       // [u.tiles * 32]: 1 = factors not finite, 2 = unknown user
     uint32_t* mask;      // [rows_pad][v.tiles]: bit i of word (r, tile): item 32 tile + i excluded
     int64_t rows_pad;    // u.tiles * 32
     const int64_t* ex_off;
@@ -390,9 +389,9 @@ __device__ __forceinline__ Scale make_scale(const Job& j) {
 // A probability is 2^(s kappa - lse2), and lse is known to 2^-24 of itself: beyond this norm, where it
 // is off by a tenth and more, a row's gradient is NaN.
 constexpr float kMostNorm = 1e6f;
-// The rows' constants of the gradient (thread t < 32 of a users' block: row r; bad as ubad).  A row
-// without one -- both coefficients 0, no items left, an unknown user -- gets lse2 = 1e30, so that its
-// p are 0.
+// The rows' constants of the gradient (thread t < 32 of a users' block: row r; bad: 1 = its factors are
+// not finite, 2 = an unknown user).  A row without one -- both coefficients 0, no items left, an
+// unknown user -- gets lse2 = 1e30, so that its p are 0.
 __device__ __forceinline__ void make_meta(const Job& j, int64_t r, int bad) {
     float lse2 = 1e30f, c0 = 0.0f, c1 = 0.0f;
     int32_t given = -1;
@@ -424,9 +423,10 @@ __device__ __forceinline__ void make_meta(const Job& j, int64_t r, int bad) {
 
 // Fragments of both sides, one block per tile of 32 rows (the users' tiles first).  A row with a
 // value that is not finite is written as zeros and marked, so that 0 * NaN cannot reach the other
-// rows' sums: an item that is not excluded gets the bias NaN, a user the mark in ubad.  So is an item
-// that its bias excludes, whose factors the scale does not count.  Bound by memory: 1 M items, k = 128
-// bf16 in 98 us (512 MB, 5.2 TB/s), 500 k with k = 256 and the transposed fragments in 152 us (768 MB).
+// rows' sums: an item that is not excluded gets the bias NaN, a user NaN results from the last kernel or
+// NaN constants.  So is an item that its bias excludes, whose factors the scale does not count.  Bound by
+// memory: 1 M items, k = 128 bf16 in 98 us (512 MB, 5.2 TB/s), 500 k with k = 256 and the transposed
+// fragments in 152 us (768 MB).
 template <int T, int KT>
 __global__ __launch_bounds__(256) void softmax_prep_kernel(Job j) {
     using P = Planes<T>;
@@ -470,7 +470,6 @@ __global__ __launch_bounds__(256) void softmax_prep_kernel(Job j) {
     if (t < 32) {
         const int64_t row = tl * 32 + t;
         if (users) {
-            j.ubad[row] = (uint8_t)bad[t];
             if (j.meta) make_meta(j, row, bad[t]);
         } else {
             float b = row < s.n ? (j.bias ? j.bias[row] : 0.0f) : kGone;
@@ -522,14 +521,14 @@ __global__ __launch_bounds__(256) void softmax_prep_kernel(Job j) {
 // to + 16 i (`to` is the same in all lanes).  Written in assembly, and not as the builtin, because
 // the compiler makes every later LDS read wait for a builtin's copy to land, the reads of the other
 // buffer too; stage_wait is the wait, and a __shared__ array filled here is only read behind one.
-// (An SALU write of m0 needs a wait state before its use; nothing else here uses m0.)
+// (An SALU write of m0 needs a wait state before its use.)
 __device__ __forceinline__ void copy_to_lds(const void* from, void* to) {
     const uint32_t at = __builtin_amdgcn_readfirstlane(
         (uint32_t)(uintptr_t)(__attribute__((address_space(3))) void*)to);
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off"
                  :
                  : "s"(at), "v"(from)
-                 : "memory");
+                 : "memory", "m0");
 }
 // n KB of fragments, the 1 KB pieces dealt over the block's waves.  stage_wait: this wave's copies
 // have landed; with the barrier behind it, everyone's have.
@@ -1931,7 +1930,6 @@ int64_t plan(const mml_item_softmax_args* a, bool grad, void* base, Job& j) {
         j.u.frag = c.take<uint4>((int64_t)j.u.tiles * ps * kt * 64);
         j.v.frag = c.take<uint4>((int64_t)j.v.tiles * ps * kt * 64);
         j.vbias = c.take<float>(items_pad);
-        j.ubad = c.take<uint8_t>(j.rows_pad);
     }
     if (a->exclude_offsets) j.mask = c.take<uint32_t>((int64_t)j.v.tiles * j.rows_pad);
     if (!grad) {
