@@ -16,6 +16,7 @@
  */
 #define _GNU_SOURCE
 #include <math.h>
+#include <omp.h>
 #include <stdatomic.h>
 #include <stdint.h>
 #include <pthread.h>
@@ -153,71 +154,183 @@ typedef struct {
 
 size_t ora_bmf_params_sizeof(void) { return sizeof(ora_bmf_params); }
 
+/* Speed only, in the large-set drivers below; every value is the plain loops', bit for bit.  A rating's
+ * (triple's) scalar product is one chain of additions whose order counts, so GROUP neighbouring ones
+ * whose rows are all different, and which therefore do not see each other's updates, have theirs made
+ * side by side before they are applied one after another.  The clones let the element-wise updates use
+ * the machine's vectors; -ffp-contract=off holds for them too. */
+#define GROUP 8
+#define ORA_CLONES __attribute__((target_clones("avx512f", "avx2", "default")))
+#define ORA_INLINE static inline __attribute__((always_inline))
+
+/* whether the n ids are all different (n <= 2 * GROUP) */
+ORA_INLINE int ora_all_differ(const int32_t* id, int n) {
+    for (int a = 1; a < n; a++) {
+        int same = 0;
+        for (int b = 0; b < a; b++) same |= id[a] == id[b];
+        if (same) return 0;
+    }
+    return 1;
+}
+
+ORA_INLINE void ora_bmf_dots(float* const* a, float* const* b, int k, float* dot) {
+    float d0 = 0.0f, d1 = 0.0f, d2 = 0.0f, d3 = 0.0f, d4 = 0.0f, d5 = 0.0f, d6 = 0.0f, d7 = 0.0f;
+    for (int c = 0; c < k; c++) {
+        d0 += a[0][c] * b[0][c];
+        d1 += a[1][c] * b[1][c];
+        d2 += a[2][c] * b[2][c];
+        d3 += a[3][c] * b[3][c];
+        d4 += a[4][c] * b[4][c];
+        d5 += a[5][c] * b[5][c];
+        d6 += a[6][c] * b[6][c];
+        d7 += a[7][c] * b[7][c];
+    }
+    dot[0] = d0, dot[1] = d1, dot[2] = d2, dot[3] = d3;
+    dot[4] = d4, dot[5] = d5, dot[6] = d6, dot[7] = d7;
+}
+
+/* Iterate's body behind the scalar product, for one rating: rows Uu and Vi, biases *bu and *bi */
+ORA_INLINE void ora_bmf_apply(const ora_bmf_params* p, float value, float dot, float* restrict Uu,
+                              float* restrict Vi, float* bu, float* bi, const int32_t* count_u,
+                              const int32_t* count_i) {
+    const int k = p->k;
+    const float lr = p->learn_rate;
+    float score_f = ((p->global_bias + *bu) + *bi) + dot;
+    double score = (double)score_f;
+    double sig = 1.0 / (1.0 + exp(-score));
+    double prediction = (double)p->min_rating + sig * (double)p->rating_range_size;
+    double err = (double)value - prediction;
+
+    float g;
+    if (p->loss == ORA_LOSS_MAE) {
+        double sgn = (err > 0) ? 1.0 : ((err < 0) ? -1.0 : 0.0);
+        g = (float)(sgn * sig * (1.0 - sig) * (double)p->rating_range_size);
+    } else if (p->loss == ORA_LOSS_LOGISTIC) {
+        g = (float)err;
+    } else {
+        g = (float)(err * sig * (1.0 - sig) * (double)p->rating_range_size);
+    }
+
+    float reg_u = p->reg_u, reg_i = p->reg_i;
+    if (p->frequency_regularization) {
+        reg_u = (float)((double)p->reg_u / sqrt((double)*count_u));
+        reg_i = (float)((double)p->reg_i / sqrt((double)*count_i));
+    }
+
+    const float blr = p->bias_learn_rate * lr;
+    if (p->update_user) *bu += blr * (g - (p->bias_reg * reg_u) * *bu);
+    if (p->update_item) *bi += blr * (g - (p->bias_reg * reg_i) * *bi);
+
+    if (p->update_user && p->update_item) {
+        for (int f = 0; f < k; f++) {
+            const double u_f = (double)Uu[f], i_f = (double)Vi[f];
+            const double delta_u = (double)g * i_f - (double)reg_u * u_f;
+            const double delta_i = (double)g * u_f - (double)reg_i * i_f;
+            Uu[f] += (float)((double)lr * delta_u);
+            Vi[f] += (float)((double)lr * delta_i);
+        }
+        return;
+    }
+    for (int f = 0; f < k; f++) {
+        double u_f = (double)Uu[f];
+        double i_f = (double)Vi[f];
+        if (p->update_user) {
+            double delta_u = (double)g * i_f - (double)reg_u * u_f;
+            Uu[f] += (float)((double)lr * delta_u);
+        }
+        if (p->update_item) {
+            double delta_i = (double)g * u_f - (double)reg_i * i_f;
+            Vi[f] += (float)((double)lr * delta_i);
+        }
+    }
+}
+
 /* BiasedMatrixFactorization.Iterate(IList<int>,bool,bool), :264-310 (with SetupLoss :247-261) */
+ORA_CLONES
 void ora_bmf_iterate(const ora_bmf_params* p, const int32_t* users, const int32_t* items,
                      const float* values, const int32_t* idx, int64_t n_idx, float* U, float* V,
                      float* bu, float* bi, const int32_t* count_by_user,
                      const int32_t* count_by_item) {
     const int k = p->k;
-    const float lr = p->learn_rate;
-    enum { AHEAD = 32 };  /* rows requested AHEAD ratings early: a cache hint, the order is kept */
-    for (int64_t n = 0; n < n_idx; n++) {
-        if (n + AHEAD < n_idx) {
-            const int32_t ahead = idx[n + AHEAD];
-            const char* pu = (const char*)(U + (int64_t)users[ahead] * k);
-            const char* pv = (const char*)(V + (int64_t)items[ahead] * k);
-            for (int c = 0; c < k * 4; c += 64) {
-                __builtin_prefetch(pu + c, 1);
-                __builtin_prefetch(pv + c, 1);
+    const int64_t ahead_by = 32;  /* rows requested so many ratings early: a cache hint */
+    for (int64_t n = 0; n < n_idx;) {
+        const int m = n + GROUP <= n_idx ? GROUP : (int)(n_idx - n);
+        int32_t u[GROUP], i[GROUP];
+        float *Uu[GROUP], *Vi[GROUP], dot[GROUP];
+        for (int x = 0; x < m; x++) {
+            if (n + x + ahead_by < n_idx) {
+                const int32_t ahead = idx[n + x + ahead_by];
+                const char* pu = (const char*)(U + (int64_t)users[ahead] * k);
+                const char* pv = (const char*)(V + (int64_t)items[ahead] * k);
+                for (int c = 0; c < k * 4; c += 64) {
+                    __builtin_prefetch(pu + c, 1);
+                    __builtin_prefetch(pv + c, 1);
+                }
+                __builtin_prefetch(bu + users[ahead], 1);
+                __builtin_prefetch(bi + items[ahead], 1);
             }
-            __builtin_prefetch(bu + users[ahead], 1);
-            __builtin_prefetch(bi + items[ahead], 1);
+            u[x] = users[idx[n + x]];
+            i[x] = items[idx[n + x]];
+            Uu[x] = U + (int64_t)u[x] * k;
+            Vi[x] = V + (int64_t)i[x] * k;
         }
-        int32_t index = idx[n];
-        int32_t u = users[index];
-        int32_t i = items[index];
-        float* Uu = U + (int64_t)u * k;
-        float* Vi = V + (int64_t)i * k;
-
-        float dot = 0.0f;
-        for (int c = 0; c < k; c++) dot += Uu[c] * Vi[c];
-        float score_f = ((p->global_bias + bu[u]) + bi[i]) + dot;
-        double score = (double)score_f;
-        double sig = 1.0 / (1.0 + exp(-score));
-        double prediction = (double)p->min_rating + sig * (double)p->rating_range_size;
-        double err = (double)values[index] - prediction;
-
-        float g;
-        if (p->loss == ORA_LOSS_MAE) {
-            double sgn = (err > 0) ? 1.0 : ((err < 0) ? -1.0 : 0.0);
-            g = (float)(sgn * sig * (1.0 - sig) * (double)p->rating_range_size);
-        } else if (p->loss == ORA_LOSS_LOGISTIC) {
-            g = (float)err;
-        } else {
-            g = (float)(err * sig * (1.0 - sig) * (double)p->rating_range_size);
-        }
-
-        float reg_u = p->reg_u, reg_i = p->reg_i;
-        if (p->frequency_regularization) {
-            reg_u = (float)((double)p->reg_u / sqrt((double)count_by_user[u]));
-            reg_i = (float)((double)p->reg_i / sqrt((double)count_by_item[i]));
-        }
-
-        const float blr = p->bias_learn_rate * lr;
-        if (p->update_user) bu[u] += blr * (g - (p->bias_reg * reg_u) * bu[u]);
-        if (p->update_item) bi[i] += blr * (g - (p->bias_reg * reg_i) * bi[i]);
-
-        for (int f = 0; f < k; f++) {
-            double u_f = (double)Uu[f];
-            double i_f = (double)Vi[f];
-            if (p->update_user) {
-                double delta_u = (double)g * i_f - (double)reg_u * u_f;
-                Uu[f] += (float)((double)lr * delta_u);
+        const int together = m == GROUP && ora_all_differ(u, GROUP) && ora_all_differ(i, GROUP);
+        if (together) ora_bmf_dots(Uu, Vi, k, dot);
+        for (int x = 0; x < m; x++) {
+            if (!together) {
+                dot[x] = 0.0f;
+                for (int c = 0; c < k; c++) dot[x] += Uu[x][c] * Vi[x][c];
             }
-            if (p->update_item) {
-                double delta_i = (double)g * u_f - (double)reg_i * i_f;
-                Vi[f] += (float)((double)lr * delta_i);
+            ora_bmf_apply(p, values[idx[n + x]], dot[x], Uu[x], Vi[x], bu + u[x], bi + i[x],
+                          count_by_user ? count_by_user + u[x] : NULL,
+                          count_by_item ? count_by_item + i[x] : NULL);
+        }
+        n += m;
+    }
+}
+
+/* The step of ora_bmf_iterate_lockstep for its ratings [x0, x1): updated copies of their rows, k + 1
+ * floats each (the bias last), in nu and nv */
+ORA_CLONES
+static void ora_bmf_lockstep_range(const ora_bmf_params* p, const int32_t* users,
+                                   const int32_t* items, const float* values, const int32_t* idx,
+                                   const int64_t* sp, int64_t x0, int64_t x1, const float* U,
+                                   const float* V, const float* bu, const float* bi,
+                                   const int32_t* count_by_user, const int32_t* count_by_item,
+                                   float* nu, float* nv, int32_t* su, int32_t* si) {
+    const int k = p->k;
+    for (int64_t x = x0; x < x1; x += GROUP) {
+        const int m = x + GROUP <= x1 ? GROUP : (int)(x1 - x);
+        float *Uo[GROUP], *Vo[GROUP], dot[GROUP];
+        for (int y = 0; y < m; y++) {
+            if (x + y + GROUP < x1) {
+                const int32_t ahead = idx[sp[x + y + GROUP]];
+                const char* pu = (const char*)(U + (int64_t)users[ahead] * k);
+                const char* pv = (const char*)(V + (int64_t)items[ahead] * k);
+                for (int c = 0; c < k * 4; c += 64) {
+                    __builtin_prefetch(pu + c, 0);
+                    __builtin_prefetch(pv + c, 0);
+                }
             }
+            const int32_t index = idx[sp[x + y]], u = users[index], i = items[index];
+            Uo[y] = nu + (x + y) * (k + 1);
+            Vo[y] = nv + (x + y) * (k + 1);
+            memcpy(Uo[y], U + (int64_t)u * k, sizeof(float) * k);
+            memcpy(Vo[y], V + (int64_t)i * k, sizeof(float) * k);
+            Uo[y][k] = bu[u];
+            Vo[y][k] = bi[i];
+            su[x + y] = u;
+            si[x + y] = i;
+        }
+        if (m == GROUP) ora_bmf_dots(Uo, Vo, k, dot);
+        for (int y = 0; y < m; y++) {
+            if (m < GROUP) {
+                dot[y] = 0.0f;
+                for (int c = 0; c < k; c++) dot[y] += Uo[y][c] * Vo[y][c];
+            }
+            ora_bmf_apply(p, values[idx[sp[x + y]]], dot[y], Uo[y], Vo[y], Uo[y] + k, Vo[y] + k,
+                          count_by_user ? count_by_user + su[x + y] : NULL,
+                          count_by_item ? count_by_item + si[x + y] : NULL);
         }
     }
 }
@@ -251,34 +364,25 @@ void ora_bmf_iterate_lockstep(const ora_bmf_params* p, const int32_t* users, con
                 if (t * R + r >= per || pos >= n_idx) continue;
                 sp[m++] = pos;
             }
-        /* every rating of the step from the model before the step: independent, so on threads
-         * (OpenMP, `threads` of them); the results land in the step's buffers, the model is not
-         * touched */
-#pragma omp parallel for schedule(static) num_threads(nt) if (nt > 1)
-        for (int64_t x = 0; x < m; ++x) {
-            const int32_t index = idx[sp[x]], u = users[index], i = items[index];
-            float* Uo = nu + x * (k + 1);
-            float* Vo = nv + x * (k + 1);
-            memcpy(Uo, U + (int64_t)u * k, sizeof(float) * k);
-            memcpy(Vo, V + (int64_t)i * k, sizeof(float) * k);
-            float bu1 = bu[u], bi1 = bi[i];
-            const int32_t zero = 0;  // the rating's rows, copied: row 0 of Uo / Vo
-            ora_bmf_iterate(p, &zero, &zero, values + index, &zero, 1, Uo, Vo, &bu1, &bi1,
-                            count_by_user ? count_by_user + u : NULL,
-                            count_by_item ? count_by_item + i : NULL);
-            Uo[k] = bu1;
-            Vo[k] = bi1;
-            su[x] = u;
-            si[x] = i;
-        }
-        for (int64_t x = 0; x < m; ++x) {  /* writes in stream order: the last one stays */
-            if (p->update_user) {
-                memcpy(U + (int64_t)su[x] * k, nu + x * (k + 1), sizeof(float) * k);
-                bu[su[x]] = nu[x * (k + 1) + k];
-            }
-            if (p->update_item) {
-                memcpy(V + (int64_t)si[x] * k, nv + x * (k + 1), sizeof(float) * k);
-                bi[si[x]] = nv[x * (k + 1) + k];
+#pragma omp parallel num_threads(nt) if (nt > 1)
+        {
+            /* every rating of the step from the model before the step: independent, a range of them
+             * per thread; the results land in the step's buffers, the model is not touched */
+            const int me = omp_get_thread_num(), all = omp_get_num_threads();
+            ora_bmf_lockstep_range(p, users, items, values, idx, sp, m * me / all,
+                                   m * (me + 1) / all, U, V, bu, bi, count_by_user, count_by_item,
+                                   nu, nv, su, si);
+#pragma omp barrier
+            /* writes in stream order, the last one stays: a row belongs to one thread */
+            for (int64_t x = 0; x < m; ++x) {
+                if (p->update_user && su[x] % all == me) {
+                    memcpy(U + (int64_t)su[x] * k, nu + x * (k + 1), sizeof(float) * k);
+                    bu[su[x]] = nu[x * (k + 1) + k];
+                }
+                if (p->update_item && si[x] % all == me) {
+                    memcpy(V + (int64_t)si[x] * k, nv + x * (k + 1), sizeof(float) * k);
+                    bi[si[x]] = nv[x * (k + 1) + k];
+                }
             }
         }
     }
@@ -995,15 +1099,15 @@ static void ora_soft_margin_update(const ora_bpr_params* p, int32_t i, int32_t j
     }
 }
 
-/* BPRMF.UpdateFactors(u,i,j,...) :330-374 (model 1: SoftMarginRankingMF's override) */
-void ora_bpr_update(const ora_bpr_params* p, int32_t u, int32_t i, int32_t j, float* U, float* V,
-                    float* bias) {
+/* BPRMF.UpdateFactors(u,i,j,...) :330-374 behind the scalar product (model 1: SoftMarginRankingMF's
+ * override) */
+ORA_INLINE void ora_bpr_apply(const ora_bpr_params* p, int32_t u, int32_t i, int32_t j, double dot,
+                              float* U, float* V, float* bias) {
     const int k = p->k;
     float* w = U + (int64_t)u * k;
     float* hi = V + (int64_t)i * k;
     float* hj = V + (int64_t)j * k;
-    double x_uij = (double)(bias[i] - bias[j]) +
-                   ora_row_scalar_product_with_row_difference(U, u, V, i, V, j, k);
+    double x_uij = (double)(bias[i] - bias[j]) + dot;
     if (p->model == 1) {
         ora_soft_margin_update(p, i, j, w, hi, hj, bias, x_uij);
         return;
@@ -1016,6 +1120,21 @@ void ora_bpr_update(const ora_bpr_params* p, int32_t u, int32_t i, int32_t j, fl
     if (p->update_j) {
         double update = -e - (double)(p->bias_reg * bias[j]);
         bias[j] += (float)((double)p->learn_rate * update);
+    }
+    if (p->update_u && p->update_i && p->update_j && i != j) { /* three different rows */
+        float *restrict rw = w, *restrict ri = hi, *restrict rj = hj;
+        const double lr = (double)p->learn_rate;
+        const float reg_u = p->reg_u, reg_i = p->reg_i, reg_j = p->reg_j;
+        for (int f = 0; f < k; f++) {
+            const float w_uf = rw[f], h_if = ri[f], h_jf = rj[f];
+            const double du = (double)(h_if - h_jf) * e - (double)(reg_u * w_uf);
+            const double di = (double)w_uf * e - (double)(reg_i * h_if);
+            const double dj = (double)(-w_uf) * e - (double)(reg_j * h_jf);
+            rw[f] = (float)((double)w_uf + lr * du);
+            ri[f] = (float)((double)h_if + lr * di);
+            rj[f] = (float)((double)h_jf + lr * dj);
+        }
+        return;
     }
     for (int f = 0; f < k; f++) {
         float w_uf = w[f], h_if = hi[f], h_jf = hj[f];
@@ -1032,6 +1151,48 @@ void ora_bpr_update(const ora_bpr_params* p, int32_t u, int32_t i, int32_t j, fl
             hj[f] = (float)((double)h_jf + (double)p->learn_rate * update);
         }
     }
+}
+ORA_CLONES
+void ora_bpr_update(const ora_bpr_params* p, int32_t u, int32_t i, int32_t j, float* U, float* V,
+                    float* bias) {
+    ora_bpr_apply(p, u, i, j,
+                  ora_row_scalar_product_with_row_difference(U, u, V, i, V, j, p->k), U, V, bias);
+}
+
+/* GROUP triples (u, i, j) in order: side by side where all their rows differ */
+ORA_CLONES
+static void ora_bpr_update_group(const ora_bpr_params* p, int32_t (*t)[3], float* U, float* V,
+                                 float* bias) {
+    const int k = p->k;
+    int32_t user[GROUP], item[2 * GROUP];
+    for (int x = 0; x < GROUP; x++) {
+        user[x] = t[x][0];
+        item[2 * x] = t[x][1];
+        item[2 * x + 1] = t[x][2];
+    }
+    if (!ora_all_differ(user, GROUP) || !ora_all_differ(item, 2 * GROUP)) {
+        for (int x = 0; x < GROUP; x++) ora_bpr_update(p, t[x][0], t[x][1], t[x][2], U, V, bias);
+        return;
+    }
+    const float *a[GROUP], *b[GROUP], *c[GROUP];
+    for (int x = 0; x < GROUP; x++) {
+        a[x] = U + (int64_t)t[x][0] * k;
+        b[x] = V + (int64_t)t[x][1] * k;
+        c[x] = V + (int64_t)t[x][2] * k;
+    }
+    /* ora_row_scalar_product_with_row_difference, the chains of four triples at a time */
+    double d[GROUP];
+    for (int x = 0; x < GROUP; x += 4) {
+        double d0 = 0.0, d1 = 0.0, d2 = 0.0, d3 = 0.0;
+        for (int f = 0; f < k; f++) {
+            d0 += (double)(a[x][f] * (b[x][f] - c[x][f]));
+            d1 += (double)(a[x + 1][f] * (b[x + 1][f] - c[x + 1][f]));
+            d2 += (double)(a[x + 2][f] * (b[x + 2][f] - c[x + 2][f]));
+            d3 += (double)(a[x + 3][f] * (b[x + 3][f] - c[x + 3][f]));
+        }
+        d[x] = d0, d[x + 1] = d1, d[x + 2] = d2, d[x + 3] = d3;
+    }
+    for (int x = 0; x < GROUP; x++) ora_bpr_apply(p, t[x][0], t[x][1], t[x][2], d[x], U, V, bias);
 }
 
 /* Loss-sample burn in BPRMF.Train :136-150 (triples drawn, never used) */
@@ -1125,7 +1286,7 @@ void ora_bpr_epoch(ora_rng* r, const ora_bpr_params* p, const int64_t* off, cons
  * latency of a 1 M x 1 M set -- triples do not depend on the factors (BPRMF.cs:216-226), so the
  * sampler can run ahead of the updates, and the rows of the next triples can be prefetched.
  * ---------------------------------------------------------------------------------------- */
-#define ORA_AHEAD 8
+#define ORA_AHEAD (2 * GROUP)
 
 static void ora_bpr_prefetch(const ora_bpr_params* p, const int32_t* t, const float* U,
                              const float* V) {
@@ -1140,13 +1301,20 @@ static void ora_bpr_prefetch(const ora_bpr_params* p, const int32_t* t, const fl
 /* UpdateFactors over given triples in order (a replay of a recorded triple stream) */
 void ora_bpr_apply_triples(const ora_bpr_params* p, const int32_t* tu, const int32_t* ti,
                            const int32_t* tj, int64_t n, float* U, float* V, float* bias) {
-    for (int64_t c = 0; c < n; c++) {
-        if (c + ORA_AHEAD < n) {
-            const int32_t t[3] = {tu[c + ORA_AHEAD], ti[c + ORA_AHEAD], tj[c + ORA_AHEAD]};
-            ora_bpr_prefetch(p, t, U, V);
+    int64_t c = 0;
+    for (; c + GROUP <= n; c += GROUP) {
+        int32_t t[GROUP][3];
+        for (int x = 0; x < GROUP; x++) {
+            const int64_t y = c + x + ORA_AHEAD;
+            if (y < n) {
+                const int32_t next[3] = {tu[y], ti[y], tj[y]};
+                ora_bpr_prefetch(p, next, U, V);
+            }
+            t[x][0] = tu[c + x], t[x][1] = ti[c + x], t[x][2] = tj[c + x];
         }
-        ora_bpr_update(p, tu[c], ti[c], tj[c], U, V, bias);
+        ora_bpr_update_group(p, t, U, V, bias);
     }
+    for (; c < n; c++) ora_bpr_update(p, tu[c], ti[c], tj[c], U, V, bias);
 }
 
 #define ORA_RING (1 << 16)
@@ -1192,19 +1360,25 @@ void ora_bpr_epoch_pipelined(ora_rng* r, const ora_bpr_params* p, const int64_t*
     atomic_init(&q->tail, 0);
     pthread_t th;
     pthread_create(&th, NULL, ora_bpr_producer, q);
-    for (int64_t c = 0; c < num_events; c++) {
+    for (int64_t c = 0; c < num_events;) {
+        const int m = c + GROUP <= num_events ? GROUP : (int)(num_events - c);
         int64_t h;
-        while ((h = atomic_load_explicit(&q->head, memory_order_acquire)) <= c) {
+        while ((h = atomic_load_explicit(&q->head, memory_order_acquire)) < c + m) {
         }
-        if (c + ORA_AHEAD < h) ora_bpr_prefetch(p, q->ring + 3 * ((c + ORA_AHEAD) % ORA_RING), U, V);
-        const int32_t* t = q->ring + 3 * (c % ORA_RING);
-        if (trace) {
-            trace[3 * c] = t[0];
-            trace[3 * c + 1] = t[1];
-            trace[3 * c + 2] = t[2];
+        int32_t t[GROUP][3];
+        for (int x = 0; x < m; x++) {
+            const int64_t y = c + x;
+            if (y + ORA_AHEAD < h)
+                ora_bpr_prefetch(p, q->ring + 3 * ((y + ORA_AHEAD) % ORA_RING), U, V);
+            memcpy(t[x], q->ring + 3 * (y % ORA_RING), sizeof t[x]);
+            if (trace) memcpy(trace + 3 * y, t[x], sizeof t[x]);
         }
-        ora_bpr_update(p, t[0], t[1], t[2], U, V, bias);
-        atomic_store_explicit(&q->tail, c + 1, memory_order_release);
+        if (m == GROUP)
+            ora_bpr_update_group(p, t, U, V, bias);
+        else
+            for (int x = 0; x < m; x++) ora_bpr_update(p, t[x][0], t[x][1], t[x][2], U, V, bias);
+        c += m;
+        atomic_store_explicit(&q->tail, c, memory_order_release);
     }
     pthread_join(th, NULL);
     free(q->ring);
@@ -1273,6 +1447,8 @@ static void ora_lu_inverse(double* a, double* inv, int n, int* piv, double* col)
 
 /* WRMF.ComputeSquareMatrix :94-108 -- float products, double sums */
 void ora_wrmf_square(const float* H, int64_t rows, int k, double* HH) {
+    /* (elements on threads; every sum in its own order) */
+#pragma omp parallel for schedule(dynamic, 1)
     for (int f1 = 0; f1 < k; f1++)
         for (int f2 = f1; f2 < k; f2++) {
             double d = 0.0;
@@ -1312,12 +1488,16 @@ static void wrmf_optimize_rows_impl(const int64_t* off, const int32_t* cols, int
                                     int64_t row_end, int64_t n_data_rows, float* W,
                                     const float* H, const double* HH, int k, double alpha,
                                     double reg, int exact) {
+    /* (rows on threads: each its own system) */
+#pragma omp parallel
+    {
     double* HC = (double*)malloc(sizeof(double) * (size_t)k * k);
     double* m = (double*)malloc(sizeof(double) * (size_t)k * k);
     double* inv = (double*)malloc(sizeof(double) * (size_t)k * k);
     double* HCp = (double*)malloc(sizeof(double) * (size_t)k);
     double* col = (double*)malloc(sizeof(double) * (size_t)k);
     int* piv = (int*)malloc(sizeof(int) * (size_t)k);
+#pragma omp for schedule(dynamic, 1)
     for (int64_t u = row_begin; u < row_end; u++) {
         int64_t b = (u < n_data_rows) ? off[u] : 0, e = (u < n_data_rows) ? off[u + 1] : 0;
         for (int f1 = 0; f1 < k; f1++)
@@ -1355,6 +1535,7 @@ static void wrmf_optimize_rows_impl(const int64_t* off, const int32_t* cols, int
     free(HCp);
     free(col);
     free(piv);
+    }
 }
 
 /* ------------------------------------------------------------------------------------------
