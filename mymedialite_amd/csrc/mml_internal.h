@@ -328,8 +328,10 @@ struct PeerGroup {
     ~PeerGroup();
     PeerGroup(const PeerGroup&) = delete;
     PeerGroup& operator=(const PeerGroup&) = delete;
-    // throws when a rank aborted (its call failed): the others then leave instead of waiting
+    // throws when a rank aborted (its call failed) or does not come within limit_s seconds: the
+    // others then leave instead of waiting.  (The slowest half-step between two barriers takes seconds.)
     void barrier();
+    double limit_s = 600.0;
     void abort();  // by a failing rank
     void reset();  // before the ranks start a call (no rank inside the group)
     // every rank's rows [bounds[r], bounds[r + 1]) of W [rows x k] copied into every other rank's

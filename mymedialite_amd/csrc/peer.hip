@@ -12,6 +12,7 @@
 //    stopping decision (the max over ranks of the last correction, as ncclMax would give); the
 //    BiasedMF DSGD ring's ranks send item groups through it (bmf.hip ring_exchange / ring_bcast,
 //    the peer-copy twins of ncclSend / ncclRecv and ncclBroadcast).
+#include <chrono>
 #include <condition_variable>
 #include <mutex>
 
@@ -108,8 +109,16 @@ void PeerGroup::barrier() {
         impl->cv.notify_all();
         return;
     }
-    impl->cv.wait(lk, [&] { return impl->generation != gen || impl->aborted; });
-    if (impl->generation == gen) fail(MML_ERR_STATE, "another shard of the context failed");
+    const bool woken = impl->cv.wait_for(lk, std::chrono::duration<double>(limit_s), [&] {
+        return impl->generation != gen || impl->aborted;
+    });
+    if (impl->generation != gen) return;
+    if (!woken) {
+        impl->aborted = true;
+        impl->cv.notify_all();
+        fail(MML_ERR_STATE, "another shard of the context did not come to a barrier");
+    }
+    fail(MML_ERR_STATE, "another shard of the context failed");
 }
 
 void PeerGroup::abort() {
