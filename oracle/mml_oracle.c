@@ -1328,12 +1328,33 @@ typedef struct {
     _Atomic int64_t head, tail;
 } ora_bpr_pipe;
 
+/* Sampling waits for memory too: a user's offsets, then its rows.  A second generator runs FAR triples
+ * ahead with the same draws (three a triple as long as none is rejected) and names the users that
+ * come, so that their offsets are requested; half way, their rows.  Hints only: where a draw was rejected
+ * they name other users for a while, and the triples are the first generator's in any case. */
+#define FAR 48
 static void* ora_bpr_producer(void* arg) {
     ora_bpr_pipe* q = (ora_bpr_pipe*)arg;
+    ora_rng ahead = *q->r;
+    for (int x = 0; x < 3 * FAR; x++) ora_rng_internal_sample(&ahead);
+    int32_t coming[FAR];
+    for (int x = 0; x < FAR; x++) coming[x] = 0;
     for (int64_t c = 0; c < q->n; c++) {
+        const int32_t user = ora_rng_next(&ahead, q->p->max_user_id + 1);
+        coming[c % FAR] = user;
+        __builtin_prefetch(q->off + user, 0);
+        const int32_t near = coming[(c + FAR / 2) % FAR];
+        for (int64_t x = q->off[near]; x < q->off[near + 1]; x += 16) {
+            __builtin_prefetch(q->rows + x, 0);
+            __builtin_prefetch(q->sorted + x, 0);
+        }
+        const int32_t before = q->r->inext;
         while (c - atomic_load_explicit(&q->tail, memory_order_acquire) >= ORA_RING) {
         }
         ora_bpr_sample_triple(q->r, q->p, q->off, q->rows, q->sorted, q->ring + 3 * (c % ORA_RING));
+        int drawn = q->r->inext - before; /* (the state goes round 55 places) */
+        if (drawn <= 0) drawn += 55;
+        for (int x = 1; x < drawn; x++) ora_rng_internal_sample(&ahead);
         atomic_store_explicit(&q->head, c + 1, memory_order_release);
     }
     return NULL;
