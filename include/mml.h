@@ -672,9 +672,10 @@ mml_status mml_item_log_probs_device(const mml_item_softmax_args* args, float* l
                                      int64_t workspace_bytes, int32_t device, void* stream);
 /* The gradient of a loss L with grad_log_probs[r] = dL / d log_probs[r] and grad_entropy[r] =
  * dL / d entropy[r] (either NULL: 0), log_norm and entropy as mml_item_log_probs_device gave them
- * (entropy only read with grad_entropy): grad_users [n_rows x num_factors] per row (a user listed
- * twice has two), grad_items [n_items x num_factors] in the factors' type with the row strides
- * ld_*, grad_bias [n_items].  Every element is written, in the same order of sums every time. */
+ * (entropy only read with grad_entropy; |grad_entropy| up to 1e8): grad_users [n_rows x num_factors]
+ * per row (a user listed twice has two), grad_items [n_items x num_factors] in the factors' type with
+ * the row strides ld_*, grad_bias [n_items].  Every element is written, in the same order of sums every
+ * time. */
 mml_status mml_item_log_probs_grad_device(const mml_item_softmax_args* args, const float* log_norm,
                                           const float* entropy, const float* grad_log_probs,
                                           const float* grad_entropy, void* grad_users,

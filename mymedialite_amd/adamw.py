@@ -10,6 +10,13 @@ from . import _native as N
 _DTYPES = {torch.float32: N.DTYPE_F32, torch.bfloat16: N.DTYPE_BF16, torch.float16: N.DTYPE_F16}
 
 
+def _overlap(tensors):
+    """Whether two of the contiguous tensors share memory"""
+    spans = sorted((x.data_ptr(), x.data_ptr() + x.numel() * x.element_size())
+                   for x in tensors if x.numel())
+    return any(x[1] > y[0] for x, y in zip(spans, spans[1:]))
+
+
 class AdamW:
     """One optimizer for a list of contiguous float32, bfloat16 or float16 tensors on one GPU.
 
@@ -38,9 +45,7 @@ class AdamW:
                 raise ValueError("parameters must be on one device")
             if not p.is_contiguous():
                 raise ValueError("parameters must be contiguous: they are updated in place")
-        spans = sorted((p.data_ptr(), p.data_ptr() + p.numel() * p.element_size())
-                       for p in self.params if p.numel())
-        if any(x[1] > y[0] for x, y in zip(spans, spans[1:])):
+        if _overlap(self.params):
             raise ValueError("a parameter is listed twice, or two overlap")
         self._device = self.params[0].device if self.params else torch.device("cuda", 0)
         blocks = [-(-p.numel() // N.ADAMW_BLOCK) for p in self.params]
@@ -68,6 +73,10 @@ class AdamW:
                                      "parameters' (scales: blocks') shapes on their device")
             setattr(self, name, x)
         self._names = names
+        if _overlap(self.params + [y for name in names for y in getattr(self, name)]):
+            raise ValueError("two of the state's tensors overlap, or one and a parameter")
+        if int(s.get("step", 0)) < 0:
+            raise ValueError("state's step must not be negative")
         self._count = torch.zeros(N.ADAMW_STATE, dtype=torch.int32, device=self._device)
         self._count[0] = int(s.get("step", 0))
         n = len(self.params)

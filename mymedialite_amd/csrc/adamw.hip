@@ -124,8 +124,9 @@ __device__ __forceinline__ void moments(const Factors& f, float g, float& m, flo
     m = fmaf(f.one1, g, f.beta1 * m);
     v = fmaf(f.one2, g * g, f.beta2 * v);
 }
-// A square root rounded as sqrtf's from the reciprocal root in fewer instructions: one step for both
-// sqrt(v) and 1 / (2 sqrt(v)), then the remainder.  For v from 2^-96 on (no term underflows).
+// A square root rounded as sqrtf's from the reciprocal root in fewer instructions: one step of
+// Goldschmidt's iteration for both sqrt(v) and 1 / (2 sqrt(v)), then the remainder (Markstein 2004).  For
+// v from 2^-96 on (no term underflows).
 __device__ __forceinline__ float normal_root(float v) {
     const float y = __builtin_amdgcn_rsqf(v);
     float g = v * y, h = 0.5f * y;

@@ -3,8 +3,8 @@
 ``item_log_probs`` gives the log probability of given items, the log normaliser, the entropy and the
 likeliest items of a batch of users; ``item_log_probs_grad`` the gradient of a loss on them.  Both
 run the HIP kernels of libmml_hip.so on torch's current stream of the factors' device and return
-without waiting; there is no CPU path.  (BPRMF.log_probs and WRMF.log_probs are the same for a
-trained recommender, on host arrays.)
+without waiting; there is no CPU path, and results carry no autograd graph.  (BPRMF.log_probs and
+WRMF.log_probs are the same for a trained recommender, on host arrays.)
 """
 from __future__ import annotations
 

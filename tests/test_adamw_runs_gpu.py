@@ -190,3 +190,58 @@ def test_states_without_rests_and_refusals():
             AdamW([p], StateBits=8, state=dict(s, rest=[bad]), **HYPER)
     with pytest.raises(ValueError, match="1 m, expected 2|state has 1 m"):
         AdamW([p, p.clone()], StateBits=8, state=s, **HYPER)
+
+
+def test_overlapping_states_and_negative_steps_are_refused():
+    p = torch.ones(300, device="cuda")
+    x, y = torch.zeros(300, device="cuda"), torch.zeros(400, device="cuda")
+    for state in ({"m": [x], "v": [x]}, {"m": [y[:300]], "v": [y[100:]]}, {"m": [p], "v": [x]}):
+        with pytest.raises(ValueError, match="overlap"):
+            AdamW([p], state=dict(state, step=1))
+    with pytest.raises(ValueError, match="negative"):
+        AdamW([p], state={"m": [x], "v": [y[:300]], "step": -1})
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_not_finite_gradients_in_whole_chunks(bits):
+    """As test_adamw_gpu.py's, in the chunks that are read four values at a time: a NaN or infinite
+    gradient spoils its own value and no neighbour's."""
+    rs = np.random.default_rng(7)
+    n = 9000
+    gs = [torch.tensor(rs.normal(0, 1, n), dtype=torch.float32, device="cuda") for _ in range(8)]
+    bad = torch.zeros(n, dtype=torch.bool, device="cuda")
+    bad[[3, 300, 2047, 2048, 4444, n - 1]] = True
+    ps = [torch.ones(n, device="cuda") for _ in range(2)]
+    a, b = (AdamW([p], StateBits=bits, **HYPER) for p in ps)
+    for t, g in enumerate(gs):
+        g[bad] = 0.0
+        spoiled = g.clone()
+        if t == 5:
+            spoiled[3], spoiled[300], spoiled[2047] = float("nan"), float("inf"), -float("inf")
+            spoiled[2048], spoiled[4444], spoiled[n - 1] = float("inf"), float("nan"), float("inf")
+        a.step([spoiled])
+        b.step([g])
+    assert torch.equal(ps[0][~bad], ps[1][~bad]) and torch.isnan(ps[0][bad]).all()
+    for name in a._names:
+        x, y = getattr(a, name)[0], getattr(b, name)[0]
+        if name.endswith("scale"):
+            assert torch.equal(x, y)
+        else:
+            assert torch.equal(x.float()[~bad], y.float()[~bad])
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_more_chunks_than_blocks(bits):
+    """A tensor that the grid's blocks walk in several turns (2,048 blocks of 1,024 or 2,048 values): each
+    value as in a tensor of its block alone."""
+    n, part = 9_000_011, 8_399_872  # the part begins at a block of 256 and is behind 4 M values
+    g = torch.randn(n, device="cuda", generator=torch.Generator("cuda").manual_seed(3))
+    whole, some = torch.ones(n, device="cuda"), torch.ones(n - part, device="cuda")
+    a = AdamW([whole], StateBits=bits, **HYPER)
+    b = AdamW([some], StateBits=bits, **HYPER)
+    for t in range(3):  # (the first steps leave no rests, whose dither goes by place)
+        a.step([g * (t + 1)])
+        b.step([g[part:] * (t + 1)])
+    assert part % 256 == 0 and torch.equal(whole[part:], some)
+    assert torch.equal(a.m[0][part:].view(torch.uint8), b.m[0].view(torch.uint8))
+    assert ((whole != 1) | (g.abs() < 1e-7)).all()  # (randn gives a few zeros)
