@@ -815,16 +815,10 @@ struct mml_bpr {
 namespace {
 
 void upload_padded(mml_bpr* h, float* dst, const float* src, int64_t rows) {
-    if (rows == 0) return;
-    MML_HIP(hipMemsetAsync(dst, 0, sizeof(float) * rows * h->ld, h->ctx->stream));
-    MML_HIP(hipMemcpy2DAsync(dst, sizeof(float) * h->ld, src, sizeof(float) * h->k,
-                             sizeof(float) * h->k, rows, hipMemcpyHostToDevice, h->ctx->stream));
+    mml::upload_rows(h->ctx->stream, dst, h->ld, src, h->k, rows);
 }
-
 void download_padded(mml_bpr* h, float* dst, const float* src, int64_t rows) {
-    if (rows == 0) return;
-    MML_HIP(hipMemcpy2DAsync(dst, sizeof(float) * h->k, src, sizeof(float) * h->ld,
-                             sizeof(float) * h->k, rows, hipMemcpyDeviceToHost, h->ctx->stream));
+    mml::download_rows(h->ctx->stream, dst, h->k, src, h->ld, rows);
 }
 
 }  // namespace

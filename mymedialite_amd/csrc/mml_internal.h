@@ -153,6 +153,11 @@ void item_auc(hipStream_t st, const float* U, int32_t ldu, int32_t n_users_model
               const int32_t* candidates, int32_t n_cand, const int32_t* users, int32_t n_eval,
               const int64_t* test_off, const int32_t* test_items, double* out_auc);
 
+// Host rows of k floats <-> device rows of ld >= k (row_copy.hip); the device's columns from k on become 0.
+// On `st`; done with the host array when the stream is.
+void upload_rows(hipStream_t st, float* dst, int32_t ld, const float* src, int32_t k, int64_t rows);
+void download_rows(hipStream_t st, float* dst, int32_t k, const float* src, int32_t ld, int64_t rows);
+
 // The softmax over the catalogue (item_softmax.hip), stream-ordered: mml_item_log_probs_* without
 // the device scope and the status.
 void item_log_probs(const mml_item_softmax_args* a, float* log_probs, float* log_norm,
