@@ -99,6 +99,8 @@ class AdamW:
             raise ValueError(f"{len(grads)} gradients for {len(self.params)} parameters")
         keep = []
         for i, (g, p) in enumerate(zip(grads, self.params)):
+            if not isinstance(g, torch.Tensor):
+                raise ValueError(f"gradient {i} is not a tensor")
             if g.shape != p.shape or g.device != self._device:
                 raise ValueError(f"gradient {i} has not its parameter's shape and device")
             if g.dtype not in _DTYPES:

@@ -200,6 +200,10 @@ def test_overlapping_states_and_negative_steps_are_refused():
             AdamW([p], state=dict(state, step=1))
     with pytest.raises(ValueError, match="negative"):
         AdamW([p], state={"m": [x], "v": [y[:300]], "step": -1})
+    o = AdamW([p], state={"m": [x], "v": [y[:300]], "step": 1})
+    with pytest.raises(ValueError, match="gradient 0 is not a tensor"):
+        o.step([None])
+    assert o.state()["step"] == 1
 
 
 @pytest.mark.parametrize("bits", [32, 8])
