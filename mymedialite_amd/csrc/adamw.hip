@@ -22,7 +22,7 @@
 // within 0.93 and 1.06 of theirs, first moments within 1.5 %.
 //
 // Memory-bound: an f32 parameter takes 28 bytes with 32-bit moments (p, m, v read and written, g
-// read), 18.06 with 8-bit ones.  71.5 M f32 values take 400 us with 32-bit moments and 270 with 8-bit
+// read), 18.06 with 8-bit ones.  71.5 M f32 values take 400 us with 32-bit moments and 267 with 8-bit
 // ones, 5.0 and 4.8 TB/s (a large copy: 4.7); small models the 8 us of a launch.  One launch covers up to
 // kMaxTensors tensors, whose addresses are
 // kernel arguments (a captured graph replays with them); the step count lives on the device, so a
@@ -39,8 +39,8 @@ namespace {
 
 constexpr int kBlock = MML_ADAMW_BLOCK;  // values per scale
 // Values per block of threads and turn: 2 groups of 4 a thread with 32-bit moments, 1 with 8-bit
-// ones, whose arithmetic wants the waves instead (8 a SIMD; 71.5 M f32 values: 270 us against 320 with
-// 5 to 7 waves, though 7 of a wave's registers are spilled; 64 M f32 values with 32-bit moments: 354 us with 2 groups, 367 with 1).
+// ones, whose arithmetic wants the waves instead (8 a SIMD; 71.5 M f32 values: 267 us against 320 with
+// 5 to 7 waves, though 8 of a wave's registers are spilled; 64 M f32 values with 32-bit moments: 354 us with 2 groups, 367 with 1).
 template <int BITS>
 constexpr int kGroupsOf4 = BITS == 32 ? 2 : 1;
 template <int BITS>
@@ -189,28 +189,33 @@ template <int UNITS>
 __device__ __forceinline__ float with_rest(float d, int32_t rest) {
     return fmaf((float)rest * (0.125f / UNITS), spacings8(d), d);
 }
-// The rest of the quotient q (value / scale) whose code stands for d; dither in [0, 1)
+// The rest of the quotient q (value / scale) whose code stands for d, plus `bias` (so that cutting off
+// rounds down); dither 0 .. 255 in 256ths of a unit, under 1, so that what is a code's value exactly, 0
+// above all, stays it.  (The NaN code's does not matter.)
 template <int UNITS>
-__device__ __forceinline__ int32_t rest_of(float q, float d, float dither) {
+__device__ __forceinline__ uint32_t rest_of(float q, float d, float dither, int bias) {
     const float units = __uint_as_float((254u << 23) - __float_as_uint(spacings8(d))) * (8.0f * UNITS);
-    const int32_t r = (int32_t)floorf(fmaf(q - d, units, dither));  // (the NaN code's does not matter)
-    return min(max(r, -UNITS / 2), UNITS / 2);
+    const int32_t r = (int32_t)fmaf(dither, 0x1p-8f, fmaf(q - d, units, (float)bias));
+    return (uint32_t)min(max(r, bias - UNITS / 2), bias + UNITS / 2);
+}
+// Both rests in a byte, m's in the low 3 bits, as two's complements.  Packed with biases of 4 and 16, whose
+// removal is an exclusive or with kBiases.
+constexpr int kBiasM = 4, kBiasV = 16;
+constexpr uint32_t kBiases = 0x84848484u;
+__device__ __forceinline__ uint32_t biased_rests(float qm, float dm, float qv, float dv, float dither) {
+    return rest_of<kUnitsM>(qm, dm, dither, kBiasM) | rest_of<kUnitsV>(qv, dv, dither, kBiasV) << 3;
 }
 __device__ __forceinline__ int32_t rest_m(uint32_t byte) { return __builtin_amdgcn_sbfe((int)byte, 0, 3); }
 __device__ __forceinline__ int32_t rest_v(uint32_t byte) { return __builtin_amdgcn_sbfe((int)byte, 3, 5); }
-__device__ __forceinline__ uint32_t rest_byte(int32_t m, int32_t v) {
-    return ((uint32_t)m & 7u) | ((uint32_t)v & 31u) << 3;
-}
 // Steps that leave no rest: v is the sum of so few terms then that a term moves it by a code's
 // spacing or more, and codes and scales alone are the state of a run that short.
 constexpr int kBareSteps = 4;
-// Multiples of the golden ratio and of another fraction, as fractions of 2^32
-constexpr uint32_t kPlace = 0x85EBCA6Bu;
-__device__ __forceinline__ uint32_t dither_at(int32_t step, int64_t i) {
-    return (uint32_t)step * 0x9E3779B9u + (uint32_t)i * kPlace;
+// The dithers of four values from the i-th on (a multiple of 4), a byte each: multiples of the golden
+// ratio and of another fraction by step and place, as fractions of 2^32, whose bytes each run through all
+// values.
+__device__ __forceinline__ uint32_t dithers_at(int32_t step, int64_t i) {
+    return (uint32_t)step * 0x9E3779B9u + (uint32_t)(i >> 2) * 0x85EBCA6Bu;
 }
-// (under 1, so that what is a code's value exactly, 0 above all, stays it)
-__device__ __forceinline__ float fraction(uint32_t x) { return (float)(x >> 8) * 0x1p-24f; }
 
 // Four finite values / scale as codes.  The quotients are rounded as a division rounds them: one
 // division for the block's reciprocal y, then q = x y corrected by its remainder (Markstein 1990).
@@ -365,13 +370,12 @@ __global__ __launch_bounds__(256, BITS == 32 ? 1 : 8) void adamw_kernel(Step s) 
                     uint32_t rests = 0;
                     if (step > kBareSteps) {
                         const f32x4 dm = decode4(cm), dv = decode4(cv);
-                        const uint32_t first = dither_at(step, at[u]);
+                        const uint32_t dithers = dithers_at(step, at[u]);
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const float dither = fraction(first + e * kPlace);
-                            rests |= rest_byte(rest_of<kUnitsM>(qm[e], dm[e], dither),
-                                               rest_of<kUnitsV>(qr[e], dv[e], dither)) << (8 * e);
-                        }
+                        for (int e = 0; e < 4; ++e)
+                            rests |= biased_rests(qm[e], dm[e], qr[e], dv[e],
+                                                  (float)(dithers >> (8 * e) & 0xFFu)) << (8 * e);
+                        rests ^= kBiases;
                     }
                     *(uint32_t*)(q.rest + at[u]) = rests;
                     if ((t & 63) == 0) {
@@ -433,12 +437,13 @@ __global__ __launch_bounds__(256, BITS == 32 ? 1 : 8) void adamw_kernel(Step s) 
                         const float least = kE4m3Min * nr;
                         const uint8_t cm = encode(m[e], nm);
                         const uint8_t cv = encode(r[e] > 0.0f && r[e] < least ? least : r[e], nr);
-                        const float dither = fraction(dither_at(step, i));
+                        const float dither =
+                            (float)(dithers_at(step, i) >> (8 * (int)(i & 3)) & 0xFFu);
                         ((uint8_t*)q.m)[i] = cm;
                         ((uint8_t*)q.v)[i] = cv;
-                        q.rest[i] = step <= kBareSteps ? 0 : (uint8_t)rest_byte(
-                            rest_of<kUnitsM>(quotient(m[e], nm), decode(cm), dither),
-                            rest_of<kUnitsV>(quotient(r[e], nr), decode(cv), dither));
+                        q.rest[i] = step <= kBareSteps ? 0 : (uint8_t)(
+                            biased_rests(quotient(m[e], nm), decode(cm), quotient(r[e], nr),
+                                         decode(cv), dither) ^ kBiases);
                     }
                 }
                 if ((t & 63) == 0) {
