@@ -24,7 +24,8 @@ class AdamW:
     waiting; it may be captured into a graph, and a replay counts its step.  ``StateBits``: 32, or
     8 for moments as e4m3 codes with one scale per 256 values (``m``, ``v`` and ``m_scale``,
     ``v_scale``; ``v`` then holds the codes of sqrt(v)) and a byte for what both codes leave
-    (``rest``; zeros where a ``state`` has none).  LearnRate, Beta1, Beta2, Epsilon and
+    (``rest``), without which changes of less than half a code's spacing, which most are, would be
+    lost; a ``state`` that has none goes on without.  LearnRate, Beta1, Beta2, Epsilon and
     WeightDecay may be changed between steps.  ``state``: the dict that ``state()`` returned (its
     tensors are used, not copied), to go on from there."""
 
@@ -52,11 +53,13 @@ class AdamW:
         kind = torch.float32 if StateBits == 32 else torch.float8_e4m3fn
         names = ("m", "v") if StateBits == 32 else ("m", "v", "m_scale", "v_scale", "rest")
         s = dict(state) if state is not None else {}
+        if state is not None and "rest" not in s:
+            names = names[:4]
         for name in names:
             scale = name.endswith("scale")
             dtype = torch.float32 if scale else torch.uint8 if name == "rest" else kind
             if name not in s:
-                if state is not None and name != "rest":
+                if state is not None:
                     raise ValueError(f"state has no {name}")
                 zeros = torch.uint8 if dtype == torch.float8_e4m3fn else dtype
                 s[name] = [torch.zeros(b if scale else p.shape, device=self._device,
@@ -86,7 +89,8 @@ class AdamW:
             t.param, t.m, t.v = p.data_ptr(), self.m[i].data_ptr(), self.v[i].data_ptr()
             if StateBits == 8:
                 t.m_scale, t.v_scale = self.m_scale[i].data_ptr(), self.v_scale[i].data_ptr()
-                t.rest = self.rest[i].data_ptr()
+                if "rest" in names:
+                    t.rest = self.rest[i].data_ptr()
             t.n, t.param_dtype = p.numel(), _DTYPES[p.dtype]
 
     @property
@@ -119,7 +123,7 @@ class AdamW:
             self._device.index, torch._C._cuda_getCurrentRawStream(self._device.index)))
 
     def state(self):
-        """{"step", "m", "v"} and with 8 bits {"m_scale", "v_scale", "rest"}: the optimizer's own tensors
+        """{"step", "m", "v"}, with 8 bits {"m_scale", "v_scale"} and {"rest"}: the optimizer's own tensors
         and the number of steps done (waits for the device)."""
         s = {n: getattr(self, n) for n in self._names}
         s["step"] = int(self._count[0])

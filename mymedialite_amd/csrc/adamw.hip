@@ -15,7 +15,8 @@
 // half a code's spacing is 3 to 6 %, so rounding to nearest gives the old code back and the change is
 // lost (over 5,000 steps roots up to 9 times too large and 2 times too small; first moments 1.5 times
 // too large under a steady gradient).  So what a code leaves of its value, within half a spacing
-// either way, is kept in a byte that both moments share: 3 bits for m in sixths of a spacing, 5 for the
+// either way, is kept in a byte that both moments share (a caller may leave it out, to go on from a
+// state of codes and scales alone): 3 bits for m in sixths of a spacing, 5 for the
 // root in thirtieths.  That is rounded with a dither, the fraction of a multiple of the golden ratio
 // that goes with step and place, so that changes of less than a unit arrive on average; the same step
 // gives the same bits.  Over 5,000 steps of steady, sparse, rising and falling gradients (beta2 = 0.999)
@@ -23,8 +24,8 @@
 // moments within 1.3 % of their size.
 //
 // Memory-bound: an f32 parameter takes 28 bytes with 32-bit moments (p, m, v read and written, g
-// read), 18.06 with 8-bit ones.  71.5 M f32 values take 400 us with 32-bit moments and 267 with 8-bit
-// ones, 5.0 and 4.8 TB/s (a large copy: 4.7); small models the 8 us of a launch.  One launch covers up to
+// read), 18.06 with 8-bit ones (16.06 without the rests).  71.5 M f32 values take 400 us with 32-bit
+// moments and 267 with 8-bit ones (233), 5.0 and 4.8 TB/s (a large copy: 4.7); small models the 8 us of a launch.  One launch covers up to
 // kMaxTensors tensors, whose addresses are kernel arguments (a captured graph replays with them); the
 // step count lives on the device, so a replay counts on.
 #include <hip/hip_runtime.h>
@@ -40,7 +41,7 @@ namespace {
 constexpr int kBlock = MML_ADAMW_BLOCK;  // values per scale
 // Values per block of threads and turn: 2 groups of 4 a thread with 32-bit moments, 1 with 8-bit
 // ones, whose arithmetic wants the waves instead (8 a SIMD; 71.5 M f32 values: 267 us against 320 with
-// 5 to 7 waves, though 8 of a wave's registers are spilled; 64 M f32 values with 32-bit moments: 354 us
+// 5 to 7 waves, though 5 of a wave's registers are spilled; 64 M f32 values with 32-bit moments: 354 us
 // with 2 groups, 367 with 1).
 template <int BITS>
 constexpr int kGroupsOf4 = BITS == 32 ? 2 : 1;
@@ -236,7 +237,7 @@ __device__ __forceinline__ f32x4 decode4(uint32_t w) {
                  __builtin_amdgcn_cvt_f32_fp8((int)w, 2), __builtin_amdgcn_cvt_f32_fp8((int)w, 3)};
 }
 
-template <int BITS>
+template <int BITS, bool REST>
 __global__ __launch_bounds__(256, BITS == 32 ? 1 : 8) void adamw_kernel(Step s) {
     constexpr int NU = kGroupsOf4<BITS>;
     const int t = threadIdx.x;
@@ -266,7 +267,7 @@ __global__ __launch_bounds__(256, BITS == 32 ? 1 : 8) void adamw_kernel(Step s) 
         if (q.vec4 && base + kChunk<BITS> <= q.n) {  // a whole chunk
             f32x4 p[NU], g[NU], m[NU], v[NU];
             int64_t at[NU];
-            uint32_t mq[NU], vq[NU], rq[NU];
+            uint32_t mq[NU], vq[NU], rq[NU] = {};
             float ms[NU], vs[NU];
 #pragma unroll
             for (int u = 0; u < NU; ++u) {
@@ -281,7 +282,7 @@ __global__ __launch_bounds__(256, BITS == 32 ? 1 : 8) void adamw_kernel(Step s) 
                 } else {
                     mq[u] = *(const uint32_t*)((const uint8_t*)q.m + at[u]);
                     vq[u] = *(const uint32_t*)((const uint8_t*)q.v + at[u]);
-                    rq[u] = *(const uint32_t*)(q.rest + at[u]);
+                    if (REST) rq[u] = *(const uint32_t*)(q.rest + at[u]);
                     // (the same in all lanes: a scalar load)
                     const int64_t b = base / kBlock +
                                       __builtin_amdgcn_readfirstlane((t >> 6) * NU + u);
@@ -294,13 +295,16 @@ __global__ __launch_bounds__(256, BITS == 32 ? 1 : 8) void adamw_kernel(Step s) 
             for (int u = 0; u < NU; ++u) {
                 f32x4 r;
                 if constexpr (BITS == 8) {
-                    const f32x4 dm = decode4(mq[u]), dv = decode4(vq[u]);
+                    f32x4 dm = decode4(mq[u]), dv = decode4(vq[u]);
+                    if constexpr (REST)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        m[u][e] = with_rest<kUnitsM>(dm[e], rest_m(rq[u] >> (8 * e))) * ms[u];
-                        const float root = with_rest<kUnitsV>(dv[e], rest_v(rq[u] >> (8 * e))) * vs[u];
-                        v[u][e] = root * root;
-                    }
+                        for (int e = 0; e < 4; ++e) {
+                            dm[e] = with_rest<kUnitsM>(dm[e], rest_m(rq[u] >> (8 * e)));
+                            dv[e] = with_rest<kUnitsV>(dv[e], rest_v(rq[u] >> (8 * e)));
+                        }
+                    m[u] = dm * ms[u];
+                    const f32x4 root = dv * vs[u];
+                    v[u] = root * root;
                 }
                 bool small = false;
 #pragma unroll
@@ -370,7 +374,7 @@ __global__ __launch_bounds__(256, BITS == 32 ? 1 : 8) void adamw_kernel(Step s) 
                     *(uint32_t*)((uint8_t*)q.m + at[u]) = cm;
                     *(uint32_t*)((uint8_t*)q.v + at[u]) = cv;
                     uint32_t rests = 0;
-                    if (step > kBareSteps) {
+                    if (REST && step > kBareSteps) {
                         const f32x4 dm = decode4(cm), dv = decode4(cv);
                         const uint32_t dithers = dithers_at(step, at[u]);
 #pragma unroll
@@ -379,7 +383,7 @@ __global__ __launch_bounds__(256, BITS == 32 ? 1 : 8) void adamw_kernel(Step s) 
                                                   (float)(dithers >> (8 * e) & 0xFFu)) << (8 * e);
                         rests ^= kBiases;
                     }
-                    *(uint32_t*)(q.rest + at[u]) = rests;
+                    if (REST) *(uint32_t*)(q.rest + at[u]) = rests;
                     if ((t & 63) == 0) {
                         q.ms[at[u] / kBlock] = nm;
                         q.vs[at[u] / kBlock] = nr;
@@ -413,7 +417,7 @@ __global__ __launch_bounds__(256, BITS == 32 ? 1 : 8) void adamw_kernel(Step s) 
                     const int64_t i = b0 + e * 64 + (t & 63);
                     m[e] = r[e] = 0.0f;
                     if (i < q.n) {
-                        const uint32_t rest = q.rest[i];
+                        const uint32_t rest = REST ? q.rest[i] : 0;
                         m[e] = with_rest<kUnitsM>(decode(((uint8_t*)q.m)[i]), rest_m(rest)) * ms;
                         const float root =
                             with_rest<kUnitsV>(decode(((uint8_t*)q.v)[i]), rest_v(rest)) * vs;
@@ -443,9 +447,10 @@ __global__ __launch_bounds__(256, BITS == 32 ? 1 : 8) void adamw_kernel(Step s) 
                             (float)(dithers_at(step, i) >> (8 * (int)(i & 3)) & 0xFFu);
                         ((uint8_t*)q.m)[i] = cm;
                         ((uint8_t*)q.v)[i] = cv;
-                        q.rest[i] = step <= kBareSteps ? 0 : (uint8_t)(
-                            biased_rests(quotient(m[e], nm), decode(cm), quotient(r[e], nr),
-                                         decode(cv), dither) ^ kBiases);
+                        if (REST)
+                            q.rest[i] = step <= kBareSteps ? 0 : (uint8_t)(
+                                biased_rests(quotient(m[e], nm), decode(cm), quotient(r[e], nr),
+                                             decode(cv), dither) ^ kBiases);
                     }
                 }
                 if ((t & 63) == 0) {
@@ -486,7 +491,6 @@ void check_tensor(const mml_adamw_tensor& x, int32_t bits) {
     if (x.n == 0) return;
     MML_REQUIRE(x.param && x.grad && x.m && x.v, "a tensor's pointer is null");
     MML_REQUIRE(bits == 32 || (x.m_scale && x.v_scale), "8-bit moments without their scales");
-    MML_REQUIRE(bits == 32 || x.rest, "8-bit moments without their rests");
 }
 
 }  // namespace
@@ -505,7 +509,14 @@ extern "C" mml_status mml_adamw_step_device(const mml_adamw_tensor* tensors, int
                     "learn_rate, epsilon and weight_decay must be finite and not negative");
         MML_REQUIRE(a.beta1 >= 0.0 && a.beta1 < 1.0 && a.beta2 >= 0.0 && a.beta2 < 1.0,
                     "beta1 and beta2 must be in [0, 1)");
-        for (int32_t i = 0; i < n_tensors; ++i) check_tensor(tensors[i], a.state_bits);
+        int32_t sized = 0, with_rest = 0;
+        for (int32_t i = 0; i < n_tensors; ++i) {
+            check_tensor(tensors[i], a.state_bits);
+            sized += tensors[i].n > 0;
+            with_rest += tensors[i].n > 0 && tensors[i].rest;
+        }
+        MML_REQUIRE(a.state_bits == 32 || with_rest == 0 || with_rest == sized,
+                    "rests of some tensors only");
         mml::DeviceScope on(device);
         Step s{};
         s.lr = a.learn_rate;
@@ -530,7 +541,7 @@ extern "C" mml_status mml_adamw_step_device(const mml_adamw_tensor* tensors, int
                 const bool vec4 = aligned(x.param, x.param_dtype == MML_DTYPE_F32 ? 16 : 8) &&
                                   aligned(x.grad, x.grad_dtype == MML_DTYPE_F32 ? 16 : 8) &&
                                   aligned(x.m, moment) && aligned(x.v, moment) &&
-                                  (a.state_bits == 32 || aligned(x.rest, 4));
+                                  aligned(x.rest, 4);
                 s.t[s.n_tensors++] = Tensor{x.param, x.grad, x.m, x.v, x.m_scale, x.v_scale, x.rest,
                                             x.n, s.chunks, (int16_t)x.param_dtype,
                                             (int16_t)x.grad_dtype, vec4};
@@ -540,9 +551,11 @@ extern "C" mml_status mml_adamw_step_device(const mml_adamw_tensor* tensors, int
             s.last = i == n_tensors;
             const uint32_t blocks = (uint32_t)std::max<int64_t>(1, std::min<int64_t>(s.chunks, 2048));
             if (a.state_bits == 32)
-                adamw_kernel<32><<<blocks, 256, 0, (hipStream_t)stream>>>(s);
+                adamw_kernel<32, false><<<blocks, 256, 0, (hipStream_t)stream>>>(s);
+            else if (with_rest)
+                adamw_kernel<8, true><<<blocks, 256, 0, (hipStream_t)stream>>>(s);
             else
-                adamw_kernel<8><<<blocks, 256, 0, (hipStream_t)stream>>>(s);
+                adamw_kernel<8, false><<<blocks, 256, 0, (hipStream_t)stream>>>(s);
             MML_HIP(hipGetLastError());
         } while (i < n_tensors);
     });

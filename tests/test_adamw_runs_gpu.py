@@ -177,19 +177,41 @@ def test_steps_repeat_bit_for_bit(at):
 
 
 def test_states_without_rests_and_refusals():
-    """A state of codes and scales alone goes on from there; rests of another type or size are refused."""
-    p = torch.ones(300, device="cuda")
+    """A state of codes and scales alone goes on as one, whatever the step: each step is that of the
+    definition from the codes, to nearest (tolerance: codes whose quotient lies within 16 EPS of the
+    middle of two may be either).  Rests of another type or size are refused."""
+    rs = np.random.default_rng(9)
+    n = 1324
+    p = torch.ones(n, device="cuda")
     a = AdamW([p], StateBits=8, **HYPER)
-    a.step([torch.full((300,), 0.5, device="cuda")])
-    s = a.state()
-    del s["rest"]
+    gs = [torch.tensor(rs.normal(0, 1, n), dtype=torch.float32, device="cuda") for _ in range(9)]
+    for g in gs[:6]:
+        a.step([g])
+    s = {k: v if k == "step" else [x.clone() for x in v] for k, v in a.state().items() if k != "rest"}
     b = AdamW([p], StateBits=8, state=s, **HYPER)
-    assert (b.rest[0] == 0).all() and b.rest[0].shape == p.shape
+    assert "rest" not in b.state() and not hasattr(b, "rest")
+    for t, g in enumerate(gs[6:], 7):
+        m, root = (np.repeat(scale[0].cpu().double().numpy(), 256)[:n] * q[0].cpu().double().numpy()
+                   for q, scale in ((b.m, b.m_scale), (b.v, b.v_scale)))
+        b.step([g])
+        g = g.cpu().double().numpy()
+        m, v = 0.9 * m + 0.1 * g, 0.999 * root ** 2 + 0.001 * g * g
+        for q, scale, x in ((b.m, b.m_scale, m), (b.v, b.v_scale, np.sqrt(v))):
+            block = np.array([np.abs(x[i:i + 256]).max() / 448 for i in range(0, n, 256)])
+            np.testing.assert_allclose(scale[0].cpu().double().numpy(), block, rtol=16 * EPS)
+            want = x / np.repeat(block, 256)[:n]
+            slack = 16 * EPS * (np.abs(want) + (np.abs(g) / np.repeat(block, 256)[:n] if x is m else 0))
+            e4m3 = lambda y: torch.tensor(y).float().to(torch.float8_e4m3fn).double().numpy()
+            lo, hi, got = e4m3(want - slack), e4m3(want + slack), q[0].cpu().double().numpy()
+            assert ((got >= np.minimum(lo, hi)) & (got <= np.maximum(lo, hi))).all(), t
+    short = torch.ones(300, device="cuda")
+    c = AdamW([short], StateBits=8, **HYPER)
+    s = c.state()
     for bad in (torch.zeros(300, device="cuda"), torch.zeros(299, dtype=torch.uint8, device="cuda")):
         with pytest.raises(ValueError, match="state's rest must"):
-            AdamW([p], StateBits=8, state=dict(s, rest=[bad]), **HYPER)
-    with pytest.raises(ValueError, match="1 m, expected 2|state has 1 m"):
-        AdamW([p, p.clone()], StateBits=8, state=s, **HYPER)
+            AdamW([short], StateBits=8, state=dict(s, rest=[bad]), **HYPER)
+    with pytest.raises(ValueError, match="state has 1 m, expected 2"):
+        AdamW([short, short.clone()], StateBits=8, state=s, **HYPER)
 
 
 def test_overlapping_states_and_negative_steps_are_refused():
