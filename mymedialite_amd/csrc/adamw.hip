@@ -16,18 +16,18 @@
 // lost (over 5,000 steps roots up to 9 times too large and 2 times too small; first moments 1.5 times
 // too large under a steady gradient).  So what a code leaves of its value, within half a spacing
 // either way, is kept in a byte that both moments share (a caller may leave it out, to go on from a
-// state of codes and scales alone): 3 bits for m in sixths of a spacing, 5 for the
-// root in thirtieths.  That is rounded with a dither, the fraction of a multiple of the golden ratio
-// that goes with step and place, so that changes of less than a unit arrive on average; the same step
-// gives the same bits.  Over 5,000 steps of steady, sparse, rising and falling gradients (beta2 = 0.999)
+// state of codes and scales alone): 3 bits for m in sixths of a spacing, 5 for the root in thirtieths.
+// That is rounded with a dither, the fraction of a multiple of the golden ratio that goes with step and
+// place, so that changes of less than a unit arrive on average; the same step gives the same bits.  Over 5,000 steps of steady, sparse, rising and falling gradients (beta2 = 0.999)
 // roots then lie within 0.93 and 1.07 of theirs, 0.89 and 1.09 where half a block's gradients stop, first
 // moments within 1.3 % of their size.
 //
 // Memory-bound: an f32 parameter takes 28 bytes with 32-bit moments (p, m, v read and written, g
-// read), 18.06 with 8-bit ones (16.06 without the rests).  71.5 M f32 values take 400 us with 32-bit
-// moments and 267 with 8-bit ones (233), 5.0 and 4.8 TB/s (a large copy: 4.7); small models the 8 us of a launch.  One launch covers up to
-// kMaxTensors tensors, whose addresses are kernel arguments (a captured graph replays with them); the
-// step count lives on the device, so a replay counts on.
+// read), 18.06 with 8-bit ones, 16.06 without the rests.  71.5 M f32 values take 400, 267 and 231 us: 5.0,
+// 4.8 and 5.0 TB/s (a large copy: 4.7).  With bf16 parameters 8-bit moments are bound by the vector
+// instructions, some 100 a value with the rests: 232 us, 167 without (862 and 719 MB).  Small models take
+// the 8 us of a launch.  One launch covers up to kMaxTensors tensors, whose addresses are kernel arguments
+// (a captured graph replays with them); the step count lives on the device, so a replay counts on.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>

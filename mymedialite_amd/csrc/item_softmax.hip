@@ -426,7 +426,7 @@ __device__ __forceinline__ void make_meta(const Job& j, int64_t r, int bad) {
 // rows' sums: an item that is not excluded gets the bias NaN, a user NaN results from the last kernel or
 // NaN constants.  So is an item that its bias excludes, whose factors the scale does not count.  Bound by
 // memory: 1 M items, k = 128 bf16 in 98 us (512 MB, 5.2 TB/s), 500 k with k = 256 and the transposed
-// fragments in 152 us (768 MB).
+// fragments in 155 us (768 MB).
 template <int T, int KT>
 __global__ __launch_bounds__(256) void softmax_prep_kernel(Job j) {
     using P = Planes<T>;
@@ -744,7 +744,7 @@ constexpr int kTileGroup = 8;  // the streamed items are padded to a multiple of
 // turn in two buffers: the next turn's tiles are on the way while this one's are used.  Lane l: user
 // l % 32, 16 of a tile's 32 items.  m, l, w: the running maximum (of scaled scores), the sum of
 // e = exp(s - m) and of e y, y = log2 e.
-// Bound by instructions and power, not memory: 2,048 x 1 M, k = 128 bf16 takes 722 us, where the SIMDs
+// Bound by instructions and power, not memory: 2,048 x 1 M, k = 128 bf16 takes 726 us, where the SIMDs
 // issue about 450 cycles of vector instructions a tile (16 exponentials of 8 cycles, 80 others of 4), 64 % of
 // the time, beside 256 of matrix instructions, at 1.95 GHz of 2.4: on zeros the same launch takes 500 us.
 template <int T, int KT, bool TOP>
@@ -1467,7 +1467,7 @@ __global__ __launch_bounds__(NT, 8) void softmax_finish_kernel(Job j) {
 // 4 and 3 against 236 with 8 and 4, which spills (a reload waits for the copies on the way); k > 128:
 // users 729 with 4 and 2 against 1,221 with 4 and 1.
 // Bound by the matrix cores and power: 1024 x 500k, k = 256 bf16 takes 3 products a side (the scores
-// again, G's two planes), 786 Gflop, in 654 us (users) and 725 (items): 1.20 and 1.08 Pflop/s, where a
+// again, G's two planes), 786 Gflop, in 669 us (users) and 723 (items): 1.17 and 1.09 Pflop/s, where a
 // large library product reaches 1.23.
 template <int T, int KT>
 constexpr int users_waves() {
