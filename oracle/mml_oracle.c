@@ -1466,10 +1466,14 @@ static void ora_lu_inverse(double* a, double* inv, int n, int* piv, double* col)
     }
 }
 
+/* Threads of ora_wrmf_square and ora_wrmf_optimize_rows (one unless set: the CPU baseline's) */
+static int ora_wrmf_threads = 1;
+void ora_wrmf_set_threads(int n) { ora_wrmf_threads = n > 0 ? n : 1; }
+
 /* WRMF.ComputeSquareMatrix :94-108 -- float products, double sums */
 void ora_wrmf_square(const float* H, int64_t rows, int k, double* HH) {
     /* (elements on threads; every sum in its own order) */
-#pragma omp parallel for schedule(dynamic, 1)
+#pragma omp parallel for schedule(dynamic, 1) num_threads(ora_wrmf_threads)
     for (int f1 = 0; f1 < k; f1++)
         for (int f2 = f1; f2 < k; f2++) {
             double d = 0.0;
@@ -1510,7 +1514,7 @@ static void wrmf_optimize_rows_impl(const int64_t* off, const int32_t* cols, int
                                     const float* H, const double* HH, int k, double alpha,
                                     double reg, int exact) {
     /* (rows on threads: each its own system) */
-#pragma omp parallel
+#pragma omp parallel num_threads(ora_wrmf_threads)
     {
     double* HC = (double*)malloc(sizeof(double) * (size_t)k * k);
     double* m = (double*)malloc(sizeof(double) * (size_t)k * k);

@@ -17,6 +17,7 @@ Drivers below mirror the reference's control flow:
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import math
 import os
@@ -888,6 +889,16 @@ def bpr_update(u, i, j, U, V, bias, *, learn_rate=0.05, reg_u=0.0025, reg_i=0.00
 
 
 # ----------------------------------------------------------------------------- WRMF
+@contextlib.contextmanager
+def _wrmf_threads():
+    """ora_wrmf_* on this process's cores inside (one thread outside, as the CPU baseline runs it)"""
+    lib().ora_wrmf_set_threads(min(16, len(os.sched_getaffinity(0))))
+    try:
+        yield
+    finally:
+        lib().ora_wrmf_set_threads(1)
+
+
 def wrmf_square(H):
     H = f32(H)
     k = H.shape[1]
@@ -900,10 +911,11 @@ def wrmf_optimize(off, cols, W, H, alpha, reg, exact_products=False):
     """WRMF.Optimize(data, W, H) (:79-92) in place on W.  exact_products: the row Gram's products
     exact in double instead of rounded to float (ora_wrmf_optimize_rows_exact; a test variant,
     the system the library's fp64 refinement solves)."""
-    HH = wrmf_square(H)
     fn = lib().ora_wrmf_optimize_rows_exact if exact_products else lib().ora_wrmf_optimize_rows
-    fn(_p(off, _i64p), _p(cols, _i32p), 0, W.shape[0], len(off) - 1, _p(W, _f32p),
-       _p(f32(H), _f32p), _p(HH, _f64p), W.shape[1], float(alpha), float(reg))
+    with _wrmf_threads():
+        HH = wrmf_square(H)
+        fn(_p(off, _i64p), _p(cols, _i32p), 0, W.shape[0], len(off) - 1, _p(W, _f32p),
+           _p(f32(H), _f32p), _p(HH, _f64p), W.shape[1], float(alpha), float(reg))
 
 
 def wrmf_train(users, items, n_users, n_items, *, seed=1, k=10, num_iter=15, alpha=1.0,
@@ -1005,7 +1017,8 @@ def wrmf_rows_check(rows, row_ids, col_ids, W, H, k, alpha=1.0, reg=0.015,
     Wr = np.zeros((len(rows), k), np.float32)
     solve = lib().ora_wrmf_optimize_rows if reference_products else \
         lib().ora_wrmf_optimize_rows_exact
-    solve(_p(off, _i64p), _p(c_, _i32p), 0, len(rows), len(rows), _p(Wr, _f32p),
-          _p(f32(H), _f32p), _p(HH, _f64p), k, float(alpha), float(reg))
+    with _wrmf_threads():
+        solve(_p(off, _i64p), _p(c_, _i32p), 0, len(rows), len(rows), _p(Wr, _f32p),
+              _p(f32(H), _f32p), _p(HH, _f64p), k, float(alpha), float(reg))
     got = np.asarray(W)[rows]
     return np.abs(got - Wr).max(1) / (1.0 + np.abs(Wr).max(1))
