@@ -691,17 +691,17 @@ mml_status mml_item_log_probs_grad_device(const mml_item_softmax_args* args, con
  *          - learn_rate m / (1 - beta1^t) / (sqrt(v / (1 - beta2^t)) + epsilon),
  * in f32, a half-precision parameter rounded once to nearest.  state_bits 32: m and v are float[n].
  * 8: m and v are e4m3 codes (uint8_t[n], the OCP format without infinities), value = code x scale
- * of its MML_ADAMW_BLOCK consecutive values, scale = largest magnitude / 448 (float[ceil(n / 256)]; 0
- * for a block of zeros, else 2^-126 at least);
- * v's codes hold sqrt(v), and one that is not zero never gets code 0.  A code is the nearest; what it
- * leaves of its value is kept in `rest` (uint8_t[n], 3 bits for m in sixths of a code's spacing, 5 for
- * sqrt(v) in thirtieths, rounded with a dither that step and place give; the first 4 steps leave none),
- * so that moments follow their recurrences though a step changes them by less than half a spacing.
- * NULL for every tensor: codes and scales alone are the state, and such changes are lost: over some
- * thousand steps roots were up to 9 times too large (where gradients fell) and 2 times too small (where
- * they rose), first moments 1.5 times too large; for runs of few steps, or to go on from such a state.  A gradient that is not
- * finite (8 bits: or whose square is not) makes that value's parameter and moments NaN or infinite
- * and no other's.  All zero is the start of both forms.
+ * of its MML_ADAMW_BLOCK consecutive values, scale = largest magnitude / 448 (float[ceil(n / 256)];
+ * 0 for a block of zeros, else 2^-126 at least); v's codes hold sqrt(v), and one that is not zero
+ * never gets code 0.  A code is the nearest; what it leaves of its value is kept in `rest`
+ * (uint8_t[n]: 3 bits for m in sixths of a code's spacing, 5 for sqrt(v) in thirtieths, rounded with
+ * a dither that step and place give; the first 4 steps leave none), so that moments follow their
+ * recurrences though a step changes them by less than half a spacing.  rest NULL for every tensor:
+ * codes and scales alone are the state, and such changes are lost: over some thousand steps roots
+ * were up to 9 times too large (where gradients fell) and 2 times too small (where they rose), first
+ * moments 1.5 times too large; for runs of few steps, or to go on from such a state.
+ * A gradient that is not finite (8 bits: or whose square is not) makes that value's parameter and
+ * moments NaN or infinite and no other's.  All zero is the start of both forms.
  * Stream-ordered like mml_item_log_probs_device, nothing allocated or read back; a captured step
  * counts on at every replay (learn_rate is replayed as captured).  step_state:
  * int32_t[MML_ADAMW_STATE] on the device, {steps done, 0, ..., 0}; one step at a time may use it.
